@@ -1,0 +1,412 @@
+"""Measured cases of the 4-bit operators and the mixture-of-experts layer: quantisation to microscaled 4-bit floats, the
+product of two quantised operands, the product of unquantised activations with quantised weights, and a whole
+mixture-of-experts MLP for the few tokens of a decoding step.
+
+A quantised row ("mx4") of k numbers is cut into blocks of 32 along k, k padded with zeros to kp, a multiple of 128:
+one byte of two e2m1 codes per pair of elements (the first in the low half) and one scale byte s per block, worth
+2^(s - 127), 255 for a block that is not a number. An operand is codes [rows, kp / 2] and scales [rows, kp / 32].
+Sizes are those of the shipped MLP graphs and of the benchmark's GEMMs (512 x 2048, 4096 x 14336), and odd ones
+between them."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+DEVICE = "cuda"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+CODES = {"f32": 0, "bf16": 1, "f16": 2, "mx4": 4}
+MOST_ELEMENTS = 4096 * 14336          # of a quantised tensor
+MOST_MULTIPLY_ADDS = 4096 * 4096 * 14336  # of a product
+MOST_EXPERT_WEIGHTS = 64 * 3 * 2048 * 1024
+
+
+def listed():
+    return [
+        # One token's activations before a 4-bit product: latency only.
+        {"name": "quantize_one_row", "op": "quantize", "form": "rows", "type": "bf16", "rows": 1, "k": 4096, "pad": 0},
+        # The hidden activations of the benchmark's MLP block.
+        {"name": "quantize_8192_rows", "op": "quantize", "form": "rows", "type": "f32", "rows": 8192, "k": 2048, "pad": 0},
+        # Weights of a layer with odd sizes, a view of wider rows, stored [k, n] as the matmuls take B.
+        {"name": "quantize_columns_odd", "op": "quantize", "form": "columns", "type": "f16", "rows": 2047, "k": 1001,
+         "pad": 7},
+        # A serving batch through a quantised layer.
+        {"name": "mx4_16_rows", "op": "product", "m": 16, "n": 4096, "k": 4096, "out": "bf16"},
+        # Sizes that no tile divides, fp32 result.
+        {"name": "mx4_ragged", "op": "product", "m": 1000, "n": 1001, "k": 1023, "out": "f32"},
+        # The FFN shape of the benchmark.
+        {"name": "mx4_ffn", "op": "product", "m": 4096, "n": 14336, "k": 4096, "out": "bf16"},
+        # One token through the same layer with 4-bit weights only.
+        {"name": "weights_one_row", "op": "weights", "type": "bf16", "m": 1, "n": 14336, "k": 4096},
+        # A serving batch in fp16.
+        {"name": "weights_32_rows", "op": "weights", "type": "f16", "m": 32, "n": 4096, "k": 4096},
+        # A prompt of odd length and sizes, fp32 activations.
+        {"name": "weights_ragged", "op": "weights", "type": "f32", "m": 300, "n": 1001, "k": 1023},
+        # One token of a decoding step, many experts on 4-bit weights.
+        {"name": "moe_one_token", "op": "moe", "type": "bf16", "weights": "mx4", "tokens": 1, "d": 2048, "h": 1024,
+         "experts": 64, "top_k": 8, "act": "swiglu"},
+        # The shipped MLP block's sizes with eight experts, biases and GELU, fp32 activations and bf16 weights.
+        {"name": "moe_16_tokens", "op": "moe", "type": "f32", "weights": "bf16", "tokens": 16, "d": 512, "h": 2048,
+         "experts": 8, "top_k": 2, "act": "gelu"},
+        # The widest batch of a step: every expert is read. Odd sizes, 16-bit weights.
+        {"name": "moe_64_tokens", "op": "moe", "type": "f16", "weights": "f16", "tokens": 64, "d": 1023, "h": 777,
+         "experts": 32, "top_k": 4, "act": "swiglu"},
+    ]
+
+
+def _size(rng, lo, hi):
+    """A size between lo and hi, even over its logarithm: as it falls, or a multiple of 8 or of 64."""
+    hi = max(lo, hi)
+    n = round(math.exp(rng.uniform(math.log(lo), math.log(hi))))
+    step = rng.choice((1, 1, 8, 64))
+    return max(lo, min(hi, (n + step - 1) // step * step))
+
+
+def draw(rng):
+    op = rng.choice(("quantize", "product", "weights", "moe"))
+    if op == "quantize":
+        k = _size(rng, 32, 14336)
+        return {"op": op, "form": rng.choice(("rows", "columns")), "type": rng.choice(sorted(TYPES)),
+                "rows": _size(rng, 1, min(8192, MOST_ELEMENTS // 4 // k)), "k": k, "pad": rng.choice((0, 0, 1, 8, 24))}
+    if op in ("product", "weights"):
+        k = _size(rng, 64, 8192)
+        n = _size(rng, 64, min(14336, MOST_ELEMENTS // k))
+        # Rows from one token on; with unquantised activations mostly few.
+        most = min(4096, MOST_MULTIPLY_ADDS // (n * k)) if op == "product" or rng.random() < 0.3 else 64
+        case = {"op": op, "m": _size(rng, 1, most), "n": n, "k": k}
+        case["out" if op == "product" else "type"] = rng.choice(sorted(TYPES))
+        return case
+    act = rng.choice(("relu", "gelu", "swiglu"))
+    experts = rng.choice((4, 8, 16, 31, 64))
+    d = _size(rng, 256, 2048)
+    mats = 3 if act == "swiglu" else 2
+    weights = rng.choice(("bf16", "f16", "mx4"))
+    h = _size(rng, 128, min(2048, MOST_EXPERT_WEIGHTS // 4 // (mats * d * experts)))
+    return {"op": op, "type": rng.choice(sorted(TYPES)), "weights": weights, "tokens": _size(rng, 1, 64), "d": d, "h": h,
+            "experts": experts, "top_k": rng.randint(1, min(8, experts)), "act": act}
+
+
+# ---------------------------------------------------------------- the format in elementary operations
+
+
+def _padded(k):
+    return (k + 127) // 128 * 128
+
+
+def _blocks(x):
+    """[..., k] as fp32 blocks [..., kp / 32, 32]."""
+    x = x.float()
+    x = torch.nn.functional.pad(x, (0, _padded(x.shape[-1]) - x.shape[-1]))
+    return x.reshape(*x.shape[:-1], -1, 32)
+
+
+def _quantize(x):
+    """Rows [..., k] to (magnitude and sign codes [..., kp / 32, 32], scale bytes [..., kp / 32]); finite inputs."""
+    b = _blocks(x)
+    amax = b.abs().amax(-1)
+    # The biased exponent of the largest magnitude, less 2 (6 = 1.5 * 2^2 is the largest code).
+    scale = ((amax.view(torch.int32) >> 23) - 2).clamp(min=0)
+    v = b.abs() * ((254 - scale) << 23).view(torch.float32).unsqueeze(-1)
+    # Codes count the magnitudes 0 .5 1 1.5 2 3 4 6; a tie goes to the even code.
+    code = (v > 0.25).int() + (v >= 0.75) + (v > 1.25) + (v >= 1.75) + (v > 2.5) + (v >= 3.5) + (v > 5.0)
+    return code + 8 * (b < 0), scale
+
+
+def _decode(code, scale):
+    """fp32 values [..., kp] of unpacked codes and scale bytes."""
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=DEVICE)
+    # 2^(scale - 127), also where that is no normal number.
+    v = table[(code & 7).long()] * (((scale.int() + 1) << 23).view(torch.float32) * 0.5).unsqueeze(-1)
+    v = torch.where(code >= 8, -v, v)
+    return v.reshape(*v.shape[:-2], -1)
+
+
+def _pack(code, scale):
+    """The operand's bytes."""
+    code = code.reshape(*code.shape[:-2], -1).to(torch.uint8)
+    return (code[..., 0::2] | (code[..., 1::2] << 4)).contiguous(), scale.to(torch.uint8).contiguous()
+
+
+def _unpack(packed, k):
+    """fp32 values [..., k] of an operand."""
+    codes, scales = packed
+    code = torch.stack((codes & 15, codes >> 4), -1).int()
+    return _decode(code.reshape(*codes.shape[:-1], -1, 32), scales)[..., :k]
+
+
+# ---------------------------------------------------------------- inputs
+
+
+def _normal(gen, shape, std=1.0):
+    return torch.empty(shape, dtype=torch.float32, device=DEVICE).normal_(0.0, std, generator=gen)
+
+
+def _activations(gen, shape):
+    """Normal values with channels of different strength, as activations have them."""
+    return _normal(gen, shape) * torch.exp(0.5 * _normal(gen, shape[-1:]))
+
+
+def _inputs(case, seed):
+    gen = torch.Generator(device=DEVICE).manual_seed(seed)
+    op = case["op"]
+    if op == "quantize":
+        shape = [case["rows"], case["k"]] if case["form"] == "rows" else [case["k"], case["rows"]]
+        wide = _activations(gen, [shape[0], shape[1] + case["pad"]]).to(TYPES[case["type"]])
+        return {"x": wide[:, :shape[1]]}
+    if op in ("product", "weights"):
+        m, n, k = case["m"], case["n"], case["k"]
+        a = _activations(gen, [m, k])
+        b = _pack(*_quantize(_normal(gen, [n, k], k ** -0.5)))
+        return {"a": _pack(*_quantize(a)) if op == "product" else a.to(TYPES[case["type"]]), "b": b}
+    d, h, e = case["d"], case["h"], case["experts"]
+    rows = 2 * h if case["act"] == "swiglu" else h
+    t = {"x": _activations(gen, [case["tokens"], d]).to(TYPES[case["type"]]),
+         "router": _normal(gen, [e, d], d ** -0.5), "b1": None, "b2": None}
+    if case["act"] != "swiglu":
+        t["b1"], t["b2"] = _normal(gen, [e, rows], 0.1), _normal(gen, [e, d], 0.1)
+    for name, shape in (("w1", [e, rows, d]), ("w2", [e, d, h])):
+        w = _normal(gen, shape, shape[-1] ** -0.5)
+        t[name] = _pack(*_quantize(w)) if case["weights"] == "mx4" else w.to(TYPES[case["weights"]])
+    return t
+
+
+def prepare(case, seed):
+    state = {"case": case, **_inputs(case, seed)}
+    if not own:
+        return state
+    import minicompiler_amd as mc
+
+    mc.library()
+    op = case["op"]
+    # On the stream that the program's tensors are made on.
+    state["mc"], state["stream"] = mc, torch.cuda.current_stream().cuda_stream
+    workspace = 0
+    if op == "quantize":
+        x = state["x"]
+        rows, k = case["rows"], case["k"]
+        state["codes"] = torch.empty(mc.mx4_code_bytes(rows, k), dtype=torch.uint8, device=DEVICE)
+        state["scales"] = torch.empty(mc.mx4_scale_bytes(rows, k), dtype=torch.uint8, device=DEVICE)
+        state["out"] = torch.empty(x.shape, dtype=x.dtype, device=DEVICE)
+    elif op == "moe":
+        state["out"] = torch.empty_like(state["x"])
+        workspace = mc.moe_workspace_bytes(CODES[case["type"]], case["tokens"], case["d"], case["h"], case["experts"],
+                                           case["top_k"])
+    else:
+        kind = case["out"] if op == "product" else case["type"]
+        state["out"] = torch.empty([case["m"], case["n"]], dtype=TYPES[kind], device=DEVICE)
+        sizes = (case["m"], case["n"], case["k"])
+        workspace = (mc.matmul_mx4_workspace_bytes(*sizes) if op == "product" else
+                     mc.matmul_mx4_weights_workspace_bytes(CODES[kind], *sizes))
+    # Zero before its first use, as the calls ask.
+    state["workspace"] = torch.zeros(workspace, dtype=torch.uint8, device=DEVICE) if workspace else None
+    torch.cuda.synchronize()
+    return state
+
+
+# ---------------------------------------------------------------- one pass
+
+
+def _address(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _run_own(state):
+    mc, case, stream, out = state["mc"], state["case"], state["stream"], state["out"]
+    op = case["op"]
+    if op == "quantize":
+        x = state["x"]
+        if case["form"] == "rows":
+            mc.quantize_mx4(CODES[case["type"]], x.data_ptr(), x.stride(0), state["codes"].data_ptr(),
+                            state["scales"].data_ptr(), case["rows"], case["k"], out.data_ptr(), stream)
+        else:
+            mc.quantize_mx4_columns(CODES[case["type"]], x.data_ptr(), x.stride(0), state["codes"].data_ptr(),
+                                    state["scales"].data_ptr(), case["k"], case["rows"], out.data_ptr(), stream)
+        return out
+    workspace = _address(state["workspace"])
+    if op == "moe":
+        w1, w2 = state["w1"], state["w2"]
+        if case["weights"] == "mx4":
+            (w1, s1), (w2, s2) = w1, w2
+        else:
+            s1 = s2 = None
+        mc.launch_moe(CODES[case["type"]], state["x"].data_ptr(), case["d"], state["router"].data_ptr(),
+                      CODES[case["weights"]], w1.data_ptr(), _address(s1), _address(state["b1"]), w2.data_ptr(),
+                      _address(s2), _address(state["b2"]), out.data_ptr(), None, None, case["tokens"], case["d"],
+                      case["h"], case["experts"], case["top_k"], case["act"], True, stream, workspace)
+        return out
+    bc, bs = state["b"]
+    if op == "product":
+        ac, scales = state["a"]
+        mc.launch_matmul_mx4(ac.data_ptr(), scales.data_ptr(), bc.data_ptr(), bs.data_ptr(), CODES[case["out"]],
+                             out.data_ptr(), case["m"], case["n"], case["k"], stream, workspace)
+    else:
+        kind = CODES[case["type"]]
+        mc.launch_matmul_mx4_weights(kind, state["a"].data_ptr(), case["k"], bc.data_ptr(), bs.data_ptr(), kind,
+                                     out.data_ptr(), case["m"], case["n"], case["k"], stream, workspace)
+    return out
+
+
+def _act(u, act):
+    if act == "relu":
+        return torch.relu(u)
+    if act == "gelu":
+        return 0.5 * u * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (u + 0.044715 * u * u * u)))
+    gate, up = u.chunk(2, -1)
+    return gate * torch.sigmoid(gate) * up
+
+
+def _moe_plain(state):
+    case = state["case"]
+    x = state["x"].float()
+    logits = x @ state["router"].t()
+    p = torch.softmax(logits, -1)
+    chosen = torch.sort(logits, dim=-1, descending=True, stable=True)[1][:, :case["top_k"]]
+    gate = torch.gather(p, -1, chosen)
+    gate = gate / gate.sum(-1, keepdim=True)
+    y = torch.zeros_like(x)
+    for e in torch.unique(chosen).tolist():
+        token, place = torch.nonzero(chosen == e, as_tuple=True)
+        if case["weights"] == "mx4":
+            w1 = _unpack(tuple(t[e] for t in state["w1"]), case["d"])
+            w2 = _unpack(tuple(t[e] for t in state["w2"]), case["h"])
+        else:
+            w1, w2 = state["w1"][e].float(), state["w2"][e].float()
+        u = x[token] @ w1.t()
+        if state["b1"] is not None:
+            u = u + state["b1"][e]
+        o = _act(u, case["act"]) @ w2.t()
+        if state["b2"] is not None:
+            o = o + state["b2"][e]
+        y.index_add_(0, token, gate[token, place, None] * o)
+    return y.to(state["x"].dtype)
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    case = state["case"]
+    op = case["op"]
+    if op == "quantize":
+        x = state["x"] if case["form"] == "rows" else state["x"].t()
+        v = _decode(*_quantize(x))[:, :case["k"]].to(x.dtype)
+        return v if case["form"] == "rows" else v.t().contiguous()
+    if op == "moe":
+        return _moe_plain(state)
+    b = _unpack(state["b"], case["k"])
+    if op == "product":
+        return (_unpack(state["a"], case["k"]) @ b.t()).to(TYPES[case["out"]])
+    return (state["a"].float() @ b.t()).to(TYPES[case["type"]])
+
+
+# ---------------------------------------------------------------- work and results
+
+
+def _bytes(kind):
+    return 4 if kind == "f32" else 2
+
+
+def _operand_bytes(rows, k):
+    return rows * _padded(k) * 17 // 32
+
+
+def work(case):
+    """Each input read once and each output written once; two operations per multiply-add. A mixture of experts reads
+    the experts that a step's tokens choose, on average of even choices."""
+    op = case["op"]
+    if op == "quantize":
+        n = case["rows"] * case["k"]
+        return {"bytes": 2 * n * _bytes(case["type"]) + _operand_bytes(case["rows"], case["k"]), "flops": 0}
+    if op in ("product", "weights"):
+        m, n, k = case["m"], case["n"], case["k"]
+        a = _operand_bytes(m, k) if op == "product" else m * k * _bytes(case["type"])
+        out = m * n * _bytes(case["out"] if op == "product" else case["type"])
+        return {"bytes": a + _operand_bytes(n, k) + out, "flops": 2 * m * n * k}
+    t, d, h, e, top = (case[s] for s in ("tokens", "d", "h", "experts", "top_k"))
+    rows = 2 * h if case["act"] == "swiglu" else h
+    read = e * (1.0 - (1.0 - top / e) ** t)
+    one = (_operand_bytes(rows, d) + _operand_bytes(d, h)) if case["weights"] == "mx4" else 2 * d * (rows + h)
+    if case["act"] != "swiglu":
+        one += 4 * (rows + d)
+    return {"bytes": int(2 * t * d * _bytes(case["type"]) + 4 * e * d + read * one),
+            "flops": 2 * t * d * e + 2 * t * top * d * (rows + h)}
+
+
+_MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _two_to(exponent):
+    """2^exponent in float64, exactly."""
+    return ((exponent.long() + 1023) << 52).view(torch.float64)
+
+
+def _exact_operand(codes, scales, k):
+    """An operand's values in float64, nibble by nibble."""
+    m = torch.tensor(_MAGNITUDES + tuple(-v for v in _MAGNITUDES), dtype=torch.float64, device=DEVICE)
+    v = torch.empty(*codes.shape[:-1], 2 * codes.shape[-1], dtype=torch.float64, device=DEVICE)
+    v[..., 0::2] = m[codes.long() % 16]
+    v[..., 1::2] = m[codes.long() // 16]
+    v *= _two_to(scales.long() - 127).repeat_interleave(32, -1)
+    return v[..., :k]
+
+
+def _exact_quantize(x):
+    """The nearest of the 15 representable values, by distance, in float64; columns of blocks padded with zeros."""
+    k = x.shape[-1]
+    out = torch.zeros(x.shape, dtype=torch.float64, device=DEVICE)
+    m = torch.tensor(_MAGNITUDES, dtype=torch.float64, device=DEVICE)
+    # Of two equal distances the even code's counts.
+    rank = torch.tensor([8, 4, 7, 3, 6, 2, 5, 1], device=DEVICE)
+    for at in range(0, k, 32):
+        b = x[:, at:at + 32].double()
+        top = b.abs().max(-1, keepdim=True)[0]
+        exponent = torch.frexp(top)[1].long() - 1 - 2
+        scale = _two_to(torch.where(top > 0, exponent, torch.zeros_like(exponent)).clamp(min=-127))
+        grid = m * scale
+        off = (b.abs().unsqueeze(-1) - grid.unsqueeze(1)).abs()
+        near = ((off == off.amin(-1, keepdim=True)) * rank).argmax(-1)
+        out[:, at:at + 32] = torch.gather(grid, 1, near) * torch.sign(b)
+    return out
+
+
+def _exact_moe(case, t):
+    x = t["x"].double()
+    logits = torch.matmul(x, t["router"].double().t())
+    out = torch.zeros_like(x)
+    for row in range(x.shape[0]):
+        line = logits[row].tolist()
+        best = sorted(range(len(line)), key=lambda e: (-line[e], e))[:case["top_k"]]
+        weight = [math.exp(line[e] - line[best[0]]) for e in best]
+        for e, g in zip(best, weight):
+            if case["weights"] == "mx4":
+                w1 = _exact_operand(t["w1"][0][e], t["w1"][1][e], case["d"])
+                w2 = _exact_operand(t["w2"][0][e], t["w2"][1][e], case["h"])
+            else:
+                w1, w2 = t["w1"][e].double(), t["w2"][e].double()
+            u = torch.mv(w1, x[row])
+            if t["b1"] is not None:
+                u = u + t["b1"][e].double()
+            if case["act"] == "relu":
+                u = u.clamp(min=0.0)
+            elif case["act"] == "gelu":
+                u = u / (1.0 + torch.exp(-2.0 * math.sqrt(2.0 / math.pi) * (u + 0.044715 * u ** 3)))
+            else:
+                u = u[:case["h"]] / (1.0 + torch.exp(-u[:case["h"]])) * u[case["h"]:]
+            o = torch.mv(w2, u)
+            if t["b2"] is not None:
+                o = o + t["b2"][e].double()
+            out[row] += g / sum(weight) * o
+    return out
+
+
+def exact(case, seed):
+    t = _inputs(case, seed)
+    op = case["op"]
+    if op == "quantize":
+        return _exact_quantize(t["x"]) if case["form"] == "rows" else _exact_quantize(t["x"].t()).t().contiguous()
+    if op == "moe":
+        return _exact_moe(case, t)
+    a = _exact_operand(*t["a"], case["k"]) if op == "product" else t["a"].double()
+    return torch.matmul(a, _exact_operand(*t["b"], case["k"]).t())
