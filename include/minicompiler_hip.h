@@ -259,6 +259,68 @@ MC_API const char* mc_matmul_kernel_name(int kernel);                           
 MC_API int mc_matmul_kernel_from_name(const char* name); /* -1 if unknown (cuda_backend.hpp:41-43) */
 MC_API int mc_matmul_supported(int kernel);              /* tensor_core_supported, matmul_kernels.hpp:39-43 */
 
+/* ---- Microscaled 4-bit floats and experts ----------------------------------
+ * No counterpart in the reference, whose lowest type is fp16. Types of these
+ * calls: 0 fp32, 1 bf16, 2 fp16, 4 "mx4". Each returns 0 or a hipError_t value;
+ * for a refused argument hipErrorInvalidValue (1), with mc_last_error() naming
+ * it. All enqueue on `stream` (a hipStream_t; NULL: the default stream), wait
+ * for nothing and allocate nothing.
+ *
+ * An mx4 operand is `rows` rows of k numbers, the products' inner dimension
+ * along the row (B of C = A B as its n columns). k is padded with zeros to
+ * kp, the next multiple of 128: codes [rows, kp / 2], two e2m1 codes per byte,
+ * element 2 i in the low half of byte i (bit 3 the sign, bits 0-2 one of 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6); scales [rows, kp / 32], one byte s per 32
+ * elements, worth 2^(s - 127), 255: NaN. 16-byte aligned codes, 4-byte
+ * aligned scales. Padding must be zero codes and no scale of 255. */
+MC_API long long mc_mx4_code_bytes(int rows, int k);
+MC_API long long mc_mx4_scale_bytes(int rows, int k);
+/* x [rows, k], rows ld elements apart, to an mx4 operand: per block of 32,
+ * s = max(0, floor(log2(largest magnitude)) + 125), each element x 2^(127 - s)
+ * rounded to the nearest code, ties to the even one, at most 6. A block with
+ * an infinity or a NaN gets s = 255 and zero codes. values (NULL: not
+ * wanted): what the codes stand for, [rows, k] without gaps, in x's type
+ * (always exact). */
+MC_API int mc_quantize_mx4(int dtype, const void* x, long long ld, void* codes, void* scales, int rows, int k,
+                           void* values, void* stream);
+/* The same of a row-major B [k, n] (rows ld elements apart), blocks down its
+ * columns: an operand of n rows of k. values (NULL: not wanted): [k, n]. */
+MC_API int mc_quantize_mx4_columns(int dtype, const void* b, long long ld, void* codes, void* scales, int k, int n,
+                                   void* values, void* stream);
+/* C[m, n] (row-major, of type c_dtype) = A B for A of m and B of n mx4 rows
+ * of k; fp32 sums, rounded once. */
+MC_API int mc_launch_matmul_mx4(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
+                                int c_dtype, void* c, int m, int n, int k, void* stream);
+/* C[m, n] = A B for A [m, k] of type a_dtype (rows lda elements apart), not
+ * rounded, and B of n mx4 rows; fp32 sums, C in c_dtype. workspace: of
+ * mc_matmul_mx4_weights_workspace_bytes bytes (0: may be NULL), 256-byte
+ * aligned; calls that overlap need one each. */
+MC_API long long mc_matmul_mx4_weights_workspace_bytes(int a_dtype, int m, int n, int k);
+MC_API int mc_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, const void* b_codes,
+                                        const void* b_scales, int c_dtype, void* c, int m, int n, int k, void* stream,
+                                        void* workspace);
+/* A mixture-of-experts MLP for 1 to 64 tokens, router and all:
+ *   p = softmax(x R^T); the top_k experts e of largest p per token (ties: the
+ *   lower index; a NaN logit counts as smallest and makes the token's gates
+ *   NaN), gates g = p, or with normalize p / (sum of the chosen p);
+ *   y = sum of g_e (act(x W1_e^T + b1_e) W2_e^T + b2_e) over the chosen.
+ * x [tokens, d] (rows ldx apart) and y [tokens, d] of type dtype; router
+ * [experts, d] fp32; W1 [experts, h, d] and W2 [experts, d, h] of type
+ * `weights` (1, 2, or 4: w*_scales then, else NULL), every row along its
+ * product's inner dimension; b1 [experts, h], b2 [experts, d] fp32 or NULL.
+ * activation: 0 ReLU, 1 GELU (tanh form), 2 SwiGLU: W1 and b1 have 2 h rows,
+ * h gate rows first, act = gate sigmoid(gate) up. chosen, gates: [tokens,
+ * top_k], largest first, NULL if not wanted. Sums in fp32 throughout. At most
+ * 512 experts and 16 per token.
+ * workspace: mc_moe_workspace_bytes bytes, 256-byte aligned, zero before the
+ * first call that uses it; calls leave it ready for the next, of any sizes
+ * that fit it. Calls that overlap need one each. */
+MC_API long long mc_moe_workspace_bytes(int dtype, int tokens, int d, int h, int experts, int top_k);
+MC_API int mc_launch_moe(int dtype, const void* x, long long ldx, const float* router, int weights, const void* w1,
+                         const void* w1_scales, const float* b1, const void* w2, const void* w2_scales,
+                         const float* b2, void* y, int* chosen, float* gates, int tokens, int d, int h, int experts,
+                         int top_k, int activation, int normalize, void* stream, void* workspace);
+
 /* Device memory, streams and events (the thin layer, for callers with no
  * other HIP runtime in the process). */
 MC_API int mc_device_count(void);

@@ -30,8 +30,10 @@ GRAPHS_DIR = PACKAGE_DIR / "graphs"
 # MatmulKernel values (include/minicompiler/hip/hip_backend.hpp).
 MATMUL_KERNELS = ["auto", "naive", "tiled", "register_tiled_128", "register_tiled_64", "vectorized",
                   "double_buffered", "split_k", "tensor_core_tf32", "tensor_core_bf16", "tensor_core_f16"]
+DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+DTYPE_MX4 = 4
 
 
 class LibraryMissing(RuntimeError):
@@ -109,6 +111,16 @@ _SIGNATURES = {
     "mc_pack_a16": (_i, [_vp, _vp, _i, _i, _vp]),
     "mc_convert_pack_a_f32": (_i, [_i, _vp, _vp, _i, _i, _vp]),
     "mc_launch_matmul_lowp_packed": (_i, [_i, _i, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "mc_mx4_code_bytes": (_ll, [_i, _i]),
+    "mc_mx4_scale_bytes": (_ll, [_i, _i]),
+    "mc_quantize_mx4": (_i, [_i, _vp, _ll, _vp, _vp, _i, _i, _vp, _vp]),
+    "mc_quantize_mx4_columns": (_i, [_i, _vp, _ll, _vp, _vp, _i, _i, _vp, _vp]),
+    "mc_launch_matmul_mx4": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp]),
+    "mc_matmul_mx4_weights_workspace_bytes": (_ll, [_i, _i, _i, _i]),
+    "mc_launch_matmul_mx4_weights": (_i, [_i, _vp, _ll, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _vp]),
+    "mc_moe_workspace_bytes": (_ll, [_i, _i, _i, _i, _i, _i]),
+    "mc_launch_moe": (_i, [_i, _vp, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
+                           _i, _vp, _vp]),
     "mc_sum_split_partials": (_i, [_vp, _vp, _sz, _i, _vp]),
     "mc_split_k_splits": (_i, [_i, _i, _i, _i, _i]),
     "mc_matmul_splits": (_i, [_i, _i, _i, _i, _i]),
@@ -691,6 +703,75 @@ def resolve_matmul_kernel(kernel: int | str, m: int, n: int, k: int, cu_count: i
 def matmul_supported(kernel: int | str) -> bool:
     kid = matmul_kernel_id(kernel) if isinstance(kernel, str) else kernel
     return bool(library().mc_matmul_supported(kid))
+
+
+# ---------------------------------------------------------------- microscaled 4-bit operands, experts
+
+
+def _check_launch(rc: int) -> None:
+    if rc != 0:
+        raise HipError(last_error(), rc)
+
+
+def mx4_code_bytes(rows: int, k: int) -> int:
+    """Bytes of the codes of an mx4 operand of `rows` rows of k (two per byte, k padded to a multiple of 128)."""
+    return int(library().mc_mx4_code_bytes(rows, k))
+
+
+def mx4_scale_bytes(rows: int, k: int) -> int:
+    """Bytes of its scales (one per 32 elements)."""
+    return int(library().mc_mx4_scale_bytes(rows, k))
+
+
+def quantize_mx4(dtype: int, x: int, ld: int, codes: int, scales: int, rows: int, k: int, values: int | None = None,
+                 stream=None) -> None:
+    """x [rows, k] (rows ld elements apart; DTYPE_F32, DTYPE_BF16 or DTYPE_F16) to an mx4 operand; values: what the
+    codes stand for, in x's type, if wanted."""
+    _check_launch(library().mc_quantize_mx4(dtype, x, ld, codes, scales, rows, k, values, _stream_handle(stream)))
+
+
+def quantize_mx4_columns(dtype: int, b: int, ld: int, codes: int, scales: int, k: int, n: int,
+                         values: int | None = None, stream=None) -> None:
+    """Row-major B [k, n] to the mx4 operand of its n columns; values: [k, n]."""
+    _check_launch(library().mc_quantize_mx4_columns(dtype, b, ld, codes, scales, k, n, values,
+                                                    _stream_handle(stream)))
+
+
+def launch_matmul_mx4(a_codes: int, a_scales: int, b_codes: int, b_scales: int, c_dtype: int, c: int, m: int, n: int,
+                      k: int, stream=None) -> None:
+    """C[m, n] of type c_dtype = A B, A of m and B of n mx4 rows of k."""
+    _check_launch(library().mc_launch_matmul_mx4(a_codes, a_scales, b_codes, b_scales, c_dtype, c, m, n, k,
+                                                 _stream_handle(stream)))
+
+
+def matmul_mx4_weights_workspace_bytes(a_dtype: int, m: int, n: int, k: int) -> int:
+    return int(library().mc_matmul_mx4_weights_workspace_bytes(a_dtype, m, n, k))
+
+
+def launch_matmul_mx4_weights(a_dtype: int, a: int, lda: int, b_codes: int, b_scales: int, c_dtype: int, c: int,
+                              m: int, n: int, k: int, stream=None, workspace: int | None = None) -> None:
+    """C[m, n] = A B, A [m, k] of a_dtype as it is (rows lda apart), B of n mx4 rows of k."""
+    _check_launch(library().mc_launch_matmul_mx4_weights(a_dtype, a, lda, b_codes, b_scales, c_dtype, c, m, n, k,
+                                                         _stream_handle(stream), workspace))
+
+
+MOE_ACTIVATIONS = {"relu": 0, "gelu": 1, "swiglu": 2}
+
+
+def moe_workspace_bytes(dtype: int, tokens: int, d: int, h: int, experts: int, top_k: int) -> int:
+    return int(library().mc_moe_workspace_bytes(dtype, tokens, d, h, experts, top_k))
+
+
+def launch_moe(dtype: int, x: int, ldx: int, router: int, weights: int, w1: int, w1_scales: int | None,
+               b1: int | None, w2: int, w2_scales: int | None, b2: int | None, y: int, chosen: int | None,
+               gates: int | None, tokens: int, d: int, h: int, experts: int, top_k: int, activation: int | str,
+               normalize: bool, stream=None, workspace: int | None = None) -> None:
+    """A mixture-of-experts MLP of 1 to 64 tokens, router included (mc_launch_moe); the workspace
+    (moe_workspace_bytes) is zero before its first use."""
+    act = MOE_ACTIVATIONS[activation] if isinstance(activation, str) else activation
+    _check_launch(library().mc_launch_moe(dtype, x, ldx, router, weights, w1, w1_scales, b1, w2, w2_scales, b2, y,
+                                          chosen, gates, tokens, d, h, experts, top_k, act, int(normalize),
+                                          _stream_handle(stream), workspace))
 
 
 # ---------------------------------------------------------------- generator

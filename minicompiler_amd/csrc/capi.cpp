@@ -8,6 +8,7 @@
 #include "hip/hip_rt.h"
 #include "hip/kernel_compiler.hpp"
 #include "hip/matmul.h"
+#include "hip/mx4.h"
 #include "hip/matmul_policy.hpp"
 #include "minicompiler/hip/hip_backend.hpp"
 #include "minicompiler/parser.hpp"
@@ -867,6 +868,75 @@ MC_API int mc_convert_pack_a_f32(int dtype, const float* a, void* packed, int m,
 MC_API int mc_launch_matmul_lowp_packed(int kernel, int dtype, const void* a_packed, const void* b, float* c, int m,
                                         int n, int k, void* stream) {
     return mchip_launch_matmul_lowp_packed(kernel, dtype, a_packed, b, c, m, n, k, stream);
+}
+
+namespace {
+
+// A launcher's result, its refusal readable with mc_last_error().
+int launched(const char* call, int rc, const char* why) {
+    if (rc != 0) g_last_error = std::string(call) + ": " + (why != nullptr ? why : mchip_error_string(rc));
+    return rc;
+}
+
+long long mx4_blocks(int rows, int k) {
+    return rows < 1 || k < 1 ? 0 : static_cast<long long>(rows) * (mchip_mx4_k(k) / 32);
+}
+
+}  // namespace
+
+MC_API long long mc_mx4_code_bytes(int rows, int k) { return mx4_blocks(rows, k) * 16; }
+
+MC_API long long mc_mx4_scale_bytes(int rows, int k) { return mx4_blocks(rows, k); }
+
+MC_API int mc_quantize_mx4(int dtype, const void* x, long long ld, void* codes, void* scales, int rows, int k,
+                           void* values, void* stream) {
+    const char* why = nullptr;
+    const int rc = mchip_quantize_mx4(dtype, x, ld, codes, scales, rows, k, values, stream, &why);
+    return launched("mc_quantize_mx4", rc, why);
+}
+
+MC_API int mc_quantize_mx4_columns(int dtype, const void* b, long long ld, void* codes, void* scales, int k, int n,
+                                   void* values, void* stream) {
+    const char* why = nullptr;
+    const int rc = mchip_quantize_mx4_columns(dtype, b, ld, codes, scales, k, n, values, stream, &why);
+    return launched("mc_quantize_mx4_columns", rc, why);
+}
+
+MC_API int mc_launch_matmul_mx4(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
+                                int c_dtype, void* c, int m, int n, int k, void* stream) {
+    const char* why = nullptr;
+    const int rc =
+        mchip_launch_matmul_mx4(a_codes, a_scales, b_codes, b_scales, c_dtype, c, m, n, k, stream, &why);
+    return launched("mc_launch_matmul_mx4", rc, why);
+}
+
+MC_API long long mc_matmul_mx4_weights_workspace_bytes(int a_dtype, int m, int n, int k) {
+    return mchip_matmul_mx4_weights_workspace_bytes(a_dtype, m, n, k);
+}
+
+MC_API int mc_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, const void* b_codes,
+                                        const void* b_scales, int c_dtype, void* c, int m, int n, int k, void* stream,
+                                        void* workspace) {
+    const char* why = nullptr;
+    const int rc = mchip_launch_matmul_mx4_weights(a_dtype, a, lda, b_codes, b_scales, c_dtype, c, m, n, k, stream,
+                                                   workspace, &why);
+    return launched("mc_launch_matmul_mx4_weights", rc, why);
+}
+
+MC_API long long mc_moe_workspace_bytes(int dtype, int tokens, int d, int h, int experts, int top_k) {
+    return mchip_moe_workspace_bytes(dtype, tokens, d, h, experts, top_k);
+}
+
+MC_API int mc_launch_moe(int dtype, const void* x, long long ldx, const float* router, int weights, const void* w1,
+                         const void* w1_scales, const float* b1, const void* w2, const void* w2_scales,
+                         const float* b2, void* y, int* chosen, float* gates, int tokens, int d, int h, int experts,
+                         int top_k, int activation, int normalize, void* stream, void* workspace) {
+    const char* why = nullptr;
+    const mchip_moe_args args{dtype, x,      ldx,    router, weights, w1,    w1_scales, b1,         w2,        w2_scales, b2,
+                              y,     chosen, gates,  tokens, d,       h,     experts,   top_k,      activation, normalize,
+                              workspace};
+    const int rc = mchip_launch_moe(&args, stream, &why);
+    return launched("mc_launch_moe", rc, why);
 }
 
 MC_API int mc_sum_split_partials(const float* partial, float* c, size_t count, int splits, void* stream) {

@@ -1,0 +1,141 @@
+// The product of two operands quantised to microscaled 4-bit floats (mx4.h):
+// C = A B^T, on v_mfma_scale_f32_16x16x128_f8f6f4, which multiplies codes and
+// scales exactly and adds in fp32.
+
+#include "mx4_device.h"
+
+namespace {
+
+using namespace mx4;
+
+// A block computes 16 kM rows by 16 kN columns of C; its kWaves waves take the
+// steps of 128 k in turn and their sums are added at the end. Fragments come
+// straight from memory: a lane's 16 bytes of codes are one block of a row, four
+// lanes read 64 bytes of it. Rows past the edge read the last row.
+template <int kM, int kN, int kWaves, int kOut>
+__global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned char* __restrict__ a_codes,
+                                                              const unsigned char* __restrict__ a_scales,
+                                                              const unsigned char* __restrict__ b_codes,
+                                                              const unsigned char* __restrict__ b_scales,
+                                                              void* __restrict__ c, int m, int n, int steps,
+                                                              unsigned tiles_n, bool wide) {
+    __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int r = lane % 16, q = lane / 16;
+    const long long row0 = static_cast<long long>(blockIdx.x / tiles_n) * 16 * kM;
+    const long long col0 = static_cast<long long>(blockIdx.x % tiles_n) * 16 * kN;
+
+    const unsigned char *ac[kM], *as[kM], *bc[kN], *bs[kN];
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+        const long long row = row0 + 16 * i + r < m ? row0 + 16 * i + r : m - 1;
+        ac[i] = a_codes + row * steps * 64 + q * 16;
+        as[i] = a_scales + row * steps * 4 + q;
+    }
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        const long long col = col0 + 16 * j + r < n ? col0 + 16 * j + r : n - 1;
+        bc[j] = b_codes + col * steps * 64 + q * 16;
+        bs[j] = b_scales + col * steps * 4 + q;
+    }
+    f32x4 acc[kM * kN];
+#pragma unroll
+    for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    for (int t = wave; t < steps; t += kWaves) {
+        i32x4 av[kM], bv[kN];
+        int sa[kM], sb[kN];
+#pragma unroll
+        for (int i = 0; i < kM; ++i) {
+            av[i] = *reinterpret_cast<const i32x4*>(ac[i] + static_cast<long long>(t) * 64);
+            sa[i] = as[i][t * 4];
+        }
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            bv[j] = *reinterpret_cast<const i32x4*>(bc[j] + static_cast<long long>(t) * 64);
+            sb[j] = bs[j][t * 4];
+        }
+#pragma unroll
+        for (int i = 0; i < kM; ++i)
+#pragma unroll
+            for (int j = 0; j < kN; ++j) acc[i * kN + j] = mfma(bv[j], sb[j], av[i], sa[i], acc[i * kN + j]);
+    }
+    add_waves<kWaves, kM * kN>(acc, space, wave, lane);
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+        const long long row = row0 + 16 * i + r;
+        if (row >= m) continue;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            const long long col = col0 + 16 * j + 4 * q;
+            if (col < n)
+                store_four<kOut>(c, row * n + col, acc[i * kN + j], static_cast<int>(n - col < 4 ? n - col : 4),
+                                 wide && col + 4 <= n);
+        }
+    }
+}
+
+struct Product {
+    const unsigned char *a_codes, *a_scales, *b_codes, *b_scales;
+    void* c;
+    int m, n, steps;
+    bool wide;
+    hipStream_t stream;
+};
+
+long long tiles(int size, int tile) { return (static_cast<long long>(size) + tile - 1) / tile; }
+
+template <int kM, int kN, int kOut>
+int launch_direct(const Product& p) {
+    constexpr int kWaves = 8;
+    const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((product_direct<kM, kN, kWaves, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64),
+                       0, p.stream, p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps,
+                       static_cast<unsigned>(tn), p.wide);
+    return hipGetLastError();
+}
+
+template <int kOut>
+int launch(const Product& p) {
+    const int cus = device_cus();
+    const auto blocks = [&](int bm, int bn) { return tiles(p.m, 16 * bm) * tiles(p.n, 16 * bn); };
+    if (p.m <= 16) {
+        if (blocks(1, 4) >= cus) return launch_direct<1, 4, kOut>(p);
+        if (blocks(1, 2) >= cus) return launch_direct<1, 2, kOut>(p);
+        return launch_direct<1, 1, kOut>(p);
+    }
+    if (p.m <= 32) {
+        if (blocks(2, 4) >= cus) return launch_direct<2, 4, kOut>(p);
+        if (blocks(2, 2) >= cus) return launch_direct<2, 2, kOut>(p);
+        return launch_direct<1, 1, kOut>(p);
+    }
+    if (blocks(4, 4) >= cus) return launch_direct<4, 4, kOut>(p);
+    if (blocks(2, 4) >= cus) return launch_direct<2, 4, kOut>(p);
+    if (blocks(2, 2) >= cus) return launch_direct<2, 2, kOut>(p);
+    return launch_direct<1, 1, kOut>(p);
+}
+
+}  // namespace
+
+extern "C" int mchip_launch_matmul_mx4(const void* a_codes, const void* a_scales, const void* b_codes,
+                                       const void* b_scales, int c_dtype, void* c, int m, int n, int k, void* stream,
+                                       const char** why) {
+    *why = nullptr;
+    if (!is_float_type(c_dtype)) *why = "the result's type is none of fp32 (0), bf16 (1), fp16 (2)";
+    else if (m < 1 || n < 1 || k < 1) *why = "a size below 1";
+    else if (k > (1 << 24)) *why = "k above 2^24";
+    else if (!a_codes || !a_scales || !b_codes || !b_scales || !c) *why = "a null operand";
+    else if (!aligned(a_codes, 16) || !aligned(b_codes, 16)) *why = "codes not 16-byte aligned";
+    else if (!aligned(a_scales, 4) || !aligned(b_scales, 4)) *why = "scales not 4-byte aligned";
+    else if (!aligned(c, size_of(c_dtype))) *why = "a result that is not aligned to its elements";
+    if (*why != nullptr) return hipErrorInvalidValue;
+    Product p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
+              static_cast<const unsigned char*>(b_codes), static_cast<const unsigned char*>(b_scales),
+              c, m, n, static_cast<int>(mchip_mx4_k(k) / kStep),
+              n % 4 == 0 && aligned(c, 4 * size_of(c_dtype)), static_cast<hipStream_t>(stream)};
+    const int rc = c_dtype == kF32 ? launch<kF32>(p) : c_dtype == kBf16 ? launch<kBf16>(p) : launch<kF16>(p);
+    if (rc == hipErrorInvalidValue) *why = "more tiles of C than one launch takes";
+    return rc;
+}

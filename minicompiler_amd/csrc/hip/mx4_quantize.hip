@@ -1,0 +1,234 @@
+// Quantisation to microscaled 4-bit floats (the format: mx4.h).
+//
+// A block of 32 with largest magnitude a: s = max(0, floor(log2 a) - 2 + 127),
+// which puts a in [4, 8) of the codes' units (6 is the largest code); each
+// element is then x 2^(127 - s), rounded to the nearest code, ties to the even
+// code, 6 beyond it. floor(log2 a) is read from the exponent field, so fields
+// 0 to 2 (where 2^(s - 127) would pass below the smallest scale) take s = 0.
+// A block with an infinity or a NaN has no scale: 255, codes 0, NaN as a whole.
+// v_cvt_scalef32_pk_fp4_f32 divides, rounds and saturates so in one step.
+//
+// Bound by memory: 2 or 4 bytes read and 17/32 written per element (and 2 or 4
+// written for `values`).
+
+#include "mx4_device.h"
+
+namespace {
+
+using namespace mx4;
+
+// The scale byte of a block from the bits of its largest magnitude (as
+// unsigned numbers, infinities and NaNs are above all others).
+__device__ __forceinline__ unsigned scale_byte(unsigned top) {
+    if (top >= 0x7f800000u) return 255u;
+    const int s = static_cast<int>(top >> 23) - 2;
+    return static_cast<unsigned>(s > 0 ? s : 0);
+}
+
+__device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+
+// Eight codes of one block, four bytes.
+__device__ __forceinline__ unsigned encode_eight(const float (&v)[8], unsigned scale) {
+    if (scale == 255u) return 0u;
+    const float f = scale_operand(scale);
+    unsigned c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], f, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], f, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], f, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], f, 3);
+    return c;
+}
+
+__device__ __forceinline__ void decode_eight_f32(unsigned codes, unsigned scale, float (&v)[8]) {
+    const float f = scale_operand(scale);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, f, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, f, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, f, 2);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, f, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
+    v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
+}
+
+// Eight values of row `row` from element `at` on (exact in x's type: a code is
+// never finer than the numbers it was rounded from).
+template <int kType>
+__device__ __forceinline__ void store_eight(void* p, long long at, const float (&v)[8], int left, bool wide) {
+    if (wide && left >= 8) {
+        if constexpr (kType == kF32) {
+            f32x4* d = reinterpret_cast<f32x4*>(static_cast<float*>(p) + at);
+            d[0] = f32x4{v[0], v[1], v[2], v[3]};
+            d[1] = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+            u16x8 h;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = to_16<kType>(v[e]);
+            *reinterpret_cast<u16x8*>(static_cast<unsigned short*>(p) + at) = h;
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < left) store_one<kType>(p, at + e, v[e]);
+}
+
+constexpr int kThreads = 256;
+
+// The largest over the four lanes of a block (lanes 4 i .. 4 i + 3).
+__device__ __forceinline__ unsigned max_of_four(unsigned v) {
+    unsigned o = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xb1, 0xf, 0xf, false));
+    v = v > o ? v : o;
+    o = static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4e, 0xf, 0xf, false));
+    return v > o ? v : o;
+}
+
+// A lane takes eight consecutive elements of a row, four neighbouring lanes a
+// block. `per_row` = kp / 8 such chunks (a multiple of 16, so a block's lanes
+// are never in two rows), chunks counted over all rows.
+template <int kType>
+__global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict__ x, long long ld,
+                                                          unsigned* __restrict__ codes,
+                                                          unsigned char* __restrict__ scales,
+                                                          void* __restrict__ values, long long rows, int k,
+                                                          unsigned per_row, bool wide, bool wide_values) {
+    const long long first = static_cast<long long>(blockIdx.x) * kThreads;
+    const long long row0 = first / per_row;
+    const unsigned in_row = static_cast<unsigned>(first - row0 * per_row) + threadIdx.x;
+    const long long row = row0 + in_row / per_row;
+    const unsigned chunk = in_row % per_row;
+    if (row >= rows) return;  // whole blocks of lanes: a row has a multiple of 16 chunks
+    const int left = k - static_cast<int>(chunk) * 8;
+    float v[8];
+    load_eight<kType>(x, row * ld + chunk * 8, left, wide, v);
+    unsigned top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const unsigned m = magnitude(v[e]);
+        top = m > top ? m : top;
+    }
+    const unsigned s = scale_byte(max_of_four(top));
+    const unsigned c = encode_eight(v, s);
+    codes[row * per_row + chunk] = c;
+    if (chunk % 4 == 0) scales[row * (per_row / 4) + chunk / 4] = static_cast<unsigned char>(s);
+    if (values != nullptr && left > 0) {
+        decode_eight_f32(c, s, v);
+        store_eight<kType>(values, row * k + chunk * 8, v, left, wide_values);
+    }
+}
+
+// A lane takes 32 elements down one column, a wave 64 neighbouring columns of
+// one block, a thread block four blocks of k.
+template <int kType>
+__global__ __launch_bounds__(kThreads) void quantize_columns(const void* __restrict__ w, long long ld,
+                                                             u32x4* __restrict__ codes,
+                                                             unsigned char* __restrict__ scales,
+                                                             void* __restrict__ values, int k, int n, int k_blocks) {
+    const int col = blockIdx.y * 64 + threadIdx.x % 64;
+    const int kb = blockIdx.x * 4 + threadIdx.x / 64;
+    if (col >= n || kb >= k_blocks) return;
+    const int k0 = kb * 32;
+    float v[32];
+    unsigned top = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = k0 + e < k ? load_one<kType>(w, (k0 + e) * ld + col) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        const unsigned m = magnitude(v[e]);
+        top = m > top ? m : top;
+    }
+    const unsigned s = scale_byte(top);
+    u32x4 c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float part[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[e] = v[8 * j + e];
+        c[j] = encode_eight(part, s);
+    }
+    codes[static_cast<long long>(col) * k_blocks + kb] = c;
+    scales[static_cast<long long>(col) * k_blocks + kb] = static_cast<unsigned char>(s);
+    if (values == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float part[8];
+        decode_eight_f32(c[j], s, part);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int kk = k0 + 8 * j + e;
+            if (kk < k) store_one<kType>(values, static_cast<long long>(kk) * n + col, part[e]);
+        }
+    }
+}
+
+const char* refusal(int dtype, const void* x, long long ld, const void* codes, const void* scales, int outer, int inner,
+                    int k, const void* values) {
+    if (!is_float_type(dtype)) return "the type is none of fp32 (0), bf16 (1), fp16 (2)";
+    if (outer < 1 || inner < 1) return "a size below 1";
+    if (k > 0x7fffff80) return "k above 2^31 - 128";
+    if (ld < inner) return "rows closer together than they are long";
+    if (x == nullptr || codes == nullptr || scales == nullptr) return "a null input or output";
+    const std::size_t size = size_of(dtype);
+    if (!aligned(x, size) || !aligned(values, size)) return "an address that is no multiple of its element's size";
+    if (!aligned(codes, 16) || !aligned(scales, 4)) return "codes not 16-byte or scales not 4-byte aligned";
+    return nullptr;
+}
+
+template <int kType>
+int launch_rows(const void* x, long long ld, void* codes, void* scales, int rows, int k, void* values,
+                hipStream_t stream, const char** why) {
+    const unsigned per_row = static_cast<unsigned>(mchip_mx4_k(k) / 8);
+    const long long blocks = (static_cast<long long>(rows) * per_row + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffLL) {
+        *why = "more elements than one launch takes (2^42)";
+        return hipErrorInvalidValue;
+    }
+    const int unit = 16 / kSize<kType>;
+    const bool wide = aligned(x, 16) && ld % unit == 0;
+    const bool wide_values = aligned(values, 16) && k % unit == 0;
+    hipLaunchKernelGGL(quantize_rows<kType>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, x, ld,
+                       static_cast<unsigned*>(codes), static_cast<unsigned char*>(scales), values,
+                       static_cast<long long>(rows), k, per_row, wide, wide_values);
+    return hipGetLastError();
+}
+
+template <int kType>
+int launch_columns(const void* w, long long ld, void* codes, void* scales, int k, int n, void* values,
+                   hipStream_t stream, const char** why) {
+    const int k_blocks = static_cast<int>(mchip_mx4_k(k) / 32);
+    const unsigned cols = static_cast<unsigned>((static_cast<long long>(n) + 63) / 64);
+    if (cols > 65535u) {
+        *why = "more columns than one launch takes (4194240)";
+        return hipErrorInvalidValue;
+    }
+    hipLaunchKernelGGL(quantize_columns<kType>, dim3(static_cast<unsigned>(k_blocks / 4), cols), dim3(kThreads), 0,
+                       stream, w, ld, static_cast<u32x4*>(codes), static_cast<unsigned char*>(scales), values, k, n,
+                       k_blocks);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+long long mchip_mx4_k(int k) { return (static_cast<long long>(k) + mx4::kStep - 1) / mx4::kStep * mx4::kStep; }
+
+int mchip_quantize_mx4(int dtype, const void* x, long long ld, void* codes, void* scales, int rows, int k, void* values,
+                       void* stream, const char** why) {
+    *why = refusal(dtype, x, ld, codes, scales, rows, k, k, values);
+    if (*why != nullptr) return hipErrorInvalidValue;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == kF32) return launch_rows<kF32>(x, ld, codes, scales, rows, k, values, s, why);
+    if (dtype == kBf16) return launch_rows<kBf16>(x, ld, codes, scales, rows, k, values, s, why);
+    return launch_rows<kF16>(x, ld, codes, scales, rows, k, values, s, why);
+}
+
+int mchip_quantize_mx4_columns(int dtype, const void* w, long long ld, void* codes, void* scales, int k, int n,
+                               void* values, void* stream, const char** why) {
+    *why = refusal(dtype, w, ld, codes, scales, k, n, k, values);
+    if (*why != nullptr) return hipErrorInvalidValue;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == kF32) return launch_columns<kF32>(w, ld, codes, scales, k, n, values, s, why);
+    if (dtype == kBf16) return launch_columns<kBf16>(w, ld, codes, scales, k, n, values, s, why);
+    return launch_columns<kF16>(w, ld, codes, scales, k, n, values, s, why);
+}
+
+}  // extern "C"
