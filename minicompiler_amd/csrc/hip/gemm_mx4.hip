@@ -2,7 +2,7 @@
 // C = A B^T, on v_mfma_scale_f32_16x16x128_f8f6f4, which multiplies codes and
 // scales exactly and adds in fp32.
 
-#include "mx4_device.h"
+#include "gemm_mx4_tiles.h"
 
 namespace {
 
@@ -76,6 +76,31 @@ __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned cha
     }
 }
 
+// Tiles in row-major order, as gemm_mfma16_fast.h has them: the grid has one
+// block per 256x256 tile plus `halves` more, for which that many of the last
+// tiles run as two blocks of 128x256.
+template <int kOut>
+__global__ __launch_bounds__(kTileThreads, 1) void product_tiles(const unsigned char* __restrict__ a_codes,
+                                                                 const unsigned char* __restrict__ a_scales,
+                                                                 const unsigned char* __restrict__ b_codes,
+                                                                 const unsigned char* __restrict__ b_scales,
+                                                                 void* __restrict__ c, int m, int n, int steps,
+                                                                 int tiles_n, int full, int vec) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kRingBytes];
+    MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);  // generic -> LDS address space
+    const int block = static_cast<int>(blockIdx.x);
+    if (block < full) {
+        product_tile<256, kOut>(lds, a_codes, a_scales, b_codes, b_scales, c, m, n, steps, block / tiles_n * 256,
+                                block % tiles_n * 256, vec);
+    } else {
+        const int t = full + (block - full) / 2;
+        const int row0 = t / tiles_n * 256 + (block - full) % 2 * 128;
+        if (row0 >= m) return;  // the last tile row has no second half
+        product_tile<128, kOut>(lds, a_codes, a_scales, b_codes, b_scales, c, m, n, steps, row0, t % tiles_n * 256,
+                                vec);
+    }
+}
+
 struct Product {
     const unsigned char *a_codes, *a_scales, *b_codes, *b_scales;
     void* c;
@@ -98,8 +123,25 @@ int launch_direct(const Product& p) {
 }
 
 template <int kOut>
+int launch_tiles(const Product& p) {
+    const int tn = static_cast<int>(tiles(p.n, kTileCols)), all = static_cast<int>(tiles(p.m, kTileRows)) * tn;
+    const int cus = device_cus(), rest = all % cus;
+    const int halves = rest <= cus / 2 ? rest : 0;
+    hipLaunchKernelGGL(product_tiles<kOut>, dim3(static_cast<unsigned>(all + halves)), dim3(kTileThreads), 0, p.stream,
+                       p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps, tn, all - halves,
+                       p.n % 8 == 0 && aligned(p.c, 16) ? 8 : p.wide ? 4 : 1);
+    return hipGetLastError();
+}
+
+// Four steps at least (a slot of scales), and 32-bit offsets from a tile's origin.
+bool tiles_fit(const Product& p) {
+    return p.steps >= 4 && p.steps <= (1 << 16) && tiles(p.m, kTileRows) * tiles(p.n, kTileCols) < (1 << 30);
+}
+
+template <int kOut>
 int launch(const Product& p) {
     const int cus = device_cus();
+    if (tiles_fit(p) && tiles(p.m, kTileRows) * tiles(p.n, kTileCols) >= cus / 2) return launch_tiles<kOut>(p);
     const auto blocks = [&](int bm, int bn) { return tiles(p.m, 16 * bm) * tiles(p.n, 16 * bn); };
     if (p.m <= 16) {
         if (blocks(1, 4) >= cus) return launch_direct<1, 4, kOut>(p);

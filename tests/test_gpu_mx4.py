@@ -176,26 +176,30 @@ def test_product_of_quantised_operands(device, mc, kind, m, n, k):
     within(ref.from_type(c.get(bits_type(dtype), (m, n)), dtype), exact, bound)
 
 
-@pytest.mark.parametrize("m,n,k", [(1500, 2100, 1100), (1024, 4096, 1536), (2300, 2049, 129)])
-def test_product_of_many_tiles(device, mc, m, n, k):
-    print(f"case mx4 product {m}x{n}x{k}", flush=True)
+@pytest.mark.parametrize("kind,m,n,k", [("f32", 1500, 2100, 1100), ("f32", 1024, 4096, 1536), ("f32", 2300, 2049, 129),
+                                        ("f32", 3000, 3001, 520), ("f32", 2900, 2820, 1290), ("bf16", 2817, 2952, 640),
+                                        ("f16", 2900, 2948, 513), ("bf16", 2900, 2950, 2049), ("f16", 4200, 2090, 898),
+                                        ("f32", 300, 40000, 1100)])
+def test_product_of_many_tiles(device, mc, kind, m, n, k):
+    print(f"case mx4 product {kind} {m}x{n}x{k}", flush=True)
+    dtype = ref.TYPES[kind]
     rng = np.random.default_rng(m)
     ac, as_, a = operand(mc, rng, m, k)
     bc, bs, b = operand(mc, rng, n, k, k ** -0.5)
-    c = Out(mc, m * n * 4)
-    mc.launch_matmul_mx4(ac.ptr, as_.ptr, bc.ptr, bs.ptr, ref.F32, c.ptr, m, n, k)
+    c = Out(mc, m * n * (4 if dtype == ref.F32 else 2))
+    mc.launch_matmul_mx4(ac.ptr, as_.ptr, bc.ptr, bs.ptr, dtype, c.ptr, m, n, k)
     mc.synchronize()
-    exact, bound = ref.product_bound(a, b, k, ref.F32)
-    within(c.get(np.float32, (m, n)).astype(np.float64), exact, bound)
+    exact, bound = ref.product_bound(a, b, k, dtype)
+    within(ref.from_type(c.get(bits_type(dtype), (m, n)), dtype), exact, bound)
 
 
-@pytest.mark.parametrize("m,n", [(3, 40), (300, 700), (1300, 2100)])
+@pytest.mark.parametrize("m,n", [(3, 40), (300, 700), (1300, 2100), (2900, 3000)])
 def test_a_block_without_a_scale_reaches_its_rows_alone(device, mc, m, n):
-    k = 400
+    k = 600
     rng = np.random.default_rng(9)
     x, w = rng.standard_normal((m, k)), rng.standard_normal((n, k))
     x[m // 2, 100] = np.nan
-    w[n // 3, 399] = np.inf
+    w[n // 3, 599] = np.inf
     (xc, xs, _), (wc, ws, _) = ref.quantize(x), ref.quantize(w)
     bufs = [mc.DeviceBuffer.from_array(t) for t in (xc, xs, wc, ws)]
     c = Out(mc, m * n * 4)
