@@ -6,22 +6,34 @@
 // ring of four 32 KiB LDS stages, the two waves of each SIMD one phase apart,
 // one reading its operands from LDS while the other multiplies.
 //
-// LDS layout of a stage: A [16 blocks of 16 rows][4 blocks of 32 k][16 rows] of
-// 16 bytes, at 0, and B likewise at 16 KiB: a fragment (16 rows, 128 k) is
-// 1 KiB read linearly, lane l at 16 l, and one fetch instruction fills one
-// fragment from 64 bytes of each of 16 rows.
+// LDS layout of a stage: rows of 64 bytes, A's 256 at 0 and B's at 16 KiB; block
+// c of row r lies at 64 r + 16 (c ^ (r / 2 % 4)). A fetch instruction fills 16
+// rows, four neighbouring lanes one row: the address unit takes four lanes'
+// adjacent 16 bytes in one access (with a lane per row it made 64 accesses of
+// an instruction and bound the kernel: 2400 a step, 8192^3 in 342 us).
+// A fragment read (lane (r, q) block q of row r) goes over every bank once per
+// 16 lanes that the LDS serves together (lanes 0-3, 12-15 and 20-27 the first);
+// of the swizzles tried, this one and one other had no conflicts.
 //
-// Scales: a row has four bytes per step. Fetched a step at a time, a fetch
-// instruction would touch 64 rows, 64 lines, for 256 bytes; instead 16 bytes
-// of each row, four steps' worth, go to one of two 8 KiB slots ([256 rows][16]
-// of A, then of B) every fourth step. A row's last 16 bytes are fetched whole
-// where its end falls inside a slot, so nothing is read outside the operand
-// (K >= 512). A lane reads its fragment row's byte for its block.
+// Scales: a row has four bytes per step. Fetched a step at a time, a load would
+// touch 64 rows, 64 lines, for 256 bytes; instead a lane takes 16 bytes of its
+// row, four steps' worth, once in four steps, and turns them (four steps of
+// four blocks) into four blocks' dwords of four steps each, in one of two 8 KiB
+// slots of LDS. A lane then reads one dword per fragment for four steps and the
+// instruction picks the step's byte. (Read from LDS a byte per fragment and
+// step, the scales took 50 of 332 us at 8192^3.) A row's last 16 bytes are
+// loaded whole where its end falls inside a slot, so nothing is read outside
+// the operand (K >= 512).
 #pragma once
 
 #include "mx4_device.h"
 
 namespace mx4 {
+
+template <int kValue>
+struct Constant {
+    static constexpr int value = kValue;
+};
 
 #define MX4_LDS __attribute__((address_space(3)))
 
@@ -73,42 +85,60 @@ __device__ __forceinline__ void fetch_b(MX4_LDS unsigned char* wr, const TileLan
     for (int i = 0; i < 2; ++i) buffer_to_lds(L.b, wr + kStageB + (L.wave * 2 + i) * 1024, L.b_src[i], t * 64);
 }
 
-// Where a slot's bytes start in a row: 16 per slot, moved back where the row ends inside.
+// Scales of steps 4 slot .. 4 slot + 3 of 64 rows (waves 0-3 of A, waves 4-7 of
+// B), as they lie in the row: 16 bytes per slot, moved back where it ends inside.
 __device__ __forceinline__ int slot_start(int slot, int scale_row) {
     const int last = scale_row - 16;
     return slot * 16 < last ? slot * 16 : last;
 }
 
-// Scales of steps 4 slot .. 4 slot + 3: waves 0-3 fetch 64 rows of A each, waves 4-7 of B.
 template <int kRows>
-__device__ __forceinline__ void fetch_scales(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int slot) {
-    buffer_to_lds(L.scales, wr + L.wave * 1024, L.scale_src, slot_start(slot, L.scale_row));
+__device__ __forceinline__ u32x4 load_scales(const TileLane<kRows>& L, int slot) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(L.scales, L.scale_src,
+                                                                           slot_start(slot, L.scale_row), 0));
 }
 
-// A memory phase: the fetch of A of step `next` (and of the scales of slot
-// `next_slot`, if it is one), and step t's operands from LDS into registers.
-// The regions written and read are distinct; __restrict__ says so, or the
-// compiler would wait for the fetch before the reads.
+// Dword q of the result: block q's bytes of the four steps.
+__device__ __forceinline__ u32x4 by_block(u32x4 v) {
+    const unsigned lo01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), lo23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+    const unsigned hi01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u), hi23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+    return u32x4{__builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
+                 __builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
+}
+
+template <int kRows>
+__device__ __forceinline__ void store_scales(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, u32x4 v, int slot) {
+    for (int late = slot * 16 - slot_start(slot, L.scale_row); late > 0; late -= 4) v = u32x4{v[1], v[2], v[3], 0};
+    *reinterpret_cast<MX4_LDS u32x4*>(wr + threadIdx.x * 16) = by_block(v);
+}
+
+// A memory phase: the fetch of A of step `next`, and step t's operands from LDS
+// into registers. The regions written and read are distinct; __restrict__ says
+// so, or the compiler would wait for the fetch before the reads.
 template <int kRows>
 __device__ __forceinline__ void memory_phase(const MX4_LDS unsigned char* __restrict__ rd,
-                                             MX4_LDS unsigned char* __restrict__ wr,
-                                             const MX4_LDS unsigned char* __restrict__ scale_rd,
-                                             MX4_LDS unsigned char* __restrict__ scale_wr, const TileLane<kRows>& L,
-                                             int next, int next_slot, int scale_at,
-                                             i32x4 (&av)[TileLane<kRows>::kRowFrags], i32x4 (&bv)[kColFrags],
-                                             int (&sa)[TileLane<kRows>::kRowFrags], int (&sb)[kColFrags]) {
-    if (next_slot >= 0) fetch_scales<kRows>(scale_wr, L, next_slot);
+                                             MX4_LDS unsigned char* __restrict__ wr, const TileLane<kRows>& L,
+                                             int next, i32x4 (&av)[TileLane<kRows>::kRowFrags],
+                                             i32x4 (&bv)[kColFrags]) {
     fetch_a<kRows>(wr, L, next);
 #pragma unroll
-    for (int f = 0; f < TileLane<kRows>::kRowFrags; ++f) {
+    for (int f = 0; f < TileLane<kRows>::kRowFrags; ++f)
         av[f] = *reinterpret_cast<const MX4_LDS i32x4*>(rd + L.a_off + f * 1024);
-        sa[f] = scale_rd[L.a_scale + f * 256 + scale_at];
-    }
 #pragma unroll
-    for (int f = 0; f < kColFrags; ++f) {
+    for (int f = 0; f < kColFrags; ++f)
         bv[f] = *reinterpret_cast<const MX4_LDS i32x4*>(rd + kStageB + L.b_off + f * 1024);
-        sb[f] = scale_rd[kSlotB + L.b_scale + f * 256 + scale_at];
-    }
+}
+
+// The fragments' scales of a slot's four steps.
+template <int kRows>
+__device__ __forceinline__ void read_scales(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L,
+                                            int (&sa)[TileLane<kRows>::kRowFrags], int (&sb)[kColFrags]) {
+#pragma unroll
+    for (int f = 0; f < TileLane<kRows>::kRowFrags; ++f)
+        sa[f] = *reinterpret_cast<const MX4_LDS int*>(rd + L.a_scale + f * 256);
+#pragma unroll
+    for (int f = 0; f < kColFrags; ++f)
+        sb[f] = *reinterpret_cast<const MX4_LDS int*>(rd + kSlotB + L.b_scale + f * 256);
 }
 
 // A wave's accumulators, first row and column (row, col): lane (r, q) holds
@@ -173,22 +203,23 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
     L.scale_row = steps * 4;
     L.a = rsrc_at(a_codes + static_cast<long long>(row0) * row_bytes);
     L.b = rsrc_at(b_codes + static_cast<long long>(col0) * row_bytes);
+    const int from = (lane % 4 ^ lane / 8 % 4) * 16;  // the block that lane's place in LDS takes
     // Rows past the edge read the last one.
     const auto row_of = [](int first, int i, int size) { return first + i < size ? i : size - 1 - first; };
 #pragma unroll
     for (int i = 0; i < Lane::kFetchA; ++i)
-        L.a_src[i] = row_of(row0, (wave * Lane::kFetchA + i) * 16 + r, m) * row_bytes + q * 16;
+        L.a_src[i] = row_of(row0, (wave * Lane::kFetchA + i) * 16 + lane / 4, m) * row_bytes + from;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) L.b_src[i] = row_of(col0, (wave * 2 + i) * 16 + r, n) * row_bytes + q * 16;
+    for (int i = 0; i < 2; ++i) L.b_src[i] = row_of(col0, (wave * 2 + i) * 16 + lane / 4, n) * row_bytes + from;
     const bool for_a = wave < 4;
     L.scales = rsrc_at(for_a ? a_scales + static_cast<long long>(row0) * L.scale_row
                              : b_scales + static_cast<long long>(col0) * L.scale_row);
     L.scale_src = row_of(for_a ? row0 : col0, (wave % 4) * 64 + lane, for_a ? m : n) * L.scale_row;
     const int wave_row = wave / 4 * (kRows / 2), wave_col = wave % 4 * 64;
-    L.a_off = wave_row * 64 + lane * 16;
-    L.b_off = wave_col * 64 + lane * 16;
-    L.a_scale = (wave_row + r) * 16 + q;
-    L.b_scale = (wave_col + r) * 16 + q;
+    L.a_off = (wave_row + r) * 64 + (q ^ r / 2 % 4) * 16;
+    L.b_off = (wave_col + r) * 64 + (q ^ r / 2 % 4) * 16;
+    L.a_scale = (wave_row + r) * 16 + q * 4;
+    L.b_scale = (wave_col + r) * 16 + q * 4;
 
     f32x4 acc[Lane::kRowFrags][kColFrags];
 #pragma unroll
@@ -200,12 +231,13 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
     MX4_LDS unsigned char* slots = lds + kStages * kStageBytes;
     const auto slot = [&](int s) { return slots + (s & 1) * kSlotBytes; };
 
-    fetch_scales<kRows>(slot(0), L, 0);
+    u32x4 scales = load_scales<kRows>(L, 0);
 #pragma unroll
     for (int t = 0; t < kStages - 1; ++t) {
         fetch_a<kRows>(stage(t), L, t);
         fetch_b<kRows>(stage(t), L, t);
     }
+    store_scales<kRows>(slot(0), L, scales, 0);
     __builtin_amdgcn_s_waitcnt(0);
     phase_barrier();
     const bool late = wave >= 4;
@@ -214,32 +246,46 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
     i32x4 av[Lane::kRowFrags], bv[kColFrags];
     int sa[Lane::kRowFrags], sb[kColFrags];
     const int last_slot = (steps - 1) / 4;
-    for (int t = 0; t < steps; ++t) {
-        // Step t + 3 goes to the stage of step t - 1, the next slot's scales to
-        // the slot of steps up to t - 1, which no wave reads any more (past the
-        // end the last step is fetched again).
+    // Step t = 4 s + j. Step t + 3 goes to the stage of step t - 1, the next
+    // slot's scales to the slot of steps up to 4 s - 1, which no wave reads any
+    // more (past the end the last step and slot are taken again).
+    const auto step = [&](int t, auto which) {
+        constexpr int j = decltype(which)::value;
         const int next = t + 3 < steps ? t + 3 : steps - 1;
-        const int s = t / 4;
-        const int next_slot = t % 4 == 0 && s < last_slot ? s + 1 : -1;
-        const int scale_at = t * 4 - slot_start(s, L.scale_row);
-        memory_phase<kRows>(stage(t), stage(t + 3), slot(s), slot(s + 1), L, next, next_slot, scale_at, av, bv, sa, sb);
+        const int s = t / 4, next_slot = s < last_slot ? s + 1 : last_slot;
+        if constexpr (j == 0) {
+            read_scales<kRows>(slot(s), L, sa, sb);
+            scales = load_scales<kRows>(L, next_slot);
+        }
+        memory_phase<kRows>(stage(t), stage(t + 3), L, next, av, bv);
+        if constexpr (j == 3) store_scales<kRows>(slot(s + 1), L, scales, next_slot);
         // The fetch of step t + 1 has landed once at most those of A and B of
-        // t + 2 and of A of t + 3 are left (loads into LDS land in order; a
-        // slot's scales, issued before A of t + 3, are then two steps early).
-        __builtin_amdgcn_s_waitcnt(0x0070 | (2 * Lane::kFetchA + 2));  // vmcnt, lgkmcnt(0)
+        // t + 2 and of A of t + 3 are left, and the scales loaded at the
+        // slot's first step between them (loads land in order).
+        __builtin_amdgcn_s_waitcnt(0x0070 | (2 * Lane::kFetchA + (j < 2 ? 3 : 2)));  // vmcnt, lgkmcnt(0)
         phase_barrier();
 #pragma unroll
         for (int i = 0; i < Lane::kRowFrags / 2; ++i)
 #pragma unroll
-            for (int j = 0; j < kColFrags; ++j) acc[i][j] = mfma(bv[j], sb[j], av[i], sa[i], acc[i][j]);
+            for (int f = 0; f < kColFrags; ++f) acc[i][f] = mfma<j>(bv[f], sb[f], av[i], sa[i], acc[i][f]);
         __builtin_amdgcn_sched_barrier(0);
         fetch_b<kRows>(stage(t + 3), L, next);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = Lane::kRowFrags / 2; i < Lane::kRowFrags; ++i)
 #pragma unroll
-            for (int j = 0; j < kColFrags; ++j) acc[i][j] = mfma(bv[j], sb[j], av[i], sa[i], acc[i][j]);
+            for (int f = 0; f < kColFrags; ++f) acc[i][f] = mfma<j>(bv[f], sb[f], av[i], sa[i], acc[i][f]);
         phase_barrier();
+    };
+    for (int t = 0;;) {
+        step(t, Constant<0>{});
+        if (++t == steps) break;
+        step(t, Constant<1>{});
+        if (++t == steps) break;
+        step(t, Constant<2>{});
+        if (++t == steps) break;
+        step(t, Constant<3>{});
+        if (++t == steps) break;
     }
     if (!late) phase_barrier();
     __builtin_amdgcn_s_waitcnt(0);

@@ -40,10 +40,12 @@ constexpr int kF32 = MCHIP_DTYPE_F32, kBf16 = MCHIP_DTYPE_BF16, kF16 = MCHIP_DTY
 template <int kType>
 constexpr int kSize = kType == kF32 ? 4 : 2;
 
+// kByte: which byte of the scale registers.
+template <int kByte = 0>
 __device__ __forceinline__ f32x4 mfma(i32x4 a, int sa, i32x4 b, int sb, f32x4 c) {
     const i32x8 a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
     const i32x8 b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, sa, 0, sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, kByte, sa, kByte, sb);
 }
 
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
