@@ -1,28 +1,35 @@
 // The large-tile body of the product of two mx4 operands (gemm_mx4.hip).
 //
-// Block tile 256x256 (or 128x256), 512 lanes = 8 waves in a 2x4 grid (two
-// waves per SIMD), each a 128x64 quadrant as 8x4 accumulators. One block per
-// CU. The schedule is that of gemm_mfma16_fast.h: K in steps of 128 through a
-// ring of four 32 KiB LDS stages, the two waves of each SIMD one phase apart,
-// one reading its operands from LDS while the other multiplies.
+// Block tile 256x256 (or 128x256) by 4 waves in a 2x2 grid, one per SIMD, each
+// a 128x128 quadrant as 8x8 accumulators (256 registers). One block per CU. The
+// 16x16x128 instruction takes 16 cycles for two 1 KiB fragments, so LDS and the
+// caches have to feed it four times as fast per element as bf16: the quadrant
+// is as large as the registers allow (a third fewer LDS reads than the 128x64
+// quadrants of 8 waves), and a fetch takes whole 128-byte lines (64-byte pieces,
+// 128 k per row, were twice the requests to L2: 8192^3 in 286 us with both).
 //
-// LDS layout of a stage: rows of 64 bytes, A's 256 at 0 and B's at 16 KiB; block
-// c of row r lies at 64 r + 16 (c ^ (r / 2 % 4)). A fetch instruction fills 16
-// rows, four neighbouring lanes one row: the address unit takes four lanes'
-// adjacent 16 bytes in one access (with a lane per row it made 64 accesses of
-// an instruction and bound the kernel: 2400 a step, 8192^3 in 342 us).
-// A fragment read (lane (r, q) block q of row r) goes over every bank once per
-// 16 lanes that the LDS serves together (lanes 0-3, 12-15 and 20-27 the first);
-// of the swizzles tried, this one and one other had no conflicts.
+// K goes in stages of 256 through two 64 KiB LDS buffers, each stage as two
+// steps of 128, each step as 8 rows of 8 products. While a step's products
+// issue, the next step's fragments are read from LDS: B's into registers of
+// their own, A's row i into row i's once its products have issued. In the second
+// step of stage s, after two rows, one barrier: every wave has read all of
+// stage s and its own share of stage s + 1 has landed, so after it stage s + 2 is
+// fetched over stage s, and stage s + 1 is read.
 //
-// Scales: a row has four bytes per step. Fetched a step at a time, a load would
-// touch 64 rows, 64 lines, for 256 bytes; instead a lane takes 16 bytes of its
-// row, four steps' worth, once in four steps, and turns them (four steps of
-// four blocks) into four blocks' dwords of four steps each, in one of two 8 KiB
+// LDS layout of a stage: rows of 128 bytes, A's 256 at 0 and B's at 32 KiB; block
+// c of row r lies at 128 r + 16 (c ^ (r / 2 % 8)). A fetch instruction fills 8
+// rows, eight neighbouring lanes one row (the address unit takes neighbours'
+// 16 bytes together; a lane per row made an access of each lane). A fragment
+// read, lane (r, q) block q of row r, touches every bank once per 16 lanes
+// that the LDS serves together (lanes 0-3, 12-15 and 20-27 the first).
+//
+// Scales: a row has 4 bytes per step. A lane takes 16 bytes of a row, four
+// steps' worth, two lanes 8 steps (a window), and turns them (four steps of four
+// blocks) into four blocks' dwords of four steps each, in one of two 16 KiB
 // slots of LDS. A lane then reads one dword per fragment for four steps and the
 // instruction picks the step's byte. (Read from LDS a byte per fragment and
 // step, the scales took 50 of 332 us at 8192^3.) A row's last 16 bytes are
-// loaded whole where its end falls inside a slot, so nothing is read outside
+// loaded whole where its end falls inside a window, so nothing is read outside
 // the operand (K >= 512).
 #pragma once
 
@@ -37,11 +44,11 @@ struct Constant {
 
 #define MX4_LDS __attribute__((address_space(3)))
 
-constexpr int kTileRows = 256, kTileCols = 256, kTileThreads = 512;
-constexpr int kStages = 4, kStageBytes = 32 * 1024, kStageB = 16 * 1024;
-constexpr int kSlotBytes = 8 * 1024, kSlotB = 4 * 1024;
-constexpr int kRingBytes = kStages * kStageBytes + 2 * kSlotBytes;
-constexpr int kColFrags = 4;
+constexpr int kTileRows = 256, kTileCols = 256, kTileThreads = 256;
+constexpr int kStageBytes = 64 * 1024, kStageB = 32 * 1024;
+constexpr int kSlotBytes = 16 * 1024, kSlotHalf = 8 * 1024, kSlotB = 4 * 1024;
+constexpr int kRingBytes = 2 * kStageBytes + 2 * kSlotBytes;
+constexpr int kColFrags = 8;
 
 __device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t rsrc, MX4_LDS unsigned char* dst, int voffset,
                                               int soffset) {
@@ -49,7 +56,7 @@ __device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t rsrc, MX4_L
 }
 
 // A workgroup barrier without a memory fence, which nothing is moved across.
-__device__ __forceinline__ void phase_barrier() {
+__device__ __forceinline__ void stage_barrier() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -57,88 +64,111 @@ __device__ __forceinline__ void phase_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_at(const unsigned char* p) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, 0x7fffffff, 0x00020000);
+// `rows` rows of `row_bytes` from p on; what lies past them reads as zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const unsigned char* p, int rows, int row_bytes) {
+    const int most = rows < kTileRows ? rows : kTileRows;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, most * row_bytes, 0x00020000);
 }
 
 template <int kRows>
 struct TileLane {
     static constexpr int kRowFrags = kRows / 32;  // of a wave
-    static constexpr int kFetchA = kRows / 128;   // instructions per wave and step
-    __amdgpu_buffer_rsrc_t a, b, scales;          // codes at the tile's origin; this wave's rows' scales
-    int a_src[kFetchA], b_src[2], scale_src;
-    int a_off, b_off, a_scale, b_scale;  // LDS offsets of the wave's first fragments and their scales
-    int scale_row;                       // bytes of scales in a row
-    int wave;
+    static constexpr int kFetchA = kRows / 32;    // instructions per wave and stage
+    static constexpr int kFetchB = 8;
+    __amdgpu_buffer_rsrc_t a, b, scales;  // codes at the tile's origin; this wave's operand's scales
+    int src[2];                           // the lane's offset in a fetch of rows 16 j .. + 7 and 16 j + 8 .. + 15
+    int scale_src;                        // ... in a load of 32 rows' scales
+    int a_off[2], b_off[2];               // LDS offsets of the wave's first fragments in each step
+    int a_scale, b_scale;                 // ... and of their scales
+    int row_bytes, scale_row;             // bytes of codes and of scales in a row
+    int wave, lane;
 };
 
+// Instruction i of this wave's share of stage s (A's first). Where K ends in the
+// middle of the last stage, lanes past the end take the half before.
 template <int kRows>
-__device__ __forceinline__ void fetch_a(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int t) {
+__device__ __forceinline__ void fetch_one(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int s, int i) {
+    constexpr int kA = TileLane<kRows>::kFetchA, kB = TileLane<kRows>::kFetchB;
+    const bool of_a = i < kA;
+    const int k = of_a ? i : i - kA;
+    const int at = s * 128;
+    const int back = at + 128 > L.row_bytes ? ((L.lane % 8 ^ (4 * (k & 1) + L.lane / 16)) & 4) * 16 : 0;
+    const int part = L.wave * (of_a ? kA : kB) + k;  // eight rows
+    buffer_to_lds(of_a ? L.a : L.b, wr + (of_a ? 0 : kStageB) + part * 1024, L.src[k & 1] - back,
+                  part * 8 * L.row_bytes + at);
+}
+
+// Part `which` of kParts of this wave's share.
+template <int kRows, int kParts>
+__device__ __forceinline__ void fetch_part(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int s, int which) {
+    constexpr int kAll = TileLane<kRows>::kFetchA + TileLane<kRows>::kFetchB;
 #pragma unroll
-    for (int i = 0; i < TileLane<kRows>::kFetchA; ++i)
-        buffer_to_lds(L.a, wr + (L.wave * TileLane<kRows>::kFetchA + i) * 1024, L.a_src[i], t * 64);
+    for (int i = 0; i < kAll; ++i)
+        if (i >= which * kAll / kParts && i < (which + 1) * kAll / kParts) fetch_one<kRows>(wr, L, s, i);
 }
 
+// Part n % 4 of window n / 4: 32 rows' scales of 8 steps, a lane 16 bytes as
+// they lie in the row, moved back where the row ends inside.
 template <int kRows>
-__device__ __forceinline__ void fetch_b(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int t) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) buffer_to_lds(L.b, wr + kStageB + (L.wave * 2 + i) * 1024, L.b_src[i], t * 64);
+__device__ __forceinline__ int scale_at(const TileLane<kRows>& L, int n) {
+    return n / 4 * 32 + L.lane % 2 * 16;
 }
-
-// Scales of steps 4 slot .. 4 slot + 3 of 64 rows (waves 0-3 of A, waves 4-7 of
-// B), as they lie in the row: 16 bytes per slot, moved back where it ends inside.
-__device__ __forceinline__ int slot_start(int slot, int scale_row) {
-    const int last = scale_row - 16;
-    return slot * 16 < last ? slot * 16 : last;
-}
-
 template <int kRows>
-__device__ __forceinline__ u32x4 load_scales(const TileLane<kRows>& L, int slot) {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(L.scales, L.scale_src,
-                                                                           slot_start(slot, L.scale_row), 0));
+__device__ __forceinline__ u32x4 load_scales(const TileLane<kRows>& L, int n) {
+    const int at = scale_at<kRows>(L, n), last = L.scale_row - 16;
+    return __builtin_bit_cast(
+        u32x4, __builtin_amdgcn_raw_buffer_load_b128(L.scales, L.scale_src + (at < last ? at : last),
+                                                     (L.wave % 2 * 128 + n % 4 * 32) * L.scale_row, 0));
 }
 
 // Dword q of the result: block q's bytes of the four steps.
 __device__ __forceinline__ u32x4 by_block(u32x4 v) {
-    const unsigned lo01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), lo23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
-    const unsigned hi01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u), hi23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+    const unsigned lo01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
+    const unsigned lo23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+    const unsigned hi01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+    const unsigned hi23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
     return u32x4{__builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
                  __builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
 }
 
+// A window's slot: [steps 0-3, steps 4-7][256 rows of A, 256 of B][16 bytes].
+// Bytes of steps past the end are zeros, a scale of 2^-127 on both sides, which
+// makes nothing of whatever codes they meet: an odd last step needs no branch.
 template <int kRows>
-__device__ __forceinline__ void store_scales(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, u32x4 v, int slot) {
-    for (int late = slot * 16 - slot_start(slot, L.scale_row); late > 0; late -= 4) v = u32x4{v[1], v[2], v[3], 0};
-    *reinterpret_cast<MX4_LDS u32x4*>(wr + threadIdx.x * 16) = by_block(v);
+__device__ __forceinline__ void store_scales(MX4_LDS unsigned char* slots, const TileLane<kRows>& L, u32x4 v, int n) {
+    // Without branches: a product's loop is one block, or the compiler moves
+    // products from before a branch behind it.
+    const int late = (scale_at<kRows>(L, n) - (L.scale_row - 16)) / 4;  // dwords moved back, if above 0
+    const bool one = late > 0 && (late & 1), two = late > 0 && (late & 2), past = late > 3;
+    v = u32x4{one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], one ? 0u : v[3]};
+    v = u32x4{two ? v[2] : v[0], two ? v[3] : v[1], two ? 0u : v[2], two ? 0u : v[3]};
+    v = u32x4{past ? 0u : v[0], past ? 0u : v[1], past ? 0u : v[2], past ? 0u : v[3]};
+    const int row = (L.wave / 2 * 256) + (L.wave % 2 * 128) + n % 4 * 32 + L.lane / 2;
+    *reinterpret_cast<MX4_LDS u32x4*>(slots + (n / 4 & 1) * kSlotBytes + L.lane % 2 * kSlotHalf + row * 16) = by_block(v);
 }
 
-// A memory phase: the fetch of A of step `next`, and step t's operands from LDS
-// into registers. The regions written and read are distinct; __restrict__ says
-// so, or the compiler would wait for the fetch before the reads.
+// One fragment of step u of the stage at `rd`, and a fragment's scales of four
+// steps. The regions read are not being written; __restrict__ says so, or the
+// compiler would wait for the fetches in flight.
 template <int kRows>
-__device__ __forceinline__ void memory_phase(const MX4_LDS unsigned char* __restrict__ rd,
-                                             MX4_LDS unsigned char* __restrict__ wr, const TileLane<kRows>& L,
-                                             int next, i32x4 (&av)[TileLane<kRows>::kRowFrags],
-                                             i32x4 (&bv)[kColFrags]) {
-    fetch_a<kRows>(wr, L, next);
-#pragma unroll
-    for (int f = 0; f < TileLane<kRows>::kRowFrags; ++f)
-        av[f] = *reinterpret_cast<const MX4_LDS i32x4*>(rd + L.a_off + f * 1024);
-#pragma unroll
-    for (int f = 0; f < kColFrags; ++f)
-        bv[f] = *reinterpret_cast<const MX4_LDS i32x4*>(rd + kStageB + L.b_off + f * 1024);
+__device__ __forceinline__ i32x4 read_a(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L, int u,
+                                        int f) {
+    return *reinterpret_cast<const MX4_LDS i32x4*>(rd + L.a_off[u] + f * 2048);
 }
-
-// The fragments' scales of a slot's four steps.
 template <int kRows>
-__device__ __forceinline__ void read_scales(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L,
-                                            int (&sa)[TileLane<kRows>::kRowFrags], int (&sb)[kColFrags]) {
-#pragma unroll
-    for (int f = 0; f < TileLane<kRows>::kRowFrags; ++f)
-        sa[f] = *reinterpret_cast<const MX4_LDS int*>(rd + L.a_scale + f * 256);
-#pragma unroll
-    for (int f = 0; f < kColFrags; ++f)
-        sb[f] = *reinterpret_cast<const MX4_LDS int*>(rd + kSlotB + L.b_scale + f * 256);
+__device__ __forceinline__ i32x4 read_b(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L, int u,
+                                        int f) {
+    return *reinterpret_cast<const MX4_LDS i32x4*>(rd + kStageB + L.b_off[u] + f * 2048);
+}
+template <int kRows>
+__device__ __forceinline__ int read_scale_a(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L,
+                                            int f) {
+    return *reinterpret_cast<const MX4_LDS int*>(rd + L.a_scale + f * 256);
+}
+template <int kRows>
+__device__ __forceinline__ int read_scale_b(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L,
+                                            int f) {
+    return *reinterpret_cast<const MX4_LDS int*>(rd + kSlotB + L.b_scale + f * 256);
 }
 
 // A wave's accumulators, first row and column (row, col): lane (r, q) holds
@@ -195,99 +225,134 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
                                              const unsigned char* b_scales, void* c, int m, int n, int steps, int row0,
                                              int col0, int vec) {
     typedef TileLane<kRows> Lane;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
-    const int row_bytes = steps * 64;
     Lane L;
     L.wave = wave;
+    L.lane = lane;
+    L.row_bytes = steps * 64;
     L.scale_row = steps * 4;
-    L.a = rsrc_at(a_codes + static_cast<long long>(row0) * row_bytes);
-    L.b = rsrc_at(b_codes + static_cast<long long>(col0) * row_bytes);
-    const int from = (lane % 4 ^ lane / 8 % 4) * 16;  // the block that lane's place in LDS takes
-    // Rows past the edge read the last one.
-    const auto row_of = [](int first, int i, int size) { return first + i < size ? i : size - 1 - first; };
+    L.a = rsrc_of(a_codes + static_cast<long long>(row0) * L.row_bytes, m - row0, L.row_bytes);
+    L.b = rsrc_of(b_codes + static_cast<long long>(col0) * L.row_bytes, n - col0, L.row_bytes);
+    // The block that the lane's place in LDS takes, of row lane / 8 of a fetch.
 #pragma unroll
-    for (int i = 0; i < Lane::kFetchA; ++i)
-        L.a_src[i] = row_of(row0, (wave * Lane::kFetchA + i) * 16 + lane / 4, m) * row_bytes + from;
+    for (int i = 0; i < 2; ++i) L.src[i] = lane / 8 * L.row_bytes + (lane % 8 ^ (4 * i + lane / 16)) * 16;
+    // Waves 0 and 1 see to A's scales, 2 and 3 to B's, 128 rows each.
+    const bool for_a = wave < 2;
+    L.scales = for_a ? rsrc_of(a_scales + static_cast<long long>(row0) * L.scale_row, m - row0, L.scale_row)
+                     : rsrc_of(b_scales + static_cast<long long>(col0) * L.scale_row, n - col0, L.scale_row);
+    L.scale_src = lane / 2 * L.scale_row;
+    const int wave_row = wave / 2 * (kRows / 2), wave_col = wave % 2 * 128;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) L.b_src[i] = row_of(col0, (wave * 2 + i) * 16 + lane / 4, n) * row_bytes + from;
-    const bool for_a = wave < 4;
-    L.scales = rsrc_at(for_a ? a_scales + static_cast<long long>(row0) * L.scale_row
-                             : b_scales + static_cast<long long>(col0) * L.scale_row);
-    L.scale_src = row_of(for_a ? row0 : col0, (wave % 4) * 64 + lane, for_a ? m : n) * L.scale_row;
-    const int wave_row = wave / 4 * (kRows / 2), wave_col = wave % 4 * 64;
-    L.a_off = (wave_row + r) * 64 + (q ^ r / 2 % 4) * 16;
-    L.b_off = (wave_col + r) * 64 + (q ^ r / 2 % 4) * 16;
+    for (int u = 0; u < 2; ++u) {
+        L.a_off[u] = (wave_row + r) * 128 + ((4 * u + q) ^ r / 2) * 16;
+        L.b_off[u] = (wave_col + r) * 128 + ((4 * u + q) ^ r / 2) * 16;
+    }
     L.a_scale = (wave_row + r) * 16 + q * 4;
     L.b_scale = (wave_col + r) * 16 + q * 4;
 
     f32x4 acc[Lane::kRowFrags][kColFrags];
+    const auto stage = [&](int s) { return lds + (s & 1) * kStageBytes; };
+    MX4_LDS unsigned char* slots = lds + 2 * kStageBytes;
+    const auto scales_of = [&](int s) { return slots + (s / 4 & 1) * kSlotBytes + (s / 2 & 1) * kSlotHalf; };
+    const int stages = (steps + 1) / 2;
+
+    // The scales' parts 0 to 5 and stages 0 and 1, all on their way at once; the
+    // first five parts go to LDS.
+    u32x4 first[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) first[i] = load_scales<kRows>(L, i);
+    u32x4 scales = load_scales<kRows>(L, 5);
+    fetch_part<kRows, 1>(stage(0), L, 0, 0);
+    fetch_part<kRows, 1>(stage(1), L, 1, 0);
 #pragma unroll
     for (int i = 0; i < Lane::kRowFrags; ++i)
 #pragma unroll
-        for (int j = 0; j < kColFrags; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    const auto stage = [&](int t) { return lds + (t & (kStages - 1)) * kStageBytes; };
-    MX4_LDS unsigned char* slots = lds + kStages * kStageBytes;
-    const auto slot = [&](int s) { return slots + (s & 1) * kSlotBytes; };
-
-    u32x4 scales = load_scales<kRows>(L, 0);
-#pragma unroll
-    for (int t = 0; t < kStages - 1; ++t) {
-        fetch_a<kRows>(stage(t), L, t);
-        fetch_b<kRows>(stage(t), L, t);
-    }
-    store_scales<kRows>(slot(0), L, scales, 0);
-    __builtin_amdgcn_s_waitcnt(0);
-    phase_barrier();
-    const bool late = wave >= 4;
-    if (late) phase_barrier();
-
-    i32x4 av[Lane::kRowFrags], bv[kColFrags];
-    int sa[Lane::kRowFrags], sb[kColFrags];
-    const int last_slot = (steps - 1) / 4;
-    // Step t = 4 s + j. Step t + 3 goes to the stage of step t - 1, the next
-    // slot's scales to the slot of steps up to 4 s - 1, which no wave reads any
-    // more (past the end the last step and slot are taken again).
-    const auto step = [&](int t, auto which) {
-        constexpr int j = decltype(which)::value;
-        const int next = t + 3 < steps ? t + 3 : steps - 1;
-        const int s = t / 4, next_slot = s < last_slot ? s + 1 : last_slot;
-        if constexpr (j == 0) {
-            read_scales<kRows>(slot(s), L, sa, sb);
-            scales = load_scales<kRows>(L, next_slot);
+        for (int j = 0; j < kColFrags; ++j) {
+            acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            asm volatile("" : "+a"(acc[i][j]));  // cleared here, while the fetch is under way
         }
-        memory_phase<kRows>(stage(t), stage(t + 3), L, next, av, bv);
-        if constexpr (j == 3) store_scales<kRows>(slot(s + 1), L, scales, next_slot);
-        // The fetch of step t + 1 has landed once at most those of A and B of
-        // t + 2 and of A of t + 3 are left, and the scales loaded at the
-        // slot's first step between them (loads land in order).
-        __builtin_amdgcn_s_waitcnt(0x0070 | (2 * Lane::kFetchA + (j < 2 ? 3 : 2)));  // vmcnt, lgkmcnt(0)
-        phase_barrier();
 #pragma unroll
-        for (int i = 0; i < Lane::kRowFrags / 2; ++i)
+    for (int i = 0; i < 5; ++i) store_scales<kRows>(slots, L, first[i], i);
+    __builtin_amdgcn_s_waitcnt(0);
+    stage_barrier();
+
+    constexpr int kI = Lane::kRowFrags, kB = kColFrags / kI;
+    i32x4 av[kI], bv[2][kColFrags];
+    int sa[kI], sb[kColFrags], sb_next[kColFrags];
 #pragma unroll
-            for (int f = 0; f < kColFrags; ++f) acc[i][f] = mfma<j>(bv[f], sb[f], av[i], sa[i], acc[i][f]);
-        __builtin_amdgcn_sched_barrier(0);
-        fetch_b<kRows>(stage(t + 3), L, next);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = Lane::kRowFrags / 2; i < Lane::kRowFrags; ++i)
-#pragma unroll
-            for (int f = 0; f < kColFrags; ++f) acc[i][f] = mfma<j>(bv[f], sb[f], av[i], sa[i], acc[i][f]);
-        phase_barrier();
-    };
-    for (int t = 0;;) {
-        step(t, Constant<0>{});
-        if (++t == steps) break;
-        step(t, Constant<1>{});
-        if (++t == steps) break;
-        step(t, Constant<2>{});
-        if (++t == steps) break;
-        step(t, Constant<3>{});
-        if (++t == steps) break;
+    for (int f = 0; f + 1 < kI; ++f) {
+        av[f] = read_a<kRows>(lds, L, 0, f);
+        sa[f] = read_scale_a<kRows>(scales_of(0), L, f);
     }
-    if (!late) phase_barrier();
+#pragma unroll
+    for (int f = 0; f < kColFrags; ++f) {
+        bv[0][f] = read_b<kRows>(lds, L, 0, f);
+        sb[f] = read_scale_b<kRows>(scales_of(0), L, f);
+    }
+
+    // Stage s, `which` = s % 2. The part of scales stored at stage s is s + 5
+    // (the fourth of a window two stages before its first use), loaded a stage
+    // before. The rows are held in their order, or the compiler would gather
+    // the reads at the end, where the next step waits for them.
+    const auto run = [&](int s, auto which) {
+        constexpr int w = decltype(which)::value;
+        const MX4_LDS unsigned char *here = stage(s), *there = stage(s + 1);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+            if (i == 0) {
+                av[kI - 1] = read_a<kRows>(here, L, 0, kI - 1);
+                if constexpr (w == 0) sa[kI - 1] = read_scale_a<kRows>(scales_of(s), L, kI - 1);
+            } else {
+                av[i - 1] = read_a<kRows>(here, L, 1, i - 1);
+            }
+#pragma unroll
+            for (int f = i * kB; f < i * kB + kB; ++f) bv[1][f] = read_b<kRows>(here, L, 1, f);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < kColFrags; ++f)
+                acc[i][f] = mfma<w * 2>(bv[0][f], sb[f], av[i], sa[i], acc[i][f]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int next = s + 2 < stages ? s + 2 : stages - 1;
+#pragma unroll
+        for (int i = 0; i < kI; ++i) {
+            if (i == 0) av[kI - 1] = read_a<kRows>(here, L, 1, kI - 1);
+            if (i == 2) {
+                __builtin_amdgcn_s_waitcnt(0);
+                stage_barrier();
+                store_scales<kRows>(slots, L, scales, s + 5);
+                scales = load_scales<kRows>(L, s + 6);
+                av[0] = read_a<kRows>(there, L, 0, 0);
+                if constexpr (w == 1) sa[0] = read_scale_a<kRows>(scales_of(s + 1), L, 0);
+            }
+            if (i >= 2) {
+                // What is left after two rows, over the other rows.
+                constexpr int kLeft = kI - 2;
+                av[i - 1] = read_a<kRows>(there, L, 0, i - 1);
+                if constexpr (w == 1) sa[i - 1] = read_scale_a<kRows>(scales_of(s + 1), L, i - 1);
+                fetch_part<kRows, kLeft>(stage(s), L, next, i - 2);
+#pragma unroll
+                for (int f = (i - 2) * kColFrags / kLeft; f < (i - 1) * kColFrags / kLeft; ++f) {
+                    bv[0][f] = read_b<kRows>(there, L, 0, f);
+                    if constexpr (w == 1) sb_next[f] = read_scale_b<kRows>(scales_of(s + 1), L, f);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < kColFrags; ++f)
+                acc[i][f] = mfma<w * 2 + 1>(bv[1][f], sb[f], av[i], sa[i], acc[i][f]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Two stages at a time, the four steps of a scale dword; what is past the
+    // end has zero scales.
+    for (int s = 0; s < stages; s += 2) {
+        run(s, Constant<0>{});
+        run(s + 1, Constant<1>{});
+#pragma unroll
+        for (int f = 0; f < kColFrags; ++f) sb[f] = sb_next[f];
+    }
     __builtin_amdgcn_s_waitcnt(0);
     store_tile<Lane::kRowFrags, kOut>(acc, c, row0 + wave_row, col0 + wave_col, m, n, lane, vec);
 }
