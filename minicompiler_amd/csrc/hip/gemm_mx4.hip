@@ -18,7 +18,7 @@ __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned cha
                                                               const unsigned char* __restrict__ b_codes,
                                                               const unsigned char* __restrict__ b_scales,
                                                               void* __restrict__ c, int m, int n, int steps,
-                                                              unsigned tiles_n, bool wide) {
+                                                              unsigned tiles_n) {
     __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
@@ -70,8 +70,7 @@ __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned cha
         for (int j = 0; j < kN; ++j) {
             const long long col = col0 + 16 * j + 4 * q;
             if (col < n)
-                store_four<kOut>(c, row * n + col, acc[i * kN + j], static_cast<int>(n - col < 4 ? n - col : 4),
-                                 wide && col + 4 <= n);
+                store_four<kOut>(c, row * n + col, acc[i * kN + j], static_cast<int>(n - col < 4 ? n - col : 4));
         }
     }
 }
@@ -85,19 +84,19 @@ __global__ __launch_bounds__(kTileThreads, 1) void product_tiles(const unsigned 
                                                                  const unsigned char* __restrict__ b_codes,
                                                                  const unsigned char* __restrict__ b_scales,
                                                                  void* __restrict__ c, int m, int n, int steps,
-                                                                 int tiles_n, int full, int vec) {
+                                                                 int tiles_n, int full, bool eights) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[kRingBytes];
     MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);  // generic -> LDS address space
     const int block = static_cast<int>(blockIdx.x);
     if (block < full) {
         product_tile<256, kOut>(lds, a_codes, a_scales, b_codes, b_scales, c, m, n, steps, block / tiles_n * 256,
-                                block % tiles_n * 256, vec);
+                                block % tiles_n * 256, eights);
     } else {
         const int t = full + (block - full) / 2;
         const int row0 = t / tiles_n * 256 + (block - full) % 2 * 128;
         if (row0 >= m) return;  // the last tile row has no second half
         product_tile<128, kOut>(lds, a_codes, a_scales, b_codes, b_scales, c, m, n, steps, row0, t % tiles_n * 256,
-                                vec);
+                                eights);
     }
 }
 
@@ -105,7 +104,6 @@ struct Product {
     const unsigned char *a_codes, *a_scales, *b_codes, *b_scales;
     void* c;
     int m, n, steps;
-    bool wide;
     hipStream_t stream;
 };
 
@@ -118,7 +116,7 @@ int launch_direct(const Product& p) {
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     hipLaunchKernelGGL((product_direct<kM, kN, kWaves, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64),
                        0, p.stream, p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps,
-                       static_cast<unsigned>(tn), p.wide);
+                       static_cast<unsigned>(tn));
     return hipGetLastError();
 }
 
@@ -128,8 +126,7 @@ int launch_tiles(const Product& p) {
     const int cus = device_cus(), rest = all % cus;
     const int halves = rest <= cus / 2 ? rest : 0;
     hipLaunchKernelGGL(product_tiles<kOut>, dim3(static_cast<unsigned>(all + halves)), dim3(kTileThreads), 0, p.stream,
-                       p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps, tn, all - halves,
-                       p.n % 8 == 0 && aligned(p.c, 16) ? 8 : p.wide ? 4 : 1);
+                       p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps, tn, all - halves, p.n % 8 == 0);
     return hipGetLastError();
 }
 
@@ -176,7 +173,7 @@ extern "C" int mchip_launch_matmul_mx4(const void* a_codes, const void* a_scales
     Product p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
               static_cast<const unsigned char*>(b_codes), static_cast<const unsigned char*>(b_scales),
               c, m, n, static_cast<int>(mchip_mx4_k(k) / kStep),
-              n % 4 == 0 && aligned(c, 4 * size_of(c_dtype)), static_cast<hipStream_t>(stream)};
+              static_cast<hipStream_t>(stream)};
     const int rc = c_dtype == kF32 ? launch<kF32>(p) : c_dtype == kBf16 ? launch<kBf16>(p) : launch<kF16>(p);
     if (rc == hipErrorInvalidValue) *why = "more tiles of C than one launch takes";
     return rc;

@@ -172,16 +172,15 @@ __device__ __forceinline__ int read_scale_b(const MX4_LDS unsigned char* __restr
 }
 
 // A wave's accumulators, first row and column (row, col): lane (r, q) holds
-// C[row + 16 i + r][col + 16 j + 4 q + v]. vec: how many columns N and C's
-// alignment let a lane store at once (1, 4, 8).
+// C[row + 16 i + r][col + 16 j + 4 q + v]. eights: N is a multiple of 8.
 template <int kRowFrags, int kOut>
 __device__ __forceinline__ void store_tile(const f32x4 (&acc)[kRowFrags][kColFrags], void* c, int row, int col, int m,
-                                           int n, int lane, int vec) {
+                                           int n, int lane, bool eights) {
     const int r = lane % 16, q = lane / 16;
     if constexpr (kOut != kF32) {
-        // Eight columns per lane where N allows 16-byte stores: odd rows of 16
+        // Eight columns per lane, so that no lane straddles the edge: odd rows of 16
         // lanes of one fragment change places with even rows of its neighbour.
-        if (vec == 8) {
+        if (eights) {
 #pragma unroll
             for (int i = 0; i < kRowFrags; ++i)
 #pragma unroll
@@ -198,7 +197,7 @@ __device__ __forceinline__ void store_tile(const f32x4 (&acc)[kRowFrags][kColFra
                     }
                     const int at_row = row + 16 * i + r, at_col = col + 16 * (j + (q & 1)) + 8 * (q >> 1);
                     if (at_row < m && at_col < n)
-                        *reinterpret_cast<u32x4*>(static_cast<unsigned short*>(c) +
+                        *reinterpret_cast<u32x4_loose*>(static_cast<unsigned short*>(c) +
                                                   static_cast<long long>(at_row) * n + at_col) = out;
                 }
             return;
@@ -212,8 +211,7 @@ __device__ __forceinline__ void store_tile(const f32x4 (&acc)[kRowFrags][kColFra
         for (int j = 0; j < kColFrags; ++j) {
             const int at_col = col + 16 * j + 4 * q;
             if (at_col < n)
-                store_four<kOut>(c, static_cast<long long>(at_row) * n + at_col, acc[i][j], n - at_col,
-                                 vec >= 4 && at_col + 4 <= n);
+                store_four<kOut>(c, static_cast<long long>(at_row) * n + at_col, acc[i][j], n - at_col);
         }
     }
 }
@@ -223,7 +221,7 @@ template <int kRows, int kOut>
 __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const unsigned char* a_codes,
                                              const unsigned char* a_scales, const unsigned char* b_codes,
                                              const unsigned char* b_scales, void* c, int m, int n, int steps, int row0,
-                                             int col0, int vec) {
+                                             int col0, bool eights) {
     typedef TileLane<kRows> Lane;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
@@ -354,7 +352,7 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
         for (int f = 0; f < kColFrags; ++f) sb[f] = sb_next[f];
     }
     __builtin_amdgcn_s_waitcnt(0);
-    store_tile<Lane::kRowFrags, kOut>(acc, c, row0 + wave_row, col0 + wave_col, m, n, lane, vec);
+    store_tile<Lane::kRowFrags, kOut>(acc, c, row0 + wave_row, col0 + wave_col, m, n, lane, eights);
 }
 
 }  // namespace mx4

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(kWaves * 64) void weights_direct(const void* __rest
                                                               const unsigned char* __restrict__ b_codes,
                                                               const unsigned char* __restrict__ b_scales,
                                                               void* __restrict__ c, int m, int n, int k, int steps,
-                                                              unsigned tiles_n, bool wide_a, bool wide_c) {
+                                                              unsigned tiles_n) {
     constexpr int kP = kPieces<kIn>;
     __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kWaves * 64) void weights_direct(const void* __rest
             for (int i = 0; i < kM; ++i) {
                 const long long row = row0 + 16 * i + r;
                 float v[8];
-                load_eight<kIn>(a, row * lda + k0, row < m ? k - k0 : 0, wide_a, v);
+                load_eight<kIn>(a, row * lda + k0, row < m ? k - k0 : 0, v);
                 cut_eight<kP>(v, x[i]);
             }
 #pragma unroll
@@ -79,8 +79,7 @@ __global__ __launch_bounds__(kWaves * 64) void weights_direct(const void* __rest
         for (int j = 0; j < kN; ++j) {
             const long long col = col0 + 16 * j + 4 * q;
             if (col < n)
-                store_four<kOut>(c, row * n + col, acc[i * kN + j], static_cast<int>(n - col < 4 ? n - col : 4),
-                                 wide_c && col + 4 <= n);
+                store_four<kOut>(c, row * n + col, acc[i * kN + j], static_cast<int>(n - col < 4 ? n - col : 4));
         }
     }
 }
@@ -91,7 +90,6 @@ struct Product {
     const unsigned char *b_codes, *b_scales;
     void* c;
     int m, n, k, steps;
-    bool wide_a, wide_c;
     hipStream_t stream;
 };
 
@@ -104,7 +102,7 @@ int launch_direct(const Product& p) {
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
     hipLaunchKernelGGL((weights_direct<kIn, kM, kN, kWaves, kOut>), dim3(static_cast<unsigned>(blocks)),
                        dim3(kWaves * 64), 0, p.stream, p.a, p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k, p.steps,
-                       static_cast<unsigned>(tn), p.wide_a, p.wide_c);
+                       static_cast<unsigned>(tn));
     return hipGetLastError();
 }
 
@@ -143,8 +141,7 @@ int mchip_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, c
     if (*why != nullptr) return hipErrorInvalidValue;
     Product p{a, lda, static_cast<const unsigned char*>(b_codes), static_cast<const unsigned char*>(b_scales),
               c, m, n, k, static_cast<int>(mchip_mx4_k(k) / kStep),
-              aligned(a, 16) && lda * static_cast<long long>(size_of(a_dtype)) % 16 == 0,
-              n % 4 == 0 && aligned(c, 4 * size_of(c_dtype)), static_cast<hipStream_t>(stream)};
+              static_cast<hipStream_t>(stream)};
     const int rc = a_dtype == kF32   ? launch<kF32>(c_dtype, p)
                    : a_dtype == kBf16 ? launch<kBf16>(c_dtype, p)
                                       : launch<kF16>(c_dtype, p);

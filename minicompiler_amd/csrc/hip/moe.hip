@@ -4,12 +4,15 @@
 //   y = sum over the chosen e of g_e (act(x W1_e^T + b1_e) W2_e^T + b2_e).
 //
 // Three launches, in stream order:
-//   moe_router  x R^T on the FP32 matrix instruction, x cut into bf16 pieces;
-//               the last block to arrive picks the experts and lists the jobs
+//   moe_router  x R^T on the FP32 matrix instruction, d shared out over blocks; x
+//               cut into bf16 pieces; the last block to arrive adds the parts
+//               of the logits in order, picks the experts and lists the jobs
 //               (one per chosen expert and 16 of its tokens);
 //   moe_up      per job and 32 (swiglu: 16) columns of h: act(x W1^T + b1), cut
 //               into bf16 pieces;
-//   moe_down    per 32 columns of y: all jobs, h W2^T weighed by the gates.
+//   moe_down    per 32 columns of y and share of the jobs' steps: h W2^T weighed
+//               by the gates; the last block of a column tile adds the shares
+//               in order.
 // Bound by the chosen experts' weights, each read once per job. Weights are the
 // matrix instruction's first operand, 16 rows of them, and a job's 16 tokens
 // the second. Products are exact (bf16 pieces of x, h and the weights), sums fp32.
@@ -23,6 +26,7 @@ namespace {
 using namespace mx4;
 
 constexpr int kMaxTokens = MCHIP_MOE_MAX_TOKENS, kMaxExperts = MCHIP_MOE_MAX_EXPERTS, kMaxTopK = MCHIP_MOE_MAX_TOP_K;
+constexpr int kMaxWidth = 1 << 20;  // of d and h
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kNone = -1;  // the token of a job's empty place
 
@@ -35,12 +39,13 @@ struct Job {
 
 // The workspace: counters (zero between calls), the jobs, then the arrays.
 struct Workspace {
-    unsigned* arrived;
-    int* jobs;            // how many
-    Job* job;             // [max_jobs]
-    float* logits;        // [tokens, experts]
-    unsigned short* x;    // [pieces][tokens][dp]
-    unsigned short* h;    // [pieces][max_jobs * 16][hp]
+    unsigned* arrived;  // [1 + column tiles of y]
+    int* jobs;          // how many
+    Job* job;           // [max_jobs]
+    float* logits;      // [parts][tokens, experts]
+    unsigned short* x;  // [pieces][tokens][dp]
+    unsigned short* h;  // [pieces][max_jobs * 16][hp]
+    float* y;           // [shares][tokens][column tiles * 32]
 };
 
 struct Sizes {
@@ -57,6 +62,21 @@ Sizes sizes_of(int tokens, int d, int h, int experts, int top_k) {
     return {tokens, d, h, experts, top_k, padded(d), padded(h), pairs < tiled ? pairs : tiled};
 }
 
+constexpr int kCols = 32;  // of y per block
+
+// The parts that d is cut into for the logits: 64 elements for each wave.
+int router_parts(int d) { return std::min((d + 64 * kWaves - 1) / (64 * kWaves), 16); }
+
+int column_tiles(int d) { return (d + kCols - 1) / kCols; }
+
+// The shares that a column tile of y is cut into: two blocks per CU in all, as
+// long as a wave has a step to do.
+int down_shares(const Sizes& s) {
+    const int want = 2 * device_cus() / column_tiles(s.d);
+    const int most = (s.max_jobs * (s.hp / kStep) + kWaves - 1) / kWaves;
+    return std::max(1, std::min({want, most, 64}));
+}
+
 int pieces_of(int dtype) { return dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1; }
 // h is an fp32 sum: 24 bits of it for an fp32 result, 16 otherwise.
 int h_pieces_of(int dtype) { return dtype == kF32 ? 3 : 2; }
@@ -70,178 +90,181 @@ std::size_t lay_out(const Sizes& s, int dtype, unsigned char* base, Workspace* w
         at += round_up(bytes);
         return p;
     };
-    w->arrived = reinterpret_cast<unsigned*>(take(sizeof(unsigned)));
+    w->arrived = reinterpret_cast<unsigned*>(take(sizeof(unsigned) * (1 + column_tiles(kMaxWidth))));
     w->jobs = reinterpret_cast<int*>(take(sizeof(int)));
     w->job = reinterpret_cast<Job*>(take(sizeof(Job) * static_cast<std::size_t>(s.max_jobs)));
-    w->logits = reinterpret_cast<float*>(take(sizeof(float) * static_cast<std::size_t>(s.tokens) * s.experts));
+    w->logits = reinterpret_cast<float*>(take(sizeof(float) * static_cast<std::size_t>(router_parts(s.d)) * s.tokens * s.experts));
     w->x = reinterpret_cast<unsigned short*>(
         take(2 * static_cast<std::size_t>(pieces_of(dtype)) * s.tokens * s.dp));
     w->h = reinterpret_cast<unsigned short*>(
         take(2 * static_cast<std::size_t>(h_pieces_of(dtype)) * s.max_jobs * 16 * s.hp));
+    w->y = reinterpret_cast<float*>(
+        take(sizeof(float) * static_cast<std::size_t>(down_shares(s)) * s.tokens * column_tiles(s.d) * kCols));
     return at;
 }
 
 // ---------------------------------------------------------------- router
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o /= 2) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o /= 2) v += __shfl_xor(v, o);
-    return v;
-}
-
-// One token's experts and gates, by one wave. A NaN logit never counts as
-// larger; it makes every gate NaN, as softmax does.
+// One token's experts and gates, by one wave, from its logits in LDS. Logits are
+// compared as unsigned numbers in the order of the floats, from 2 up; a NaN
+// counts as 1, smaller than all, and a chosen one as 0. A NaN makes every gate
+// NaN, as softmax does.
 __device__ void choose(const float* logits, int experts, int top_k, bool normalize, int lane, int* chosen, float* gate) {
     constexpr int kEach = kMaxExperts / 64;
-    float l[kEach];
-    float top = -__builtin_inff();
+    unsigned key[kEach];
+    unsigned best = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
+        key[j] = 0;
+        if (64 * j >= experts) continue;
         const int e = lane + 64 * j;
-        l[j] = e < experts ? mc_split_load(logits + e) : -__builtin_inff();
-        top = fmaxf(top, l[j]);
+        if (e < experts) {
+            const float l = logits[e] + 0.0f;  // -0 to 0
+            const unsigned u = __builtin_bit_cast(unsigned, l);
+            key[j] = l != l ? 1u : u >> 31 ? ~u : u | 0x80000000u;
+        }
+        best = key[j] > best ? key[j] : best;
     }
-    top = wave_max(top);
+    const unsigned first = wave_max(best);
+    const float top = __builtin_bit_cast(float, first >> 31 ? first & 0x7fffffffu : ~first);
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
-        if (lane + 64 * j < experts) sum += expf(l[j] - top);
+        if (64 * j < experts && lane + 64 * j < experts) sum += expf(logits[lane + 64 * j] - top);
     sum = wave_sum(sum);
-    unsigned taken = 0;
-    float kept = 0.0f;
+    float kept = 0.0f, mine = 0.0f;
     for (int i = 0; i < top_k; ++i) {
-        float best = -__builtin_inff();
-        int at = 0x7fffffff;
+        unsigned most = 0, at = 0xffffffffu;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int e = lane + 64 * j;
-            if (e >= experts || (taken >> j & 1u)) continue;
-            if (at == 0x7fffffff || l[j] > best) {
-                best = l[j] > -__builtin_inff() ? l[j] : -__builtin_inff();
-                at = e;
+        for (int j = 0; j < kEach; ++j)
+            if (64 * j < experts && key[j] > most) {
+                most = key[j];
+                at = static_cast<unsigned>(lane + 64 * j);
             }
-        }
+        const unsigned winner = wave_max(most);
+        const unsigned e = wave_min(most == winner ? at : 0xffffffffu);
 #pragma unroll
-        for (int o = 32; o > 0; o /= 2) {
-            const float other = __shfl_xor(best, o);
-            const int e = __shfl_xor(at, o);
-            if (other > best || (other == best && e < at)) {
-                best = other;
-                at = e;
-            }
-        }
-        if (at % 64 == lane) taken |= 1u << (at / 64);
-        // The chosen expert's own logit (NaN if it is one).
-        const float p = expf(mc_split_load(logits + at) - top) / sum;
+        for (int j = 0; j < kEach; ++j)
+            if (e == static_cast<unsigned>(lane + 64 * j)) key[j] = 0;
+        const float p = expf(logits[e] - top) / sum;
         kept += p;
-        if (lane == 0) {
-            chosen[i] = at;
-            gate[i] = p;
+        if (lane == i) {
+            mine = p;
+            chosen[i] = static_cast<int>(e);
         }
     }
-    if (normalize && lane == 0)
-        for (int i = 0; i < top_k; ++i) gate[i] /= kept;
+    if (lane < top_k) gate[lane] = normalize ? mine / kept : mine;
 }
 
-// The jobs from the chosen experts in LDS, by the whole block: a thread per expert.
+// The jobs from the chosen experts in LDS, by the whole block: a thread per
+// expert for their places, then one per chosen pair.
 __device__ void list_jobs(const Workspace& w, const Sizes& s, const int (*chosen)[kMaxTopK],
-                          const float (*gate)[kMaxTopK], int* scan) {
-    const int e = threadIdx.x;
-    unsigned long long mask = 0;
-    if (e < s.experts)
-        for (int t = 0; t < s.tokens; ++t)
-            for (int i = 0; i < s.top_k; ++i)
-                if (chosen[t][i] == e) mask |= 1ull << t;
-    const int mine = (__builtin_popcountll(mask) + 15) / 16;
-    scan[e] = mine;
+                          const float (*gate)[kMaxTopK], unsigned long long* mask, int* place) {
+    static_assert(kThreads == kMaxExperts);
+    const int e = threadIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    mask[e] = 0;
     __syncthreads();
-    for (int o = 1; o < kMaxExperts; o *= 2) {
-        const int add = e >= o ? scan[e - o] : 0;
-        __syncthreads();
-        scan[e] += add;
-        __syncthreads();
+    for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads)
+        atomicOr(mask + chosen[i / s.top_k][i % s.top_k], 1ull << (i / s.top_k));
+    __syncthreads();
+    const int count = __builtin_popcountll(mask[e]), mine = (count + 15) / 16;
+    int before = mine;
+    for (int o = 1; o < 64; o *= 2) {
+        const int add = __shfl_up(before, o);
+        if (lane >= o) before += add;
     }
-    if (e == kMaxExperts - 1) *w.jobs = scan[e];
-    int at = scan[e] - mine;
-    for (int n = 0; n < mine; ++n, ++at) {
-        Job& job = w.job[at];
-        job.expert = e;
-        for (int i = 0; i < 16; ++i) {
-            int t = kNone;
-            float g = 0.0f;
-            if (mask != 0) {
-                t = __builtin_ctzll(mask);
-                mask &= mask - 1;
-                for (int j = 0; j < s.top_k; ++j)
-                    if (chosen[t][j] == e) g = gate[t][j];
-            }
-            job.token[i] = t;
-            job.gate[i] = g;
-        }
+    if (lane == 63) place[kMaxExperts + wave] = before;
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) before += place[kMaxExperts + v];
+    if (e == kMaxExperts - 1) *w.jobs = before;
+    place[e] = before - mine;
+    for (int n = 0; n < mine; ++n) w.job[before - mine + n].expert = e;
+    for (int i = count; i < 16 * mine; ++i) {
+        Job& job = w.job[before - mine + i / 16];
+        job.token[i % 16] = kNone;
+        job.gate[i % 16] = 0.0f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads) {
+        const int t = i / s.top_k, j = i % s.top_k, to = chosen[t][j];
+        const int rank = __builtin_popcountll(mask[to] & ((1ull << t) - 1));
+        Job& job = w.job[place[to] + rank / 16];
+        job.token[rank % 16] = t;
+        job.gate[rank % 16] = gate[t][j];
     }
 }
 
-// 16 experts by 16 tokens of the logits; the waves take 16-wide steps of d in
-// turn. v_mfma_f32_16x16x4_f32: lane (r, q) supplies row or column r, element q.
+// 16 experts by 16 tokens of the logits over one part of d, 64 elements at a time
+// for each wave. v_mfma_f32_16x16x4_f32: lane (r, q) supplies row or column r,
+// element q; here a lane's four elements go to four instructions.
 template <int kIn>
 __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ x, long long ldx,
                                                        const float* __restrict__ router, Workspace w, Sizes s,
                                                        bool normalize, int* __restrict__ chosen_out,
                                                        float* __restrict__ gates_out) {
     constexpr int kP = kPieces<kIn>;
+    extern __shared__ float logits[];  // [tokens, experts], in the last block
     __shared__ f32x4 space[kWaves / 2 * 64];
     __shared__ int chosen[kMaxTokens][kMaxTopK];
     __shared__ float gate[kMaxTokens][kMaxTopK];
-    __shared__ int scan[kMaxExperts];
+    __shared__ unsigned long long mask[kMaxExperts];
+    __shared__ int place[kMaxExperts + kWaves];
     __shared__ int flag;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
-    const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
-    const int blocks = gridDim.x * gridDim.y, block = blockIdx.y * gridDim.x + blockIdx.x;
+    const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16, parts = gridDim.z;
+    const int blocks = gridDim.x * gridDim.y * parts;
+    const int block = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    const long long all_logits = static_cast<long long>(s.tokens) * s.experts;
 
     const long long expert = e0 + r < s.experts ? e0 + r : s.experts - 1;
     const long long token = t0 + r < s.tokens ? t0 + r : s.tokens - 1;
     f32x4 acc[1] = {{0.0f, 0.0f, 0.0f, 0.0f}};
-    for (int k0 = wave * 16; k0 < s.d; k0 += kWaves * 16) {
-        const int k = k0 + 4 * q;
+    for (int k0 = (blockIdx.z * kWaves + wave) * 64; k0 < s.d; k0 += parts * kWaves * 64) {
+        f32x4 a[4], b[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool in = k + j < s.d;
-            const float a = in ? router[expert * s.d + k + j] : 0.0f;
-            const float b = in ? load_one<kIn>(x, token * ldx + k + j) : 0.0f;
-            acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc[0], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + 16 * i + 4 * q;
+            a[i] = load_four<kF32>(router, expert * s.d + k, s.d - k);
+            b[i] = load_four<kIn>(x, token * ldx + k, s.d - k);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][j], b[i][j], acc[0], 0, 0, 0);
     }
     add_waves<kWaves, 1>(acc, space, wave, lane);
     if (wave == 0 && t0 + r < s.tokens) {
+        float* out = w.logits + blockIdx.z * all_logits + static_cast<long long>(t0 + r) * s.experts + e0 + 4 * q;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-            if (e0 + 4 * q + v < s.experts)
-                mc_split_store(w.logits + static_cast<long long>(t0 + r) * s.experts + e0 + 4 * q + v, acc[0][v]);
+            if (e0 + 4 * q + v < s.experts) mc_split_store(out + v, acc[0][v]);
     }
 
     // x in pieces, rows padded with zeros, shared out over the blocks.
     const long long all = static_cast<long long>(s.tokens) * s.dp;
-    for (long long i = static_cast<long long>(block) * kThreads + threadIdx.x; i < all;
-         i += static_cast<long long>(blocks) * kThreads) {
+    for (long long i = (static_cast<long long>(block) * kThreads + threadIdx.x) * 8; i < all;
+         i += static_cast<long long>(blocks) * kThreads * 8) {
         const int t = static_cast<int>(i / s.dp), k = static_cast<int>(i % s.dp);
-        float piece[kP];
-        cut<kP>(k < s.d ? load_one<kIn>(x, t * ldx + k) : 0.0f, piece);
+        float v[8];
+        load_eight<kIn>(x, t * ldx + k, s.d - k, v);
+        u32x4 out[kP];
+        cut_eight<kP>(v, out);
 #pragma unroll
-        for (int p = 0; p < kP; ++p)
-            w.x[p * all + i] = static_cast<unsigned short>(__builtin_bit_cast(unsigned, piece[p]) >> 16);
+        for (int p = 0; p < kP; ++p) *reinterpret_cast<u32x4*>(w.x + p * all + i) = out[p];
     }
 
     if (!mc_split_last_arrival(w.arrived, blocks, &flag)) return;
-    for (int t = wave; t < s.tokens; t += kWaves)
-        choose(w.logits + static_cast<long long>(t) * s.experts, s.experts, s.top_k, normalize, lane, chosen[t], gate[t]);
+    for (int i = threadIdx.x; i < all_logits; i += kThreads) {
+        float sum = mc_split_load(w.logits + i);
+        for (int z = 1; z < parts; ++z) sum += mc_split_load(w.logits + z * all_logits + i);
+        logits[i] = sum;
+    }
     __syncthreads();
-    list_jobs(w, s, chosen, gate, scan);
+    for (int t = wave; t < s.tokens; t += kWaves)
+        choose(logits + t * s.experts, s.experts, s.top_k, normalize, lane, chosen[t], gate[t]);
+    __syncthreads();
+    list_jobs(w, s, chosen, gate, mask, place);
     for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads) {
         const int t = i / s.top_k, j = i % s.top_k;
         if (chosen_out != nullptr) chosen_out[i] = chosen[t][j];
@@ -261,7 +284,6 @@ struct Weights {
     const void* base;
     const unsigned char* scales;
     int k, kp;
-    bool wide;
 
     __device__ __forceinline__ static int offset(int q, int s) { return kType == kMx4 ? 32 * q + 8 * s : 32 * s + 8 * q; }
 
@@ -281,8 +303,8 @@ struct Weights {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const int k0 = t * kStep + offset(q, s);
-                if (wide && k0 + 8 <= k) {
-                    st.raw[s] = *reinterpret_cast<const u32x4*>(p + k0);
+                if (k0 + 8 <= k) {
+                    st.raw[s] = *reinterpret_cast<const u32x4_loose*>(p + k0);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -313,15 +335,19 @@ struct Weights {
     }
 };
 
-// acc[i] += rows[i] (16 weight rows) times the columns `col` (a lane's own
-// row of the pieces, `plane` elements apart), over step t.
-template <int kType, int kP, int kTiles>
-__device__ __forceinline__ void multiply_step(const Weights<kType>& w, const long long (&rows)[kTiles],
-                                              const unsigned short* col, long long plane, bool has, int t, int q,
-                                              f32x4 (&acc)[kTiles]) {
-    typename Weights<kType>::Step st[kTiles];
+template <int kType, int kTiles>
+__device__ __forceinline__ void load_step(const Weights<kType>& w, const long long (&rows)[kTiles], int t, int q,
+                                          typename Weights<kType>::Step (&st)[kTiles]) {
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) st[i] = w.load(rows[i], t, q);
+}
+
+// acc[i] += step t of 16 weight rows, loaded, times the columns `col` (a lane's
+// own row of the pieces, `plane` elements apart; has: there is one).
+template <int kType, int kP, int kTiles>
+__device__ __forceinline__ void multiply_step(const typename Weights<kType>::Step (&st)[kTiles],
+                                              const unsigned short* col, long long plane, bool has, int t, int q,
+                                              f32x4 (&acc)[kTiles]) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         u32x4 x[kP];
@@ -354,16 +380,17 @@ template <int kType, int kP, int kHP, int kAct>
 __global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const float* __restrict__ b1, Workspace w,
                                                    Sizes s) {
     constexpr bool kGated = kAct == MCHIP_MOE_SWIGLU;
-    constexpr int kTiles = 2, kCols = kGated ? 16 : 32;
+    constexpr int kTiles = 2, kUpCols = kGated ? 16 : 32;
     __shared__ f32x4 space[kWaves / 2 * kTiles * 64];
-    if (static_cast<int>(blockIdx.y) >= *w.jobs) return;
     const Job& job = w.job[blockIdx.y];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
-    const int h0 = blockIdx.x * kCols;
-    const int token = job.token[r];
+    const int h0 = blockIdx.x * kUpCols;
+    // The job is read beside the number of jobs, not after it; past the last, it is not used.
+    const int jobs = *w.jobs, expert = job.expert, token = job.token[r];
+    if (static_cast<int>(blockIdx.y) >= jobs) return;
     const long long all_rows = kGated ? 2LL * s.h : s.h;
-    const long long first = job.expert * all_rows;
+    const long long first = expert * all_rows;
     long long rows[kTiles];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
@@ -375,9 +402,17 @@ __global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const floa
     for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const long long plane = static_cast<long long>(s.tokens) * s.dp;
     const unsigned short* col = w.x + static_cast<long long>(token == kNone ? 0 : token) * s.dp;
-    if (h0 < s.h)
-        for (int t = wave; t < s.dp / kStep; t += kWaves)
-            multiply_step<kType, kP, kTiles>(w1, rows, col, plane, token != kNone, t, q, acc);
+    if (h0 < s.h) {
+        const int steps = s.dp / kStep;
+        typename Weights<kType>::Step now[kTiles], next[kTiles];
+        if (wave < steps) load_step<kType, kTiles>(w1, rows, wave, q, now);
+        for (int t = wave; t < steps; t += kWaves) {
+            if (t + kWaves < steps) load_step<kType, kTiles>(w1, rows, t + kWaves, q, next);
+            multiply_step<kType, kP, kTiles>(now, col, plane, token != kNone, t, q, acc);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) now[i] = next[i];
+        }
+    }
     add_waves<kWaves, kTiles>(acc, space, wave, lane);
     if (wave != 0) return;
     const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
@@ -406,54 +441,90 @@ __global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const floa
     }
 }
 
-// 32 columns of y for all tokens. A wave adds every job's share of its steps of
-// h into its own LDS tile (no two lanes the same element); the tiles are added
-// in wave order.
+// 32 columns of y for all tokens and one share of the jobs' steps (all jobs' steps
+// in a row, cut evenly over the shares' waves). A wave adds each of its jobs'
+// parts, weighed, to its own LDS tile (no two lanes the same element); the tiles
+// are added in wave order, the shares in their order by the last block to arrive.
 template <int kType, int kP, int kOut>
 __global__ __launch_bounds__(kThreads) void moe_down(Weights<kType> w2, const float* __restrict__ b2, Workspace w,
                                                      Sizes s, void* __restrict__ y) {
-    constexpr int kTiles = 2, kCols = 16 * kTiles;
-    __shared__ float tile[kWaves][kMaxTokens][kCols];
+    constexpr int kTiles = kCols / 16;
+    extern __shared__ float tile[];  // [kWaves][tokens][kCols]
+    __shared__ int flag;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
-    const int d0 = blockIdx.x * kCols;
-    for (int i = lane; i < s.tokens * kCols; i += 64) (&tile[wave][0][0])[i] = 0.0f;
-    const int jobs = *w.jobs;
+    const int d0 = blockIdx.x * kCols, shares = gridDim.y;
+    const int cells = s.tokens * kCols;
+    float* mine = tile + wave * cells;
+    for (int i = lane; i < cells; i += 64) mine[i] = 0.0f;
+    const int steps = s.hp / kStep, units = *w.jobs * steps;
+    const int waves = shares * kWaves, each = units / waves, more = units % waves;
+    const int index = blockIdx.y * kWaves + wave;
+    const int from = index * each + (index < more ? index : more), to = from + each + (index < more ? 1 : 0);
     const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
-    for (int n = 0; n < jobs; ++n) {
-        const Job& job = w.job[n];
-        const int token = job.token[r];
-        const float gate = job.gate[r];
-        const long long first = static_cast<long long>(job.expert) * s.d;
-        long long rows[kTiles];
-        f32x4 acc[kTiles];
+
+    const auto rows_of = [&](int expert, long long (&rows)[kTiles]) {
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
             const int col = d0 + 16 * i + r;
-            rows[i] = first + (col < s.d ? col : s.d - 1);
-            acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            rows[i] = static_cast<long long>(expert) * s.d + (col < s.d ? col : s.d - 1);
+        }
+    };
+    int u = from;
+    while (u < to) {
+        const int n = u / steps, last = (n + 1) * steps < to ? (n + 1) * steps : to;
+        const Job& job = w.job[n];
+        const int expert = job.expert, token = job.token[r];
+        const float gate = job.gate[r];
+        long long rows[kTiles];
+        rows_of(expert, rows);
+        f32x4 acc[kTiles];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (b2 != nullptr && u == n * steps) {  // the job's first step brings the bias
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int c = d0 + 16 * i + 4 * q + v;
+                    if (c < s.d) acc[i][v] = b2[static_cast<long long>(expert) * s.d + c];
+                }
         }
         const unsigned short* col = w.h + (static_cast<long long>(n) * 16 + r) * s.hp;
-        for (int t = wave; t < s.hp / kStep; t += kWaves)
-            multiply_step<kType, kP, kTiles>(w2, rows, col, h_plane, token != kNone, t, q, acc);
-        if (token == kNone) continue;
+        typename Weights<kType>::Step now[kTiles], next[kTiles];
+        load_step<kType, kTiles>(w2, rows, u - n * steps, q, now);
+        for (; u < last; ++u) {
+            if (u + 1 < last) load_step<kType, kTiles>(w2, rows, u + 1 - n * steps, q, next);
+            multiply_step<kType, kP, kTiles>(now, col, h_plane, token != kNone, u - n * steps, q, acc);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i)
+            for (int i = 0; i < kTiles; ++i) now[i] = next[i];
+        }
+        if (token != kNone) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int c = 16 * i + 4 * q + v;
-                float o = acc[i][v];
-                if (b2 != nullptr && wave == 0 && d0 + c < s.d) o += b2[first + d0 + c];
-                tile[wave][token][c] += gate * o;
-            }
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mine[token * kCols + 16 * i + 4 * q + v] += gate * acc[i][v];
+        }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < s.tokens * kCols; i += kThreads) {
+    const long long row = static_cast<long long>(gridDim.x) * kCols, plane = s.tokens * row;
+    for (int i = threadIdx.x; i < cells; i += kThreads) {
         const int t = i / kCols, c = i % kCols;
-        if (d0 + c >= s.d) continue;
         float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) sum += tile[v][t][c];
+        for (int v = 0; v < kWaves; ++v) sum += tile[v * cells + i];
+        if (shares > 1)
+            mc_split_store(w.y + blockIdx.y * plane + t * row + d0 + c, sum);
+        else if (d0 + c < s.d)
+            store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum);
+    }
+    if (shares == 1 || !mc_split_last_arrival(w.arrived + 1 + blockIdx.x, shares, &flag)) return;
+    for (int i = threadIdx.x; i < cells; i += kThreads) {
+        const int t = i / kCols, c = i % kCols;
+        if (d0 + c >= s.d) continue;
+        const float* at = w.y + t * row + d0 + c;
+        float sum = mc_split_load(at);
+        for (int v = 1; v < shares; ++v) sum += mc_split_load(at + v * plane);
         store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum);
     }
 }
@@ -462,18 +533,19 @@ __global__ __launch_bounds__(kThreads) void moe_down(Weights<kType> w2, const fl
 
 template <int kType>
 Weights<kType> weights(const void* base, const void* scales, int k) {
-    return {base, static_cast<const unsigned char*>(scales), k, padded(k), k % 8 == 0 && aligned(base, 16)};
+    return {base, static_cast<const unsigned char*>(scales), k, padded(k)};
 }
 
 template <int kIn, int kType, int kAct>
 int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, hipStream_t stream) {
     constexpr int kHP = kIn == kF32 ? 3 : 2;
-    constexpr int kCols = kAct == MCHIP_MOE_SWIGLU ? 16 : 32;
+    constexpr int kUpCols = kAct == MCHIP_MOE_SWIGLU ? 16 : 32;
     hipLaunchKernelGGL((moe_up<kType, kPieces<kIn>, kHP, kAct>),
-                       dim3(static_cast<unsigned>(s.hp / kCols), static_cast<unsigned>(s.max_jobs)), dim3(kThreads), 0,
+                       dim3(static_cast<unsigned>(s.hp / kUpCols), static_cast<unsigned>(s.max_jobs)), dim3(kThreads), 0,
                        stream, weights<kType>(a.w1, a.w1_scales, s.d), a.b1, w, s);
-    hipLaunchKernelGGL((moe_down<kType, kHP, kIn>), dim3(static_cast<unsigned>((s.d + 31) / 32)), dim3(kThreads), 0,
-                       stream, weights<kType>(a.w2, a.w2_scales, s.h), a.b2, w, s, a.y);
+    hipLaunchKernelGGL((moe_down<kType, kHP, kIn>), 
+                       dim3(static_cast<unsigned>(column_tiles(s.d)), static_cast<unsigned>(down_shares(s))),
+                       dim3(kThreads), sizeof(float) * kWaves * s.tokens * kCols, stream, weights<kType>(a.w2, a.w2_scales, s.h), a.b2, w, s, a.y);
     return hipGetLastError();
 }
 
@@ -490,8 +562,9 @@ int launch(const mchip_moe_args& a, hipStream_t stream) {
     Workspace w;
     lay_out(s, a.dtype, static_cast<unsigned char*>(a.workspace), &w);
     hipLaunchKernelGGL(moe_router<kIn>,
-                       dim3(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16)),
-                       dim3(kThreads), 0, stream, a.x, a.ldx, a.router, w, s, a.normalize != 0, a.chosen, a.gates);
+                       dim3(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16),
+                            static_cast<unsigned>(router_parts(s.d))),
+                       dim3(kThreads), sizeof(float) * s.tokens * s.experts, stream, a.x, a.ldx, a.router, w, s, a.normalize != 0, a.chosen, a.gates);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.weights == kBf16) return launch_act<kIn, kBf16>(a, w, s, stream);
@@ -509,7 +582,7 @@ const char* refusal(const mchip_moe_args& a) {
     if (a.experts > kMaxExperts) return "more than 512 experts";
     if (a.top_k > kMaxTopK) return "more than 16 experts for a token";
     if (a.top_k > a.experts) return "more experts for a token than there are";
-    if (a.d > (1 << 20) || a.h > (1 << 20)) return "rows longer than 2^20";
+    if (a.d > kMaxWidth || a.h > kMaxWidth) return "rows longer than 2^20";
     if (a.ldx < a.d) return "rows of x closer together than they are long";
     if (!a.x || !a.router || !a.w1 || !a.w2 || !a.y || !a.workspace) return "a null operand";
     if (a.weights == kMx4 && (!a.w1_scales || !a.w2_scales)) return "mx4 weights without scales";
@@ -526,8 +599,8 @@ const char* refusal(const mchip_moe_args& a) {
 extern "C" {
 
 long long mchip_moe_workspace_bytes(int dtype, int tokens, int d, int h, int experts, int top_k) {
-    if (!is_float_type(dtype) || tokens < 1 || tokens > kMaxTokens || d < 1 || h < 1 || d > (1 << 20) ||
-        h > (1 << 20) || experts < 1 || experts > kMaxExperts || top_k < 1 || top_k > kMaxTopK)
+    if (!is_float_type(dtype) || tokens < 1 || tokens > kMaxTokens || d < 1 || h < 1 || d > kMaxWidth ||
+        h > kMaxWidth || experts < 1 || experts > kMaxExperts || top_k < 1 || top_k > kMaxTopK)
         return 0;
     Workspace w;
     return static_cast<long long>(lay_out(sizes_of(tokens, d, h, experts, top_k), dtype, nullptr, &w));

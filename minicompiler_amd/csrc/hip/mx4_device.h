@@ -82,18 +82,23 @@ __device__ __forceinline__ void store_one(void* p, long long i, float v) {
         static_cast<unsigned short*>(p)[i] = to_16<kType>(v);
 }
 
-// Four consecutive elements of a row of C at element `at`; `wide`: the row
-// has all four and the address is aligned to them.
+// Vectors at any address of their elements (one load all the same).
+typedef f32x4 f32x4_loose __attribute__((aligned(4)));
+typedef u16x8 u16x8_loose __attribute__((aligned(2)));
+typedef u32x4 u32x4_loose __attribute__((aligned(2)));
+typedef u16x4 u16x4_loose __attribute__((aligned(2)));
+
+// The first `left` of four consecutive elements of a row of C at element `at`.
 template <int kType>
-__device__ __forceinline__ void store_four(void* c, long long at, f32x4 v, int left, bool wide) {
-    if (wide) {
+__device__ __forceinline__ void store_four(void* c, long long at, f32x4 v, int left) {
+    if (left >= 4) {
         if constexpr (kType == kF32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(c) + at) = v;
+            *reinterpret_cast<f32x4_loose*>(static_cast<float*>(c) + at) = v;
         } else {
             u16x4 h;
 #pragma unroll
             for (int e = 0; e < 4; ++e) h[e] = to_16<kType>(v[e]);
-            *reinterpret_cast<u16x4*>(static_cast<unsigned short*>(c) + at) = h;
+            *reinterpret_cast<u16x4_loose*>(static_cast<unsigned short*>(c) + at) = h;
         }
         return;
     }
@@ -102,13 +107,12 @@ __device__ __forceinline__ void store_four(void* c, long long at, f32x4 v, int l
         if (e < left) store_one<kType>(c, at + e, v[e]);
 }
 
-// Eight consecutive elements from element `at` as fp32, zeros from `left` on;
-// `wide`: the address is aligned to 16 bytes.
+// Eight consecutive elements from element `at` as fp32, zeros from `left` on.
 template <int kType>
-__device__ __forceinline__ void load_eight(const void* p, long long at, int left, bool wide, float (&v)[8]) {
-    if (wide && left >= 8) {
+__device__ __forceinline__ void load_eight(const void* p, long long at, int left, float (&v)[8]) {
+    if (left >= 8) {
         if constexpr (kType == kF32) {
-            const f32x4* s = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+            const f32x4_loose* s = reinterpret_cast<const f32x4_loose*>(static_cast<const float*>(p) + at);
             const f32x4 lo = s[0], hi = s[1];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -116,7 +120,7 @@ __device__ __forceinline__ void load_eight(const void* p, long long at, int left
                 v[4 + e] = hi[e];
             }
         } else {
-            const u16x8 s = *reinterpret_cast<const u16x8*>(static_cast<const unsigned short*>(p) + at);
+            const u16x8 s = *reinterpret_cast<const u16x8_loose*>(static_cast<const unsigned short*>(p) + at);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = to_f32<kType>(s[e]);
         }
@@ -124,6 +128,45 @@ __device__ __forceinline__ void load_eight(const void* p, long long at, int left
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = e < left ? load_one<kType>(p, at + e) : 0.0f;
+}
+
+// Four.
+template <int kType>
+__device__ __forceinline__ f32x4 load_four(const void* p, long long at, int left) {
+    f32x4 v;
+    if (left >= 4) {
+        if constexpr (kType == kF32) return *reinterpret_cast<const f32x4_loose*>(static_cast<const float*>(p) + at);
+        const u16x4 s = *reinterpret_cast<const u16x4_loose*>(static_cast<const unsigned short*>(p) + at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = to_f32<kType>(s[e]);
+        return v;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < left ? load_one<kType>(p, at + e) : 0.0f;
+    return v;
+}
+
+// Reductions over the 64 lanes, the result in every lane (as a scalar).
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#define MX4_STEP(ctrl, rows)                                                                                     \
+    {                                                                                                            \
+        const unsigned o =                                                                                       \
+            static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xf, false)); \
+        v = v > o ? v : o;                                                                                       \
+    }
+    MX4_STEP(0x111, 0xf) MX4_STEP(0x112, 0xf) MX4_STEP(0x114, 0xf) MX4_STEP(0x118, 0xf)
+    MX4_STEP(0x142, 0xa) MX4_STEP(0x143, 0xc)
+#undef MX4_STEP
+    return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+__device__ __forceinline__ unsigned wave_min(unsigned v) { return ~wave_max(~v); }
+__device__ __forceinline__ float wave_sum(float v) {
+#define MX4_STEP(ctrl, rows) \
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false));
+    MX4_STEP(0x111, 0xf) MX4_STEP(0x112, 0xf) MX4_STEP(0x114, 0xf) MX4_STEP(0x118, 0xf)
+    MX4_STEP(0x142, 0xa) MX4_STEP(0x143, 0xc)
+#undef MX4_STEP
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // The high halves of two registers in one (a: low half).

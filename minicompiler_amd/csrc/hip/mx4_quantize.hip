@@ -52,17 +52,17 @@ __device__ __forceinline__ void decode_eight_f32(unsigned codes, unsigned scale,
 // Eight values of row `row` from element `at` on (exact in x's type: a code is
 // never finer than the numbers it was rounded from).
 template <int kType>
-__device__ __forceinline__ void store_eight(void* p, long long at, const float (&v)[8], int left, bool wide) {
-    if (wide && left >= 8) {
+__device__ __forceinline__ void store_eight(void* p, long long at, const float (&v)[8], int left) {
+    if (left >= 8) {
         if constexpr (kType == kF32) {
-            f32x4* d = reinterpret_cast<f32x4*>(static_cast<float*>(p) + at);
+            f32x4_loose* d = reinterpret_cast<f32x4_loose*>(static_cast<float*>(p) + at);
             d[0] = f32x4{v[0], v[1], v[2], v[3]};
             d[1] = f32x4{v[4], v[5], v[6], v[7]};
         } else {
             u16x8 h;
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] = to_16<kType>(v[e]);
-            *reinterpret_cast<u16x8*>(static_cast<unsigned short*>(p) + at) = h;
+            *reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(p) + at) = h;
         }
         return;
     }
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict
                                                           unsigned* __restrict__ codes,
                                                           unsigned char* __restrict__ scales,
                                                           void* __restrict__ values, long long rows, int k,
-                                                          unsigned per_row, bool wide, bool wide_values) {
+                                                          unsigned per_row) {
     const long long first = static_cast<long long>(blockIdx.x) * kThreads;
     const long long row0 = first / per_row;
     const unsigned in_row = static_cast<unsigned>(first - row0 * per_row) + threadIdx.x;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict
     if (row >= rows) return;  // whole blocks of lanes: a row has a multiple of 16 chunks
     const int left = k - static_cast<int>(chunk) * 8;
     float v[8];
-    load_eight<kType>(x, row * ld + chunk * 8, left, wide, v);
+    load_eight<kType>(x, row * ld + chunk * 8, left, v);
     unsigned top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict
     if (chunk % 4 == 0) scales[row * (per_row / 4) + chunk / 4] = static_cast<unsigned char>(s);
     if (values != nullptr && left > 0) {
         decode_eight_f32(c, s, v);
-        store_eight<kType>(values, row * k + chunk * 8, v, left, wide_values);
+        store_eight<kType>(values, row * k + chunk * 8, v, left);
     }
 }
 
@@ -181,12 +181,9 @@ int launch_rows(const void* x, long long ld, void* codes, void* scales, int rows
         *why = "more elements than one launch takes (2^42)";
         return hipErrorInvalidValue;
     }
-    const int unit = 16 / kSize<kType>;
-    const bool wide = aligned(x, 16) && ld % unit == 0;
-    const bool wide_values = aligned(values, 16) && k % unit == 0;
     hipLaunchKernelGGL(quantize_rows<kType>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, x, ld,
                        static_cast<unsigned*>(codes), static_cast<unsigned char*>(scales), values,
-                       static_cast<long long>(rows), k, per_row, wide, wide_values);
+                       static_cast<long long>(rows), k, per_row);
     return hipGetLastError();
 }
 
