@@ -43,8 +43,8 @@ struct Workspace {
     int* jobs;          // how many
     Job* job;           // [max_jobs]
     float* logits;      // [parts][tokens, experts]
-    unsigned short* x;  // [pieces][tokens][dp]
-    unsigned short* h;  // [pieces][max_jobs * 16][hp]
+    unsigned short* x;  // [pieces][dp / 8][tokens][8]: a token's eight elements beside its neighbours'
+    unsigned short* h;  // [pieces][max_jobs][hp / 8][16][8]
     float* y;           // [shares][tokens][column tiles * 32]
 };
 
@@ -69,15 +69,15 @@ int router_parts(int d) { return std::min((d + 64 * kWaves - 1) / (64 * kWaves),
 
 int column_tiles(int d) { return (d + kCols - 1) / kCols; }
 
-// The shares that a column tile of y is cut into: two blocks per CU in all, as
-// long as a wave has a step to do.
+// The shares that a column tile of y is cut into: a block for each CU (the
+// kernel's registers leave room for one), as long as a wave has a step to do.
 int down_shares(const Sizes& s) {
-    const int want = 2 * device_cus() / column_tiles(s.d);
+    const int want = device_cus() / column_tiles(s.d);
     const int most = (s.max_jobs * (s.hp / kStep) + kWaves - 1) / kWaves;
     return std::max(1, std::min({want, most, 64}));
 }
 
-int pieces_of(int dtype) { return dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1; }
+int pieces_of(int dtype) { return dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1; }  // at most
 // h is an fp32 sum: 24 bits of it for an fp32 result, 16 otherwise.
 int h_pieces_of(int dtype) { return dtype == kF32 ? 3 : 2; }
 
@@ -105,55 +105,92 @@ std::size_t lay_out(const Sizes& s, int dtype, unsigned char* base, Workspace* w
 
 // ---------------------------------------------------------------- router
 
-// One token's experts and gates, by one wave, from its logits in LDS. Logits are
-// compared as unsigned numbers in the order of the floats, from 2 up; a NaN
-// counts as 1, smaller than all, and a chosen one as 0. A NaN makes every gate
-// NaN, as softmax does.
-__device__ void choose(const float* logits, int experts, int top_k, bool normalize, int lane, int* chosen, float* gate) {
-    constexpr int kEach = kMaxExperts / 64;
-    unsigned key[kEach];
-    unsigned best = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        key[j] = 0;
-        if (64 * j >= experts) continue;
-        const int e = lane + 64 * j;
-        if (e < experts) {
-            const float l = logits[e] + 0.0f;  // -0 to 0
-            const unsigned u = __builtin_bit_cast(unsigned, l);
-            key[j] = l != l ? 1u : u >> 31 ? ~u : u | 0x80000000u;
-        }
-        best = key[j] > best ? key[j] : best;
-    }
-    const unsigned first = wave_max(best);
-    const float top = __builtin_bit_cast(float, first >> 31 ? first & 0x7fffffffu : ~first);
+// parts[0] + parts[plane] + ... (`count` of them, in order), written by other
+// blocks. Eight loads at a time are under way: one after the other, 16 of them
+// took 16 us.
+__device__ __forceinline__ float add_parts(const float* parts, long long plane, int count) {
     float sum = 0.0f;
+    for (int v = 0; v < count; v += 8) {
+        float part[8];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
-        if (64 * j < experts && lane + 64 * j < experts) sum += expf(logits[lane + 64 * j] - top);
-    sum = wave_sum(sum);
-    float kept = 0.0f, mine = 0.0f;
-    for (int i = 0; i < top_k; ++i) {
-        unsigned most = 0, at = 0xffffffffu;
+        for (int j = 0; j < 8; ++j) part[j] = v + j < count ? mc_split_load(parts + (v + j) * plane) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (v + j < count) sum += part[j];
+    }
+    return sum;
+}
+
+// The experts and gates of kTokens tokens from `first` on, by one wave, from
+// their logits in LDS; kEach: experts per lane. Logits are compared as unsigned
+// numbers in the order of the floats, from 2 up; a NaN counts as 1, smaller than
+// all, and a chosen one as 0. A NaN makes every gate NaN, as softmax does. A
+// reduction over the wave is a chain of dependent instructions: several tokens'
+// chains go side by side.
+template <int kEach, int kTokens>
+__device__ void choose(const float* logits, int first, const Sizes& s, bool normalize, int lane,
+                       int (*chosen)[kMaxTopK], float (*gate)[kMaxTopK]) {
+    unsigned key[kTokens][kEach];
+    float top[kTokens], sum[kTokens];
+    int mine[kTokens];  // lane i: the i-th expert
+#pragma unroll
+    for (int n = 0; n < kTokens; ++n) {
+        const int t = first + n < s.tokens ? first + n : s.tokens - 1;
+        float l[kEach];
+        unsigned best = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int e = lane + 64 * j;
+            l[j] = e < s.experts ? logits[t * s.experts + e] + 0.0f : 0.0f;  // -0 to 0
+            const unsigned u = __builtin_bit_cast(unsigned, l[j]);
+            key[n][j] = e >= s.experts ? 0u : l[j] != l[j] ? 1u : u >> 31 ? ~u : u | 0x80000000u;
+            best = key[n][j] > best ? key[n][j] : best;
+        }
+        const unsigned most = wave_max(best);
+        top[n] = __builtin_bit_cast(float, most >> 31 ? most & 0x7fffffffu : ~most);
+        float part = 0.0f;
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
-            if (64 * j < experts && key[j] > most) {
-                most = key[j];
-                at = static_cast<unsigned>(lane + 64 * j);
-            }
-        const unsigned winner = wave_max(most);
-        const unsigned e = wave_min(most == winner ? at : 0xffffffffu);
+            if (lane + 64 * j < s.experts) part += expf(l[j] - top[n]);
+        sum[n] = wave_sum(part);
+        mine[n] = 0;
+    }
+    for (int i = 0; i < s.top_k; ++i) {
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
-            if (e == static_cast<unsigned>(lane + 64 * j)) key[j] = 0;
-        const float p = expf(logits[e] - top) / sum;
-        kept += p;
-        if (lane == i) {
-            mine = p;
-            chosen[i] = static_cast<int>(e);
+        for (int n = 0; n < kTokens; ++n) {
+            unsigned most = 0, at = 0xffffffffu;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+                if (key[n][j] > most) {
+                    most = key[n][j];
+                    at = static_cast<unsigned>(lane + 64 * j);
+                }
+            const unsigned winner = wave_max(most);
+            const unsigned e = wave_min(most == winner ? at : 0xffffffffu);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+                if (e == static_cast<unsigned>(lane + 64 * j)) key[n][j] = 0;
+            if (lane == i) mine[n] = static_cast<int>(e);
         }
     }
-    if (lane < top_k) gate[lane] = normalize ? mine / kept : mine;
+#pragma unroll
+    for (int n = 0; n < kTokens; ++n) {
+        const int t = first + n;
+        if (t >= s.tokens) break;
+        const float p = lane < s.top_k ? expf(logits[t * s.experts + mine[n]] - top[n]) / sum[n] : 0.0f;
+        const float kept = wave_sum(p);
+        if (lane < s.top_k) {
+            chosen[t][lane] = mine[n];
+            gate[t][lane] = normalize ? p / kept : p;
+        }
+    }
+}
+
+template <int kEach, int kTokens>
+__device__ __forceinline__ void choose_all(const float* logits, const Sizes& s, bool normalize, int wave, int lane,
+                                           int (*chosen)[kMaxTopK], float (*gate)[kMaxTopK]) {
+    for (int t = wave * kTokens; t < s.tokens; t += kWaves * kTokens)
+        choose<kEach, kTokens>(logits, t, s, normalize, lane, chosen, gate);
 }
 
 // The jobs from the chosen experts in LDS, by the whole block: a thread per
@@ -197,7 +234,7 @@ __device__ void list_jobs(const Workspace& w, const Sizes& s, const int (*chosen
 // 16 experts by 16 tokens of the logits over one part of d, 64 elements at a time
 // for each wave. v_mfma_f32_16x16x4_f32: lane (r, q) supplies row or column r,
 // element q; here a lane's four elements go to four instructions.
-template <int kIn>
+template <int kIn, bool kHalf>
 __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ x, long long ldx,
                                                        const float* __restrict__ router, Workspace w, Sizes s,
                                                        bool normalize, int* __restrict__ chosen_out,
@@ -241,28 +278,35 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
             if (e0 + 4 * q + v < s.experts) mc_split_store(out + v, acc[0][v]);
     }
 
-    // x in pieces, rows padded with zeros, shared out over the blocks.
-    const long long all = static_cast<long long>(s.tokens) * s.dp;
-    for (long long i = (static_cast<long long>(block) * kThreads + threadIdx.x) * 8; i < all;
-         i += static_cast<long long>(blocks) * kThreads * 8) {
-        const int t = static_cast<int>(i / s.dp), k = static_cast<int>(i % s.dp);
+    // x in pieces, padded with zeros, shared out over the blocks.
+    const int chunks = s.tokens * (s.dp / 8);
+    for (int i = block * kThreads + threadIdx.x; i < chunks; i += blocks * kThreads) {
+        const int t = i % s.tokens, k = i / s.tokens * 8;
         float v[8];
         load_eight<kIn>(x, t * ldx + k, s.d - k, v);
+        if constexpr (kHalf) {
+            u16x8 same;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) same[e] = to_16<kF16>(v[e]);
+            *reinterpret_cast<u16x8*>(w.x + static_cast<long long>(i) * 8) = same;
+            continue;
+        }
         u32x4 out[kP];
         cut_eight<kP>(v, out);
 #pragma unroll
-        for (int p = 0; p < kP; ++p) *reinterpret_cast<u32x4*>(w.x + p * all + i) = out[p];
+        for (int p = 0; p < kP; ++p)
+            *reinterpret_cast<u32x4*>(w.x + (static_cast<long long>(p) * chunks + i) * 8) = out[p];
     }
 
     if (!mc_split_last_arrival(w.arrived, blocks, &flag)) return;
-    for (int i = threadIdx.x; i < all_logits; i += kThreads) {
-        float sum = mc_split_load(w.logits + i);
-        for (int z = 1; z < parts; ++z) sum += mc_split_load(w.logits + z * all_logits + i);
-        logits[i] = sum;
-    }
+    for (int i = threadIdx.x; i < all_logits; i += kThreads) logits[i] = add_parts(w.logits + i, all_logits, parts);
     __syncthreads();
-    for (int t = wave; t < s.tokens; t += kWaves)
-        choose(logits + t * s.experts, s.experts, s.top_k, normalize, lane, chosen[t], gate[t]);
+    if (s.experts > 128)
+        choose_all<kMaxExperts / 64, 1>(logits, s, normalize, wave, lane, chosen, gate);
+    else if (s.experts > 64 || s.tokens <= kWaves)
+        choose_all<2, 1>(logits, s, normalize, wave, lane, chosen, gate);
+    else
+        choose_all<1, 4>(logits, s, normalize, wave, lane, chosen, gate);
     __syncthreads();
     list_jobs(w, s, chosen, gate, mask, place);
     for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads) {
@@ -274,98 +318,161 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
 
 // ---------------------------------------------------------------- experts' products
 
-// Rows of an expert's weights in steps of 128: lane (r, q) supplies row r in
-// four instructions s. 16-bit rows: elements 32 s + 8 q .. + 7 of the step
-// (whole 64-byte pieces per instruction); mx4: 32 q + 8 s .. + 7 (block q of
-// the step is the lane's own 16 bytes).
-template <int kType>
-struct Weights {
-    static constexpr int kPiecesW = kType == kF16 ? 2 : 1;
-    const void* base;
-    const unsigned char* scales;
-    int k, kp;
-
-    __device__ __forceinline__ static int offset(int q, int s) { return kType == kMx4 ? 32 * q + 8 * s : 32 * s + 8 * q; }
+// kTiles tiles of 16 rows of an expert's weights and 16 tokens' pieces, in steps
+// of 128 elements. Lane (r, q) supplies row and token r in four instructions s:
+// of 16-bit rows elements 32 s + 8 q .. + 7 of the step (whole 64-byte pieces per
+// load), of mx4 ones 32 q + 8 s .. + 7 (block q of the step is its 16 bytes).
+// kOdd: 16-bit rows that start at odd elements, or some of them. Loads at odd
+// elements halved the rate (101 MB of W1 in 61 us, 30 with even rows): a lane
+// takes the whole dwords that its elements lie in, and shifts.
+// kHalf: fp16 rows and tokens multiplied as they are.
+template <int kType, int kTiles, int kP, bool kOdd, bool kHalf>
+struct Stream {
+    static constexpr bool kQuant = kType == kMx4;
+    static constexpr int kPiecesW = kType == kF16 && !kHalf ? 2 : 1;
+    static constexpr int kRaw = kQuant ? 1 : 4;
 
     struct Step {
-        u32x4 raw[4];
-        float scale;
+        u32x4 w[kTiles][kRaw];
+        unsigned more[kTiles][kOdd ? kRaw : 1];  // the dword behind w
+        unsigned scales;  // lane 16 i + r: of row r of tile i
+        u32x4 x[4][kP];
     };
 
-    __device__ __forceinline__ Step load(long long row, int t, int q) const {
-        Step st;
-        if constexpr (kType == kMx4) {
-            st.raw[0] = *reinterpret_cast<const u32x4*>(static_cast<const unsigned char*>(base) + row * (kp / 2) +
-                                                        t * 64 + q * 16);
-            st.scale = scale_operand(scales[row * (kp / 32) + t * 4 + q]);
+    const unsigned char* rows[kTiles];  // lane's, mx4: at its block
+    const unsigned char* scale_row;
+    int shift[kTiles];
+    const unsigned short* x;  // lane's token, at its chunk
+    long long x_plane, x_chunk;
+    int k, r, q;
+    bool has;
+
+    __device__ __forceinline__ static int offset(int q, int s) { return kQuant ? 32 * q + 8 * s : 32 * s + 8 * q; }
+
+    // row_of(i): the row of the weights that lane has in tile i.
+    template <typename Rows>
+    __device__ __forceinline__ void open(const void* base, const unsigned char* scales, int k_, Rows row_of) {
+        const int lane = threadIdx.x % 64;
+        r = lane % 16, q = lane / 16, k = k_;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            const long long row = row_of(i);
+            if constexpr (kQuant) {
+                rows[i] = static_cast<const unsigned char*>(base) + row * (padded(k) / 2) + q * 16;
+                if (q == i) scale_row = scales + row * (padded(k) / 32);
+            } else {
+                const unsigned char* p = static_cast<const unsigned char*>(base) + row * k * 2;
+                shift[i] = kOdd ? static_cast<int>(reinterpret_cast<std::uintptr_t>(p) & 2) : 0;
+                rows[i] = p - shift[i];
+            }
+        }
+    }
+
+    // Chunks of eight elements of a token, `chunk` apart, in pieces `plane` apart; has: there is a token.
+    __device__ __forceinline__ void tokens(const unsigned short* p, long long chunk, long long plane, bool has_) {
+        x = p, x_chunk = chunk, x_plane = plane, has = has_;
+    }
+
+    __device__ __forceinline__ void load(int t, Step& st) const {
+        if constexpr (kQuant) {
+            static_assert(kTiles <= 4);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+                st.w[i][0] = *reinterpret_cast<const u32x4*>(rows[i] + static_cast<long long>(t) * 64);
+            // A dword per row from one lane each, shared out later: a byte per
+            // lane would be as many accesses as the codes.
+            if (q < kTiles) st.scales = *reinterpret_cast<const unsigned*>(scale_row + t * 4);
         } else {
-            const unsigned short* p = static_cast<const unsigned short*>(base) + row * k;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k0 = t * kStep + offset(q, s);
-                if (k0 + 8 <= k) {
-                    st.raw[s] = *reinterpret_cast<const u32x4_loose*>(p + k0);
-                } else {
+            for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const unsigned lo = k0 + 2 * j < k ? p[k0 + 2 * j] : 0u;
-                        const unsigned hi = k0 + 2 * j + 1 < k ? p[k0 + 2 * j + 1] : 0u;
-                        st.raw[s][j] = lo | hi << 16;
+                for (int s = 0; s < 4; ++s) {
+                    const int k0 = t * kStep + offset(q, s);
+                    const unsigned char* p = rows[i] + k0 * 2;
+                    if (k0 + 8 <= k) {
+                        st.w[i][s] = *reinterpret_cast<const u32x4_dwords*>(p);
+                        // Unshifted lanes take the last dword again: the next may lie past the weights.
+                        if constexpr (kOdd) st.more[i][s] = *reinterpret_cast<const unsigned*>(p + 12 + 2 * shift[i]);
+                    } else {
+                        unsigned e[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            e[j] = k0 + j < k ? *reinterpret_cast<const unsigned short*>(p + shift[i] + 2 * j) : 0u;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) st.w[i][s][j] = e[2 * j] | e[2 * j + 1] << 16;
+                        if constexpr (kOdd) {  // as if loaded shifted
+                            if (shift[i] != 0) {
+                                st.more[i][s] = e[7];
+#pragma unroll
+                                for (int j = 3; j > 0; --j) st.w[i][s][j] = e[2 * j - 1] | e[2 * j] << 16;
+                                st.w[i][s][0] = e[0] << 16;
+                            }
+                        }
                     }
                 }
             }
         }
-        return st;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int p = 0; p < kP; ++p)
+                st.x[s][p] = has ? *reinterpret_cast<const u32x4*>(x + p * x_plane + (t * kStep + offset(q, s)) / 8 * x_chunk)
+                                 : u32x4{0, 0, 0, 0};
     }
 
-    __device__ __forceinline__ static void operand(const Step& st, int s, u32x4 (&out)[kPiecesW]) {
-        if constexpr (kType == kMx4) {
-            out[0] = decode_eight(st.raw[0][s], st.scale);
-        } else if constexpr (kType == kBf16) {
-            out[0] = st.raw[s];
-        } else {
-            float v[8];
+    __device__ __forceinline__ void multiply(const Step& st, f32x4 (&acc)[kTiles]) const {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[2 * j] = to_f32<kF16>(st.raw[s][j] & 0xffffu);
-                v[2 * j + 1] = to_f32<kF16>(st.raw[s][j] >> 16);
+        for (int i = 0; i < kTiles; ++i) {
+            float scale = 0.0f;
+            if constexpr (kQuant) {
+                const int of_row = __builtin_amdgcn_ds_bpermute((16 * i + r) * 4, static_cast<int>(st.scales));
+                scale = scale_operand(static_cast<unsigned>(of_row) >> (8 * q) & 255u);
             }
-            cut_eight<2>(v, out);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                u32x4 w[kPiecesW];
+                if constexpr (kQuant) {
+                    w[0] = decode_eight(st.w[i][0][s], scale);
+                } else {
+                    u32x4 raw = st.w[i][s];
+                    if constexpr (kOdd) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            raw[j] = __builtin_amdgcn_alignbyte(j < 3 ? st.w[i][s][j + 1] : st.more[i][s], raw[j], shift[i]);
+                    }
+                    if constexpr (kType == kBf16 || kHalf) {
+                        w[0] = raw;
+                    } else {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            v[2 * j] = to_f32<kF16>(raw[j] & 0xffffu);
+                            v[2 * j + 1] = to_f32<kF16>(raw[j] >> 16);
+                        }
+                        cut_eight<2>(v, w);
+                    }
+                }
+#pragma unroll
+                for (int wp = 0; wp < kPiecesW; ++wp)
+#pragma unroll
+                    for (int p = 0; p < kP; ++p)
+                        acc[i] = kHalf ? mfma_f16(w[wp], st.x[s][p], acc[i]) : mfma_bf16(w[wp], st.x[s][p], acc[i]);
+            }
+        }
+    }
+
+    // acc[i] += steps from, from + by, .. below to; one step is under way while another is multiplied.
+    __device__ __forceinline__ void run(int from, int to, int by, f32x4 (&acc)[kTiles]) const {
+        if (from >= to) return;
+        Step now, next;
+        load(from, now);
+        for (int t = from; t < to; t += by) {
+            if (t + by < to) load(t + by, next);
+            multiply(now, acc);
+            now = next;
         }
     }
 };
-
-template <int kType, int kTiles>
-__device__ __forceinline__ void load_step(const Weights<kType>& w, const long long (&rows)[kTiles], int t, int q,
-                                          typename Weights<kType>::Step (&st)[kTiles]) {
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) st[i] = w.load(rows[i], t, q);
-}
-
-// acc[i] += step t of 16 weight rows, loaded, times the columns `col` (a lane's
-// own row of the pieces, `plane` elements apart; has: there is one).
-template <int kType, int kP, int kTiles>
-__device__ __forceinline__ void multiply_step(const typename Weights<kType>::Step (&st)[kTiles],
-                                              const unsigned short* col, long long plane, bool has, int t, int q,
-                                              f32x4 (&acc)[kTiles]) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        u32x4 x[kP];
-        const int k0 = t * kStep + Weights<kType>::offset(q, s);
-#pragma unroll
-        for (int p = 0; p < kP; ++p)
-            x[p] = has ? *reinterpret_cast<const u32x4*>(col + p * plane + k0) : u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-            u32x4 a[Weights<kType>::kPiecesW];
-            Weights<kType>::operand(st[i], s, a);
-#pragma unroll
-            for (int wp = 0; wp < Weights<kType>::kPiecesW; ++wp)
-#pragma unroll
-                for (int p = 0; p < kP; ++p) acc[i] = mfma_bf16(a[wp], x[p], acc[i]);
-        }
-    }
-}
 
 template <int kAct>
 __device__ __forceinline__ float activate(float u, float up) {
@@ -374,16 +481,17 @@ __device__ __forceinline__ float activate(float u, float up) {
     return 0.5f * u * (1.0f + tanhf(0.79788456080286536f * (u + 0.044715f * u * u * u)));
 }
 
-// A job's h for 16 kTiles (swiglu: 16) columns from blockIdx.x on. Columns from
-// h to hp are written as zeros.
-template <int kType, int kP, int kHP, int kAct>
-__global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const float* __restrict__ b1, Workspace w,
-                                                   Sizes s) {
+// A job's h for 32 (swiglu: 16) columns from blockIdx.x on. Columns from h to hp
+// are written as zeros.
+// kHalf: x was kept in fp16, as the weights are (one piece).
+template <int kType, int kP, int kHP, int kAct, bool kOdd, bool kHalf>
+__global__ __launch_bounds__(kThreads) void moe_up(const void* __restrict__ w1, const unsigned char* __restrict__ w1_scales,
+                                                   const float* __restrict__ b1, Workspace w, Sizes s) {
     constexpr bool kGated = kAct == MCHIP_MOE_SWIGLU;
     constexpr int kTiles = 2, kUpCols = kGated ? 16 : 32;
     __shared__ f32x4 space[kWaves / 2 * kTiles * 64];
     const Job& job = w.job[blockIdx.y];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
     const int h0 = blockIdx.x * kUpCols;
     // The job is read beside the number of jobs, not after it; past the last, it is not used.
@@ -391,27 +499,18 @@ __global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const floa
     if (static_cast<int>(blockIdx.y) >= jobs) return;
     const long long all_rows = kGated ? 2LL * s.h : s.h;
     const long long first = expert * all_rows;
-    long long rows[kTiles];
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-        const int col = h0 + (kGated ? 0 : 16 * i) + r;
-        rows[i] = first + (col < s.h ? col : s.h - 1) + (kGated && i == 1 ? s.h : 0);
-    }
     f32x4 acc[kTiles];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const long long plane = static_cast<long long>(s.tokens) * s.dp;
-    const unsigned short* col = w.x + static_cast<long long>(token == kNone ? 0 : token) * s.dp;
     if (h0 < s.h) {
-        const int steps = s.dp / kStep;
-        typename Weights<kType>::Step now[kTiles], next[kTiles];
-        if (wave < steps) load_step<kType, kTiles>(w1, rows, wave, q, now);
-        for (int t = wave; t < steps; t += kWaves) {
-            if (t + kWaves < steps) load_step<kType, kTiles>(w1, rows, t + kWaves, q, next);
-            multiply_step<kType, kP, kTiles>(now, col, plane, token != kNone, t, q, acc);
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) now[i] = next[i];
-        }
+        Stream<kType, kTiles, kP, kOdd, kHalf> in;
+        in.open(w1, w1_scales, s.d, [&](int i) {
+            const int col = h0 + (kGated ? 0 : 16 * i) + r;
+            return first + (col < s.h ? col : s.h - 1) + (kGated && i == 1 ? s.h : 0);
+        });
+        in.tokens(w.x + (token == kNone ? 0 : token) * 8, 8LL * s.tokens, static_cast<long long>(s.tokens) * s.dp,
+                  token != kNone);
+        in.run(wave, s.dp / kStep, kWaves, acc);
     }
     add_waves<kWaves, kTiles>(acc, space, wave, lane);
     if (wave != 0) return;
@@ -436,8 +535,8 @@ __global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const floa
         }
 #pragma unroll
         for (int p = 0; p < kHP; ++p)
-            *reinterpret_cast<u16x4*>(w.h + p * h_plane + (static_cast<long long>(blockIdx.y) * 16 + r) * s.hp + c0) =
-                out[p];
+            *reinterpret_cast<u16x4*>(w.h + p * h_plane + static_cast<long long>(blockIdx.y) * 16 * s.hp +
+                                      (c0 / 8 * 16 + r) * 8 + c0 % 8) = out[p];
     }
 }
 
@@ -445,13 +544,14 @@ __global__ __launch_bounds__(kThreads) void moe_up(Weights<kType> w1, const floa
 // in a row, cut evenly over the shares' waves). A wave adds each of its jobs'
 // parts, weighed, to its own LDS tile (no two lanes the same element); the tiles
 // are added in wave order, the shares in their order by the last block to arrive.
-template <int kType, int kP, int kOut>
-__global__ __launch_bounds__(kThreads) void moe_down(Weights<kType> w2, const float* __restrict__ b2, Workspace w,
-                                                     Sizes s, void* __restrict__ y) {
+template <int kType, int kP, int kOut, bool kOdd>
+__global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2, const unsigned char* __restrict__ w2_scales,
+                                                     const float* __restrict__ b2, Workspace w, Sizes s,
+                                                     void* __restrict__ y) {
     constexpr int kTiles = kCols / 16;
     extern __shared__ float tile[];  // [kWaves][tokens][kCols]
     __shared__ int flag;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
     const int d0 = blockIdx.x * kCols, shares = gridDim.y;
     const int cells = s.tokens * kCols;
@@ -463,21 +563,12 @@ __global__ __launch_bounds__(kThreads) void moe_down(Weights<kType> w2, const fl
     const int from = index * each + (index < more ? index : more), to = from + each + (index < more ? 1 : 0);
     const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
 
-    const auto rows_of = [&](int expert, long long (&rows)[kTiles]) {
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-            const int col = d0 + 16 * i + r;
-            rows[i] = static_cast<long long>(expert) * s.d + (col < s.d ? col : s.d - 1);
-        }
-    };
     int u = from;
     while (u < to) {
         const int n = u / steps, last = (n + 1) * steps < to ? (n + 1) * steps : to;
         const Job& job = w.job[n];
         const int expert = job.expert, token = job.token[r];
         const float gate = job.gate[r];
-        long long rows[kTiles];
-        rows_of(expert, rows);
         f32x4 acc[kTiles];
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -490,15 +581,14 @@ __global__ __launch_bounds__(kThreads) void moe_down(Weights<kType> w2, const fl
                     if (c < s.d) acc[i][v] = b2[static_cast<long long>(expert) * s.d + c];
                 }
         }
-        const unsigned short* col = w.h + (static_cast<long long>(n) * 16 + r) * s.hp;
-        typename Weights<kType>::Step now[kTiles], next[kTiles];
-        load_step<kType, kTiles>(w2, rows, u - n * steps, q, now);
-        for (; u < last; ++u) {
-            if (u + 1 < last) load_step<kType, kTiles>(w2, rows, u + 1 - n * steps, q, next);
-            multiply_step<kType, kP, kTiles>(now, col, h_plane, token != kNone, u - n * steps, q, acc);
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) now[i] = next[i];
-        }
+        Stream<kType, kTiles, kP, kOdd, false> in;
+        in.open(w2, w2_scales, s.h, [&](int i) {
+            const int col = d0 + 16 * i + r;
+            return static_cast<long long>(expert) * s.d + (col < s.d ? col : s.d - 1);
+        });
+        in.tokens(w.h + static_cast<long long>(n) * 16 * s.hp + r * 8, 16 * 8, h_plane, token != kNone);
+        in.run(u - n * steps, last - n * steps, 1, acc);
+        u = last;
         if (token != kNone) {
 #pragma unroll
             for (int i = 0; i < kTiles; ++i)
@@ -522,38 +612,42 @@ __global__ __launch_bounds__(kThreads) void moe_down(Weights<kType> w2, const fl
     for (int i = threadIdx.x; i < cells; i += kThreads) {
         const int t = i / kCols, c = i % kCols;
         if (d0 + c >= s.d) continue;
-        const float* at = w.y + t * row + d0 + c;
-        float sum = mc_split_load(at);
-        for (int v = 1; v < shares; ++v) sum += mc_split_load(at + v * plane);
+        const float sum = add_parts(w.y + t * row + d0 + c, plane, shares);
         store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum);
     }
 }
 
 // ---------------------------------------------------------------- launches
 
-template <int kType>
-Weights<kType> weights(const void* base, const void* scales, int k) {
-    return {base, static_cast<const unsigned char*>(scales), k, padded(k)};
-}
-
-template <int kIn, int kType, int kAct>
+template <int kIn, int kType, int kAct, bool kOdd>
 int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, hipStream_t stream) {
     constexpr int kHP = kIn == kF32 ? 3 : 2;
     constexpr int kUpCols = kAct == MCHIP_MOE_SWIGLU ? 16 : 32;
-    hipLaunchKernelGGL((moe_up<kType, kPieces<kIn>, kHP, kAct>),
+    constexpr bool kHalf = kIn == kF16 && kType == kF16;
+    hipLaunchKernelGGL((moe_up<kType, kHalf ? 1 : kPieces<kIn>, kHP, kAct, kOdd, kHalf>),
                        dim3(static_cast<unsigned>(s.hp / kUpCols), static_cast<unsigned>(s.max_jobs)), dim3(kThreads), 0,
-                       stream, weights<kType>(a.w1, a.w1_scales, s.d), a.b1, w, s);
-    hipLaunchKernelGGL((moe_down<kType, kHP, kIn>), 
+                       stream, a.w1, static_cast<const unsigned char*>(a.w1_scales), a.b1, w, s);
+    hipLaunchKernelGGL((moe_down<kType, kHP, kIn, kOdd>),
                        dim3(static_cast<unsigned>(column_tiles(s.d)), static_cast<unsigned>(down_shares(s))),
-                       dim3(kThreads), sizeof(float) * kWaves * s.tokens * kCols, stream, weights<kType>(a.w2, a.w2_scales, s.h), a.b2, w, s, a.y);
+                       dim3(kThreads), sizeof(float) * kWaves * s.tokens * kCols, stream, a.w2,
+                       static_cast<const unsigned char*>(a.w2_scales), a.b2, w, s, a.y);
     return hipGetLastError();
+}
+
+template <int kIn, int kType, int kAct>
+int launch_odd(const mchip_moe_args& a, const Workspace& w, const Sizes& s, hipStream_t stream) {
+    if constexpr (kType != kMx4) {
+        if (s.d % 2 != 0 || s.h % 2 != 0 || !aligned(a.w1, 4) || !aligned(a.w2, 4))
+            return launch_experts<kIn, kType, kAct, true>(a, w, s, stream);
+    }
+    return launch_experts<kIn, kType, kAct, false>(a, w, s, stream);
 }
 
 template <int kIn, int kType>
 int launch_act(const mchip_moe_args& a, const Workspace& w, const Sizes& s, hipStream_t stream) {
-    if (a.activation == MCHIP_MOE_RELU) return launch_experts<kIn, kType, MCHIP_MOE_RELU>(a, w, s, stream);
-    if (a.activation == MCHIP_MOE_GELU) return launch_experts<kIn, kType, MCHIP_MOE_GELU>(a, w, s, stream);
-    return launch_experts<kIn, kType, MCHIP_MOE_SWIGLU>(a, w, s, stream);
+    if (a.activation == MCHIP_MOE_RELU) return launch_odd<kIn, kType, MCHIP_MOE_RELU>(a, w, s, stream);
+    if (a.activation == MCHIP_MOE_GELU) return launch_odd<kIn, kType, MCHIP_MOE_GELU>(a, w, s, stream);
+    return launch_odd<kIn, kType, MCHIP_MOE_SWIGLU>(a, w, s, stream);
 }
 
 template <int kIn>
@@ -561,10 +655,16 @@ int launch(const mchip_moe_args& a, hipStream_t stream) {
     const Sizes s = sizes_of(a.tokens, a.d, a.h, a.experts, a.top_k);
     Workspace w;
     lay_out(s, a.dtype, static_cast<unsigned char*>(a.workspace), &w);
-    hipLaunchKernelGGL(moe_router<kIn>,
-                       dim3(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16),
-                            static_cast<unsigned>(router_parts(s.d))),
-                       dim3(kThreads), sizeof(float) * s.tokens * s.experts, stream, a.x, a.ldx, a.router, w, s, a.normalize != 0, a.chosen, a.gates);
+    const dim3 grid(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16),
+                    static_cast<unsigned>(router_parts(s.d)));
+    const auto router = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), sizeof(float) * s.tokens * s.experts, stream, a.x, a.ldx,
+                           a.router, w, s, a.normalize != 0, a.chosen, a.gates);
+    };
+    if (kIn == kF16 && a.weights == kF16)
+        router(moe_router<kIn, kIn == kF16>);
+    else
+        router(moe_router<kIn, false>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.weights == kBf16) return launch_act<kIn, kBf16>(a, w, s, stream);

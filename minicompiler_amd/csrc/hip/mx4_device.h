@@ -32,7 +32,7 @@ typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 128;  // elements of k per matrix instruction
 constexpr int kF32 = MCHIP_DTYPE_F32, kBf16 = MCHIP_DTYPE_BF16, kF16 = MCHIP_DTYPE_F16, kMx4 = MCHIP_DTYPE_MX4;
@@ -51,6 +51,11 @@ __device__ __forceinline__ f32x4 mfma(i32x4 a, int sa, i32x4 b, int sb, f32x4 c)
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
+}
+
+__device__ __forceinline__ f32x4 mfma_f16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
 }
 
 // A 16-bit value, or an fp32 one, as fp32 (exact).
@@ -86,6 +91,7 @@ __device__ __forceinline__ void store_one(void* p, long long i, float v) {
 typedef f32x4 f32x4_loose __attribute__((aligned(4)));
 typedef u16x8 u16x8_loose __attribute__((aligned(2)));
 typedef u32x4 u32x4_loose __attribute__((aligned(2)));
+typedef u32x4 u32x4_dwords __attribute__((aligned(4)));
 typedef u16x4 u16x4_loose __attribute__((aligned(2)));
 
 // The first `left` of four consecutive elements of a row of C at element `at`.

@@ -98,6 +98,27 @@ def test_sizes(device, mc, weights, tokens, d, h, experts, top_k, act):
         check(mc, 2, kind, weights, tokens, d, h, experts, top_k, act, normalize=tokens % 2 == 0, bias=experts % 2 == 1)
 
 
+@pytest.mark.parametrize("weights", [ref.BF16, ref.F16])
+def test_rows_that_start_at_odd_elements(device, mc, weights):
+    """Weights a 2-byte step past a dword, and subnormal fp16 ones among them."""
+    tokens, d, h, experts, top_k = 9, 150, 90, 5, 2
+    rng = np.random.default_rng(21)
+    net = layer(mc, rng, weights, d, h, experts, "gelu", True)
+    for name, shape in (("1", (experts, h, d)), ("2", (experts, d, h))):
+        w = rng.standard_normal(shape) * shape[2] ** -0.5
+        w[:, ::3] *= 2.0 ** -14
+        bits = ref.to_type(w, weights)
+        buf = mc.DeviceBuffer.from_array(np.concatenate([np.zeros(1, bits.dtype), bits.reshape(-1)]))
+        net["keep"].append(buf)
+        net["w" + name], net["v" + name] = buf.ptr + 2, ref.from_type(bits, weights)
+    bits, router, (chosen, gates, _, _, err) = inputs(rng, tokens, d, experts, ref.F16, top_k, True)
+    y, got, _ = run(mc, net, bits, ref.F16, router, weights, h, top_k, "gelu", True)
+    assert np.array_equal(got, chosen)
+    exact, bound = ref.moe(ref.from_type(bits, ref.F16), net["v1"], net["vb1"], net["v2"], net["vb2"], chosen, gates, "gelu",
+                           err, ref.F16)
+    within(y, exact, bound)
+
+
 def test_strided_rows_on_a_stream(device, mc):
     s = mc.Stream()
     for pad in (1, 8):
