@@ -5,10 +5,12 @@
 //
 // Three launches, in stream order:
 //   moe_router  x R^T on the FP32 matrix instruction, d shared out over blocks; x
-//               cut into bf16 pieces; the last block to arrive adds the parts
-//               of the logits in order, picks the experts and lists the jobs
-//               (one per chosen expert and 16 of its tokens);
-//   moe_up      per job and 32 (swiglu: 16) columns of h: act(x W1^T + b1), cut
+//               cut into bf16 pieces; for more than 8 tokens the last block of 16
+//               tokens adds the parts of their logits in order and picks their
+//               experts, and the last of all lists the jobs (one per chosen
+//               expert and 16 of its tokens);
+//   moe_up      (up to 8 tokens: every block picks the experts for itself, which
+//               is less than waiting for one that does;) per job and 32 (swiglu: 16) columns of h: act(x W1^T + b1), cut
 //               into bf16 pieces;
 //   moe_down    per 32 columns of y and share of the jobs' steps: h W2^T weighed
 //               by the gates; the last block of a column tile adds the shares
@@ -28,6 +30,8 @@ using namespace mx4;
 constexpr int kMaxTokens = MCHIP_MOE_MAX_TOKENS, kMaxExperts = MCHIP_MOE_MAX_EXPERTS, kMaxTopK = MCHIP_MOE_MAX_TOP_K;
 constexpr int kMaxWidth = 1 << 20;  // of d and h
 constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kFirstColumn = 1 + kMaxTokens / 16;  // counter of the first column tile of y
+constexpr int kFew = 8;    // tokens for which every block of moe_up picks the experts
 constexpr int kNone = -1;  // the token of a job's empty place
 
 // A job's tokens and what they weigh.
@@ -39,8 +43,10 @@ struct Job {
 
 // The workspace: counters (zero between calls), the jobs, then the arrays.
 struct Workspace {
-    unsigned* arrived;  // [1 + column tiles of y]
+    unsigned* arrived;  // [1 + token tiles + column tiles of y]
     int* jobs;          // how many
+    int* chosen;        // [tokens][kMaxTopK]
+    float* gate;
     Job* job;           // [max_jobs]
     float* logits;      // [parts][tokens, experts]
     unsigned short* x;  // [pieces][dp / 8][tokens][8]: a token's eight elements beside its neighbours'
@@ -90,8 +96,10 @@ std::size_t lay_out(const Sizes& s, int dtype, unsigned char* base, Workspace* w
         at += round_up(bytes);
         return p;
     };
-    w->arrived = reinterpret_cast<unsigned*>(take(sizeof(unsigned) * (1 + column_tiles(kMaxWidth))));
+    w->arrived = reinterpret_cast<unsigned*>(take(sizeof(unsigned) * (kFirstColumn + column_tiles(kMaxWidth))));
     w->jobs = reinterpret_cast<int*>(take(sizeof(int)));
+    w->chosen = reinterpret_cast<int*>(take(sizeof(int) * kMaxTokens * kMaxTopK));
+    w->gate = reinterpret_cast<float*>(take(sizeof(float) * kMaxTokens * kMaxTopK));
     w->job = reinterpret_cast<Job*>(take(sizeof(Job) * static_cast<std::size_t>(s.max_jobs)));
     w->logits = reinterpret_cast<float*>(take(sizeof(float) * static_cast<std::size_t>(router_parts(s.d)) * s.tokens * s.experts));
     w->x = reinterpret_cast<unsigned short*>(
@@ -128,14 +136,14 @@ __device__ __forceinline__ float add_parts(const float* parts, long long plane, 
 // reduction over the wave is a chain of dependent instructions: several tokens'
 // chains go side by side.
 template <int kEach, int kTokens>
-__device__ void choose(const float* logits, int first, const Sizes& s, bool normalize, int lane,
+__device__ void choose(const float* logits, int from, int first, int to, const Sizes& s, bool normalize, int lane,
                        int (*chosen)[kMaxTopK], float (*gate)[kMaxTopK]) {
     unsigned key[kTokens][kEach];
     float top[kTokens], sum[kTokens];
     int mine[kTokens];  // lane i: the i-th expert
 #pragma unroll
     for (int n = 0; n < kTokens; ++n) {
-        const int t = first + n < s.tokens ? first + n : s.tokens - 1;
+        const int t = (first + n < to ? first + n : to - 1) - from;
         float l[kEach];
         unsigned best = 0;
 #pragma unroll
@@ -176,8 +184,8 @@ __device__ void choose(const float* logits, int first, const Sizes& s, bool norm
 #pragma unroll
     for (int n = 0; n < kTokens; ++n) {
         const int t = first + n;
-        if (t >= s.tokens) break;
-        const float p = lane < s.top_k ? expf(logits[t * s.experts + mine[n]] - top[n]) / sum[n] : 0.0f;
+        if (t >= to) break;
+        const float p = lane < s.top_k ? expf(logits[(t - from) * s.experts + mine[n]] - top[n]) / sum[n] : 0.0f;
         const float kept = wave_sum(p);
         if (lane < s.top_k) {
             chosen[t][lane] = mine[n];
@@ -186,11 +194,30 @@ __device__ void choose(const float* logits, int first, const Sizes& s, bool norm
     }
 }
 
+// Tokens `from` to `to` of the logits (from `logits` on, in LDS), a few for each of the block's waves.
 template <int kEach, int kTokens>
-__device__ __forceinline__ void choose_all(const float* logits, const Sizes& s, bool normalize, int wave, int lane,
-                                           int (*chosen)[kMaxTopK], float (*gate)[kMaxTopK]) {
-    for (int t = wave * kTokens; t < s.tokens; t += kWaves * kTokens)
-        choose<kEach, kTokens>(logits, t, s, normalize, lane, chosen, gate);
+__device__ __forceinline__ void choose_all(const float* logits, int from, int to, const Sizes& s, bool normalize,
+                                           int wave, int waves, int lane, int (*chosen)[kMaxTopK],
+                                           float (*gate)[kMaxTopK]) {
+    for (int t = from + wave * kTokens; t < to; t += waves * kTokens)
+        choose<kEach, kTokens>(logits, from, t, to, s, normalize, lane, chosen, gate);
+}
+
+// The logits of tokens `from` to `to` added up into LDS, and their experts and gates.
+__device__ __forceinline__ void route(const Workspace& w, const Sizes& s, int parts, int from, int to, bool normalize,
+                                      float* logits, int (*chosen)[kMaxTopK], float (*gate)[kMaxTopK]) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, lane = threadIdx.x % 64;
+    const long long plane = static_cast<long long>(s.tokens) * s.experts;
+    for (int i = threadIdx.x; i < (to - from) * s.experts; i += blockDim.x)
+        logits[i] = add_parts(w.logits + from * s.experts + i, plane, parts);
+    __syncthreads();
+    if (s.experts > 128)
+        choose_all<kMaxExperts / 64, 1>(logits, from, to, s, normalize, wave, waves, lane, chosen, gate);
+    else if (to - from <= waves)
+        choose_all<2, 1>(logits, from, to, s, normalize, wave, waves, lane, chosen, gate);
+    else
+        choose_all<2, 2>(logits, from, to, s, normalize, wave, waves, lane, chosen, gate);
+    __syncthreads();
 }
 
 // The jobs from the chosen experts in LDS, by the whole block: a thread per
@@ -231,6 +258,44 @@ __device__ void list_jobs(const Workspace& w, const Sizes& s, const int (*chosen
     }
 }
 
+// The same for up to 8 tokens (a job per chosen expert) into `jobs`, by blocks
+// of at least 128 threads, a thread per chosen pair; returns how many.
+__device__ int list_few_jobs(const Sizes& s, const int (*chosen)[kMaxTopK], const float (*gate)[kMaxTopK],
+                             unsigned* mask, int* counts, Job* jobs) {
+    const int i = threadIdx.x, t = i / s.top_k, j = i % s.top_k;
+    const bool pair = i < s.tokens * s.top_k;
+    const int e = pair ? chosen[t][j] : 0;
+    if (pair) mask[e] = 0;
+    __syncthreads();
+    if (pair) atomicOr(mask + e, 1u << t);
+    __syncthreads();
+    const bool first = pair && __builtin_ctz(mask[e]) == t;
+    const unsigned long long firsts = __ballot(first);
+    if (i % 64 == 0 && i < 128) counts[i / 64] = __builtin_popcountll(firsts);
+    __syncthreads();
+    if (first) {
+        const int n = (i >= 64 ? counts[0] : 0) + __builtin_popcountll(firsts & ((1ull << i % 64) - 1));
+        Job& job = jobs[n];
+        job.expert = e;
+        unsigned left = mask[e];
+        for (int place = 0; place < 16; ++place) {
+            int to = kNone;
+            float g = 0.0f;
+            if (left != 0) {
+                to = __builtin_ctz(left);
+                left &= left - 1;
+                for (int k = 0; k < s.top_k; ++k)
+                    if (chosen[to][k] == e) g = gate[to][k];
+            }
+            job.token[place] = to;
+            job.gate[place] = g;
+        }
+    }
+    const int all = counts[0] + counts[1];
+    __syncthreads();
+    return all;
+}
+
 // 16 experts by 16 tokens of the logits over one part of d, 64 elements at a time
 // for each wave. v_mfma_f32_16x16x4_f32: lane (r, q) supplies row or column r,
 // element q; here a lane's four elements go to four instructions.
@@ -240,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
                                                        bool normalize, int* __restrict__ chosen_out,
                                                        float* __restrict__ gates_out) {
     constexpr int kP = kPieces<kIn>;
-    extern __shared__ float logits[];  // [tokens, experts], in the last block
+    extern __shared__ float logits[];  // [16, experts], in the last block of 16 tokens
     __shared__ f32x4 space[kWaves / 2 * 64];
     __shared__ int chosen[kMaxTokens][kMaxTopK];
     __shared__ float gate[kMaxTokens][kMaxTopK];
@@ -298,16 +363,23 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
             *reinterpret_cast<u32x4*>(w.x + (static_cast<long long>(p) * chunks + i) * 8) = out[p];
     }
 
-    if (!mc_split_last_arrival(w.arrived, blocks, &flag)) return;
-    for (int i = threadIdx.x; i < all_logits; i += kThreads) logits[i] = add_parts(w.logits + i, all_logits, parts);
-    __syncthreads();
-    if (s.experts > 128)
-        choose_all<kMaxExperts / 64, 1>(logits, s, normalize, wave, lane, chosen, gate);
-    else if (s.experts > 64 || s.tokens <= kWaves)
-        choose_all<2, 1>(logits, s, normalize, wave, lane, chosen, gate);
-    else
-        choose_all<1, 4>(logits, s, normalize, wave, lane, chosen, gate);
-    __syncthreads();
+    if (s.tokens <= kFew) return;
+    if (!mc_split_last_arrival(w.arrived + 1 + blockIdx.y, gridDim.x * parts, &flag)) return;
+    const int t1 = t0 + 16 < s.tokens ? t0 + 16 : s.tokens;
+    route(w, s, parts, t0, t1, normalize, logits, chosen, gate);
+    if (gridDim.y > 1) {
+        for (int i = threadIdx.x; i < (t1 - t0) * kMaxTopK; i += kThreads) {
+            mc_split_store(reinterpret_cast<float*>(w.chosen) + t0 * kMaxTopK + i,
+                           __builtin_bit_cast(float, chosen[t0][i]));
+            mc_split_store(w.gate + t0 * kMaxTopK + i, gate[t0][i]);
+        }
+        if (!mc_split_last_arrival(w.arrived, gridDim.y, &flag)) return;
+        for (int i = threadIdx.x; i < s.tokens * kMaxTopK; i += kThreads) {
+            chosen[0][i] = __builtin_bit_cast(int, mc_split_load(reinterpret_cast<const float*>(w.chosen) + i));
+            gate[0][i] = mc_split_load(w.gate + i);
+        }
+        __syncthreads();
+    }
     list_jobs(w, s, chosen, gate, mask, place);
     for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads) {
         const int t = i / s.top_k, j = i % s.top_k;
@@ -460,18 +532,6 @@ struct Stream {
             }
         }
     }
-
-    // acc[i] += steps from, from + by, .. below to; one step is under way while another is multiplied.
-    __device__ __forceinline__ void run(int from, int to, int by, f32x4 (&acc)[kTiles]) const {
-        if (from >= to) return;
-        Step now, next;
-        load(from, now);
-        for (int t = from; t < to; t += by) {
-            if (t + by < to) load(t + by, next);
-            multiply(now, acc);
-            now = next;
-        }
-    }
 };
 
 template <int kAct>
@@ -481,62 +541,122 @@ __device__ __forceinline__ float activate(float u, float up) {
     return 0.5f * u * (1.0f + tanhf(0.79788456080286536f * (u + 0.044715f * u * u * u)));
 }
 
-// A job's h for 32 (swiglu: 16) columns from blockIdx.x on. Columns from h to hp
-// are written as zeros.
+// h of jobs, 32 (swiglu: 16) columns at a time: every job's column tiles in a row
+// are cut evenly over the blocks, so that the grid does not depend on how many
+// jobs there are. The waves take a tile's steps in turn, and the next step, of
+// the next tile too, is under way while one is multiplied and while the waves'
+// sums are added (a block per tile waited for its job, its weights and its sums
+// in turn: 143 MB of mx4 in 42 us). Columns from h to hp are written as zeros.
 // kHalf: x was kept in fp16, as the weights are (one piece).
+template <int kType>
+constexpr int kUpWaves = kType == kMx4 ? 8 : 4;  // 16-bit weights take the registers of two mx4 waves
+
 template <int kType, int kP, int kHP, int kAct, bool kOdd, bool kHalf>
-__global__ __launch_bounds__(kThreads) void moe_up(const void* __restrict__ w1, const unsigned char* __restrict__ w1_scales,
-                                                   const float* __restrict__ b1, Workspace w, Sizes s) {
+__global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __restrict__ w1,
+                                                               const unsigned char* __restrict__ w1_scales,
+                                                               const float* __restrict__ b1, Workspace w, Sizes s,
+                                                               int parts, bool normalize,
+                                                               int* __restrict__ chosen_out,
+                                                               float* __restrict__ gates_out) {
     constexpr bool kGated = kAct == MCHIP_MOE_SWIGLU;
-    constexpr int kTiles = 2, kUpCols = kGated ? 16 : 32;
-    __shared__ f32x4 space[kWaves / 2 * kTiles * 64];
-    const Job& job = w.job[blockIdx.y];
+    constexpr int kTiles = 2, kUpCols = kGated ? 16 : 32, kWaves = kUpWaves<kType>, kThreads = 64 * kWaves;
+    typedef Stream<kType, kTiles, kP, kOdd, kHalf> In;
+    __shared__ f32x4 space[2][kWaves][kTiles][64];
+    extern __shared__ float logits[];  // for few tokens: [tokens, experts], then their jobs
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-    const int r = lane % 16, q = lane / 16;
-    const int h0 = blockIdx.x * kUpCols;
-    // The job is read beside the number of jobs, not after it; past the last, it is not used.
-    const int jobs = *w.jobs, expert = job.expert, token = job.token[r];
-    if (static_cast<int>(blockIdx.y) >= jobs) return;
-    const long long all_rows = kGated ? 2LL * s.h : s.h;
-    const long long first = expert * all_rows;
-    f32x4 acc[kTiles];
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (h0 < s.h) {
-        Stream<kType, kTiles, kP, kOdd, kHalf> in;
+    const int r = lane % 16;
+    const int tiles = s.hp / kUpCols, steps = s.dp / kStep;
+    const Job* jobs = w.job;
+    int count;
+    if (s.tokens <= kFew) {
+        __shared__ int chosen[kFew][kMaxTopK];
+        __shared__ float gate[kFew][kMaxTopK];
+        __shared__ unsigned mask[kMaxExperts];
+        __shared__ int counts[2];
+        Job* few = reinterpret_cast<Job*>(logits + s.tokens * s.experts);
+        route(w, s, parts, 0, s.tokens, normalize, logits, chosen, gate);
+        count = list_few_jobs(s, chosen, gate, mask, counts, few);
+        jobs = few;
+        if (blockIdx.x == 0) {  // for moe_down and the caller
+            if (threadIdx.x == 0) *w.jobs = count;
+            for (int i = threadIdx.x; i < count * static_cast<int>(sizeof(Job) / 4); i += kThreads)
+                reinterpret_cast<int*>(w.job)[i] = reinterpret_cast<const int*>(few)[i];
+            for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads) {
+                if (chosen_out != nullptr) chosen_out[i] = chosen[i / s.top_k][i % s.top_k];
+                if (gates_out != nullptr) gates_out[i] = gate[i / s.top_k][i % s.top_k];
+            }
+        }
+    } else {
+        count = *w.jobs;
+    }
+    const long long all = static_cast<long long>(count) * tiles;
+    const int from = static_cast<int>(blockIdx.x * all / gridDim.x), to = static_cast<int>((blockIdx.x + 1) * all / gridDim.x);
+    if (from >= to) return;
+    const int h_rows = kGated ? 2 * s.h : s.h;
+
+    int job = from / tiles, expert = jobs[job].expert, token = jobs[job].token[r];
+    const auto open = [&](int u, In& in) {
+        if (u / tiles != job) {
+            job = u / tiles;
+            expert = jobs[job].expert;
+            token = jobs[job].token[r];
+        }
+        const int h0 = u % tiles * kUpCols;
         in.open(w1, w1_scales, s.d, [&](int i) {
             const int col = h0 + (kGated ? 0 : 16 * i) + r;
-            return first + (col < s.h ? col : s.h - 1) + (kGated && i == 1 ? s.h : 0);
+            return static_cast<long long>(expert) * h_rows + (col < s.h ? col : s.h - 1) + (kGated && i == 1 ? s.h : 0);
         });
         in.tokens(w.x + (token == kNone ? 0 : token) * 8, 8LL * s.tokens, static_cast<long long>(s.tokens) * s.dp,
                   token != kNone);
-        in.run(wave, s.dp / kStep, kWaves, acc);
-    }
-    add_waves<kWaves, kTiles>(acc, space, wave, lane);
-    if (wave != 0) return;
-    const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
+    };
+    In in;
+    typename In::Step now, next;
+    open(from, in);
+    if (wave < steps) in.load(wave, now);
+    for (int u = from; u < to; ++u) {
+        const int of_job = u / tiles, of_expert = expert, h0 = u % tiles * kUpCols;
+        f32x4 acc[kTiles];
 #pragma unroll
-    for (int i = 0; i < (kGated ? 1 : kTiles); ++i) {
-        const int c0 = h0 + 16 * i + 4 * q;
-        u16x4 out[kHP];
+        for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = wave; t < steps; t += kWaves) {
+            // Decoding needs nothing of `in` but the lane's place: it may move on first.
+            if (t + kWaves < steps) {
+                in.load(t + kWaves, next);
+            } else if (u + 1 < to) {
+                open(u + 1, in);
+                in.load(wave, next);
+            }
+            in.multiply(now, acc);
+            now = next;
+        }
+        if (wave >= steps && u + 1 < to) open(u + 1, in);
+        f32x4(&sums)[kWaves][kTiles][64] = space[u & 1];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            float u = acc[i][v], up = kGated ? acc[1][v] : 0.0f;
-            const bool in = c0 + v < s.h;
-            if (b1 != nullptr && in) {
-                u += b1[first + c0 + v];
-                if (kGated) up += b1[first + s.h + c0 + v];
+        for (int i = 0; i < kTiles; ++i) sums[wave][i][lane] = acc[i];
+        __syncthreads();
+        // A thread per element: lane's values v of a tile are columns 4 q + v of token r.
+        for (int o = threadIdx.x; o < (kGated ? 256 : 512); o += kThreads) {
+            const int at = o % 256, tile = o / 256, er = at / 4 % 16, col = h0 + 16 * tile + at / 64 * 4 + at % 4;
+            const auto sum = [&](int i) {
+                float v = 0.0f;
+#pragma unroll
+                for (int n = 0; n < kWaves; ++n) v += reinterpret_cast<const float*>(sums[n][i])[at];
+                return v;
+            };
+            float a = sum(tile), up = kGated ? sum(1) : 0.0f;
+            const bool in_h = col < s.h;
+            if (b1 != nullptr && in_h) {
+                a += b1[static_cast<long long>(of_expert) * h_rows + col];
+                if (kGated) up += b1[static_cast<long long>(of_expert) * h_rows + s.h + col];
             }
             float piece[kHP];
-            cut<kHP>(in ? activate<kAct>(u, up) : 0.0f, piece);
+            cut<kHP>(in_h ? activate<kAct>(a, up) : 0.0f, piece);
+            const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
 #pragma unroll
             for (int p = 0; p < kHP; ++p)
-                out[p][v] = static_cast<unsigned short>(__builtin_bit_cast(unsigned, piece[p]) >> 16);
+                w.h[p * h_plane + static_cast<long long>(of_job) * 16 * s.hp + (col / 8 * 16 + er) * 8 + col % 8] =
+                    static_cast<unsigned short>(__builtin_bit_cast(unsigned, piece[p]) >> 16);
         }
-#pragma unroll
-        for (int p = 0; p < kHP; ++p)
-            *reinterpret_cast<u16x4*>(w.h + p * h_plane + static_cast<long long>(blockIdx.y) * 16 * s.hp +
-                                      (c0 / 8 * 16 + r) * 8 + c0 % 8) = out[p];
     }
 }
 
@@ -563,37 +683,59 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
     const int from = index * each + (index < more ? index : more), to = from + each + (index < more ? 1 : 0);
     const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
 
-    int u = from;
-    while (u < to) {
-        const int n = u / steps, last = (n + 1) * steps < to ? (n + 1) * steps : to;
-        const Job& job = w.job[n];
-        const int expert = job.expert, token = job.token[r];
-        const float gate = job.gate[r];
-        f32x4 acc[kTiles];
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (b2 != nullptr && u == n * steps) {  // the job's first step brings the bias
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const int c = d0 + 16 * i + 4 * q + v;
-                    if (c < s.d) acc[i][v] = b2[static_cast<long long>(expert) * s.d + c];
-                }
-        }
-        Stream<kType, kTiles, kP, kOdd, false> in;
+    typedef Stream<kType, kTiles, kP, kOdd, false> In;
+    In in;
+    typename In::Step now, next;
+    int expert = 0, token = kNone;
+    float gate = 0.0f;
+    const auto open = [&](int n) {
+        expert = w.job[n].expert;
+        token = w.job[n].token[r];
+        gate = w.job[n].gate[r];
         in.open(w2, w2_scales, s.h, [&](int i) {
             const int col = d0 + 16 * i + r;
             return static_cast<long long>(expert) * s.d + (col < s.d ? col : s.d - 1);
         });
         in.tokens(w.h + static_cast<long long>(n) * 16 * s.hp + r * 8, 16 * 8, h_plane, token != kNone);
-        in.run(u - n * steps, last - n * steps, 1, acc);
-        u = last;
-        if (token != kNone) {
+    };
+    int n = from / steps, t = from % steps;
+    if (from < to) {
+        open(n);
+        in.load(t, now);
+    }
+    for (int u = from; u < to;) {
+        const int of_expert = expert, of_token = token;
+        const float of_gate = gate;
+        f32x4 acc[kTiles];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (b2 != nullptr && t == 0) {  // the job's first step brings the bias
 #pragma unroll
             for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) mine[token * kCols + 16 * i + 4 * q + v] += gate * acc[i][v];
+                for (int v = 0; v < 4; ++v) {
+                    const int c = d0 + 16 * i + 4 * q + v;
+                    if (c < s.d) acc[i][v] = b2[static_cast<long long>(of_expert) * s.d + c];
+                }
+        }
+        // To the job's end or the wave's; the next step, of the next job too, is under way meanwhile.
+        for (bool same = true; same && u < to; ++u) {
+            if (u + 1 < to) {
+                if (++t == steps) {
+                    t = 0;
+                    same = false;
+                    open(++n);
+                }
+                in.load(t, next);
+            }
+            in.multiply(now, acc);
+            now = next;
+        }
+        if (of_token != kNone) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) mine[of_token * kCols + 16 * i + 4 * q + v] += of_gate * acc[i][v];
         }
     }
     __syncthreads();
@@ -608,7 +750,7 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
         else if (d0 + c < s.d)
             store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum);
     }
-    if (shares == 1 || !mc_split_last_arrival(w.arrived + 1 + blockIdx.x, shares, &flag)) return;
+    if (shares == 1 || !mc_split_last_arrival(w.arrived + kFirstColumn + blockIdx.x, shares, &flag)) return;
     for (int i = threadIdx.x; i < cells; i += kThreads) {
         const int t = i / kCols, c = i % kCols;
         if (d0 + c >= s.d) continue;
@@ -624,9 +766,14 @@ int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, 
     constexpr int kHP = kIn == kF32 ? 3 : 2;
     constexpr int kUpCols = kAct == MCHIP_MOE_SWIGLU ? 16 : 32;
     constexpr bool kHalf = kIn == kF16 && kType == kF16;
+    // As many blocks as the registers let run at once, about.
+    const long long units = static_cast<long long>(s.max_jobs) * (s.hp / kUpCols);
+    const long long blocks = static_cast<long long>(kType == kMx4 ? 2 : 3) * device_cus();
+    const std::size_t few = s.tokens <= kFew ? sizeof(float) * s.tokens * s.experts + sizeof(Job) * s.max_jobs : 0;
     hipLaunchKernelGGL((moe_up<kType, kHalf ? 1 : kPieces<kIn>, kHP, kAct, kOdd, kHalf>),
-                       dim3(static_cast<unsigned>(s.hp / kUpCols), static_cast<unsigned>(s.max_jobs)), dim3(kThreads), 0,
-                       stream, a.w1, static_cast<const unsigned char*>(a.w1_scales), a.b1, w, s);
+                       dim3(static_cast<unsigned>(std::min(blocks, units))), dim3(64 * kUpWaves<kType>), few, stream, a.w1,
+                       static_cast<const unsigned char*>(a.w1_scales), a.b1, w, s, router_parts(s.d), a.normalize != 0,
+                       a.chosen, a.gates);
     hipLaunchKernelGGL((moe_down<kType, kHP, kIn, kOdd>),
                        dim3(static_cast<unsigned>(column_tiles(s.d)), static_cast<unsigned>(down_shares(s))),
                        dim3(kThreads), sizeof(float) * kWaves * s.tokens * kCols, stream, a.w2,
@@ -658,7 +805,7 @@ int launch(const mchip_moe_args& a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16),
                     static_cast<unsigned>(router_parts(s.d)));
     const auto router = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), sizeof(float) * s.tokens * s.experts, stream, a.x, a.ldx,
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), sizeof(float) * 16 * s.experts, stream, a.x, a.ldx,
                            a.router, w, s, a.normalize != 0, a.chosen, a.gates);
     };
     if (kIn == kF16 && a.weights == kF16)
