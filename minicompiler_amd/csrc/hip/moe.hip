@@ -113,20 +113,26 @@ std::size_t lay_out(const Sizes& s, int dtype, unsigned char* base, Workspace* w
 
 // ---------------------------------------------------------------- router
 
-// parts[0] + parts[plane] + ... (`count` of them, in order), written by other
-// blocks. Eight loads at a time are under way: one after the other, 16 of them
-// took 16 us.
-__device__ __forceinline__ float add_parts(const float* parts, long long plane, int count) {
-    float sum = 0.0f;
+// sum[n] = parts[n][0] + parts[n][plane] + ... (`count` of them, in order),
+// written by other blocks. Eight loads of each are under way: one after the
+// other, 16 of them took 16 us.
+template <int kEach>
+__device__ __forceinline__ void add_parts(const float* const (&parts)[kEach], long long plane, int count,
+                                          float (&sum)[kEach]) {
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) sum[n] = 0.0f;
     for (int v = 0; v < count; v += 8) {
-        float part[8];
+        float part[kEach][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) part[j] = v + j < count ? mc_split_load(parts + (v + j) * plane) : 0.0f;
+        for (int n = 0; n < kEach; ++n)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (v + j < count) sum += part[j];
+            for (int j = 0; j < 8; ++j) part[n][j] = v + j < count ? mc_split_load(parts[n] + (v + j) * plane) : 0.0f;
+#pragma unroll
+        for (int n = 0; n < kEach; ++n)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (v + j < count) sum[n] += part[n][j];
     }
-    return sum;
 }
 
 // The experts and gates of kTokens tokens from `first` on, by one wave, from
@@ -208,8 +214,15 @@ __device__ __forceinline__ void route(const Workspace& w, const Sizes& s, int pa
                                       float* logits, int (*chosen)[kMaxTopK], float (*gate)[kMaxTopK]) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, lane = threadIdx.x % 64;
     const long long plane = static_cast<long long>(s.tokens) * s.experts;
-    for (int i = threadIdx.x; i < (to - from) * s.experts; i += blockDim.x)
-        logits[i] = add_parts(w.logits + from * s.experts + i, plane, parts);
+    const int all = (to - from) * s.experts;
+    for (int i = threadIdx.x; i < all; i += 2 * blockDim.x) {
+        const int second = i + static_cast<int>(blockDim.x);
+        const float* at[2] = {w.logits + from * s.experts + i, w.logits + from * s.experts + (second < all ? second : i)};
+        float sum[2];
+        add_parts<2>(at, plane, parts, sum);
+        logits[i] = sum[0];
+        if (second < all) logits[second] = sum[1];
+    }
     __syncthreads();
     if (s.experts > 128)
         choose_all<kMaxExperts / 64, 1>(logits, from, to, s, normalize, wave, waves, lane, chosen, gate);
@@ -396,7 +409,8 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
 // load), of mx4 ones 32 q + 8 s .. + 7 (block q of the step is its 16 bytes).
 // kOdd: 16-bit rows that start at odd elements, or some of them. Loads at odd
 // elements halved the rate (101 MB of W1 in 61 us, 30 with even rows): a lane
-// takes the whole dwords that its elements lie in, and shifts.
+// takes the four dwords from the one with its first element on, gets the fifth,
+// with its last, from the lane behind, and shifts.
 // kHalf: fp16 rows and tokens multiplied as they are.
 template <int kType, int kTiles, int kP, bool kOdd, bool kHalf>
 struct Stream {
@@ -406,7 +420,8 @@ struct Stream {
 
     struct Step {
         u32x4 w[kTiles][kRaw];
-        unsigned more[kTiles][kOdd ? kRaw : 1];  // the dword behind w
+        unsigned behind[kTiles];  // odd rows, lanes of q = 0: the dword behind the step
+        int shift[kTiles];
         unsigned scales;  // lane 16 i + r: of row r of tile i
         u32x4 x[4][kP];
     };
@@ -457,31 +472,32 @@ struct Stream {
         } else {
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
+                if constexpr (kOdd) st.shift[i] = shift[i];
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
                     const int k0 = t * kStep + offset(q, s);
                     const unsigned char* p = rows[i] + k0 * 2;
                     if (k0 + 8 <= k) {
                         st.w[i][s] = *reinterpret_cast<const u32x4_dwords*>(p);
-                        // Unshifted lanes take the last dword again: the next may lie past the weights.
-                        if constexpr (kOdd) st.more[i][s] = *reinterpret_cast<const unsigned*>(p + 12 + 2 * shift[i]);
                     } else {
-                        unsigned e[8];
+                        // Element by element; e[0] is the one before, which a shifted row's first dword holds.
+                        unsigned e[9];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            e[j] = k0 + j < k ? *reinterpret_cast<const unsigned short*>(p + shift[i] + 2 * j) : 0u;
+                        for (int j = 0; j < 9; ++j)
+                            e[j] = k0 + j - 1 >= 0 && k0 + j - 1 < k
+                                       ? *reinterpret_cast<const unsigned short*>(p + shift[i] + 2 * (j - 1))
+                                       : 0u;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) st.w[i][s][j] = e[2 * j] | e[2 * j + 1] << 16;
-                        if constexpr (kOdd) {  // as if loaded shifted
-                            if (shift[i] != 0) {
-                                st.more[i][s] = e[7];
-#pragma unroll
-                                for (int j = 3; j > 0; --j) st.w[i][s][j] = e[2 * j - 1] | e[2 * j] << 16;
-                                st.w[i][s][0] = e[0] << 16;
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            const bool back = kOdd && shift[i] != 0;
+                            st.w[i][s][j] = (back ? e[2 * j] : e[2 * j + 1]) | (back ? e[2 * j + 1] : e[2 * j + 2]) << 16;
                         }
                     }
                 }
+                if constexpr (kOdd)
+                    st.behind[i] = q == 0 && shift[i] != 0 && (t + 1) * kStep - 1 < k
+                                       ? *reinterpret_cast<const unsigned*>(rows[i] + (t + 1) * kStep * 2)
+                                       : 0u;
             }
         }
 #pragma unroll
@@ -508,9 +524,13 @@ struct Stream {
                 } else {
                     u32x4 raw = st.w[i][s];
                     if constexpr (kOdd) {
+                        // Chunk 4 s + q's fifth dword is the first of chunk 4 s + q + 1.
+                        const unsigned give = q != 0 ? raw[0] : s < 3 ? st.w[i][s < 3 ? s + 1 : 3][0] : st.behind[i];
+                        const unsigned fifth = static_cast<unsigned>(
+                            __builtin_amdgcn_ds_bpermute(((16 * q + r + 16) & 63) * 4, static_cast<int>(give)));
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            raw[j] = __builtin_amdgcn_alignbyte(j < 3 ? st.w[i][s][j + 1] : st.more[i][s], raw[j], shift[i]);
+                            raw[j] = __builtin_amdgcn_alignbyte(j < 3 ? st.w[i][s][j + 1] : fifth, raw[j], st.shift[i]);
                     }
                     if constexpr (kType == kBf16 || kHalf) {
                         w[0] = raw;
@@ -751,11 +771,19 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
             store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum);
     }
     if (shares == 1 || !mc_split_last_arrival(w.arrived + kFirstColumn + blockIdx.x, shares, &flag)) return;
-    for (int i = threadIdx.x; i < cells; i += kThreads) {
-        const int t = i / kCols, c = i % kCols;
-        if (d0 + c >= s.d) continue;
-        const float sum = add_parts(w.y + t * row + d0 + c, plane, shares);
-        store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum);
+    constexpr int kEach = kMaxTokens * kCols / kThreads;
+    const float* parts[kEach];
+    float sum[kEach];
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {  // past the last cell: the first one's, not stored
+        const int i = threadIdx.x + n * kThreads, t = i / kCols, c = i % kCols;
+        parts[n] = w.y + (i < cells ? t * row + d0 + c : d0);
+    }
+    add_parts<kEach>(parts, plane, shares, sum);
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+        const int i = threadIdx.x + n * kThreads, t = i / kCols, c = i % kCols;
+        if (i < cells && d0 + c < s.d) store_one<kOut>(y, static_cast<long long>(t) * s.d + d0 + c, sum[n]);
     }
 }
 
