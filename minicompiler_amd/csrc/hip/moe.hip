@@ -426,7 +426,8 @@ struct Stream {
         u32x4 x[4][kP];
     };
 
-    const unsigned char* rows[kTiles];  // lane's, mx4: at its block
+    __amdgpu_buffer_rsrc_t rows[kTiles];  // from each tile's first row on, to the weights' end
+    int at[kTiles];                       // lane's row and chunk
     const unsigned char* scale_row;
     int shift[kTiles];
     const unsigned short* x;  // lane's token, at its chunk
@@ -436,21 +437,24 @@ struct Stream {
 
     __device__ __forceinline__ static int offset(int q, int s) { return kQuant ? 32 * q + 8 * s : 32 * s + 8 * q; }
 
-    // row_of(i): the row of the weights that lane has in tile i.
-    template <typename Rows>
-    __device__ __forceinline__ void open(const void* base, const unsigned char* scales, int k_, Rows row_of) {
+    // first(i): tile i's first row of `all`, the same in every lane.
+    template <typename First>
+    __device__ __forceinline__ void open(const void* base, const unsigned char* scales, int k_, long long all, First first) {
         const int lane = threadIdx.x % 64;
         r = lane % 16, q = lane / 16, k = k_;
+        const int row_bytes = kQuant ? padded(k) / 2 : 2 * k;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
-            const long long row = row_of(i);
+            const long long row = first(i), left = all - row;
+            const unsigned char* p = static_cast<const unsigned char*>(base) + row * row_bytes;
+            const int odd = kOdd ? static_cast<int>(reinterpret_cast<std::uintptr_t>(p) & 2) : 0;
+            // Whole dwords, to the one with the last element: what lies past it reads as zeros.
+            const int bytes = (odd + (left < 16 ? static_cast<int>(left) : 16) * row_bytes + 3) & ~3;
+            rows[i] = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p - odd), 0, bytes, 0x00020000);
+            shift[i] = kOdd ? (odd + r * row_bytes) & 2 : 0;
+            at[i] = odd + r * row_bytes - shift[i] + 16 * q;
             if constexpr (kQuant) {
-                rows[i] = static_cast<const unsigned char*>(base) + row * (padded(k) / 2) + q * 16;
-                if (q == i) scale_row = scales + row * (padded(k) / 32);
-            } else {
-                const unsigned char* p = static_cast<const unsigned char*>(base) + row * k * 2;
-                shift[i] = kOdd ? static_cast<int>(reinterpret_cast<std::uintptr_t>(p) & 2) : 0;
-                rows[i] = p - shift[i];
+                if (q == i) scale_row = scales + (row + (r < left ? r : 0)) * (padded(k) / 32);
             }
         }
     }
@@ -465,39 +469,22 @@ struct Stream {
             static_assert(kTiles <= 4);
 #pragma unroll
             for (int i = 0; i < kTiles; ++i)
-                st.w[i][0] = *reinterpret_cast<const u32x4*>(rows[i] + static_cast<long long>(t) * 64);
+                st.w[i][0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows[i], at[i], t * 64, 0));
             // A dword per row from one lane each, shared out later: a byte per
             // lane would be as many accesses as the codes.
             if (q < kTiles) st.scales = *reinterpret_cast<const unsigned*>(scale_row + t * 4);
         } else {
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
-                if constexpr (kOdd) st.shift[i] = shift[i];
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int k0 = t * kStep + offset(q, s);
-                    const unsigned char* p = rows[i] + k0 * 2;
-                    if (k0 + 8 <= k) {
-                        st.w[i][s] = *reinterpret_cast<const u32x4_dwords*>(p);
-                    } else {
-                        // Element by element; e[0] is the one before, which a shifted row's first dword holds.
-                        unsigned e[9];
-#pragma unroll
-                        for (int j = 0; j < 9; ++j)
-                            e[j] = k0 + j - 1 >= 0 && k0 + j - 1 < k
-                                       ? *reinterpret_cast<const unsigned short*>(p + shift[i] + 2 * (j - 1))
-                                       : 0u;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const bool back = kOdd && shift[i] != 0;
-                            st.w[i][s][j] = (back ? e[2 * j] : e[2 * j + 1]) | (back ? e[2 * j + 1] : e[2 * j + 2]) << 16;
-                        }
-                    }
+                for (int s = 0; s < 4; ++s)
+                    st.w[i][s] = __builtin_bit_cast(
+                        u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows[i], at[i] + 64 * s, t * 256, 0));
+                if constexpr (kOdd) {
+                    st.shift[i] = shift[i];
+                    if (q == 0)
+                        st.behind[i] = __builtin_amdgcn_raw_buffer_load_b32(rows[i], at[i] + 256, t * 256, 0);
                 }
-                if constexpr (kOdd)
-                    st.behind[i] = q == 0 && shift[i] != 0 && (t + 1) * kStep - 1 < k
-                                       ? *reinterpret_cast<const unsigned*>(rows[i] + (t + 1) * kStep * 2)
-                                       : 0u;
             }
         }
 #pragma unroll
@@ -506,6 +493,25 @@ struct Stream {
             for (int p = 0; p < kP; ++p)
                 st.x[s][p] = has ? *reinterpret_cast<const u32x4*>(x + p * x_plane + (t * kStep + offset(q, s)) / 8 * x_chunk)
                                  : u32x4{0, 0, 0, 0};
+    }
+
+    // Whether step t reaches past the end of 16-bit rows, into the next one's elements;
+    // those to zeros (x has zeros there, but they may be no numbers).
+    __device__ __forceinline__ bool past_end(int t) const { return !kQuant && (t + 1) * kStep > k; }
+    __device__ __forceinline__ void cut_off(int t, Step& st) const {
+        if constexpr (!kQuant) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int low = t * kStep + offset(q, s) + 2 * j - (kOdd && st.shift[i] != 0 ? 1 : 0);
+                        st.w[i][s][j] &= (low < k ? 0xffffu : 0u) | (low + 1 < k ? 0xffff0000u : 0u);
+                    }
+                if constexpr (kOdd) st.behind[i] = 0;
+            }
+        }
     }
 
     __device__ __forceinline__ void multiply(const Step& st, f32x4 (&acc)[kTiles]) const {
@@ -614,17 +620,16 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
     if (from >= to) return;
     const int h_rows = kGated ? 2 * s.h : s.h;
 
-    int job = from / tiles, expert = jobs[job].expert, token = jobs[job].token[r];
+    int job = from / tiles, expert = __builtin_amdgcn_readfirstlane(jobs[job].expert), token = jobs[job].token[r];
     const auto open = [&](int u, In& in) {
         if (u / tiles != job) {
             job = u / tiles;
-            expert = jobs[job].expert;
+            expert = __builtin_amdgcn_readfirstlane(jobs[job].expert);
             token = jobs[job].token[r];
         }
-        const int h0 = u % tiles * kUpCols;
-        in.open(w1, w1_scales, s.d, [&](int i) {
-            const int col = h0 + (kGated ? 0 : 16 * i) + r;
-            return static_cast<long long>(expert) * h_rows + (col < s.h ? col : s.h - 1) + (kGated && i == 1 ? s.h : 0);
+        const int h0 = u % tiles * kUpCols < s.h ? u % tiles * kUpCols : 0;  // past h: not used
+        in.open(w1, w1_scales, s.d, static_cast<long long>(s.experts) * h_rows, [&](int i) {
+            return static_cast<long long>(expert) * h_rows + (kGated ? h0 + i * s.h : h0 + 16 * i < s.h ? h0 + 16 * i : 0);
         });
         in.tokens(w.x + (token == kNone ? 0 : token) * 8, 8LL * s.tokens, static_cast<long long>(s.tokens) * s.dp,
                   token != kNone);
@@ -632,22 +637,20 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
     In in;
     typename In::Step now, next;
     open(from, in);
-    if (wave < steps) in.load(wave, now);
+    if (wave < steps) in.load(wave, next);
     for (int u = from; u < to; ++u) {
         const int of_job = u / tiles, of_expert = expert, h0 = u % tiles * kUpCols;
         f32x4 acc[kTiles];
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         for (int t = wave; t < steps; t += kWaves) {
-            // Decoding needs nothing of `in` but the lane's place: it may move on first.
-            if (t + kWaves < steps) {
-                in.load(t + kWaves, next);
-            } else if (u + 1 < to) {
-                open(u + 1, in);
-                in.load(wave, next);
-            }
-            in.multiply(now, acc);
             now = next;
+            const int then = t + kWaves < steps ? t + kWaves : wave;
+            const bool move = then == wave;  // to the next tile (multiplying needs nothing of `in` but the lane's place)
+            if (move && u + 1 < to) open(u + 1, in);
+            if (!move || u + 1 < to) in.load(then, next);
+            if (in.past_end(t)) in.cut_off(t, now);
+            in.multiply(now, acc);
         }
         if (wave >= steps && u + 1 < to) open(u + 1, in);
         f32x4(&sums)[kWaves][kTiles][64] = space[u & 1];
@@ -709,19 +712,18 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
     int expert = 0, token = kNone;
     float gate = 0.0f;
     const auto open = [&](int n) {
-        expert = w.job[n].expert;
+        expert = __builtin_amdgcn_readfirstlane(w.job[n].expert);
         token = w.job[n].token[r];
         gate = w.job[n].gate[r];
-        in.open(w2, w2_scales, s.h, [&](int i) {
-            const int col = d0 + 16 * i + r;
-            return static_cast<long long>(expert) * s.d + (col < s.d ? col : s.d - 1);
+        in.open(w2, w2_scales, s.h, static_cast<long long>(s.experts) * s.d, [&](int i) {
+            return static_cast<long long>(expert) * s.d + (d0 + 16 * i < s.d ? d0 + 16 * i : d0);
         });
         in.tokens(w.h + static_cast<long long>(n) * 16 * s.hp + r * 8, 16 * 8, h_plane, token != kNone);
     };
     int n = from / steps, t = from % steps;
     if (from < to) {
         open(n);
-        in.load(t, now);
+        in.load(t, next);
     }
     for (int u = from; u < to;) {
         const int of_expert = expert, of_token = token;
@@ -740,16 +742,16 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
         }
         // To the job's end or the wave's; the next step, of the next job too, is under way meanwhile.
         for (bool same = true; same && u < to; ++u) {
-            if (u + 1 < to) {
-                if (++t == steps) {
-                    t = 0;
-                    same = false;
-                    open(++n);
-                }
-                in.load(t, next);
-            }
-            in.multiply(now, acc);
             now = next;
+            const int of_t = t;
+            if (++t == steps) {
+                t = 0;
+                same = false;
+                if (u + 1 < to) open(++n);
+            }
+            if (u + 1 < to) in.load(t, next);
+            if (in.past_end(of_t)) in.cut_off(of_t, now);
+            in.multiply(now, acc);
         }
         if (of_token != kNone) {
 #pragma unroll
