@@ -3,6 +3,7 @@
 // scales exactly and adds in fp32.
 
 #include "gemm_mx4_tiles.h"
+#include "mx4_rows.h"
 
 namespace {
 
@@ -10,8 +11,7 @@ using namespace mx4;
 
 // A block computes 16 kM rows by 16 kN columns of C; its kWaves waves take the
 // steps of 128 k in turn and their sums are added at the end. Fragments come
-// straight from memory: a lane's 16 bytes of codes are one block of a row, four
-// lanes read 64 bytes of it. Rows past the edge read the last row.
+// straight from memory, the next step's while one is multiplied.
 template <int kM, int kN, int kWaves, int kOut>
 __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned char* __restrict__ a_codes,
                                                               const unsigned char* __restrict__ a_scales,
@@ -20,45 +20,41 @@ __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned cha
                                                               void* __restrict__ c, int m, int n, int steps,
                                                               unsigned tiles_n) {
     __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
     const long long row0 = static_cast<long long>(blockIdx.x / tiles_n) * 16 * kM;
     const long long col0 = static_cast<long long>(blockIdx.x % tiles_n) * 16 * kN;
-
-    const unsigned char *ac[kM], *as[kM], *bc[kN], *bs[kN];
-#pragma unroll
-    for (int i = 0; i < kM; ++i) {
-        const long long row = row0 + 16 * i + r < m ? row0 + 16 * i + r : m - 1;
-        ac[i] = a_codes + row * steps * 64 + q * 16;
-        as[i] = a_scales + row * steps * 4 + q;
-    }
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
-        const long long col = col0 + 16 * j + r < n ? col0 + 16 * j + r : n - 1;
-        bc[j] = b_codes + col * steps * 64 + q * 16;
-        bs[j] = b_scales + col * steps * 4 + q;
-    }
+    Rows<kMx4, kM> a;
+    Rows<kMx4, kN> b;
+    a.open(a_codes, a_scales, steps * kStep, m, [&](int i) { return row0 + 16 * i < m ? row0 + 16 * i : 0; });
+    b.open(b_codes, b_scales, steps * kStep, n, [&](int j) { return col0 + 16 * j < n ? col0 + 16 * j : 0; });
     f32x4 acc[kM * kN];
 #pragma unroll
     for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
+    typename Rows<kMx4, kM>::Step a_now, a_next;
+    typename Rows<kMx4, kN>::Step b_now, b_next;
+    if (wave < steps) {
+        a.load(wave, a_next);
+        b.load(wave, b_next);
+    }
     for (int t = wave; t < steps; t += kWaves) {
-        i32x4 av[kM], bv[kN];
+        a_now = a_next;
+        b_now = b_next;
+        if (t + kWaves < steps) {
+            a.load(t + kWaves, a_next);
+            b.load(t + kWaves, b_next);
+        }
         int sa[kM], sb[kN];
 #pragma unroll
-        for (int i = 0; i < kM; ++i) {
-            av[i] = *reinterpret_cast<const i32x4*>(ac[i] + static_cast<long long>(t) * 64);
-            sa[i] = as[i][t * 4];
-        }
+        for (int i = 0; i < kM; ++i) sa[i] = static_cast<int>(a.scale(a_now, i));
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            bv[j] = *reinterpret_cast<const i32x4*>(bc[j] + static_cast<long long>(t) * 64);
-            sb[j] = bs[j][t * 4];
-        }
+        for (int j = 0; j < kN; ++j) sb[j] = static_cast<int>(b.scale(b_now, j));
 #pragma unroll
         for (int i = 0; i < kM; ++i)
 #pragma unroll
-            for (int j = 0; j < kN; ++j) acc[i * kN + j] = mfma(bv[j], sb[j], av[i], sa[i], acc[i * kN + j]);
+            for (int j = 0; j < kN; ++j)
+                acc[i * kN + j] = mfma(__builtin_bit_cast(i32x4, b_now.w[j][0]), sb[j],
+                                       __builtin_bit_cast(i32x4, a_now.w[i][0]), sa[i], acc[i * kN + j]);
     }
     add_waves<kWaves, kM * kN>(acc, space, wave, lane);
     if (wave != 0) return;

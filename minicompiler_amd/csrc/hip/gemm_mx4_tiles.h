@@ -42,27 +42,11 @@ struct Constant {
     static constexpr int value = kValue;
 };
 
-#define MX4_LDS __attribute__((address_space(3)))
-
 constexpr int kTileRows = 256, kTileCols = 256, kTileThreads = 256;
 constexpr int kStageBytes = 64 * 1024, kStageB = 32 * 1024;
 constexpr int kSlotBytes = 16 * 1024, kSlotHalf = 8 * 1024, kSlotB = 4 * 1024;
 constexpr int kRingBytes = 2 * kStageBytes + 2 * kSlotBytes;
 constexpr int kColFrags = 8;
-
-__device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t rsrc, MX4_LDS unsigned char* dst, int voffset,
-                                              int soffset) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, reinterpret_cast<MX4_LDS void*>(dst), 16, voffset, soffset, 0, 0);
-}
-
-// A workgroup barrier without a memory fence, which nothing is moved across.
-__device__ __forceinline__ void stage_barrier() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
 
 // `rows` rows of `row_bytes` from p on; what lies past them reads as zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const unsigned char* p, int rows, int row_bytes) {
@@ -273,7 +257,7 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
 #pragma unroll
     for (int i = 0; i < 5; ++i) store_scales<kRows>(slots, L, first[i], i);
     __builtin_amdgcn_s_waitcnt(0);
-    stage_barrier();
+    lds_barrier();
 
     constexpr int kI = Lane::kRowFrags, kB = kColFrags / kI;
     i32x4 av[kI], bv[2][kColFrags];
@@ -318,7 +302,7 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
             if (i == 0) av[kI - 1] = read_a<kRows>(here, L, 1, kI - 1);
             if (i == 2) {
                 __builtin_amdgcn_s_waitcnt(0);
-                stage_barrier();
+                lds_barrier();
                 store_scales<kRows>(slots, L, scales, s + 5);
                 scales = load_scales<kRows>(L, s + 6);
                 av[0] = read_a<kRows>(there, L, 0, 0);

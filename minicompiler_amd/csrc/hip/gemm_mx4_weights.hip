@@ -5,67 +5,152 @@
 // exact in bf16: a weight (two significant bits and a power of two), and A cut
 // into one, two or three bf16 pieces (8, 11 or 24 significant bits), each
 // multiplied by the same weights into the same fp32 sum.
+//
+//   weights_few     up to 8 rows: A cut by every wave as it reads it;
+//   cut_rows        A's pieces into the workspace, for the two below:
+//   weights_direct  few tiles: a block's waves share out k, fragments come
+//                   straight from memory;
+//   weights_tiles   many: 128x128 tiles, k in stages through LDS.
+// The pieces are kept as [pieces][kp / 8][rows][8], a row's eight elements beside
+// its neighbours', so that a fragment of 16 rows is read in whole lines.
 
-#include "mx4_device.h"
+#include "mx4_rows.h"
 
 namespace {
 
 using namespace mx4;
 
-// A block computes 16 kM rows by 16 kN columns of C; its kWaves waves take the
-// steps of 128 k in turn and their sums are added at the end. Lane (r, q) of a
-// wave holds block q of weight row r: dword s of its codes, decoded, is the
-// operand of instruction s, so group q supplies elements 32 q + 8 s .. + 7.
-template <int kIn, int kM, int kN, int kWaves, int kOut>
-__global__ __launch_bounds__(kWaves * 64) void weights_direct(const void* __restrict__ a, long long lda,
-                                                              const unsigned char* __restrict__ b_codes,
-                                                              const unsigned char* __restrict__ b_scales,
-                                                              void* __restrict__ c, int m, int n, int k, int steps,
-                                                              unsigned tiles_n) {
-    constexpr int kP = kPieces<kIn>;
-    __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-    const int r = lane % 16, q = lane / 16;
-    const long long row0 = static_cast<long long>(blockIdx.x / tiles_n) * 16 * kM;
-    const long long col0 = static_cast<long long>(blockIdx.x % tiles_n) * 16 * kN;
+constexpr int kFew = 8;
+constexpr int kWaves = 8;
 
-    const unsigned char *bc[kN], *bs[kN];
+// ---------------------------------------------------------------- few rows
+
+// Four instructions' operands of 16 rows of A from element k0 = 128 t on, cut into
+// pieces; zeros past k and for lanes without a row.
+template <int kIn>
+__device__ __forceinline__ void cut_step(const void* a, long long at, bool has, int k0, int k, int q,
+                                         u32x4 (&x)[4][kPieces<kIn>]) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const int e = k0 + 32 * q + 8 * s;
+        float v[8];
+        load_eight<kIn>(a, at + e, has ? k - e : 0, v);
+        cut_eight<kPieces<kIn>>(v, x[s]);
+    }
+}
+
+// 16 kN columns of C for all rows (at most 16); the waves take the steps of 128 k
+// in turn, the next one under way while one is multiplied.
+template <int kIn, int kN, int kOut>
+__global__ __launch_bounds__(kWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
+                                                           const unsigned char* __restrict__ b_codes,
+                                                           const unsigned char* __restrict__ b_scales,
+                                                           void* __restrict__ c, int m, int n, int k) {
+    constexpr int kP = kPieces<kIn>;
+    __shared__ f32x4 space[kWaves / 2 * kN * 64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep;
+    const long long col0 = static_cast<long long>(blockIdx.x) * 16 * kN;
+    Rows<kMx4, kN> b;
+    b.open(b_codes, b_scales, k, n, [&](int j) { return col0 + 16 * j < n ? col0 + 16 * j : 0; });
+    const bool has = r < m;
+    const long long at = has ? r * lda : 0;
+    f32x4 acc[kN];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    typename Rows<kMx4, kN>::Step now, next;
+    if (wave < steps) b.load(wave, next);
+    for (int t = wave; t < steps; t += kWaves) {
+        now = next;
+        if (t + kWaves < steps) b.load(t + kWaves, next);
+        u32x4 x[4][kP];
+        cut_step<kIn>(a, at, has, t * kStep, k, q, x);
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            const float scale = scale_operand(b.scale(now, j));
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const u32x4 w = decode_eight(now.w[j][0][s], scale);
+#pragma unroll
+                for (int p = 0; p < kP; ++p) acc[j] = mfma_bf16(w, x[s][p], acc[j]);
+            }
+        }
+    }
+    add_waves<kWaves, kN>(acc, space, wave, lane);
+    if (wave != 0 || !has) return;
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
-        const long long col = col0 + 16 * j + r < n ? col0 + 16 * j + r : n - 1;
-        bc[j] = b_codes + col * steps * 64 + q * 16;
-        bs[j] = b_scales + col * steps * 4 + q;
+        const long long col = col0 + 16 * j + 4 * q;
+        if (col < n) store_four<kOut>(c, r * static_cast<long long>(n) + col, acc[j], static_cast<int>(n - col < 4 ? n - col : 4));
     }
+}
+
+// ---------------------------------------------------------------- pieces
+
+// A lane a row's eight elements; neighbouring lanes neighbouring rows, so that
+// the pieces are written in whole lines.
+template <int kIn>
+__global__ __launch_bounds__(256) void cut_rows(const void* __restrict__ a, long long lda, unsigned short* __restrict__ out,
+                                                int m, int rows, int k, int chunks) {
+    constexpr int kP = kPieces<kIn>;
+    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<long long>(rows) * chunks;
+    if (i >= all) return;
+    const int row = static_cast<int>(i % rows), e = static_cast<int>(i / rows) * 8;
+    float v[8];
+    load_eight<kIn>(a, row < m ? row * lda + e : 0, row < m ? k - e : 0, v);
+    u32x4 x[kP];
+    cut_eight<kP>(v, x);
+#pragma unroll
+    for (int p = 0; p < kP; ++p) *reinterpret_cast<u32x4*>(out + (p * all + i) * 8) = x[p];
+}
+
+// 16 kM rows by 16 kN columns of C per block, A in pieces (`rows` of them, a multiple of 16).
+template <int kP, int kM, int kN, int kOut>
+__global__ __launch_bounds__(kWaves * 64) void weights_direct(const unsigned short* __restrict__ a,
+                                                              const unsigned char* __restrict__ b_codes,
+                                                              const unsigned char* __restrict__ b_scales,
+                                                              void* __restrict__ c, int m, int rows, int n, int k,
+                                                              unsigned tiles_n) {
+    __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep;
+    const int row0 = static_cast<int>(blockIdx.x / tiles_n) * 16 * kM;
+    const long long col0 = static_cast<long long>(blockIdx.x % tiles_n) * 16 * kN;
+    Rows<kMx4, kN> b;
+    b.open(b_codes, b_scales, k, n, [&](int j) { return col0 + 16 * j < n ? col0 + 16 * j : 0; });
+    const unsigned short* x[kM];
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+        const int row = row0 + 16 * i < rows ? row0 + 16 * i + r : r;
+        x[i] = a + (static_cast<long long>(4 * q) * rows + row) * 8;
+    }
+    const long long plane = static_cast<long long>(rows) * padded(k), chunk = 8LL * rows;
     f32x4 acc[kM * kN];
 #pragma unroll
     for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
+    typename Rows<kMx4, kN>::Step now, next;
+    if (wave < steps) b.load(wave, next);
     for (int t = wave; t < steps; t += kWaves) {
-        u32x4 codes[kN];
+        now = next;
+        if (t + kWaves < steps) b.load(t + kWaves, next);
         float scale[kN];
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            codes[j] = *reinterpret_cast<const u32x4*>(bc[j] + static_cast<long long>(t) * 64);
-            scale[j] = scale_operand(bs[j][t * 4]);
-        }
+        for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const int k0 = t * kStep + 32 * q + 8 * s;
-            u32x4 x[kM][kP];
+            u32x4 xs[kM][kP];
 #pragma unroll
-            for (int i = 0; i < kM; ++i) {
-                const long long row = row0 + 16 * i + r;
-                float v[8];
-                load_eight<kIn>(a, row * lda + k0, row < m ? k - k0 : 0, v);
-                cut_eight<kP>(v, x[i]);
-            }
+            for (int i = 0; i < kM; ++i)
+#pragma unroll
+                for (int p = 0; p < kP; ++p)
+                    xs[i][p] = *reinterpret_cast<const u32x4*>(x[i] + p * plane + (t * 16 + s) * chunk);
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-                const u32x4 w = decode_eight(codes[j][s], scale[j]);
+                const u32x4 w = decode_eight(now.w[j][0][s], scale[j]);
 #pragma unroll
                 for (int i = 0; i < kM; ++i)
 #pragma unroll
-                    for (int p = 0; p < kP; ++p) acc[i * kN + j] = mfma_bf16(w, x[i][p], acc[i * kN + j]);
+                    for (int p = 0; p < kP; ++p) acc[i * kN + j] = mfma_bf16(w, xs[i][p], acc[i * kN + j]);
             }
         }
     }
@@ -73,57 +158,222 @@ __global__ __launch_bounds__(kWaves * 64) void weights_direct(const void* __rest
     if (wave != 0) return;
 #pragma unroll
     for (int i = 0; i < kM; ++i) {
-        const long long row = row0 + 16 * i + r;
+        const int row = row0 + 16 * i + r;
         if (row >= m) continue;
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
             const long long col = col0 + 16 * j + 4 * q;
             if (col < n)
-                store_four<kOut>(c, row * n + col, acc[i * kN + j], static_cast<int>(n - col < 4 ? n - col : 4));
+                store_four<kOut>(c, static_cast<long long>(row) * n + col, acc[i * kN + j],
+                                 static_cast<int>(n - col < 4 ? n - col : 4));
         }
     }
 }
+
+// ---------------------------------------------------------------- large tiles
+
+constexpr int kTile = 128, kTileThreads = 256;
+constexpr int kStageA = 16 * 1024, kStagesA = 3;
+constexpr int kStageB = 8 * 1024 + 512;  // codes, then a dword of scales per row
+constexpr int kLdsBytes = kStagesA * kStageA + 2 * kStageB;
+
+// 128x128 tiles by 4 waves in a 2x2 grid, each a 64x64 quadrant as 4x4
+// accumulators; two blocks per CU, so that one multiplies while the other
+// waits. A step of 128 k brings one stage of B (codes and scales), decoded once
+// into registers, and 2 kP stages of A, each a piece's half of the chunks (those
+// of instructions 0 and 1, then 2 and 3: chunks 4 q + 2 h and 4 q + 2 h + 1).
+//
+// LDS: A as [8 chunks][128 rows][16 bytes], as it lies in memory, a fetch
+// instruction 64 rows of a chunk, a fragment read 16 rows of four chunks, no bank
+// twice per 16 lanes; B's rows of 64 bytes, block c at c ^ (r / 2 % 4). One
+// barrier per stage: stage i has landed and stage i - 1 has been read, so i + 2
+// is fetched over it.
+template <int kP, int kOut>
+__global__ __launch_bounds__(kTileThreads, 2) void weights_tiles(const unsigned short* __restrict__ a,
+                                                                 const unsigned char* __restrict__ b_codes,
+                                                                 const unsigned char* __restrict__ b_scales,
+                                                                 void* __restrict__ c, int m, int rows, int n, int k,
+                                                                 int tiles_n) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kLdsBytes];
+    MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int r = lane % 16, q = lane / 16;
+    const int kp = padded(k), steps = kp / kStep, stages = steps * 2 * kP;
+    const int row0 = static_cast<int>(blockIdx.x) / tiles_n * kTile, col0 = static_cast<int>(blockIdx.x) % tiles_n * kTile;
+
+    // What lies past the operands reads as zeros.
+    const int a_left = rows - row0 < kTile ? rows - row0 : kTile, b_left = n - col0 < kTile ? n - col0 : kTile;
+    const long long plane = static_cast<long long>(rows) * kp;
+    const unsigned char* b_tile = b_codes + static_cast<long long>(col0) * (kp / 2);
+    const __amdgpu_buffer_rsrc_t b_rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(b_tile), 0, b_left * (kp / 2), 0x00020000);
+    const __amdgpu_buffer_rsrc_t s_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char*>(b_scales + static_cast<long long>(col0) * (kp / 32)), 0, b_left * (kp / 32), 0x00020000);
+    // Waves 2 i and 2 i + 1 fetch rows 0-63 and 64-127 of chunks 4 j + 2 h + i, j = 0..3.
+    const int a_row = wave % 2 * 64 + lane;
+    const int b_src = (wave * 32 + lane / 4) * (kp / 2) + (lane % 4 ^ lane / 8 % 4) * 16;
+
+    const auto fetch_a = [&](int i) {
+        const int t = i / (2 * kP), p = i % (2 * kP) / 2, h = i % 2;
+        MX4_LDS unsigned char* to = lds + i % kStagesA * kStageA;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int chunk = 4 * j + 2 * h + wave / 2;
+            const unsigned short* from = a + p * plane + (static_cast<long long>(t * 16 + chunk) * rows + row0) * 8;
+            const __amdgpu_buffer_rsrc_t rsrc =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(from), 0, a_left * 16, 0x00020000);
+            buffer_to_lds(rsrc, to + (2 * j + wave / 2) * 2048 + wave % 2 * 1024, a_row * 16, 0);
+        }
+    };
+    const auto fetch_b = [&](int t) {
+        MX4_LDS unsigned char* to = lds + kStagesA * kStageA + (t & 1) * kStageB;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) buffer_to_lds(b_rsrc, to + (wave * 2 + j) * 1024, b_src + j * 16 * (kp / 2), t * 64);
+        if (wave < 2)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(s_rsrc, reinterpret_cast<MX4_LDS void*>(to + 8192 + wave * 256), 4,
+                                                     (wave * 64 + lane) * (kp / 32), t * 4, 0, 0);
+    };
+
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int wave_row = wave / 2 * 64, wave_col = wave % 2 * 64;
+    fetch_b(0);
+    fetch_a(0);
+    fetch_a(1);
+    int i = 0;
+    for (int t = 0; t < steps; ++t) {
+        u32x4 w[4][4];
+#pragma unroll
+        for (int part = 0; part < 2 * kP; ++part, ++i) {
+            // Stage i (and this step's B, fetched before) has landed once the four fetches of i + 1 are left;
+            // this wave's reads of stage i - 1 are over.
+            __builtin_amdgcn_s_waitcnt(0x0074);  // vmcnt(4), lgkmcnt(0)
+            lds_barrier();
+            if (part == 0 && t + 1 < steps) fetch_b(t + 1);
+            fetch_a(i + 2 < stages ? i + 2 : stages - 1);
+            const MX4_LDS unsigned char* from = lds + i % kStagesA * kStageA;
+            if (part == 0) {
+                const MX4_LDS unsigned char* b = lds + kStagesA * kStageA + (t & 1) * kStageB;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = wave_col + 16 * j + r;
+                    const u32x4 codes = *reinterpret_cast<const MX4_LDS u32x4*>(b + row * 64 + (q ^ r / 2 % 4) * 16);
+                    const float scale = scale_operand(b[8192 + row * 4 + q]);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) w[j][s] = decode_eight(codes[s], scale);
+                }
+            }
+            u32x4 x[4][2];
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                    x[f][s] = *reinterpret_cast<const MX4_LDS u32x4*>(from + (2 * q + s) * 2048 + (wave_row + 16 * f + r) * 16);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[f][j] = mfma_bf16(w[j][part % 2 * 2 + s], x[f][s], acc[f][j]);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // no fetch may land in LDS that is another block's
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+        const int row = row0 + wave_row + 16 * f + r;
+        if (row >= m) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int col = col0 + wave_col + 16 * j + 4 * q;
+            if (col < n) store_four<kOut>(c, static_cast<long long>(row) * n + col, acc[f][j], n - col);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
 
 struct Product {
     const void* a;
     long long lda;
     const unsigned char *b_codes, *b_scales;
     void* c;
-    int m, n, k, steps;
+    int m, n, k;
+    unsigned short* pieces;
     hipStream_t stream;
 };
 
-long long tiles(int size, int tile) { return (static_cast<long long>(size) + tile - 1) / tile; }
+long long tiles(long long size, int tile) { return (size + tile - 1) / tile; }
+int piece_rows(int m) { return (m + 15) / 16 * 16; }
 
-template <int kIn, int kM, int kN, int kOut>
-int launch_direct(const Product& p) {
-    constexpr int kWaves = 8;
-    const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((weights_direct<kIn, kM, kN, kWaves, kOut>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(kWaves * 64), 0, p.stream, p.a, p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k, p.steps,
-                       static_cast<unsigned>(tn));
+template <int kIn, int kN, int kOut>
+int launch_few(const Product& p) {
+    hipLaunchKernelGGL((weights_few<kIn, kN, kOut>), dim3(static_cast<unsigned>(tiles(p.n, 16 * kN))), dim3(kWaves * 64), 0,
+                       p.stream, p.a, p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
     return hipGetLastError();
 }
 
+template <int kP, int kM, int kN, int kOut>
+int launch_direct(const Product& p) {
+    const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((weights_direct<kP, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64), 0, p.stream,
+                       p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k, static_cast<unsigned>(tn));
+    return hipGetLastError();
+}
+
+template <int kP, int kOut>
+int launch_pieces(const Product& p) {
+    const int cus = device_cus();
+    const auto blocks = [&](int bm, int bn) { return tiles(p.m, 16 * bm) * tiles(p.n, 16 * bn); };
+    // 32-bit offsets from a tile's origin.
+    if (blocks(8, 8) >= cus && p.k <= (1 << 22) && tiles(p.m, kTile) * tiles(p.n, kTile) < 0x7fffffffLL) {
+        hipLaunchKernelGGL((weights_tiles<kP, kOut>), dim3(static_cast<unsigned>(blocks(8, 8))), dim3(kTileThreads), 0, p.stream,
+                           p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
+                           static_cast<int>(tiles(p.n, kTile)));
+        return hipGetLastError();
+    }
+    if (p.m > 32 && blocks(4, 2) >= cus) return launch_direct<kP, 4, 2, kOut>(p);
+    if (p.m > 16 && blocks(2, 2) >= cus) return launch_direct<kP, 2, 2, kOut>(p);
+    if (p.m > 16) return launch_direct<kP, 2, 1, kOut>(p);
+    if (blocks(1, 2) >= cus) return launch_direct<kP, 1, 2, kOut>(p);
+    return launch_direct<kP, 1, 1, kOut>(p);
+}
+
 template <int kIn, int kOut>
-int launch_shape(const Product& p) {
-    if (p.m <= 16) return launch_direct<kIn, 1, 2, kOut>(p);
-    return launch_direct<kIn, 2, 2, kOut>(p);
+int launch(const Product& p) {
+    if (p.m <= kFew) {
+        if (tiles(p.n, 32) >= device_cus()) return launch_few<kIn, 2, kOut>(p);
+        return launch_few<kIn, 1, kOut>(p);
+    }
+    const int rows = piece_rows(p.m), chunks = padded(p.k) / 8;
+    const long long blocks = tiles(static_cast<long long>(rows) * chunks, 256);
+    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(cut_rows<kIn>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, p.stream, p.a, p.lda, p.pieces, p.m,
+                       rows, p.k, chunks);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return launch_pieces<kPieces<kIn>, kOut>(p);
 }
 
 template <int kIn>
-int launch(int c_dtype, const Product& p) {
-    if (c_dtype == kF32) return launch_shape<kIn, kF32>(p);
-    if (c_dtype == kBf16) return launch_shape<kIn, kBf16>(p);
-    return launch_shape<kIn, kF16>(p);
+int launch_out(int c_dtype, const Product& p) {
+    if (c_dtype == kF32) return launch<kIn, kF32>(p);
+    if (c_dtype == kBf16) return launch<kIn, kBf16>(p);
+    return launch<kIn, kF16>(p);
 }
 
 }  // namespace
 
 extern "C" {
 
-long long mchip_matmul_mx4_weights_workspace_bytes(int a_dtype, int m, int n, int k) { return 0; }
+long long mchip_matmul_mx4_weights_workspace_bytes(int a_dtype, int m, int n, int k) {
+    if (!is_float_type(a_dtype) || m <= kFew || n < 1 || k < 1 || k > (1 << 24)) return 0;
+    const int pieces = a_dtype == kF32 ? kPieces<kF32> : a_dtype == kBf16 ? kPieces<kBf16> : kPieces<kF16>;
+    return 2LL * pieces * ((static_cast<long long>(m) + 15) / 16 * 16) * padded(k);
+}
 
 int mchip_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, const void* b_codes,
                                     const void* b_scales, int c_dtype, void* c, int m, int n, int k, void* stream,
@@ -131,6 +381,7 @@ int mchip_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, c
     *why = nullptr;
     if (!is_float_type(a_dtype) || !is_float_type(c_dtype)) *why = "a type that is none of fp32 (0), bf16 (1), fp16 (2)";
     else if (m < 1 || n < 1 || k < 1) *why = "a size below 1";
+    else if (m > (1 << 30)) *why = "m above 2^30";
     else if (k > (1 << 24)) *why = "k above 2^24";
     else if (lda < k) *why = "rows of A closer together than they are long";
     else if (!a || !b_codes || !b_scales || !c) *why = "a null operand";
@@ -138,13 +389,14 @@ int mchip_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, c
     else if (!aligned(b_scales, 4)) *why = "scales not 4-byte aligned";
     else if (!aligned(a, size_of(a_dtype)) || !aligned(c, size_of(c_dtype)))
         *why = "an address that is no multiple of its element's size";
+    else if (m > kFew && (workspace == nullptr || !aligned(workspace, 256)))
+        *why = "no workspace, or one that is not 256-byte aligned";
     if (*why != nullptr) return hipErrorInvalidValue;
     Product p{a, lda, static_cast<const unsigned char*>(b_codes), static_cast<const unsigned char*>(b_scales),
-              c, m, n, k, static_cast<int>(mchip_mx4_k(k) / kStep),
-              static_cast<hipStream_t>(stream)};
-    const int rc = a_dtype == kF32   ? launch<kF32>(c_dtype, p)
-                   : a_dtype == kBf16 ? launch<kBf16>(c_dtype, p)
-                                      : launch<kF16>(c_dtype, p);
+              c, m, n, k, static_cast<unsigned short*>(workspace), static_cast<hipStream_t>(stream)};
+    const int rc = a_dtype == kF32   ? launch_out<kF32>(c_dtype, p)
+                   : a_dtype == kBf16 ? launch_out<kBf16>(c_dtype, p)
+                                      : launch_out<kF16>(c_dtype, p);
     if (rc == hipErrorInvalidValue) *why = "more tiles of C than one launch takes";
     return rc;
 }

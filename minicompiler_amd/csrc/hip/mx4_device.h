@@ -225,6 +225,24 @@ __device__ __forceinline__ u32x4 decode_eight(unsigned codes, float scale) {
 // scale byte (they read no more of it; field 0 counts as 2^-127, 255 as NaN).
 __device__ __forceinline__ float scale_operand(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
 
+#define MX4_LDS __attribute__((address_space(3)))
+
+// 16 bytes per lane from memory to LDS without registers, lane l at dst + 16 l.
+__device__ __forceinline__ void buffer_to_lds(__amdgpu_buffer_rsrc_t rsrc, MX4_LDS unsigned char* dst, int voffset,
+                                              int soffset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, reinterpret_cast<MX4_LDS void*>(dst), 16, voffset, soffset, 0, 0);
+}
+
+// A workgroup barrier without a memory fence (which would wait for fetches in
+// flight), which nothing is moved across.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // The partial sums of a block's waves (kWaves, a power of two; each `kCount`
 // vectors per lane) added up in wave 0, pairs in a fixed order: half the waves
 // write, the other half add. `space`: kWaves / 2 * kCount * 64 vectors.

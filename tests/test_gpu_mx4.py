@@ -213,7 +213,9 @@ def test_a_block_without_a_scale_reaches_its_rows_alone(device, mc, m, n):
 
 WEIGHTS = [(1, 1, 1, 0), (1, 14, 130, 0), (1, 1000, 4096, 0), (2, 33, 77, 3), (5, 128, 512, 8), (16, 257, 1023, 0),
            (17, 64, 257, 1), (32, 500, 640, 0), (33, 100, 128, 4), (64, 129, 300, 0), (65, 300, 1000, 0),
-           (128, 256, 256, 0), (200, 77, 2048, 8), (300, 513, 129, 5), (700, 600, 520, 0)]
+           (128, 256, 256, 0), (200, 77, 2048, 8), (300, 513, 129, 5), (700, 600, 520, 0),
+           (8, 5000, 384, 1), (9, 4100, 250, 0), (40, 4097, 700, 2), (130, 4500, 200, 0), (2050, 2060, 390, 0),
+           (2200, 2201, 640, 3)]
 
 
 @pytest.mark.parametrize("kind", sorted(ref.TYPES))
