@@ -25,22 +25,72 @@ constexpr int kWaves = 8;
 
 // ---------------------------------------------------------------- few rows
 
-// Four instructions' operands of 16 rows of A from element k0 = 128 t on, cut into
-// pieces; zeros past k and for lanes without a row.
+// Eight elements of a row, as they lie in memory; zeros from `left` on.
 template <int kIn>
-__device__ __forceinline__ void cut_step(const void* a, long long at, bool has, int k0, int k, int q,
-                                         u32x4 (&x)[4][kPieces<kIn>]) {
+struct Eight {
+    u32x4 v[kIn == kF32 ? 2 : 1];
+
+    __device__ __forceinline__ void load(const void* a, long long at, int left) {
+        if (left >= 8) {
+            if constexpr (kIn == kF32) {
+                const u32x4_dwords* p = reinterpret_cast<const u32x4_dwords*>(static_cast<const float*>(a) + at);
+                v[0] = p[0];
+                v[1] = p[1];
+            } else {
+                v[0] = *reinterpret_cast<const u32x4_loose*>(static_cast<const unsigned short*>(a) + at);
+            }
+            return;
+        }
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        const int e = k0 + 32 * q + 8 * s;
-        float v[8];
-        load_eight<kIn>(a, at + e, has ? k - e : 0, v);
-        cut_eight<kPieces<kIn>>(v, x[s]);
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (kIn == kF32) {
+                v[e / 4][e % 4] = e < left ? static_cast<const unsigned*>(a)[at + e] : 0u;
+            } else {
+                const unsigned h = e < left ? static_cast<const unsigned short*>(a)[at + e] : 0u;
+                v[0][e / 2] = e % 2 ? v[0][e / 2] | h << 16 : h;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void pieces(u32x4 (&out)[kPieces<kIn>]) const {
+        if constexpr (kIn == kBf16) {
+            out[0] = v[0];
+        } else {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned word = kIn == kF32 ? v[kIn == kF32 ? e / 4 : 0][e % 4] : v[0][e / 2 % 4];
+                f[e] = to_f32<kIn>(kIn == kF32 ? word : e % 2 ? word >> 16 : word & 0xffffu);
+            }
+            cut_eight<kPieces<kIn>>(f, out);
+        }
+    }
+};
+
+// The steps from `first` on, kWaves apart, of the weights `b`, four under way at
+// a time: fetch(t) is called, and then the step's multiplied. (One at a time, the
+// steps' latencies added up: 31 MB in 14 us.) What fetch loads for step t is
+// loaded before the weights of step t + 4 kWaves, because loads arrive in order.
+template <typename Weights, typename Fetch, typename Multiply>
+__device__ __forceinline__ void four_ahead(const Weights& b, int first, int steps, Fetch fetch, Multiply multiply) {
+    typename Weights::Step ring[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (first + j * kWaves < steps) b.load(first + j * kWaves, ring[j]);
+    for (int t = first; t < steps;) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (t >= steps) break;
+            fetch(t);
+            multiply(t, ring[j]);
+            if (t + 4 * kWaves < steps) b.load(t + 4 * kWaves, ring[j]);
+            t += kWaves;
+        }
     }
 }
 
 // 16 kN columns of C for all rows (at most 16); the waves take the steps of 128 k
-// in turn, the next one under way while one is multiplied.
+// in turn.
 template <int kIn, int kN, int kOut>
 __global__ __launch_bounds__(kWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
                                                            const unsigned char* __restrict__ b_codes,
@@ -58,24 +108,32 @@ __global__ __launch_bounds__(kWaves * 64) void weights_few(const void* __restric
     f32x4 acc[kN];
 #pragma unroll
     for (int j = 0; j < kN; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    typename Rows<kMx4, kN>::Step now, next;
-    if (wave < steps) b.load(wave, next);
-    for (int t = wave; t < steps; t += kWaves) {
-        now = next;
-        if (t + kWaves < steps) b.load(t + kWaves, next);
-        u32x4 x[4][kP];
-        cut_step<kIn>(a, at, has, t * kStep, k, q, x);
+    Eight<kIn> x[4];
+    four_ahead(
+        b, wave, steps,
+        [&](int t) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            const float scale = scale_operand(b.scale(now, j));
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const u32x4 w = decode_eight(now.w[j][0][s], scale);
-#pragma unroll
-                for (int p = 0; p < kP; ++p) acc[j] = mfma_bf16(w, x[s][p], acc[j]);
+            for (int i = 0; i < 4; ++i) {
+                const int e = t * kStep + 32 * q + 8 * i;
+                x[i].load(a, at + e, has ? k - e : 0);
             }
-        }
-    }
+        },
+        [&](int, const typename Rows<kMx4, kN>::Step& now) {
+            float scale[kN];
+#pragma unroll
+            for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u32x4 piece[kP];
+                x[i].pieces(piece);
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    const u32x4 w = decode_eight(now.w[j][0][i], scale[j]);
+#pragma unroll
+                    for (int p = 0; p < kP; ++p) acc[j] = mfma_bf16(w, piece[p], acc[j]);
+                }
+            }
+        });
     add_waves<kWaves, kN>(acc, space, wave, lane);
     if (wave != 0 || !has) return;
 #pragma unroll
@@ -128,32 +186,33 @@ __global__ __launch_bounds__(kWaves * 64) void weights_direct(const unsigned sho
     f32x4 acc[kM * kN];
 #pragma unroll
     for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    typename Rows<kMx4, kN>::Step now, next;
-    if (wave < steps) b.load(wave, next);
-    for (int t = wave; t < steps; t += kWaves) {
-        now = next;
-        if (t + kWaves < steps) b.load(t + kWaves, next);
-        float scale[kN];
+    u32x4 xs[4][kM][kP];
+    four_ahead(
+        b, wave, steps,
+        [&](int t) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            u32x4 xs[kM][kP];
-#pragma unroll
-            for (int i = 0; i < kM; ++i)
-#pragma unroll
-                for (int p = 0; p < kP; ++p)
-                    xs[i][p] = *reinterpret_cast<const u32x4*>(x[i] + p * plane + (t * 16 + s) * chunk);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const u32x4 w = decode_eight(now.w[j][0][s], scale[j]);
+            for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int i = 0; i < kM; ++i)
 #pragma unroll
-                    for (int p = 0; p < kP; ++p) acc[i * kN + j] = mfma_bf16(w, xs[i][p], acc[i * kN + j]);
-            }
-        }
-    }
+                    for (int p = 0; p < kP; ++p)
+                        xs[e][i][p] = *reinterpret_cast<const u32x4*>(x[i] + p * plane + (t * 16 + e) * chunk);
+        },
+        [&](int, const typename Rows<kMx4, kN>::Step& now) {
+            float scale[kN];
+#pragma unroll
+            for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    const u32x4 w = decode_eight(now.w[j][0][e], scale[j]);
+#pragma unroll
+                    for (int i = 0; i < kM; ++i)
+#pragma unroll
+                        for (int p = 0; p < kP; ++p) acc[i * kN + j] = mfma_bf16(w, xs[e][i][p], acc[i * kN + j]);
+                }
+        });
     add_waves<kWaves, kM * kN>(acc, space, wave, lane);
     if (wave != 0) return;
 #pragma unroll
@@ -335,7 +394,9 @@ int launch_pieces(const Product& p) {
                            static_cast<int>(tiles(p.n, kTile)));
         return hipGetLastError();
     }
-    if (p.m > 32 && blocks(4, 2) >= cus) return launch_direct<kP, 4, 2, kOut>(p);
+    if constexpr (kP < 3) {  // three pieces of 64 rows do not fit the registers
+        if (p.m > 32 && blocks(4, 2) >= cus) return launch_direct<kP, 4, 2, kOut>(p);
+    }
     if (p.m > 16 && blocks(2, 2) >= cus) return launch_direct<kP, 2, 2, kOut>(p);
     if (p.m > 16) return launch_direct<kP, 2, 1, kOut>(p);
     if (blocks(1, 2) >= cus) return launch_direct<kP, 1, 2, kOut>(p);
