@@ -21,16 +21,29 @@ namespace {
 using namespace mx4;
 
 constexpr int kFew = 8;
-constexpr int kWaves = 8;
+constexpr int kFewWaves = 16;
 
 // ---------------------------------------------------------------- few rows
 
-// Eight elements of a row, as they lie in memory; zeros from `left` on.
+// These kernels' code is kept short: a launch meets a cold instruction cache, and
+// on an MI355X every 128 bytes of straight code cost about 0.2 us (31 MB through
+// 8.5 KB of code with four steps of each wave unrolled in 12.4 us, through 3.2 KB
+// in 11.4; 9 MB and fp32 rows 9.6 and 7.2), so the loop has one copy of its body,
+// and 16 waves two steps each where 8 had four.
+
+// Eight elements of a row as they lie in memory.
 template <int kIn>
 struct Eight {
     u32x4 v[kIn == kF32 ? 2 : 1];
 
-    __device__ __forceinline__ void load(const void* a, long long at, int left) {
+    // From byte `at` of the rows on; what lies past them reads as zeros.
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rows, int at, int step_at) {
+        v[0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at, step_at, 0));
+        if constexpr (kIn == kF32)
+            v[1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at + 16, step_at, 0));
+    }
+    // At any address and any distance.
+    __device__ __forceinline__ void load_loose(const void* a, long long at, int left) {
         if (left >= 8) {
             if constexpr (kIn == kF32) {
                 const u32x4_dwords* p = reinterpret_cast<const u32x4_dwords*>(static_cast<const float*>(a) + at);
@@ -51,6 +64,15 @@ struct Eight {
             }
         }
     }
+    // Zeros from element `left` on.
+    __device__ __forceinline__ void cut_off(int left) {
+#pragma unroll
+        for (int e = 0; e < 8; e += kIn == kF32 ? 1 : 2) {
+            unsigned keep = e < left ? 0xffffu : 0u;
+            keep |= (kIn == kF32 ? e : e + 1) < left ? 0xffff0000u : 0u;
+            v[kIn == kF32 ? e / 4 : 0][kIn == kF32 ? e % 4 : e / 2 % 4] &= keep;
+        }
+    }
 
     __device__ __forceinline__ void pieces(u32x4 (&out)[kPieces<kIn>]) const {
         if constexpr (kIn == kBf16) {
@@ -67,74 +89,73 @@ struct Eight {
     }
 };
 
-// The steps from `first` on, kWaves apart, of the weights `b`, four under way at
-// a time: fetch(t) is called, and then the step's multiplied. (One at a time, the
-// steps' latencies added up: 31 MB in 14 us.) What fetch loads for step t is
-// loaded before the weights of step t + 4 kWaves, because loads arrive in order.
-template <typename Weights, typename Fetch, typename Multiply>
-__device__ __forceinline__ void four_ahead(const Weights& b, int first, int steps, Fetch fetch, Multiply multiply) {
-    typename Weights::Step ring[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (first + j * kWaves < steps) b.load(first + j * kWaves, ring[j]);
-    for (int t = first; t < steps;) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (t >= steps) break;
-            fetch(t);
-            multiply(t, ring[j]);
-            if (t + 4 * kWaves < steps) b.load(t + 4 * kWaves, ring[j]);
-            t += kWaves;
-        }
-    }
-}
-
-// 16 kN columns of C for all rows (at most 16); the waves take the steps of 128 k
-// in turn.
-template <int kIn, int kN, int kOut>
-__global__ __launch_bounds__(kWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
-                                                           const unsigned char* __restrict__ b_codes,
-                                                           const unsigned char* __restrict__ b_scales,
-                                                           void* __restrict__ c, int m, int n, int k) {
-    constexpr int kP = kPieces<kIn>;
-    __shared__ f32x4 space[kWaves / 2 * kN * 64];
+// 16 kN columns of C for all rows (at most 8); the waves take the steps of 128 k
+// in turn, the next one under way while one is multiplied. kLoose: rows that do
+// not all start at dwords, or more than 2 GiB of them.
+template <int kIn, int kN, int kOut, bool kLoose>
+__global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
+                                                              const unsigned char* __restrict__ b_codes,
+                                                              const unsigned char* __restrict__ b_scales,
+                                                              void* __restrict__ c, int m, int n, int k) {
+    constexpr int kP = kPieces<kIn>, kSizeIn = kSize<kIn>;
+    __shared__ f32x4 space[kFewWaves / 2 * kN * 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep;
     const long long col0 = static_cast<long long>(blockIdx.x) * 16 * kN;
     Rows<kMx4, kN> b;
     b.open(b_codes, b_scales, k, n, [&](int j) { return col0 + 16 * j < n ? col0 + 16 * j : 0; });
     const bool has = r < m;
-    const long long at = has ? r * lda : 0;
+    const int bytes = kLoose ? 0 : static_cast<int>(((m - 1) * lda + k) * kSizeIn + 3) & ~3;
+    const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a), 0, bytes, 0x00020000);
+    // Lanes without a row read past the end, zeros.
+    const int at = has ? static_cast<int>(r * lda + 32 * q) * kSizeIn : 0x7ffffff0;
     f32x4 acc[kN];
 #pragma unroll
     for (int j = 0; j < kN; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    Eight<kIn> x[4];
-    four_ahead(
-        b, wave, steps,
-        [&](int t) {
+
+    struct Step {
+        Eight<kIn> x[4];
+        typename Rows<kMx4, kN>::Step w;
+    } now, next;
+    const auto load = [&](int t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kLoose) {
                 const int e = t * kStep + 32 * q + 8 * i;
-                x[i].load(a, at + e, has ? k - e : 0);
+                next.x[i].load_loose(a, has ? r * lda + e : 0, has ? k - e : 0);
+            } else {
+                next.x[i].load(rows, has ? at + 8 * i * kSizeIn : at, t * kStep * kSizeIn);
             }
-        },
-        [&](int, const typename Rows<kMx4, kN>::Step& now) {
-            float scale[kN];
+        }
+        b.load(t, next.w);
+    };
+    int t = wave;
+    if (t < steps) load(t);
+    while (t < steps) {
+        now = next;
+        const int then = t + kFewWaves;
+        if (then < steps) load(then);
+        if (!kLoose && (t + 1) * kStep > k) {
 #pragma unroll
-            for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
+            for (int i = 0; i < 4; ++i) now.x[i].cut_off(k - (t * kStep + 32 * q + 8 * i));
+        }
+        float scale[kN];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                u32x4 piece[kP];
-                x[i].pieces(piece);
+        for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now.w, j));
 #pragma unroll
-                for (int j = 0; j < kN; ++j) {
-                    const u32x4 w = decode_eight(now.w[j][0][i], scale[j]);
+        for (int i = 0; i < 4; ++i) {
+            u32x4 piece[kP];
+            now.x[i].pieces(piece);
 #pragma unroll
-                    for (int p = 0; p < kP; ++p) acc[j] = mfma_bf16(w, piece[p], acc[j]);
-                }
+            for (int j = 0; j < kN; ++j) {
+                const u32x4 w = decode_eight(now.w.w[j][0][i], scale[j]);
+#pragma unroll
+                for (int p = 0; p < kP; ++p) acc[j] = mfma_bf16(w, piece[p], acc[j]);
             }
-        });
-    add_waves<kWaves, kN>(acc, space, wave, lane);
+        }
+        t = then;
+    }
+    add_waves<kFewWaves, kN>(acc, space, wave, lane);
     if (wave != 0 || !has) return;
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
@@ -162,14 +183,24 @@ __global__ __launch_bounds__(256) void cut_rows(const void* __restrict__ a, long
     for (int p = 0; p < kP; ++p) *reinterpret_cast<u32x4*>(out + (p * all + i) * 8) = x[p];
 }
 
-// 16 kM rows by 16 kN columns of C per block, A in pieces (`rows` of them, a multiple of 16).
-template <int kP, int kM, int kN, int kOut>
-__global__ __launch_bounds__(kWaves * 64) void weights_direct(const unsigned short* __restrict__ a,
+// 16 kM rows by 16 kN columns of C per block, A in pieces (`rows` of them, a
+// multiple of 16). A step's pieces are loaded before the next step's weights,
+// because loads arrive in order; where they would take too many registers, by
+// instruction.
+template <int kPieceRows, int kN>
+struct Direct {
+    static constexpr bool kPiecesFirst = kPieceRows <= 4;
+    static constexpr int kWaves = kPieceRows <= 2 || (kPieceRows <= 4 && kN == 1) ? 16 : 8;  // as the registers allow
+};
+
+template <typename Shape, int kP, int kM, int kN, int kOut>
+__global__ __launch_bounds__(64 * Shape::kWaves) void weights_direct(const unsigned short* __restrict__ a,
                                                               const unsigned char* __restrict__ b_codes,
                                                               const unsigned char* __restrict__ b_scales,
                                                               void* __restrict__ c, int m, int rows, int n, int k,
                                                               unsigned tiles_n) {
-    __shared__ f32x4 space[kWaves / 2 * kM * kN * 64];
+    constexpr int kW = Shape::kWaves;
+    __shared__ f32x4 space[kW / 2 * kM * kN * 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep;
     const int row0 = static_cast<int>(blockIdx.x / tiles_n) * 16 * kM;
@@ -186,34 +217,40 @@ __global__ __launch_bounds__(kWaves * 64) void weights_direct(const unsigned sho
     f32x4 acc[kM * kN];
 #pragma unroll
     for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    u32x4 xs[4][kM][kP];
-    four_ahead(
-        b, wave, steps,
-        [&](int t) {
+    typename Rows<kMx4, kN>::Step now, next;
+    if (wave < steps) b.load(wave, next);
+    for (int t = wave; t < steps; t += kW) {
+        now = next;
+        u32x4 xs[4][kM][kP];
+        const auto load = [&](int e) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int i = 0; i < kM; ++i)
+#pragma unroll
+                for (int p = 0; p < kP; ++p)
+                    xs[e][i][p] = *reinterpret_cast<const u32x4*>(x[i] + p * plane + (t * 16 + e) * chunk);
+        };
+        if constexpr (Shape::kPiecesFirst) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) load(e);
+        }
+        if (t + kW < steps) b.load(t + kW, next);
+        float scale[kN];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (!Shape::kPiecesFirst) load(e);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const u32x4 w = decode_eight(now.w[j][0][e], scale[j]);
 #pragma unroll
                 for (int i = 0; i < kM; ++i)
 #pragma unroll
-                    for (int p = 0; p < kP; ++p)
-                        xs[e][i][p] = *reinterpret_cast<const u32x4*>(x[i] + p * plane + (t * 16 + e) * chunk);
-        },
-        [&](int, const typename Rows<kMx4, kN>::Step& now) {
-            float scale[kN];
-#pragma unroll
-            for (int j = 0; j < kN; ++j) scale[j] = scale_operand(b.scale(now, j));
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int j = 0; j < kN; ++j) {
-                    const u32x4 w = decode_eight(now.w[j][0][e], scale[j]);
-#pragma unroll
-                    for (int i = 0; i < kM; ++i)
-#pragma unroll
-                        for (int p = 0; p < kP; ++p) acc[i * kN + j] = mfma_bf16(w, xs[e][i][p], acc[i * kN + j]);
-                }
-        });
-    add_waves<kWaves, kM * kN>(acc, space, wave, lane);
+                    for (int p = 0; p < kP; ++p) acc[i * kN + j] = mfma_bf16(w, xs[e][i][p], acc[i * kN + j]);
+            }
+        }
+    }
+    add_waves<kW, kM * kN>(acc, space, wave, lane);
     if (wave != 0) return;
 #pragma unroll
     for (int i = 0; i < kM; ++i) {
@@ -369,17 +406,25 @@ int piece_rows(int m) { return (m + 15) / 16 * 16; }
 
 template <int kIn, int kN, int kOut>
 int launch_few(const Product& p) {
-    hipLaunchKernelGGL((weights_few<kIn, kN, kOut>), dim3(static_cast<unsigned>(tiles(p.n, 16 * kN))), dim3(kWaves * 64), 0,
-                       p.stream, p.a, p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
-    return hipGetLastError();
+    const long long size = kSize<kIn>;
+    const bool loose = !aligned(p.a, 4) || p.lda * size % 4 != 0 || ((p.m - 1) * p.lda + p.k) * size > 0x7fffff00LL;
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles(p.n, 16 * kN))), dim3(kFewWaves * 64), 0, p.stream, p.a,
+                           p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
+        return static_cast<int>(hipGetLastError());
+    };
+    if (loose) return go(weights_few<kIn, kN, kOut, true>);
+    return go(weights_few<kIn, kN, kOut, false>);
 }
 
 template <int kP, int kM, int kN, int kOut>
 int launch_direct(const Product& p) {
+    typedef Direct<kP * kM, kN> Shape;
     const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((weights_direct<kP, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64), 0, p.stream,
-                       p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k, static_cast<unsigned>(tn));
+    hipLaunchKernelGGL((weights_direct<Shape, kP, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(64 * Shape::kWaves),
+                       0, p.stream, p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
+                       static_cast<unsigned>(tn));
     return hipGetLastError();
 }
 
@@ -406,7 +451,14 @@ int launch_pieces(const Product& p) {
 template <int kIn, int kOut>
 int launch(const Product& p) {
     if (p.m <= kFew) {
-        if (tiles(p.n, 32) >= device_cus()) return launch_few<kIn, 2, kOut>(p);
+        // One block of 16 waves runs on a CU at a time. Rounds of blocks, each as
+        // long as its columns and a fixed part take: 14336 columns of k = 4096
+        // by 64 per block in 8.9 us, by 32 (two rounds) in 11.4.
+        const auto cost = [&](int wide) { return tiles(tiles(p.n, 16 * wide), device_cus()) * (2 * wide + 3); };
+        if constexpr (kIn != kF32) {  // fp32 rows by 64 columns do not fit the registers
+            if (cost(4) < cost(2) && cost(4) < cost(1)) return launch_few<kIn, 4, kOut>(p);
+        }
+        if (cost(2) < cost(1)) return launch_few<kIn, 2, kOut>(p);
         return launch_few<kIn, 1, kOut>(p);
     }
     const int rows = piece_rows(p.m), chunks = padded(p.k) / 8;

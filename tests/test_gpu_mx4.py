@@ -258,6 +258,21 @@ def test_infinities_and_nans_of_unquantised_rows(device, mc, kind, m):
     assert np.all(np.isnan(got[2])) and np.all(np.isfinite(got[1])) and np.all(np.isfinite(got[3:]))
 
 
+def test_few_rows_more_than_2_gib_apart(device, mc):
+    m, n, k, lda = 3, 40, 200, (1 << 30) + 24
+    rng = np.random.default_rng(31)
+    bits = ref.to_type(rng.standard_normal((m, k)), ref.BF16)
+    a = mc.DeviceBuffer(2 * ((m - 1) * lda + k))
+    for i in range(m):
+        upload_at(mc, a, 2 * i * lda, bits[i])
+    bc, bs, b = operand(mc, rng, n, k)
+    c = Out(mc, m * n * 4)
+    mc.launch_matmul_mx4_weights(ref.BF16, a.ptr, lda, bc.ptr, bs.ptr, ref.F32, c.ptr, m, n, k)
+    mc.synchronize()
+    exact, bound = ref.product_bound(ref.from_type(bits, ref.BF16), b, k, ref.F32)
+    within(c.get(np.float32, (m, n)).astype(np.float64), exact, bound)
+
+
 def test_operands_of_more_than_4_gib(device, mc):
     """The last rows of a weight operand whose codes and scales lie past 2^32 and 2^28 bytes."""
     n, k, last = 540000, 16384, 48
