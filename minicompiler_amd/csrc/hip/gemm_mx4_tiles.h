@@ -31,6 +31,14 @@
 // step, the scales took 50 of 332 us at 8192^3.) A row's last 16 bytes are
 // loaded whole where its end falls inside a window, so nothing is read outside
 // the operand (K >= 512).
+//
+// Measured, bf16 out: 4096x14336x4096 137-142 us (3.4-3.5 PFLOP/s), 8192^3
+// 250-265 us (4.1-4.4). A loop of the instruction alone, on random data in
+// registers, runs at 7.4 PFLOP/s: the chip lowers its clock (1.9 GHz here). With
+// the fetch left out the loop's matrix units are busy 64% instead of 57%, with
+// the scales' work left out as well 70%, and 72% without LDS reads; the rest is
+// a tile's start and its store, which all blocks do at one time (13 of 250 us).
+// 8 waves with quadrants of 128x64 took 261 us where 4 took 254.
 #pragma once
 
 #include "mx4_device.h"
@@ -82,13 +90,13 @@ __device__ __forceinline__ void fetch_one(MX4_LDS unsigned char* wr, const TileL
                   part * 8 * L.row_bytes + at);
 }
 
-// Part `which` of kParts of this wave's share.
-template <int kRows, int kParts>
-__device__ __forceinline__ void fetch_part(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int s, int which) {
+// Instructions `from` to `to` of them.
+template <int kRows>
+__device__ __forceinline__ void fetch_range(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int s, int from, int to) {
     constexpr int kAll = TileLane<kRows>::kFetchA + TileLane<kRows>::kFetchB;
 #pragma unroll
     for (int i = 0; i < kAll; ++i)
-        if (i >= which * kAll / kParts && i < (which + 1) * kAll / kParts) fetch_one<kRows>(wr, L, s, i);
+        if (i >= from && i < to) fetch_one<kRows>(wr, L, s, i);
 }
 
 // Part n % 4 of window n / 4: 32 rows' scales of 8 steps, a lane 16 bytes as
@@ -105,30 +113,45 @@ __device__ __forceinline__ u32x4 load_scales(const TileLane<kRows>& L, int n) {
                                                      (L.wave % 2 * 128 + n % 4 * 32) * L.scale_row, 0));
 }
 
-// Dword q of the result: block q's bytes of the four steps.
-__device__ __forceinline__ u32x4 by_block(u32x4 v) {
-    const unsigned lo01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);
-    const unsigned lo23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
-    const unsigned hi01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
-    const unsigned hi23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
-    return u32x4{__builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
-                 __builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
-}
-
 // A window's slot: [steps 0-3, steps 4-7][256 rows of A, 256 of B][16 bytes].
 // Bytes of steps past the end are zeros, a scale of 2^-127 on both sides, which
 // makes nothing of whatever codes they meet: an odd last step needs no branch.
+// (Without branches: a product's loop is one block, or the compiler moves
+// products from before a branch behind it.) In six pieces, to go between products.
+template <int kRows, int kPiece>
+__device__ __forceinline__ void store_scales_piece(MX4_LDS unsigned char* slots, const TileLane<kRows>& L, u32x4& v, int n) {
+    const int late = (scale_at<kRows>(L, n) - (L.scale_row - 16)) / 4;  // dwords moved back, if above 0
+    if constexpr (kPiece == 0) {
+        const bool one = late > 0 && (late & 1);
+        v = u32x4{one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], one ? 0u : v[3]};
+    } else if constexpr (kPiece == 1) {
+        const bool two = late > 0 && (late & 2);
+        v = u32x4{two ? v[2] : v[0], two ? v[3] : v[1], two ? 0u : v[2], two ? 0u : v[3]};
+    } else if constexpr (kPiece == 2) {
+        const bool past = late > 3;
+        v = u32x4{past ? 0u : v[0], past ? 0u : v[1], past ? 0u : v[2], past ? 0u : v[3]};
+    } else if constexpr (kPiece == 3) {
+        // Pairs of steps: blocks 0 and 1 of steps 0 and 1, of 2 and 3; blocks 2 and 3.
+        v = u32x4{__builtin_amdgcn_perm(v[1], v[0], 0x05010400u), __builtin_amdgcn_perm(v[3], v[2], 0x05010400u),
+                  __builtin_amdgcn_perm(v[1], v[0], 0x07030602u), __builtin_amdgcn_perm(v[3], v[2], 0x07030602u)};
+    } else if constexpr (kPiece == 4) {
+        // Dword q: block q's bytes of the four steps.
+        v = u32x4{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u), __builtin_amdgcn_perm(v[1], v[0], 0x07060302u),
+                  __builtin_amdgcn_perm(v[3], v[2], 0x05040100u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u)};
+    } else {
+        const int row = (L.wave / 2 * 256) + (L.wave % 2 * 128) + n % 4 * 32 + L.lane / 2;
+        *reinterpret_cast<MX4_LDS u32x4*>(slots + (n / 4 & 1) * kSlotBytes + L.lane % 2 * kSlotHalf + row * 16) = v;
+    }
+}
+
 template <int kRows>
 __device__ __forceinline__ void store_scales(MX4_LDS unsigned char* slots, const TileLane<kRows>& L, u32x4 v, int n) {
-    // Without branches: a product's loop is one block, or the compiler moves
-    // products from before a branch behind it.
-    const int late = (scale_at<kRows>(L, n) - (L.scale_row - 16)) / 4;  // dwords moved back, if above 0
-    const bool one = late > 0 && (late & 1), two = late > 0 && (late & 2), past = late > 3;
-    v = u32x4{one ? v[1] : v[0], one ? v[2] : v[1], one ? v[3] : v[2], one ? 0u : v[3]};
-    v = u32x4{two ? v[2] : v[0], two ? v[3] : v[1], two ? 0u : v[2], two ? 0u : v[3]};
-    v = u32x4{past ? 0u : v[0], past ? 0u : v[1], past ? 0u : v[2], past ? 0u : v[3]};
-    const int row = (L.wave / 2 * 256) + (L.wave % 2 * 128) + n % 4 * 32 + L.lane / 2;
-    *reinterpret_cast<MX4_LDS u32x4*>(slots + (n / 4 & 1) * kSlotBytes + L.lane % 2 * kSlotHalf + row * 16) = by_block(v);
+    store_scales_piece<kRows, 0>(slots, L, v, n);
+    store_scales_piece<kRows, 1>(slots, L, v, n);
+    store_scales_piece<kRows, 2>(slots, L, v, n);
+    store_scales_piece<kRows, 3>(slots, L, v, n);
+    store_scales_piece<kRows, 4>(slots, L, v, n);
+    store_scales_piece<kRows, 5>(slots, L, v, n);
 }
 
 // One fragment of step u of the stage at `rd`, and a fragment's scales of four
@@ -153,6 +176,36 @@ template <int kRows>
 __device__ __forceinline__ int read_scale_b(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L,
                                             int f) {
     return *reinterpret_cast<const MX4_LDS int*>(rd + kSlotB + L.b_scale + f * 256);
+}
+
+// acc += a b in acc's own registers. Written out, because the compiler, with the
+// products held in their places, gives them other registers and copies (8192^3
+// in 311 us); it also keeps asm statements in their order. What it no longer
+// knows: a value is there only after the instruction's passes (settle()).
+template <int kByte>
+__device__ __forceinline__ void mfma_in_place(f32x4& acc, i32x4 a, int sa, i32x4 b, int sb) {
+    if constexpr (kByte == 0)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(acc)
+                     : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    else if constexpr (kByte == 1)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                     : "+a"(acc)
+                     : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    else if constexpr (kByte == 2)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0] cbsz:4 blgp:4"
+                     : "+a"(acc)
+                     : "v"(a), "v"(b), "v"(sa), "v"(sb));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0] cbsz:4 blgp:4"
+                     : "+a"(acc)
+                     : "v"(a), "v"(b), "v"(sa), "v"(sb));
+}
+
+// Between the last product and the first use of its value: its passes are over.
+__device__ __forceinline__ void settle() {
+    asm volatile("s_nop 15\n s_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // A wave's accumulators, first row and column (row, col): lane (r, q) holds
@@ -245,8 +298,12 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
 #pragma unroll
     for (int i = 0; i < 5; ++i) first[i] = load_scales<kRows>(L, i);
     u32x4 scales = load_scales<kRows>(L, 5);
-    fetch_part<kRows, 1>(stage(0), L, 0, 0);
-    fetch_part<kRows, 1>(stage(1), L, 1, 0);
+    // The fetch of a stage is spread over the rows between two barriers and a
+    // few behind the second: the address unit takes 16 cycles for an
+    // instruction, and a wave that waits for it multiplies nothing.
+    constexpr int kI = Lane::kRowFrags, kAll = Lane::kFetchA + Lane::kFetchB, kEarly = kAll * 5 / 8;
+    fetch_range<kRows>(stage(0), L, 0, 0, kAll);
+    fetch_range<kRows>(stage(1), L, 1, 0, kEarly);
 #pragma unroll
     for (int i = 0; i < Lane::kRowFrags; ++i)
 #pragma unroll
@@ -259,7 +316,7 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
     __builtin_amdgcn_s_waitcnt(0);
     lds_barrier();
 
-    constexpr int kI = Lane::kRowFrags, kB = kColFrags / kI;
+    constexpr int kB = kColFrags / kI;
     i32x4 av[kI], bv[2][kColFrags];
     int sa[kI], sb[kColFrags], sb_next[kColFrags];
 #pragma unroll
@@ -275,56 +332,72 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
 
     // Stage s, `which` = s % 2. The part of scales stored at stage s is s + 5
     // (the fourth of a window two stages before its first use), loaded a stage
-    // before. The rows are held in their order, or the compiler would gather
-    // the reads at the end, where the next step waits for them.
+    // before. Every product is held in its place, with one piece of the other
+    // work behind it: the matrix unit is busy meanwhile, and a product leaves
+    // room for a few instructions; gathered between the rows they left it idle.
     const auto run = [&](int s, auto which) {
         constexpr int w = decltype(which)::value;
         const MX4_LDS unsigned char *here = stage(s), *there = stage(s + 1);
+        const int rest = s + 1 < stages ? s + 1 : stages - 1, next = s + 2 < stages ? s + 2 : stages - 1;
 #pragma unroll
         for (int i = 0; i < kI; ++i) {
-            if (i == 0) {
-                av[kI - 1] = read_a<kRows>(here, L, 0, kI - 1);
-                if constexpr (w == 0) sa[kI - 1] = read_scale_a<kRows>(scales_of(s), L, kI - 1);
-            } else {
-                av[i - 1] = read_a<kRows>(here, L, 1, i - 1);
+#pragma unroll
+            for (int f = 0; f < kColFrags; ++f) {
+                mfma_in_place<w * 2>(acc[i][f], bv[0][f], sb[f], av[i], sa[i]);
+                if (f == 0 && i == 0) {
+                    av[kI - 1] = read_a<kRows>(here, L, 0, kI - 1);
+                    if constexpr (w == 0) sa[kI - 1] = read_scale_a<kRows>(scales_of(s), L, kI - 1);
+                }
+                if (f == 0 && i > 0) av[i - 1] = read_a<kRows>(here, L, 1, i - 1);
+                if (f > 0 && f <= kB) bv[1][i * kB + f - 1] = read_b<kRows>(here, L, 1, i * kB + f - 1);
+                // The rest of stage s + 1.
+                if (i < kI / 2 && f >= 4) {
+                    const int from = kEarly + i * (kAll - kEarly) / (kI / 2), to = kEarly + (i + 1) * (kAll - kEarly) / (kI / 2);
+                    if (from + f - 4 < to) fetch_one<kRows>(stage(s + 1), L, rest, from + f - 4);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int f = i * kB; f < i * kB + kB; ++f) bv[1][f] = read_b<kRows>(here, L, 1, f);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int f = 0; f < kColFrags; ++f)
-                acc[i][f] = mfma<w * 2>(bv[0][f], sb[f], av[i], sa[i], acc[i][f]);
-            __builtin_amdgcn_sched_barrier(0);
         }
-        const int next = s + 2 < stages ? s + 2 : stages - 1;
 #pragma unroll
         for (int i = 0; i < kI; ++i) {
-            if (i == 0) av[kI - 1] = read_a<kRows>(here, L, 1, kI - 1);
             if (i == 2) {
                 __builtin_amdgcn_s_waitcnt(0);
                 lds_barrier();
-                store_scales<kRows>(slots, L, scales, s + 5);
-                scales = load_scales<kRows>(L, s + 6);
-                av[0] = read_a<kRows>(there, L, 0, 0);
-                if constexpr (w == 1) sa[0] = read_scale_a<kRows>(scales_of(s + 1), L, 0);
             }
-            if (i >= 2) {
-                // What is left after two rows, over the other rows.
-                constexpr int kLeft = kI - 2;
-                av[i - 1] = read_a<kRows>(there, L, 0, i - 1);
-                if constexpr (w == 1) sa[i - 1] = read_scale_a<kRows>(scales_of(s + 1), L, i - 1);
-                fetch_part<kRows, kLeft>(stage(s), L, next, i - 2);
 #pragma unroll
-                for (int f = (i - 2) * kColFrags / kLeft; f < (i - 1) * kColFrags / kLeft; ++f) {
-                    bv[0][f] = read_b<kRows>(there, L, 0, f);
-                    if constexpr (w == 1) sb_next[f] = read_scale_b<kRows>(scales_of(s + 1), L, f);
+            for (int f = 0; f < kColFrags; ++f) {
+                mfma_in_place<w * 2 + 1>(acc[i][f], bv[1][f], sb[f], av[i], sa[i]);
+                if (f == 0 && i == 0) av[kI - 1] = read_a<kRows>(here, L, 1, kI - 1);
+                if (i >= 2) {
+                    // What is left after two rows, over the other rows.
+                    constexpr int kLeft = kI - 2;
+                    if (f == 0) {
+                        av[i - 1] = read_a<kRows>(there, L, 0, i - 1);
+                        if constexpr (w == 1) sa[i - 1] = read_scale_a<kRows>(scales_of(s + 1), L, i - 1);
+                        if (i == 2) {
+                            av[0] = read_a<kRows>(there, L, 0, 0);
+                            if constexpr (w == 1) sa[0] = read_scale_a<kRows>(scales_of(s + 1), L, 0);
+                        }
+                    }
+                    const int from = (i - 2) * kEarly / kLeft, to = (i - 1) * kEarly / kLeft;
+                    if (f >= 4 && from + f - 4 < to) fetch_one<kRows>(stage(s), L, next, from + f - 4);
+                    const int b0 = (i - 2) * kColFrags / kLeft, b1 = (i - 1) * kColFrags / kLeft;
+                    if (f > 0 && b0 + f - 1 < b1) {
+                        bv[0][b0 + f - 1] = read_b<kRows>(there, L, 0, b0 + f - 1);
+                        if constexpr (w == 1) sb_next[b0 + f - 1] = read_scale_b<kRows>(scales_of(s + 1), L, b0 + f - 1);
+                    }
                 }
+                if (i == 3) {
+                    if (f == 0) store_scales_piece<kRows, 0>(slots, L, scales, s + 5);
+                    if (f == 1) store_scales_piece<kRows, 1>(slots, L, scales, s + 5);
+                    if (f == 2) store_scales_piece<kRows, 2>(slots, L, scales, s + 5);
+                    if (f == 3) store_scales_piece<kRows, 3>(slots, L, scales, s + 5);
+                    if (f == 4) store_scales_piece<kRows, 4>(slots, L, scales, s + 5);
+                    if (f == 5) store_scales_piece<kRows, 5>(slots, L, scales, s + 5);
+                    if (f == 6) scales = load_scales<kRows>(L, s + 6);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int f = 0; f < kColFrags; ++f)
-                acc[i][f] = mfma<w * 2 + 1>(bv[1][f], sb[f], av[i], sa[i], acc[i][f]);
-            __builtin_amdgcn_sched_barrier(0);
         }
     };
     // Two stages at a time, the four steps of a scale dword; what is past the
@@ -334,8 +407,15 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const u
         run(s + 1, Constant<1>{});
 #pragma unroll
         for (int f = 0; f < kColFrags; ++f) sb[f] = sb_next[f];
+        // A product's operand may have been written two instructions before it at the latest.
+        asm volatile("s_nop 1" ::: "memory");
     }
     __builtin_amdgcn_s_waitcnt(0);
+    settle();
+#pragma unroll
+    for (int i = 0; i < Lane::kRowFrags; ++i)
+#pragma unroll
+        for (int j = 0; j < kColFrags; ++j) asm volatile("" : "+a"(acc[i][j]));  // read behind it only
     store_tile<Lane::kRowFrags, kOut>(acc, c, row0 + wave_row, col0 + wave_col, m, n, lane, eights);
 }
 
