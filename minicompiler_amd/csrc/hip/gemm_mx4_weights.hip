@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
                                                               const unsigned char* __restrict__ b_scales,
                                                               void* __restrict__ c, int m, int n, int k) {
     constexpr int kP = kPieces<kIn>, kSizeIn = kSize<kIn>;
-    __shared__ f32x4 space[kFewWaves / 2 * kN * 64];
+    __shared__ f32x4 space[kFewWaves * kN * 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep;
     const long long col0 = static_cast<long long>(blockIdx.x) * 16 * kN;
@@ -155,13 +155,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
         }
         t = then;
     }
-    add_waves<kFewWaves, kN>(acc, space, wave, lane);
-    if (wave != 0 || !has) return;
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
+    sum_waves<kFewWaves>(acc, space, wave, lane, [&](int j, f32x4 sum) {
         const long long col = col0 + 16 * j + 4 * q;
-        if (col < n) store_four<kOut>(c, r * static_cast<long long>(n) + col, acc[j], static_cast<int>(n - col < 4 ? n - col : 4));
-    }
+        if (has && col < n)
+            store_four<kOut>(c, r * static_cast<long long>(n) + col, sum, static_cast<int>(n - col < 4 ? n - col : 4));
+    });
 }
 
 // ---------------------------------------------------------------- pieces
@@ -200,7 +198,7 @@ __global__ __launch_bounds__(64 * Shape::kWaves) void weights_direct(const unsig
                                                               void* __restrict__ c, int m, int rows, int n, int k,
                                                               unsigned tiles_n) {
     constexpr int kW = Shape::kWaves;
-    __shared__ f32x4 space[kW / 2 * kM * kN * 64];
+    __shared__ f32x4 space[kW * kM * kN * 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep;
     const int row0 = static_cast<int>(blockIdx.x / tiles_n) * 16 * kM;
@@ -250,20 +248,12 @@ __global__ __launch_bounds__(64 * Shape::kWaves) void weights_direct(const unsig
             }
         }
     }
-    add_waves<kW, kM * kN>(acc, space, wave, lane);
-    if (wave != 0) return;
-#pragma unroll
-    for (int i = 0; i < kM; ++i) {
-        const int row = row0 + 16 * i + r;
-        if (row >= m) continue;
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            const long long col = col0 + 16 * j + 4 * q;
-            if (col < n)
-                store_four<kOut>(c, static_cast<long long>(row) * n + col, acc[i * kN + j],
-                                 static_cast<int>(n - col < 4 ? n - col : 4));
-        }
-    }
+    sum_waves<kW>(acc, space, wave, lane, [&](int i, f32x4 sum) {
+        const int row = row0 + 16 * (i / kN) + r;
+        const long long col = col0 + 16 * (i % kN) + 4 * q;
+        if (row < m && col < n)
+            store_four<kOut>(c, static_cast<long long>(row) * n + col, sum, static_cast<int>(n - col < 4 ? n - col : 4));
+    });
 }
 
 // ---------------------------------------------------------------- large tiles

@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
                                                        float* __restrict__ gates_out) {
     constexpr int kP = kPieces<kIn>;
     extern __shared__ float logits[];  // [16, experts], in the last block of 16 tokens
-    __shared__ f32x4 space[kWaves / 2 * 64];
+    __shared__ f32x4 space[kWaves * 64];
     __shared__ int chosen[kMaxTokens][kMaxTopK];
     __shared__ float gate[kMaxTokens][kMaxTopK];
     __shared__ unsigned long long mask[kMaxExperts];
@@ -346,13 +346,12 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][j], b[i][j], acc[0], 0, 0, 0);
     }
-    add_waves<kWaves, 1>(acc, space, wave, lane);
-    if (wave == 0 && t0 + r < s.tokens) {
+    sum_waves<kWaves>(acc, space, wave, lane, [&](int, f32x4 sum) {
         float* out = w.logits + blockIdx.z * all_logits + static_cast<long long>(t0 + r) * s.experts + e0 + 4 * q;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-            if (e0 + 4 * q + v < s.experts) mc_split_store(out + v, acc[0][v]);
-    }
+            if (t0 + r < s.tokens && e0 + 4 * q + v < s.experts) mc_split_store(out + v, sum[v]);
+    });
 
     // x in pieces, padded with zeros, shared out over the blocks.
     const int chunks = s.tokens * (s.dp / 8);

@@ -243,23 +243,20 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// The partial sums of a block's waves (kWaves, a power of two; each `kCount`
-// vectors per lane) added up in wave 0, pairs in a fixed order: half the waves
-// write, the other half add. `space`: kWaves / 2 * kCount * 64 vectors.
-template <int kWaves, int kCount>
-__device__ __forceinline__ void add_waves(f32x4 (&acc)[kCount], f32x4* space, int wave, int lane) {
+// The partial sums of a block's waves (each kCount vectors per lane) added up in
+// wave order, vector i by wave i % kWaves, which hands it to take(i, sum): short
+// code, and all waves store. `space`: kWaves * kCount * 64 vectors.
+template <int kWaves, int kCount, typename Take>
+__device__ __forceinline__ void sum_waves(const f32x4 (&acc)[kCount], f32x4* space, int wave, int lane, Take take) {
 #pragma unroll
-    for (int half = kWaves / 2; half > 0; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
+    for (int i = 0; i < kCount; ++i) space[(wave * kCount + i) * 64 + lane] = acc[i];
+    __syncthreads();
+#pragma unroll 1
+    for (int i = wave; i < kCount; i += kWaves) {
+        f32x4 sum = space[i * 64 + lane];
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) space[((wave - half) * kCount + i) * 64 + lane] = acc[i];
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int i = 0; i < kCount; ++i) acc[i] += space[(wave * kCount + i) * 64 + lane];
-        }
-        __syncthreads();
+        for (int v = 1; v < kWaves; ++v) sum += space[(v * kCount + i) * 64 + lane];
+        take(i, sum);
     }
 }
 
