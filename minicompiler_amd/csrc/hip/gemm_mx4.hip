@@ -52,12 +52,18 @@ __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned cha
         for (int i = 0; i < kM; ++i) sa[i] = static_cast<int>(a.scale(a_now, i));
 #pragma unroll
         for (int j = 0; j < kN; ++j) sb[j] = static_cast<int>(b.scale(b_now, j));
+        i32x4 av[kM], bv[kN];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) av[i][e] = static_cast<int>(a.pass(a_now.w[i][0][e]));
+#pragma unroll
+            for (int j = 0; j < kN; ++j) bv[j][e] = static_cast<int>(b.pass(b_now.w[j][0][e]));
+        }
 #pragma unroll
         for (int i = 0; i < kM; ++i)
 #pragma unroll
-            for (int j = 0; j < kN; ++j)
-                acc[i * kN + j] = mfma(__builtin_bit_cast(i32x4, b_now.w[j][0]), sb[j],
-                                       __builtin_bit_cast(i32x4, a_now.w[i][0]), sa[i], acc[i * kN + j]);
+            for (int j = 0; j < kN; ++j) acc[i * kN + j] = mfma(bv[j], sb[j], av[i], sa[i], acc[i * kN + j]);
     }
     sum_waves<kWaves>(acc, space, wave, lane, [&](int i, f32x4 sum) {
         const long long row = row0 + 16 * (i / kN) + r, col = col0 + 16 * (i % kN) + 4 * q;

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
             now.x[i].pieces(piece);
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-                const u32x4 w = decode_eight(now.w.w[j][0][i], scale[j]);
+                const u32x4 w = decode_eight(b.pass(now.w.w[j][0][i]), scale[j]);
 #pragma unroll
                 for (int p = 0; p < kP; ++p) acc[j] = mfma_bf16(w, piece[p], acc[j]);
             }
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64 * Shape::kWaves) void weights_direct(const unsig
             if constexpr (!Shape::kPiecesFirst) load(e);
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-                const u32x4 w = decode_eight(now.w[j][0][e], scale[j]);
+                const u32x4 w = decode_eight(b.pass(now.w[j][0][e]), scale[j]);
 #pragma unroll
                 for (int i = 0; i < kM; ++i)
 #pragma unroll
