@@ -107,8 +107,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
     const bool has = r < m;
     const int bytes = kLoose ? 0 : static_cast<int>(((m - 1) * lda + k) * kSizeIn + 3) & ~3;
     const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a), 0, bytes, 0x00020000);
-    // Lanes without a row read past the end, zeros.
-    const int at = has ? static_cast<int>(r * lda + 32 * q) * kSizeIn : 0x7ffffff0;
+    const int at = kLoose ? 0 : static_cast<int>((has ? r : 0) * lda + 32 * q) * kSizeIn;
     f32x4 acc[kN];
 #pragma unroll
     for (int j = 0; j < kN; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -124,11 +123,12 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
                 const int e = t * kStep + 32 * q + 8 * i;
                 next.x[i].load_loose(a, has ? r * lda + e : 0, has ? k - e : 0);
             } else {
-                next.x[i].load(rows, has ? at + 8 * i * kSizeIn : at, t * kStep * kSizeIn);
+                if (has) next.x[i].load(rows, at + 8 * i * kSizeIn, t * kStep * kSizeIn);  // the others stay zeros
             }
         }
         b.load(t, next.w);
     };
+    next.x[0] = next.x[1] = next.x[2] = next.x[3] = Eight<kIn>{};
     int t = wave;
     if (t < steps) load(t);
     while (t < steps) {

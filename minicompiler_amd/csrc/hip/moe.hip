@@ -270,41 +270,83 @@ __device__ void list_jobs(const Workspace& w, const Sizes& s, const int (*chosen
 }
 
 // The same for up to 8 tokens (a job per chosen expert) into `jobs`, by blocks
-// of at least 128 threads, a thread per chosen pair; returns how many.
+// of at least 128 threads, a thread per chosen pair; returns how many. The jobs'
+// places and the masks of the experts have been cleared (clear_few_jobs).
 __device__ int list_few_jobs(const Sizes& s, const int (*chosen)[kMaxTopK], const float (*gate)[kMaxTopK],
-                             unsigned* mask, int* counts, Job* jobs) {
+                             unsigned* mask, int* place, int* counts, Job* jobs) {
     const int i = threadIdx.x, t = i / s.top_k, j = i % s.top_k;
     const bool pair = i < s.tokens * s.top_k;
     const int e = pair ? chosen[t][j] : 0;
-    if (pair) mask[e] = 0;
-    __syncthreads();
+    const float g = pair ? gate[t][j] : 0.0f;
+    if (s.tokens == 1) {  // every pair a job
+        if (pair) {
+            jobs[i].expert = e;
+            jobs[i].token[0] = 0;
+            jobs[i].gate[0] = g;
+        }
+        __syncthreads();
+        return s.top_k;
+    }
     if (pair) atomicOr(mask + e, 1u << t);
     __syncthreads();
-    const bool first = pair && __builtin_ctz(mask[e]) == t;
-    const unsigned long long firsts = __ballot(first);
+    const unsigned before = pair ? mask[e] & ((1u << t) - 1) : 1u;
+    const unsigned long long firsts = __ballot(before == 0);
     if (i % 64 == 0 && i < 128) counts[i / 64] = __builtin_popcountll(firsts);
     __syncthreads();
-    if (first) {
+    if (before == 0) {
         const int n = (i >= 64 ? counts[0] : 0) + __builtin_popcountll(firsts & ((1ull << i % 64) - 1));
-        Job& job = jobs[n];
-        job.expert = e;
-        unsigned left = mask[e];
-        for (int place = 0; place < 16; ++place) {
-            int to = kNone;
-            float g = 0.0f;
-            if (left != 0) {
-                to = __builtin_ctz(left);
-                left &= left - 1;
-                for (int k = 0; k < s.top_k; ++k)
-                    if (chosen[to][k] == e) g = gate[to][k];
-            }
-            job.token[place] = to;
-            job.gate[place] = g;
-        }
+        place[e] = n;
+        jobs[n].expert = e;
     }
-    const int all = counts[0] + counts[1];
     __syncthreads();
-    return all;
+    if (pair) {
+        Job& job = jobs[place[e]];
+        job.token[__builtin_popcount(before)] = t;
+        job.gate[__builtin_popcount(before)] = g;
+    }
+    __syncthreads();
+    return counts[0] + counts[1];
+}
+
+__device__ __forceinline__ void clear_few_jobs(const Sizes& s, unsigned* mask, Job* jobs) {
+    for (int i = threadIdx.x; i < s.experts; i += blockDim.x) mask[i] = 0;
+    for (int i = threadIdx.x; i < 16 * s.max_jobs; i += blockDim.x) {
+        jobs[i / 16].token[i % 16] = kNone;
+        jobs[i / 16].gate[i % 16] = 0.0f;
+    }
+}
+
+// x in pieces, padded with zeros, and zeros for the end of h, by `blocks` blocks
+// of moe_router of their own (by those with the logits it took 1.2 of 13 us).
+template <int kIn, bool kHalf>
+__device__ __forceinline__ void cut_tokens(const void* __restrict__ x, long long ldx, const Workspace& w, const Sizes& s,
+                                           int block, int blocks) {
+    constexpr int kP = kPieces<kIn>;
+    const int chunks = s.tokens * (s.dp / 8);
+    for (int i = block * kThreads + threadIdx.x; i < chunks; i += blocks * kThreads) {
+        const int t = i % s.tokens, k = i / s.tokens * 8;
+        float v[8];
+        load_eight<kIn>(x, t * ldx + k, s.d - k, v);
+        if constexpr (kHalf) {
+            u16x8 same;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) same[e] = to_16<kF16>(v[e]);
+            *reinterpret_cast<u16x8*>(w.x + static_cast<long long>(i) * 8) = same;
+            continue;
+        }
+        u32x4 out[kP];
+        cut_eight<kP>(v, out);
+#pragma unroll
+        for (int p = 0; p < kP; ++p)
+            *reinterpret_cast<u32x4*>(w.x + (static_cast<long long>(p) * chunks + i) * 8) = out[p];
+    }
+
+    // h's columns past its last tile of 16, in all jobs, to zeros.
+    const int pad = s.hp / 8 - (s.h + 15) / 16 * 2, pads = (kIn == kF32 ? 3 : 2) * s.max_jobs * pad * 16;
+    for (int i = block * kThreads + threadIdx.x; i < pads; i += blocks * kThreads) {
+        const long long row = i / (pad * 16) + 1LL;  // ends of jobs, of all pieces
+        *reinterpret_cast<u32x4*>(w.h + row * 16 * s.hp - (i % (pad * 16) + 1) * 8) = u32x4{0, 0, 0, 0};
+    }
 }
 
 // 16 experts by 16 tokens of the logits over one part of d, 64 elements at a time
@@ -315,7 +357,6 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
                                                        const float* __restrict__ router, Workspace w, Sizes s,
                                                        bool normalize, int* __restrict__ chosen_out,
                                                        float* __restrict__ gates_out) {
-    constexpr int kP = kPieces<kIn>;
     extern __shared__ float logits[];  // [16, experts], in the last block of 16 tokens
     __shared__ f32x4 space[kWaves * 64];
     __shared__ int chosen[kMaxTokens][kMaxTopK];
@@ -325,9 +366,12 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
     __shared__ int flag;
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
-    const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16, parts = gridDim.z;
-    const int blocks = gridDim.x * gridDim.y * parts;
-    const int block = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16, parts = gridDim.z / 2;
+    if (static_cast<int>(blockIdx.z) >= parts) {
+        const int block = ((blockIdx.z - parts) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+        cut_tokens<kIn, kHalf>(x, ldx, w, s, block, gridDim.x * gridDim.y * parts);
+        return;
+    }
     const long long all_logits = static_cast<long long>(s.tokens) * s.experts;
 
     const long long expert = e0 + r < s.experts ? e0 + r : s.experts - 1;
@@ -352,26 +396,6 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
         for (int v = 0; v < 4; ++v)
             if (t0 + r < s.tokens && e0 + 4 * q + v < s.experts) mc_split_store(out + v, sum[v]);
     });
-
-    // x in pieces, padded with zeros, shared out over the blocks.
-    const int chunks = s.tokens * (s.dp / 8);
-    for (int i = block * kThreads + threadIdx.x; i < chunks; i += blocks * kThreads) {
-        const int t = i % s.tokens, k = i / s.tokens * 8;
-        float v[8];
-        load_eight<kIn>(x, t * ldx + k, s.d - k, v);
-        if constexpr (kHalf) {
-            u16x8 same;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) same[e] = to_16<kF16>(v[e]);
-            *reinterpret_cast<u16x8*>(w.x + static_cast<long long>(i) * 8) = same;
-            continue;
-        }
-        u32x4 out[kP];
-        cut_eight<kP>(v, out);
-#pragma unroll
-        for (int p = 0; p < kP; ++p)
-            *reinterpret_cast<u32x4*>(w.x + (static_cast<long long>(p) * chunks + i) * 8) = out[p];
-    }
 
     if (s.tokens <= kFew) return;
     if (!mc_split_last_arrival(w.arrived + 1 + blockIdx.y, gridDim.x * parts, &flag)) return;
@@ -463,7 +487,8 @@ __device__ __forceinline__ float activate(float u, float up) {
 // jobs there are. The waves take a tile's steps in turn, and the next step, of
 // the next tile too, is under way while one is multiplied and while the waves'
 // sums are added (a block per tile waited for its job, its weights and its sums
-// in turn: 143 MB of mx4 in 42 us). Columns from h to hp are written as zeros.
+// in turn: 143 MB of mx4 in 42 us). Columns past h are written as zeros (past
+// the last tile by moe_router).
 // kHalf: x was kept in fp16, as the weights are (one piece).
 template <int kType>
 constexpr int kUpWaves = kType == kMx4 ? 8 : 4;  // 16-bit weights take the registers of two mx4 waves
@@ -482,22 +507,22 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
     extern __shared__ float logits[];  // for few tokens: [tokens, experts], then their jobs
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16;
-    const int tiles = s.hp / kUpCols, steps = s.dp / kStep;
-    const Job* jobs = w.job;
+    const int tiles = (s.h + kUpCols - 1) / kUpCols, steps = s.dp / kStep;
+    Job* jobs = reinterpret_cast<Job*>(logits);  // the block's, from `first_job` on
     int count;
     if (s.tokens <= kFew) {
         __shared__ int chosen[kFew][kMaxTopK];
         __shared__ float gate[kFew][kMaxTopK];
         __shared__ unsigned mask[kMaxExperts];
-        __shared__ int counts[2];
-        Job* few = reinterpret_cast<Job*>(logits + s.tokens * s.experts);
+        __shared__ int place[kMaxExperts], counts[2];
+        jobs = reinterpret_cast<Job*>(logits + s.tokens * s.experts);
+        clear_few_jobs(s, mask, jobs);
         route(w, s, parts, 0, s.tokens, normalize, logits, chosen, gate);
-        count = list_few_jobs(s, chosen, gate, mask, counts, few);
-        jobs = few;
+        count = list_few_jobs(s, chosen, gate, mask, place, counts, jobs);
         if (blockIdx.x == 0) {  // for moe_down and the caller
             if (threadIdx.x == 0) *w.jobs = count;
             for (int i = threadIdx.x; i < count * static_cast<int>(sizeof(Job) / 4); i += kThreads)
-                reinterpret_cast<int*>(w.job)[i] = reinterpret_cast<const int*>(few)[i];
+                reinterpret_cast<int*>(w.job)[i] = reinterpret_cast<const int*>(jobs)[i];
             for (int i = threadIdx.x; i < s.tokens * s.top_k; i += kThreads) {
                 if (chosen_out != nullptr) chosen_out[i] = chosen[i / s.top_k][i % s.top_k];
                 if (gates_out != nullptr) gates_out[i] = gate[i / s.top_k][i % s.top_k];
@@ -507,18 +532,29 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
         count = *w.jobs;
     }
     const long long all = static_cast<long long>(count) * tiles;
-    const int from = static_cast<int>(blockIdx.x * all / gridDim.x), to = static_cast<int>((blockIdx.x + 1) * all / gridDim.x);
+    // (Said to be the same in all lanes: a descriptor that may differ is loaded through lane by lane.)
+    const int from = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * all / gridDim.x));
+    const int to = __builtin_amdgcn_readfirstlane(static_cast<int>((blockIdx.x + 1) * all / gridDim.x));
     if (from >= to) return;
+    int first_job = 0;
+    if (s.tokens > kFew) {
+        first_job = from / tiles;
+        const int dwords = ((to - 1) / tiles - first_job + 1) * static_cast<int>(sizeof(Job) / 4);
+        for (int i = threadIdx.x; i < dwords; i += kThreads)
+            reinterpret_cast<int*>(jobs)[i] = reinterpret_cast<const int*>(w.job + first_job)[i];
+        __syncthreads();
+    }
     const int h_rows = kGated ? 2 * s.h : s.h;
+    const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
 
-    int job = from / tiles, expert = __builtin_amdgcn_readfirstlane(jobs[job].expert), token = jobs[job].token[r];
+    int job = kNone, expert = 0, token = kNone;
     const auto open = [&](int u, In& in) {
         if (u / tiles != job) {
             job = u / tiles;
-            expert = __builtin_amdgcn_readfirstlane(jobs[job].expert);
-            token = jobs[job].token[r];
+            expert = __builtin_amdgcn_readfirstlane(jobs[job - first_job].expert);
+            token = jobs[job - first_job].token[r];
         }
-        const int h0 = u % tiles * kUpCols < s.h ? u % tiles * kUpCols : 0;  // past h: not used
+        const int h0 = u % tiles * kUpCols;
         in.open(w1, w1_scales, s.d, static_cast<long long>(s.experts) * h_rows, [&](int i) {
             return static_cast<long long>(expert) * h_rows + (kGated ? h0 + i * s.h : h0 + 16 * i < s.h ? h0 + 16 * i : 0);
         });
@@ -564,7 +600,6 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
             }
             float piece[kHP];
             cut<kHP>(in_h ? activate<kAct>(a, up) : 0.0f, piece);
-            const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
 #pragma unroll
             for (int p = 0; p < kHP; ++p)
                 w.h[p * h_plane + static_cast<long long>(of_job) * 16 * s.hp + (col / 8 * 16 + er) * 8 + col % 8] =
@@ -589,7 +624,6 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
     const int d0 = blockIdx.x * kCols, shares = gridDim.y;
     const int cells = s.tokens * kCols;
     float* mine = tile + wave * cells;
-    for (int i = lane; i < cells; i += 64) mine[i] = 0.0f;
     const int steps = s.hp / kStep, units = *w.jobs * steps;
     const int waves = shares * kWaves, each = units / waves, more = units % waves;
     const int index = blockIdx.y * kWaves + wave;
@@ -615,6 +649,7 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
         open(n);
         in.load(t, next);
     }
+    for (int i = lane * 4; i < cells; i += 256) *reinterpret_cast<f32x4*>(mine + i) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int u = from; u < to;) {
         const int of_expert = expert, of_token = token;
         const float of_gate = gate;
@@ -686,11 +721,14 @@ int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, 
     constexpr int kUpCols = kAct == MCHIP_MOE_SWIGLU ? 16 : 32;
     constexpr bool kHalf = kIn == kF16 && kType == kF16;
     // As many blocks as the registers let run at once, about.
-    const long long units = static_cast<long long>(s.max_jobs) * (s.hp / kUpCols);
+    const long long units = static_cast<long long>(s.max_jobs) * ((s.h + kUpCols - 1) / kUpCols);
     const long long blocks = static_cast<long long>(kType == kMx4 ? 2 : 3) * device_cus();
-    const std::size_t few = s.tokens <= kFew ? sizeof(float) * s.tokens * s.experts + sizeof(Job) * s.max_jobs : 0;
+    // A block's jobs: all of few tokens' (behind their logits), or those of its share of the units.
+    const long long grid = std::min(blocks, units);
+    const std::size_t jobs = s.tokens <= kFew ? s.max_jobs : std::min<long long>(s.max_jobs, s.max_jobs / grid + 2);
+    const std::size_t lds = sizeof(Job) * jobs + (s.tokens <= kFew ? sizeof(float) * s.tokens * s.experts : 0);
     hipLaunchKernelGGL((moe_up<kType, kHalf ? 1 : kPieces<kIn>, kHP, kAct, kOdd, kHalf>),
-                       dim3(static_cast<unsigned>(std::min(blocks, units))), dim3(64 * kUpWaves<kType>), few, stream, a.w1,
+                       dim3(static_cast<unsigned>(grid)), dim3(64 * kUpWaves<kType>), lds, stream, a.w1,
                        static_cast<const unsigned char*>(a.w1_scales), a.b1, w, s, router_parts(s.d), a.normalize != 0,
                        a.chosen, a.gates);
     hipLaunchKernelGGL((moe_down<kType, kHP, kIn, kOdd>),
@@ -722,7 +760,7 @@ int launch(const mchip_moe_args& a, hipStream_t stream) {
     Workspace w;
     lay_out(s, a.dtype, static_cast<unsigned char*>(a.workspace), &w);
     const dim3 grid(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16),
-                    static_cast<unsigned>(router_parts(s.d)));
+                    static_cast<unsigned>(2 * router_parts(s.d)));
     const auto router = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(kThreads), sizeof(float) * 16 * s.experts, stream, a.x, a.ldx,
                            a.router, w, s, a.normalize != 0, a.chosen, a.gates);
