@@ -132,7 +132,12 @@ __global__ __launch_bounds__(kColumnThreads) void quantize_columns(const void* _
                                                              void* __restrict__ values, int k, int n, int k_blocks) {
     typedef std::conditional_t<kType == kF32, float, unsigned short> Element;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, q = lane / 16;
-    const int col = blockIdx.y * 64 + wave % 4 * 16 + lane % 16, kb = blockIdx.x * 4 + wave / 4;
+    // Blocks go to the XCDs in turn; consecutive steps of one, so that its L2 joins
+    // their pieces of a line of codes or scales.
+    const unsigned block = blockIdx.y * gridDim.x + blockIdx.x, all = gridDim.x * gridDim.y;
+    const unsigned mine = block % 8 * (all / 8) + block / 8, at_block = block < all / 8 * 8 ? mine : block;
+    const int col = static_cast<int>(at_block / gridDim.x) * 64 + wave % 4 * 16 + lane % 16;
+    const int kb = static_cast<int>(at_block % gridDim.x) * 4 + wave / 4;
     const int k0 = kb * 32 + q * 8, last = k - 1;
     const bool has = col < n;
     const Element* at = static_cast<const Element*>(w) + (has ? col : n - 1);
