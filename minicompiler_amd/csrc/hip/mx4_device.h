@@ -93,6 +93,7 @@ typedef u16x8 u16x8_loose __attribute__((aligned(2)));
 typedef u32x4 u32x4_loose __attribute__((aligned(2)));
 typedef u32x4 u32x4_dwords __attribute__((aligned(4)));
 typedef u16x4 u16x4_loose __attribute__((aligned(2)));
+typedef unsigned u32_loose __attribute__((aligned(2)));
 
 // The first `left` of four consecutive elements of a row of C at element `at`.
 template <int kType>

@@ -9,7 +9,9 @@
 // v_cvt_scalef32_pk_fp4_f32 divides, rounds and saturates so in one step.
 //
 // Bound by memory: 2 or 4 bytes read and 17/32 written per element (and 2 or 4
-// written for `values`).
+// written for `values`, past the caches: the codes are what is read next). By
+// rows 8192x2048 fp32 with values in 24.8 us (5.8 TB/s; 28.6 with plain stores),
+// 4096x14336 bf16 45 us (5.9), one row of 4096 1.5 us: a launch.
 
 #include <type_traits>
 
@@ -58,13 +60,14 @@ __device__ __forceinline__ void store_eight(void* p, long long at, const float (
     if (left >= 8) {
         if constexpr (kType == kF32) {
             f32x4_loose* d = reinterpret_cast<f32x4_loose*>(static_cast<float*>(p) + at);
-            d[0] = f32x4{v[0], v[1], v[2], v[3]};
-            d[1] = f32x4{v[4], v[5], v[6], v[7]};
+            const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+            __builtin_nontemporal_store(lo, d);
+            __builtin_nontemporal_store(hi, d + 1);
         } else {
             u16x8 h;
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] = to_16<kType>(v[e]);
-            *reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(p) + at) = h;
+            __builtin_nontemporal_store(h, reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(p) + at));
         }
         return;
     }
@@ -117,54 +120,84 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict
     }
 }
 
-// A lane takes eight elements down one column, the lanes 16 q + r, q = 0..3, a
-// block of column r; a wave 16 neighbouring columns, a thread block 64 columns
+// A lane takes eight elements down kPer neighbouring columns, the lanes 16 q + r,
+// q = 0..3, a block of them; a wave 16 kPer columns, a thread block 64 kPer
 // (whole lines of 16-bit rows) of four blocks of k (a step, 64 bytes of codes per
 // column). Rows past k are read as the last one and count as zeros. Code is
 // short, since a launch meets a cold instruction cache (32 elements per lane,
-// 5.5 KB of code: 1001x2047 fp16 in 6.9 us).
+// 5.5 KB of code: 1001x2047 fp16 in 6.9 us, so in 4.4). With values 4096x4096
+// fp32 25 us (5.8 TB/s; 37 with plain stores), 4096x14336 bf16 74 us (3.6 TB/s:
+// codes come in pieces of 4 bytes, 64 to a column and block). Loads past the
+// caches took 92: a line of x is read by several lanes' loads.
 constexpr int kColumnThreads = 1024;
 
-template <int kType>
+template <int kType, int kPer>
 __global__ __launch_bounds__(kColumnThreads) void quantize_columns(const void* __restrict__ w, long long ld,
-                                                             unsigned* __restrict__ codes,
-                                                             unsigned char* __restrict__ scales,
-                                                             void* __restrict__ values, int k, int n, int k_blocks) {
+                                                                   unsigned* __restrict__ codes,
+                                                                   unsigned char* __restrict__ scales,
+                                                                   void* __restrict__ values, int k, int n,
+                                                                   int k_blocks) {
     typedef std::conditional_t<kType == kF32, float, unsigned short> Element;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, q = lane / 16;
     // Blocks go to the XCDs in turn; consecutive steps of one, so that its L2 joins
     // their pieces of a line of codes or scales.
     const unsigned block = blockIdx.y * gridDim.x + blockIdx.x, all = gridDim.x * gridDim.y;
     const unsigned mine = block % 8 * (all / 8) + block / 8, at_block = block < all / 8 * 8 ? mine : block;
-    const int col = static_cast<int>(at_block / gridDim.x) * 64 + wave % 4 * 16 + lane % 16;
+    const int col = static_cast<int>(at_block / gridDim.x) * 64 * kPer + (wave % 4 * 16 + lane % 16) * kPer;
     const int kb = static_cast<int>(at_block % gridDim.x) * 4 + wave / 4;
     const int k0 = kb * 32 + q * 8, last = k - 1;
     const bool has = col < n;
-    const Element* at = static_cast<const Element*>(w) + (has ? col : n - 1);
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = load_one<kType>(at, (k0 + e < last ? k0 + e : last) * ld);
-    unsigned top = 0;
+    const Element* at = static_cast<const Element*>(w) + (has ? col : n - kPer);
+    float v[kPer][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        v[e] = k0 + e < k ? v[e] : 0.0f;
-        const unsigned m = magnitude(v[e]);
-        top = m > top ? m : top;
+        const Element* row = at + (k0 + e < last ? k0 + e : last) * ld;
+        if constexpr (kPer == 1) {
+            v[0][e] = load_one<kType>(row, 0);
+        } else {
+            const unsigned two = *reinterpret_cast<const u32_loose*>(row);
+            v[0][e] = to_f32<kType>(two & 0xffffu);
+            v[1][e] = to_f32<kType>(two >> 16);
+        }
     }
-    u32x2 other = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(top, top, false, false));
-    top = other[0] > other[1] ? other[0] : other[1];
-    other = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(top, top, false, false));
-    top = other[0] > other[1] ? other[0] : other[1];
-    const unsigned s = scale_byte(top), c = encode_eight(v, s);
+    unsigned c[kPer], s[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        unsigned top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[j][e] = k0 + e < k ? v[j][e] : 0.0f;
+            const unsigned m = magnitude(v[j][e]);
+            top = m > top ? m : top;
+        }
+        u32x2 other = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(top, top, false, false));
+        top = other[0] > other[1] ? other[0] : other[1];
+        other = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(top, top, false, false));
+        s[j] = scale_byte(other[0] > other[1] ? other[0] : other[1]);
+        c[j] = encode_eight(v[j], s[j]);
+    }
     if (!has) return;
-    codes[(static_cast<long long>(col) * k_blocks + kb) * 4 + q] = c;
-    if (q == 0) scales[static_cast<long long>(col) * k_blocks + kb] = static_cast<unsigned char>(s);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        codes[(static_cast<long long>(col + j) * k_blocks + kb) * 4 + q] = c[j];
+        if (q == 0) scales[static_cast<long long>(col + j) * k_blocks + kb] = static_cast<unsigned char>(s[j]);
+    }
     if (values == nullptr) return;
-    decode_eight_f32(c, s, v);
     Element* to = static_cast<Element*>(values) + col;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (k0 + e < k) store_one<kType>(to, static_cast<long long>(k0 + e) * n, v[e]);
+    for (int j = 0; j < kPer; ++j) decode_eight_f32(c[j], s[j], v[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (k0 + e >= k) continue;
+        Element* row = to + static_cast<long long>(k0 + e) * n;
+        if constexpr (kType == kF32)
+            __builtin_nontemporal_store(v[0][e], row);
+        else if constexpr (kPer == 1)
+            __builtin_nontemporal_store(to_16<kType>(v[0][e]), row);
+        else
+            __builtin_nontemporal_store(to_16<kType>(v[0][e]) | static_cast<unsigned>(to_16<kType>(v[1][e])) << 16,
+                                        reinterpret_cast<u32_loose*>(row));
+    }
 }
 
 const char* refusal(int dtype, const void* x, long long ld, const void* codes, const void* scales, int outer, int inner,
@@ -199,15 +232,21 @@ template <int kType>
 int launch_columns(const void* w, long long ld, void* codes, void* scales, int k, int n, void* values,
                    hipStream_t stream, const char** why) {
     const int k_blocks = static_cast<int>(mchip_mx4_k(k) / 32);
-    const unsigned cols = static_cast<unsigned>((static_cast<long long>(n) + 63) / 64);
-    if (cols > 65535u) {
-        *why = "more columns than one launch takes (4194240)";
-        return hipErrorInvalidValue;
+    const auto go = [&](auto kernel, int per) {
+        const unsigned cols = static_cast<unsigned>((static_cast<long long>(n) + 64 * per - 1) / (64 * per));
+        if (cols > 65535u) {
+            *why = "more columns than one launch takes (4194240)";
+            return static_cast<int>(hipErrorInvalidValue);
+        }
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(k_blocks / 4), cols), dim3(kColumnThreads), 0, stream, w, ld,
+                           static_cast<unsigned*>(codes), static_cast<unsigned char*>(scales), values, k, n, k_blocks);
+        return static_cast<int>(hipGetLastError());
+    };
+    if constexpr (kType != kF32) {
+        // Two columns to a lane load dwords (4096x14336 bf16 with values: 74 us, 80 by one).
+        if (n % 2 == 0) return go(quantize_columns<kType, 2>, 2);
     }
-    hipLaunchKernelGGL(quantize_columns<kType>, dim3(static_cast<unsigned>(k_blocks / 4), cols), dim3(kColumnThreads), 0,
-                       stream, w, ld, static_cast<unsigned*>(codes), static_cast<unsigned char*>(scales), values, k, n,
-                       k_blocks);
-    return hipGetLastError();
+    return go(quantize_columns<kType, 1>, 1);
 }
 
 }  // namespace
