@@ -135,7 +135,6 @@ bool tiles_fit(const Product& p) {
 template <int kOut>
 int launch(const Product& p) {
     const int cus = device_cus();
-    if (tiles_fit(p) && tiles(p.m, kTileRows) * tiles(p.n, kTileCols) >= cus / 2) return launch_tiles<kOut>(p);
     const auto blocks = [&](int bm, int bn) { return tiles(p.m, 16 * bm) * tiles(p.n, 16 * bn); };
     if (p.m <= 16) {
         if (blocks(1, 4) >= cus) return launch_direct<1, 4, kOut>(p);
@@ -147,7 +146,16 @@ int launch(const Product& p) {
         if (blocks(2, 2) >= cus) return launch_direct<2, 2, kOut>(p);
         return launch_direct<1, 1, kOut>(p);
     }
-    if (blocks(4, 4) >= cus) return launch_direct<4, 4, kOut>(p);
+    // A round of 256x256 tiles takes as long as 2.25 rounds of 64x64 (24 and 10.4 us each at
+    // k = 4096), however few of the CUs have one: 2048x3840x4096, 120 tiles, in 26 us, by 64x64
+    // in 77; 1024x2560x600 in 10.9 and 16.0.
+    const long long large = blocks(4, 4), rounds = (large + cus - 1) / cus;
+    const long long tile_rounds = (tiles(p.m, kTileRows) * tiles(p.n, kTileCols) + cus - 1) / cus;
+    if (tiles_fit(p) && 4 * large >= 9 * cus * tile_rounds) return launch_tiles<kOut>(p);
+    // 64x64 per block read the least, one block to a CU at a time: where that leaves no
+    // round a fifth empty (1000x1001x8000 in 19.3 us, 22.4 by 32x64; 1400x1001x4096,
+    // 352 blocks on 256 CUs, in 20.4, 17.0 by 32x64).
+    if (large >= cus && 5 * large >= 4 * rounds * cus) return launch_direct<4, 4, kOut>(p);
     if (blocks(2, 4) >= cus) return launch_direct<2, 4, kOut>(p);
     if (blocks(2, 2) >= cus) return launch_direct<2, 2, kOut>(p);
     return launch_direct<1, 1, kOut>(p);

@@ -422,8 +422,10 @@ template <int kP, int kOut>
 int launch_pieces(const Product& p) {
     const int cus = device_cus();
     const auto blocks = [&](int bm, int bn) { return tiles(p.m, 16 * bm) * tiles(p.n, 16 * bn); };
-    // 32-bit offsets from a tile's origin.
-    if (blocks(8, 8) >= cus && p.k <= (1 << 22) && tiles(p.m, kTile) * tiles(p.n, kTile) < 0x7fffffffLL) {
+    // 128x128 tiles: where three quarters of the CUs have one (512x4096x4096 bf16, 128 of them, in
+    // 42 us, by the direct kernel in 33; fp16 64 in 76 and 27, which grows with their number).
+    // (32-bit offsets from a tile's origin.)
+    if (4 * blocks(8, 8) >= 3 * cus && p.k <= (1 << 22) && tiles(p.m, kTile) * tiles(p.n, kTile) < 0x7fffffffLL) {
         hipLaunchKernelGGL((weights_tiles<kP, kOut>), dim3(static_cast<unsigned>(blocks(8, 8))), dim3(kTileThreads), 0, p.stream,
                            p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
                            static_cast<int>(tiles(p.n, kTile)));
