@@ -5,19 +5,26 @@
 //
 // Three launches, in stream order:
 //   moe_router  x R^T on the FP32 matrix instruction, d shared out over blocks; x
-//               cut into bf16 pieces; for more than 8 tokens the last block of 16
-//               tokens adds the parts of their logits in order and picks their
-//               experts, and the last of all lists the jobs (one per chosen
-//               expert and 16 of its tokens);
-//   moe_up      (up to 8 tokens: every block picks the experts for itself, which
-//               is less than waiting for one that does;) per job and 32 (swiglu: 16) columns of h: act(x W1^T + b1), cut
-//               into bf16 pieces;
+//               cut into bf16 pieces by blocks of their own; for more than 8
+//               tokens the last block of 16 tokens adds the parts of their logits
+//               in order and picks their experts, and the last of all lists the
+//               jobs (one per chosen expert and 16 of its tokens);
+//   moe_up      per job and 32 (swiglu: 16) columns of h: act(x W1^T + b1), cut
+//               into bf16 pieces. Up to 8 tokens every block picks the experts for
+//               itself, which is less than waiting for one that does;
 //   moe_down    per 32 columns of y and share of the jobs' steps: h W2^T weighed
 //               by the gates; the last block of a column tile adds the shares
 //               in order.
-// Bound by the chosen experts' weights, each read once per job. Weights are the
+// Bound by the chosen experts' weights, each read once per job, and for few
+// tokens by the chain of launches, routing and trips to memory. Weights are the
 // matrix instruction's first operand, 16 rows of them, and a job's 16 tokens
 // the second. Products are exact (bf16 pieces of x, h and the weights), sums fp32.
+//
+// Measured (router, up, down, and all of it in steady repetition): one token, 8
+// of 64 mx4 experts of 2048x1024: 3.3, 9.5, 6.8, 22 us (27 MB); 16 tokens, 8 bf16
+// experts of 512x2048, fp32: 7.7, 7.8, 8.6, 29 us (34 MB); 64 tokens, 32 fp16
+// experts of 1023x777: 12.4, 25.5, 22.4, 68 us (153 MB; with rows of 1024 and 768
+// elements 11.3, 20, 15: rows at odd places cost a quarter of the rate).
 
 #include "mx4_rows.h"
 
