@@ -110,7 +110,7 @@ template <int kM, int kN, int kOut>
 int launch_direct(const Product& p) {
     constexpr int kWaves = 8;
     const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (!fits_launch(blocks, kWaves * 64)) return hipErrorInvalidValue;
     hipLaunchKernelGGL((product_direct<kM, kN, kWaves, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64),
                        0, p.stream, p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps,
                        static_cast<unsigned>(tn));
@@ -129,7 +129,7 @@ int launch_tiles(const Product& p) {
 
 // Four steps at least (a slot of scales), and 32-bit offsets from a tile's origin.
 bool tiles_fit(const Product& p) {
-    return p.steps >= 4 && p.steps <= (1 << 16) && tiles(p.m, kTileRows) * tiles(p.n, kTileCols) < (1 << 30);
+    return p.steps >= 4 && p.steps <= (1 << 16) && fits_launch(tiles(p.m, kTileRows) * tiles(p.n, kTileCols) * 2, kTileThreads);
 }
 
 template <int kOut>

@@ -403,8 +403,10 @@ template <int kIn, int kN, int kOut>
 int launch_few(const Product& p) {
     const long long size = kSize<kIn>;
     const bool loose = !aligned(p.a, 4) || p.lda * size % 4 != 0 || ((p.m - 1) * p.lda + p.k) * size > 0x7fffff00LL;
+    const long long blocks = tiles(p.n, 16 * kN);
+    if (!fits_launch(blocks, kFewWaves * 64)) return hipErrorInvalidValue;
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles(p.n, 16 * kN))), dim3(kFewWaves * 64), 0, p.stream, p.a,
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kFewWaves * 64), 0, p.stream, p.a,
                            p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
         return static_cast<int>(hipGetLastError());
     };
@@ -416,7 +418,7 @@ template <int kP, int kM, int kN, int kOut>
 int launch_direct(const Product& p) {
     typedef Direct<kP * kM, kN> Shape;
     const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (!fits_launch(blocks, 64 * Shape::kWaves)) return hipErrorInvalidValue;
     hipLaunchKernelGGL((weights_direct<Shape, kP, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(64 * Shape::kWaves),
                        0, p.stream, p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
                        static_cast<unsigned>(tn));
@@ -430,7 +432,7 @@ int launch_pieces(const Product& p) {
     // 128x128 tiles: where three quarters of the CUs have one (512x4096x4096 bf16, 128 of them, in
     // 42 us, by the direct kernel in 33; fp16 64 in 76 and 27, which grows with their number).
     // (32-bit offsets from a tile's origin.)
-    if (4 * blocks(8, 8) >= 3 * cus && p.k <= (1 << 22) && tiles(p.m, kTile) * tiles(p.n, kTile) < 0x7fffffffLL) {
+    if (4 * blocks(8, 8) >= 3 * cus && p.k <= (1 << 22) && fits_launch(blocks(8, 8), kTileThreads)) {
         hipLaunchKernelGGL((weights_tiles<kP, kOut>), dim3(static_cast<unsigned>(blocks(8, 8))), dim3(kTileThreads), 0, p.stream,
                            p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
                            static_cast<int>(tiles(p.n, kTile)));
@@ -460,7 +462,7 @@ int launch(const Product& p) {
     }
     const int rows = piece_rows(p.m), chunks = padded(p.k) / 8;
     const long long blocks = tiles(static_cast<long long>(rows) * chunks, 256);
-    if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (!fits_launch(blocks, 256)) return hipErrorInvalidValue;
     hipLaunchKernelGGL(cut_rows<kIn>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, p.stream, p.a, p.lda, p.pieces, p.m,
                        rows, p.k, chunks);
     const hipError_t e = hipGetLastError();

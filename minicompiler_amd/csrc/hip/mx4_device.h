@@ -265,6 +265,9 @@ inline bool is_float_type(int dtype) {
     return dtype == MCHIP_DTYPE_F32 || dtype == MCHIP_DTYPE_BF16 || dtype == MCHIP_DTYPE_F16;
 }
 
+// A launch takes fewer than 2^32 threads along a dimension of its grid.
+inline bool fits_launch(long long blocks, int threads) { return blocks < (1LL << 32) / threads; }
+
 // CUs of the current device, asked once per device.
 inline int device_cus() {
     static std::atomic<int> cache[64];

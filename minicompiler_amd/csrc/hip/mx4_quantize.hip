@@ -213,33 +213,53 @@ const char* refusal(int dtype, const void* x, long long ld, const void* codes, c
     return nullptr;
 }
 
+// `elements` of x's type from p on (or null).
 template <int kType>
-int launch_rows(const void* x, long long ld, void* codes, void* scales, int rows, int k, void* values,
-                hipStream_t stream, const char** why) {
-    const unsigned per_row = static_cast<unsigned>(mchip_mx4_k(k) / 8);
-    const long long blocks = (static_cast<long long>(rows) * per_row + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffffLL) {
-        *why = "more elements than one launch takes (2^42)";
-        return hipErrorInvalidValue;
-    }
-    hipLaunchKernelGGL(quantize_rows<kType>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, x, ld,
-                       static_cast<unsigned*>(codes), static_cast<unsigned char*>(scales), values,
-                       static_cast<long long>(rows), k, per_row);
-    return hipGetLastError();
+const void* offset(const void* p, long long elements) {
+    return p == nullptr ? nullptr : static_cast<const unsigned char*>(p) + elements * kSize<kType>;
+}
+template <int kType>
+void* offset(void* p, long long elements) {
+    return const_cast<void*>(offset<kType>(static_cast<const void*>(p), elements));
 }
 
+// As many rows at a time as a launch takes.
+template <int kType>
+int launch_rows(const void* x, long long ld, void* codes, void* scales, int rows, int k, void* values,
+                hipStream_t stream) {
+    const unsigned per_row = static_cast<unsigned>(mchip_mx4_k(k) / 8);
+    const long long most = ((1LL << 32) - kThreads) / per_row;
+    for (long long from = 0; from < rows; from += most) {
+        const long long count = std::min(most, rows - from);
+        const unsigned blocks = static_cast<unsigned>((count * per_row + kThreads - 1) / kThreads);
+        hipLaunchKernelGGL(quantize_rows<kType>, dim3(blocks), dim3(kThreads), 0, stream, offset<kType>(x, from * ld), ld,
+                           static_cast<unsigned*>(codes) + from * per_row,
+                           static_cast<unsigned char*>(scales) + from * (per_row / 4), offset<kType>(values, from * k), count,
+                           k, per_row);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+// As much of k at a time as a launch takes.
 template <int kType>
 int launch_columns(const void* w, long long ld, void* codes, void* scales, int k, int n, void* values,
                    hipStream_t stream, const char** why) {
-    const int k_blocks = static_cast<int>(mchip_mx4_k(k) / 32);
+    const int k_blocks = static_cast<int>(mchip_mx4_k(k) / 32), most = (1 << 22) - 1;  // steps
     const auto go = [&](auto kernel, int per) {
         const unsigned cols = static_cast<unsigned>((static_cast<long long>(n) + 64 * per - 1) / (64 * per));
         if (cols > 65535u) {
             *why = "more columns than one launch takes (4194240)";
             return static_cast<int>(hipErrorInvalidValue);
         }
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(k_blocks / 4), cols), dim3(kColumnThreads), 0, stream, w, ld,
-                           static_cast<unsigned*>(codes), static_cast<unsigned char*>(scales), values, k, n, k_blocks);
+        for (int step = 0; step < k_blocks / 4; step += most) {
+            const int steps = std::min(most, k_blocks / 4 - step), from = step * kStep;
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(steps), cols), dim3(kColumnThreads), 0, stream,
+                               offset<kType>(w, from * ld), ld, static_cast<unsigned*>(codes) + step * 16LL,
+                               static_cast<unsigned char*>(scales) + step * 4LL,
+                               offset<kType>(values, static_cast<long long>(from) * n), k - from, n, k_blocks);
+        }
         return static_cast<int>(hipGetLastError());
     };
     if constexpr (kType != kF32) {
@@ -260,9 +280,9 @@ int mchip_quantize_mx4(int dtype, const void* x, long long ld, void* codes, void
     *why = refusal(dtype, x, ld, codes, scales, rows, k, k, values);
     if (*why != nullptr) return hipErrorInvalidValue;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == kF32) return launch_rows<kF32>(x, ld, codes, scales, rows, k, values, s, why);
-    if (dtype == kBf16) return launch_rows<kBf16>(x, ld, codes, scales, rows, k, values, s, why);
-    return launch_rows<kF16>(x, ld, codes, scales, rows, k, values, s, why);
+    if (dtype == kF32) return launch_rows<kF32>(x, ld, codes, scales, rows, k, values, s);
+    if (dtype == kBf16) return launch_rows<kBf16>(x, ld, codes, scales, rows, k, values, s);
+    return launch_rows<kF16>(x, ld, codes, scales, rows, k, values, s);
 }
 
 int mchip_quantize_mx4_columns(int dtype, const void* w, long long ld, void* codes, void* scales, int k, int n,

@@ -141,6 +141,42 @@ def test_quantize_rows_more_than_4_gib_apart(device, mc):
     assert np.array_equal(scales.get(np.uint8, want[1].shape), want[1])
 
 
+def download_at(mc, buf, offset, dtype, shape):
+    out = np.empty(shape, dtype=dtype)
+    assert mc.library().mc_memcpy_dtoh(out.ctypes.data, buf.ptr + offset, out.nbytes) == 0
+    return out
+
+
+@pytest.mark.parametrize("rows,k", [(1, (1 << 29) + 300), ((1 << 24) + 3, 2048)])
+def test_quantize_more_than_one_launch(device, mc, rows, k):
+    """2^29 rows of one column, 2^35 elements by rows: more threads than a launch has. The ends of both."""
+    columns = rows == 1
+    most = 4096  # elements at each end
+    rng = np.random.default_rng(9)
+    bits = ref.to_type(rng.standard_normal((2, most)), ref.BF16)
+    x = mc.DeviceBuffer(2 * rows * k)
+    x.fill_bytes(0)
+    # From an element that starts a row, and a step of one.
+    last = (k - most) // 128 * 128 if columns else rows * k - most
+    upload_at(mc, x, 0, bits[0])
+    upload_at(mc, x, 2 * last, bits[1])
+    codes, scales = mc.DeviceBuffer(mc.mx4_code_bytes(rows, k)), mc.DeviceBuffer(mc.mx4_scale_bytes(rows, k))
+    codes.fill_bytes(255)
+    scales.fill_bytes(255)
+    if columns:
+        mc.quantize_mx4_columns(ref.BF16, x.ptr, 1, codes.ptr, scales.ptr, k, 1)
+    else:
+        mc.quantize_mx4(ref.BF16, x.ptr, k, codes.ptr, scales.ptr, rows, k)
+    mc.synchronize()
+    for at, end in ((0, bits[0]), (last, bits[1])):
+        want = ref.quantize(ref.from_type(end, ref.BF16).reshape(1, -1))
+        assert np.array_equal(download_at(mc, codes, at // 2, np.uint8, want[0].shape), want[0])
+        assert np.array_equal(download_at(mc, scales, at // 32, np.uint8, want[1].shape), want[1])
+    middle = rows * k // 2 // 4096 * 4096
+    assert not download_at(mc, codes, middle // 2, np.uint8, (1 << 20,)).any()
+    assert not download_at(mc, scales, middle // 32, np.uint8, (1 << 16,)).any()
+
+
 # ---------------------------------------------------------------- products
 
 
