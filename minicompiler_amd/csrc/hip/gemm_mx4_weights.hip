@@ -6,7 +6,7 @@
 // into one, two or three bf16 pieces (8, 11 or 24 significant bits), each
 // multiplied by the same weights into the same fp32 sum.
 //
-//   weights_few     up to 8 rows: A cut by every wave as it reads it;
+//   weights_few     up to 16 rows: A cut by every wave as it reads it;
 //   cut_rows        A's pieces into the workspace, for the two below:
 //   weights_direct  few tiles: a block's waves share out k, fragments come
 //                   straight from memory;
@@ -20,7 +20,7 @@ namespace {
 
 using namespace mx4;
 
-constexpr int kFew = 8;
+constexpr int kFew = 16;
 constexpr int kFewWaves = 16;
 
 // ---------------------------------------------------------------- few rows
@@ -89,10 +89,12 @@ struct Eight {
     }
 };
 
-// 16 kN columns of C for all rows (at most 8); the waves take the steps of 128 k
+// 16 kN columns of C for all rows (at most 16); the waves take the steps of 128 k
 // in turn, the next one under way while one is multiplied. Bound by the weights
 // and a launch's latency: one row by 14336x4096 in 7.6 us (31 MB at 4.1 TB/s),
-// two by 4096x4096 in 3.7. kLoose: rows that do
+// two by 4096x4096 in 3.7. 16 bf16 rows take 10.4 us a call where a launch that
+// cuts them and one that multiplies took 12.0, 12 fp16 rows by 4096x4096 6.9 and
+// 8.2, fp32 ones 10.1 and 9.7. kLoose: rows that do
 // not all start at dwords, or more than 2 GiB of them.
 template <int kIn, int kN, int kOut, bool kLoose>
 __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
@@ -441,10 +443,8 @@ int launch_pieces(const Product& p) {
     if constexpr (kP < 3) {  // three pieces of 64 rows do not fit the registers
         if (p.m > 32 && blocks(4, 2) >= cus) return launch_direct<kP, 4, 2, kOut>(p);
     }
-    if (p.m > 16 && blocks(2, 2) >= cus) return launch_direct<kP, 2, 2, kOut>(p);
-    if (p.m > 16) return launch_direct<kP, 2, 1, kOut>(p);
-    if (blocks(1, 2) >= cus) return launch_direct<kP, 1, 2, kOut>(p);
-    return launch_direct<kP, 1, 1, kOut>(p);
+    if (blocks(2, 2) >= cus) return launch_direct<kP, 2, 2, kOut>(p);
+    return launch_direct<kP, 2, 1, kOut>(p);
 }
 
 template <int kIn, int kOut>

@@ -53,9 +53,9 @@ def test_weights(mc):
     for match, kw in [("type", {"dt": 4}), ("type", {"ct": 7}), ("size", {"m": 0}), ("closer", {"lda": 7}),
                       ("null", {"a": None}), ("null", {"bc": None}), ("codes", {"bc": P + 1}),
                       ("scales", {"bs": P + 2}), ("element", {"a": P + 1}), ("element", {"c": P + 1}),
-                      ("workspace", {"m": 9, "ws": None}), ("workspace", {"m": 100, "ws": P + 128})]:
+                      ("workspace", {"m": 17, "ws": None}), ("workspace", {"m": 100, "ws": P + 128})]:
         refused(mc, match, call, **kw)
-    assert mc.matmul_mx4_weights_workspace_bytes(1, 8, 64, 64) == 0  # few rows need none
+    assert mc.matmul_mx4_weights_workspace_bytes(1, 16, 64, 64) == 0  # few rows need none
     assert mc.matmul_mx4_weights_workspace_bytes(9, 4, 4, 4) == 0
 
 
