@@ -7,6 +7,8 @@
 // multiplied by the same weights into the same fp32 sum.
 //
 //   weights_few     up to 16 rows: A cut by every wave as it reads it;
+//   weights_whole   up to 32 rows of 16 bits, not cut: fp16 ones by the fp16
+//                   instruction, scales applied to its sums;
 //   cut_rows        A's pieces into the workspace, for the two below:
 //   weights_direct  few tiles: a block's waves share out k, fragments come
 //                   straight from memory;
@@ -21,6 +23,7 @@ namespace {
 using namespace mx4;
 
 constexpr int kFew = 16;
+constexpr int kWholeRows = 32;
 constexpr int kFewWaves = 16;
 
 // ---------------------------------------------------------------- few rows
@@ -92,9 +95,9 @@ struct Eight {
 // 16 kN columns of C for all rows (at most 16); the waves take the steps of 128 k
 // in turn, the next one under way while one is multiplied. Bound by the weights
 // and a launch's latency: one row by 14336x4096 in 7.6 us (31 MB at 4.1 TB/s),
-// two by 4096x4096 in 3.7. 16 bf16 rows take 10.4 us a call where a launch that
-// cuts them and one that multiplies took 12.0, 12 fp16 rows by 4096x4096 6.9 and
-// 8.2, fp32 ones 10.1 and 9.7. kLoose: rows that do
+// two by 4096x4096 in 3.7. 16 bf16 rows by 14336x4096 take 10.4 us a call where
+// a launch that cuts them and one that multiplies took 12.0, 12 fp32 rows by
+// 4096x4096 10.1 and 9.7. kLoose: rows that do
 // not all start at dwords, or more than 2 GiB of them.
 template <int kIn, int kN, int kOut, bool kLoose>
 __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
@@ -163,6 +166,137 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
         const long long col = col0 + 16 * j + 4 * q;
         if (has && col < n)
             store_four<kOut>(c, r * static_cast<long long>(n) + col, sum, static_cast<int>(n - col < 4 ? n - col : 4));
+    });
+}
+
+// ---------------------------------------------------------------- 16-bit rows as they are
+
+// 16 kM rows by 16 kN columns of C per block, 16-bit rows that start at dwords,
+// straight from memory: no pieces and no workspace. The waves take the steps of
+// 128 k in turn. Instruction s of a step multiplies its block s (lane (r, q)
+// elements 8 q .. + 7 of it), so that one scale holds for all that it adds up:
+// fp16 rows meet the bare codes (exact in fp16) in a sum from zero, which the
+// scale multiplies as it joins the others (a power of two: one rounding, the
+// sum's); bf16 ones the scaled weights. Neighbouring lanes load 64 bytes of a row
+// and pass them on (mx4_rows.h). Bound by A, which every block reads from its L2
+// and passes on through LDS (256 KiB for 32 rows of 4096). A call on 32 fp16 rows
+// by 4096x4096 takes 9.4 us (10.5 in two launches, cutting and weights_direct),
+// by 6144x2048 7.2 (11.0); bf16 7.6 (8.0) and 6.0 (8.2); 16 fp16 rows by
+// 4096x4096 5.9 (7.2 by weights_few), bf16 5.3 (6.5).
+template <int kN>
+constexpr int kWhole = kN == 1 ? 16 : 8;  // waves, as the registers allow
+
+template <int kIn, int kM, int kN, int kOut>
+__global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __restrict__ a, int lda,
+                                                                const unsigned char* __restrict__ b_codes,
+                                                                const unsigned char* __restrict__ b_scales,
+                                                                void* __restrict__ c, int m, int n, int k) {
+    __shared__ f32x4 space[kWhole<kN> * kM * kN * 64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep, row_bytes = padded(k) / 2;
+    const long long col0 = static_cast<long long>(blockIdx.x) * 16 * kN;
+    typedef Rows<kIn, kM, false, true> A;
+    A x;
+    x.open(a, nullptr, k, m, [&](int i) { return 16 * i; }, lda);
+    __amdgpu_buffer_rsrc_t codes[kN];
+    const unsigned char* scale_row = b_scales;
+    const int at = lane / 4 * row_bytes + lane % 4 * 4;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        const long long col = col0 + 16 * j < n ? col0 + 16 * j : 0, left = n - col;
+        codes[j] = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(b_codes + col * row_bytes), 0,
+                                                     (left < 16 ? static_cast<int>(left) : 16) * row_bytes, 0x00020000);
+        if (q == j) scale_row = b_scales + (col + (r < left ? r : 0)) * (padded(k) / 32);
+    }
+    f32x4 acc[kM * kN];
+#pragma unroll
+    for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    struct Step {
+        typename A::Step x;
+        unsigned w[kN][4], scales;  // lane 16 j + r: of column r of tile j
+    } now, next;
+    const auto load = [&](int t) {
+        x.load(t, next.x);
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                next.w[j][s] = __builtin_amdgcn_raw_buffer_load_b32(codes[j], at + 16 * s, t * 64, 0);
+        next.scales = q < kN ? *reinterpret_cast<const unsigned*>(scale_row + t * 4) : 0u;
+    };
+    const auto of_column = [&](int j, int column, unsigned v) {
+        return static_cast<unsigned>(__builtin_amdgcn_ds_bpermute((16 * j + column) * 4, static_cast<int>(v)));
+    };
+    unsigned nans = 0;  // high bits of bytes: a scale of 255 in lane's column
+    int t = wave;
+    if (t < steps) load(t);
+    while (t < steps) {
+        now = next;
+        const int then = t + kWhole<kN>;
+        if (then < steps) load(then);
+        if (x.past_end(t)) x.cut_off(t, now.x);
+        if constexpr (kIn == kF16) nans |= (~now.scales - 0x01010101u) & now.scales & 0x80808080u;
+        unsigned scales[kN][kIn == kF16 ? 4 : 1];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            if constexpr (kIn == kF16) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) scales[j][v] = of_column(j, 4 * q + v, now.scales);
+            } else {
+                scales[j][0] = of_column(j, r, now.scales);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            __builtin_amdgcn_sched_barrier(0);  // or the registers of four overflow
+            u32x4 rows[kM][1];
+#pragma unroll
+            for (int i = 0; i < kM; ++i) x.operand(now.x, i, s, 1.0f, rows[i]);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const unsigned w = x.pass(now.w[j][s]);
+                if constexpr (kIn == kF16) {
+                    const u32x4 of_codes = decode_eight_f16(w);
+                    f32x4 scale;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        // 2^(byte - 127), of byte 0 too.
+                        const unsigned bits = (s < 3 ? scales[j][v] << (23 - 8 * s) : scales[j][v] >> 1) & 0x7f800000u;
+                        scale[v] = __builtin_bit_cast(float, bits > 0x00400000u ? bits : 0x00400000u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kM; ++i) {
+                        const f32x4 sum = mfma_f16(of_codes, rows[i][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                        for (int v = 0; v < 4; ++v)
+                            acc[i * kN + j][v] = __builtin_fmaf(sum[v], scale[v], acc[i * kN + j][v]);
+                    }
+                } else {
+                    const u32x4 scaled = decode_eight(w, scale_operand(scales[j][0] >> 8 * s & 255u));
+#pragma unroll
+                    for (int i = 0; i < kM; ++i) acc[i * kN + j] = mfma_bf16(scaled, rows[i][0], acc[i * kN + j]);
+                }
+            }
+        }
+        t = then;
+    }
+    if constexpr (kIn == kF16) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const bool nan = of_column(j, 4 * q + v, nans) != 0;
+#pragma unroll
+                for (int i = 0; i < kM; ++i)
+                    acc[i * kN + j][v] = nan ? __builtin_nanf("") : acc[i * kN + j][v];
+            }
+    }
+    sum_waves<kWhole<kN>>(acc, space, wave, lane, [&](int i, f32x4 sum) {
+        const int row = 16 * (i / kN) + r;
+        const long long col = col0 + 16 * (i % kN) + 4 * q;
+        if (row < m && col < n)
+            store_four<kOut>(c, static_cast<long long>(row) * n + col, sum, static_cast<int>(n - col < 4 ? n - col : 4));
     });
 }
 
@@ -416,6 +550,15 @@ int launch_few(const Product& p) {
     return go(weights_few<kIn, kN, kOut, false>);
 }
 
+template <int kIn, int kM, int kN, int kOut>
+int launch_whole(const Product& p) {
+    const long long blocks = tiles(p.n, 16 * kN);
+    if (!fits_launch(blocks, kWhole<kN> * 64)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((weights_whole<kIn, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWhole<kN> * 64), 0,
+                       p.stream, p.a, static_cast<int>(p.lda), p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
+    return hipGetLastError();
+}
+
 template <int kP, int kM, int kN, int kOut>
 int launch_direct(const Product& p) {
     typedef Direct<kP * kM, kN> Shape;
@@ -449,11 +592,30 @@ int launch_pieces(const Product& p) {
 
 template <int kIn, int kOut>
 int launch(const Product& p) {
+    // One block of these runs on a CU at a time. Rounds of blocks, each as
+    // long as its columns and a fixed part take: one row by 14336 columns of
+    // k = 4096, 64 per block, in 8.9 us, 32 (two rounds) in 11.4.
+    const auto cost = [&](int wide) { return tiles(tiles(p.n, 16 * wide), device_cus()) * (2 * wide + 3); };
+    if constexpr (kIn != kF32) {
+        if (p.m <= kWholeRows && aligned(p.a, 4) && p.lda % 2 == 0 && p.lda < (1 << 26)) {
+            const bool by_16 = cost(1) <= cost(2) && cost(1) <= cost(4);
+            if (p.m > 16) {
+                // 32 rows by 4096x8192 bf16 (pieces then need no cutting) in 11.7 us both ways, by 4096x14336
+                // 21.2 and 19.3 by weights_direct, by 4096x4096 7.6 and 8.0.
+                if (!by_16) {
+                    if (cost(4) < cost(2)) return launch_whole<kIn, 2, 4, kOut>(p);
+                    return launch_whole<kIn, 2, 2, kOut>(p);
+                }
+                if (kIn == kF16 || p.k <= 8192) return launch_whole<kIn, 2, 1, kOut>(p);
+            } else if (by_16 && p.k > kWhole<1> * kStep && (kIn == kF16 || p.m >= 8)) {
+                // From a wave's second step on; weights_few's short code is faster below (12 rows by 1000x1000
+                // in 4.1 us, 4.6 here), for wide blocks (16 fp16 rows by 14336x4096: 11.2 and 13.9), and for bf16
+                // rows that are too few to crowd its loads (2 by 4096x4096: 4.3 and 5.1; 8: 5.4 and 5.2).
+                return launch_whole<kIn, 1, 1, kOut>(p);
+            }
+        }
+    }
     if (p.m <= kFew) {
-        // One block of 16 waves runs on a CU at a time. Rounds of blocks, each as
-        // long as its columns and a fixed part take: 14336 columns of k = 4096
-        // by 64 per block in 8.9 us, by 32 (two rounds) in 11.4.
-        const auto cost = [&](int wide) { return tiles(tiles(p.n, 16 * wide), device_cus()) * (2 * wide + 3); };
         if constexpr (kIn != kF32) {  // fp32 rows by 64 columns do not fit the registers
             if (cost(4) < cost(2) && cost(4) < cost(1)) return launch_few<kIn, 4, kOut>(p);
         }

@@ -220,6 +220,16 @@ __device__ __forceinline__ u32x4 decode_eight(unsigned codes, float scale) {
     return r;
 }
 
+// Without it, as the fp16 one's.
+__device__ __forceinline__ u32x4 decode_eight_f16(unsigned codes) {
+    u32x4 r;
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 0));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 1));
+    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 2));
+    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.0f, 3));
+    return r;
+}
+
 // The scale as the conversions take it: an fp32 whose exponent field is the
 // scale byte (they read no more of it; field 0 counts as 2^-127, 255 as NaN).
 __device__ __forceinline__ float scale_operand(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }

@@ -335,3 +335,56 @@ def test_operands_of_more_than_4_gib(device, mc):
         exact, bound = ref.product_bound(left, np.concatenate([np.ones((1, k)), tail]), k, ref.F32)
         within(got[n - last:], exact[0, 1:], bound[0, 1:])
         within(got[:n - last], exact[0, 0], bound[0, 0])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,pad", [(17, 16, 128, 0), (18, 40, 2050, 0), (31, 100, 4099, 1), (32, 4130, 300, 2),
+                                       (25, 5000, 2333, 3), (29, 33, 77, 5), (32, 8200, 130, 64)])
+def test_rows_of_16_bits_that_start_at_dwords(device, mc, kind, m, n, k, pad):
+    """Even distances between rows: read as they are, up to 32 of them; block scales over the whole range."""
+    print(f"case mx4 weights {kind} {m}x{n}x{k} pad {pad}", flush=True)
+    dtype = ref.TYPES[kind]
+    rng = np.random.default_rng(m * 11 + n + k)
+    bits = ref.to_type(rng.standard_normal((m, k)) * np.exp(rng.standard_normal(k)), dtype)
+    a = device_rows(mc, bits, k + pad)
+    bc, bs, b = operand(mc, rng, n, k, k ** -0.5)
+    c = Out(mc, m * n * 4)
+    workspace = mc.DeviceBuffer(mc.matmul_mx4_weights_workspace_bytes(dtype, m, n, k))
+    mc.launch_matmul_mx4_weights(dtype, a.ptr, k + pad, bc.ptr, bs.ptr, ref.F32, c.ptr, m, n, k, None, workspace.ptr)
+    mc.synchronize()
+    exact, bound = ref.product_bound(ref.from_type(bits, dtype), b, 3 * k, ref.F32)
+    within(c.get(np.float32, (m, n)).astype(np.float64), exact, bound)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [40, 4200])
+def test_scales_at_the_ends_and_of_no_number(device, mc, kind, n):
+    """Rows of powers of two meet columns of one scale each, from 2^-127 to 2^120: exact in fp32 down to 2^-126;
+    255 makes its columns NaN, whatever their codes."""
+    m, k, dtype = 32, 300, ref.TYPES[kind]
+    kp = ref.padded(k)
+    a_bits = ref.to_type(np.tile(2.0 ** (np.arange(m) % 4).reshape(m, 1), (1, k)), dtype)
+    codes, scales = np.zeros((n, kp // 2), np.uint8), np.zeros((n, kp // 32), np.uint8)
+    codes[:, 60] = 0x42  # elements 120 and 121: 1 and 2
+    scales[:, 3] = np.arange(n) * 31 % 248
+    bad = np.arange(n) % 7 == 3
+    scales[bad, 3] = 255
+    codes[np.arange(n) % 14 == 3, 60] = 0
+    a, bc, bs = device_rows(mc, a_bits, k), mc.DeviceBuffer.from_array(codes), mc.DeviceBuffer.from_array(scales)
+    c = Out(mc, m * n * 4)
+    workspace = mc.DeviceBuffer(mc.matmul_mx4_weights_workspace_bytes(dtype, m, n, k))
+    mc.launch_matmul_mx4_weights(dtype, a.ptr, k, bc.ptr, bs.ptr, ref.F32, c.ptr, m, n, k, None, workspace.ptr)
+    mc.synchronize()
+    got = c.get(np.float32, (m, n)).astype(np.float64)
+    assert np.all(np.isnan(got[:, bad]))
+    want = 3.0 * 2.0 ** (np.arange(m) % 4).reshape(m, 1) * 2.0 ** (scales[~bad, 3].astype(np.float64) - 127)
+    normal = want >= 2.0 ** -126
+    assert normal.mean() > 0.95 and np.array_equal(got[:, ~bad][normal], want[normal])
+    assert np.all(got[:, ~bad][~normal] <= 2.0 ** -126)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,pad", [(1, 30, 2050, 0), (3, 100, 4097, 1), (9, 1000, 2200, 6), (16, 4096, 2052, 0),
+                                       (32, 70, 9000, 0)])
+def test_few_rows_of_16_bits_and_a_long_k(device, mc, kind, m, n, k, pad):
+    test_rows_of_16_bits_that_start_at_dwords(device, mc, kind, m, n, k, pad)
