@@ -177,27 +177,38 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
 // elements 8 q .. + 7 of it), so that one scale holds for all that it adds up:
 // fp16 rows meet the bare codes (exact in fp16) in a sum from zero, which the
 // scale multiplies as it joins the others (a power of two: one rounding, the
-// sum's); bf16 ones the scaled weights. Neighbouring lanes load 64 bytes of a row
-// and pass them on (mx4_rows.h). Bound by A, which every block reads from its L2
-// and passes on through LDS (256 KiB for 32 rows of 4096). A call on 32 fp16 rows
-// by 4096x4096 takes 9.4 us (10.5 in two launches, cutting and weights_direct),
-// by 6144x2048 7.2 (11.0); bf16 7.6 (8.0) and 6.0 (8.2); 16 fp16 rows by
-// 4096x4096 5.9 (7.2 by weights_few), bf16 5.3 (6.5).
-template <int kN>
-constexpr int kWhole = kN == 1 ? 16 : 8;  // waves, as the registers allow
+// sum's); bf16 ones the scaled weights.
+//
+// A wave's steps of A go to LDS without registers, one multiplied while the next
+// is under way; lanes 4 g .. 4 g + 3 fetch 64 bytes of row g, chunk c of it to
+// slot c ^ (g / 4), so that 16 lanes read 16 rows' chunks from all banks. Bound by
+// A, which every block reads from its L2 (256 KiB for 32 rows of 4096), and the
+// scales' work. A call on 32 fp16 rows by 4096x4096 takes 7.4 us (9.4 with A in
+// registers, passed on between lanes; 10.4 in two launches, cutting and
+// weights_direct), by 6144x2048 6.9 (11.0), by 14336x4096 16.5 (17.9); bf16 6.6
+// (7.9), 5.6 (8.3) and 13.7 (15.0); 16 fp16 rows by 4096x4096 5.8 (7.2 by
+// weights_few), bf16 5.3 (6.5).
+// 16 waves of 16 rows, 8 of 32: two steps of A each are 128 KiB of LDS.
+template <int kM>
+constexpr int kWhole = 16 / kM;
 
 template <int kIn, int kM, int kN, int kOut>
-__global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __restrict__ a, int lda,
+__global__ __launch_bounds__(kWhole<kM> * 64) void weights_whole(const void* __restrict__ a, int lda,
                                                                 const unsigned char* __restrict__ b_codes,
                                                                 const unsigned char* __restrict__ b_scales,
                                                                 void* __restrict__ c, int m, int n, int k) {
-    __shared__ f32x4 space[kWhole<kN> * kM * kN * 64];
+    constexpr int kTileBytes = 4096, kStepBytes = kM * kTileBytes;  // of A: 16 rows by 128
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kWhole<kM> * 2 * kStepBytes];
+    static_assert(sizeof smem >= sizeof(f32x4) * kWhole<kM> * kM * kN * 64);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16, steps = padded(k) / kStep, row_bytes = padded(k) / 2;
     const long long col0 = static_cast<long long>(blockIdx.x) * 16 * kN;
-    typedef Rows<kIn, kM, false, true> A;
-    A x;
-    x.open(a, nullptr, k, m, [&](int i) { return 16 * i; }, lda);
+    MX4_LDS unsigned char* const mine = (MX4_LDS unsigned char*)(smem) + wave * 2 * kStepBytes;
+    // To the last row's last dword; rows past it read as zeros.
+    const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<void*>(a), 0, (2 * ((m - 1) * lda + k) + 3) & ~3, 0x00020000);
+    const int a_at = 2 * (lane / 4 * lda + 8 * (lane % 4 ^ lane / 16)), a_from = 64 * r + 16 * (q ^ r / 4);
+    const int from = (4 * r + q) * 4;  // where a column's dword q was loaded
     __amdgpu_buffer_rsrc_t codes[kN];
     const unsigned char* scale_row = b_scales;
     const int at = lane / 4 * row_bytes + lane % 4 * 4;
@@ -213,11 +224,14 @@ __global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __r
     for (int i = 0; i < kM * kN; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     struct Step {
-        typename A::Step x;
         unsigned w[kN][4], scales;  // lane 16 j + r: of column r of tile j
     } now, next;
-    const auto load = [&](int t) {
-        x.load(t, next.x);
+    const auto load = [&](int t, int half) {
+#pragma unroll
+        for (int i = 0; i < kM; ++i)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                buffer_to_lds(rows, mine + half * kStepBytes + i * kTileBytes + s * 1024, a_at + 32 * lda * i + 64 * s, t * 256);
 #pragma unroll
         for (int j = 0; j < kN; ++j)
 #pragma unroll
@@ -229,13 +243,29 @@ __global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __r
         return static_cast<unsigned>(__builtin_amdgcn_ds_bpermute((16 * j + column) * 4, static_cast<int>(v)));
     };
     unsigned nans = 0;  // high bits of bytes: a scale of 255 in lane's column
-    int t = wave;
-    if (t < steps) load(t);
+    int t = wave, half = 0;
+    if (t < steps) load(t, 0);
     while (t < steps) {
+        const int then = t + kWhole<kM>;
+        // This step has landed; the reads of the other half are over.
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
         now = next;
-        const int then = t + kWhole<kN>;
-        if (then < steps) load(then);
-        if (x.past_end(t)) x.cut_off(t, now.x);
+        if (then < steps) load(then, half ^ 1);
+        if ((t + 1) * kStep > k) {  // the next row's elements, or a gap's, to zeros
+#pragma unroll 1
+            for (int i = 0; i < 4 * kM; ++i) {
+                MX4_LDS u32x4* const of_row = reinterpret_cast<MX4_LDS u32x4*>(mine + half * kStepBytes + i * 1024 + a_from);
+                u32x4 x = *of_row;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at_k = t * kStep + i % 4 * 32 + 8 * q + 2 * e;
+                    x[e] &= (at_k < k ? 0xffffu : 0u) | (at_k + 1 < k ? 0xffff0000u : 0u);
+                }
+                *of_row = x;
+            }
+        }
         if constexpr (kIn == kF16) nans |= (~now.scales - 0x01010101u) & now.scales & 0x80808080u;
         unsigned scales[kN][kIn == kF16 ? 4 : 1];
 #pragma unroll
@@ -249,13 +279,13 @@ __global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __r
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            __builtin_amdgcn_sched_barrier(0);  // or the registers of four overflow
-            u32x4 rows[kM][1];
+            u32x4 x[kM];
 #pragma unroll
-            for (int i = 0; i < kM; ++i) x.operand(now.x, i, s, 1.0f, rows[i]);
+            for (int i = 0; i < kM; ++i)
+                x[i] = *reinterpret_cast<const MX4_LDS u32x4*>(mine + half * kStepBytes + i * kTileBytes + s * 1024 + a_from);
 #pragma unroll
             for (int j = 0; j < kN; ++j) {
-                const unsigned w = x.pass(now.w[j][s]);
+                const unsigned w = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(now.w[j][s])));
                 if constexpr (kIn == kF16) {
                     const u32x4 of_codes = decode_eight_f16(w);
                     f32x4 scale;
@@ -267,7 +297,7 @@ __global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __r
                     }
 #pragma unroll
                     for (int i = 0; i < kM; ++i) {
-                        const f32x4 sum = mfma_f16(of_codes, rows[i][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        const f32x4 sum = mfma_f16(of_codes, x[i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
                         for (int v = 0; v < 4; ++v)
                             acc[i * kN + j][v] = __builtin_fmaf(sum[v], scale[v], acc[i * kN + j][v]);
@@ -275,11 +305,12 @@ __global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __r
                 } else {
                     const u32x4 scaled = decode_eight(w, scale_operand(scales[j][0] >> 8 * s & 255u));
 #pragma unroll
-                    for (int i = 0; i < kM; ++i) acc[i * kN + j] = mfma_bf16(scaled, rows[i][0], acc[i * kN + j]);
+                    for (int i = 0; i < kM; ++i) acc[i * kN + j] = mfma_bf16(scaled, x[i], acc[i * kN + j]);
                 }
             }
         }
         t = then;
+        half ^= 1;
     }
     if constexpr (kIn == kF16) {
 #pragma unroll
@@ -292,7 +323,8 @@ __global__ __launch_bounds__(kWhole<kN> * 64) void weights_whole(const void* __r
                     acc[i * kN + j][v] = nan ? __builtin_nanf("") : acc[i * kN + j][v];
             }
     }
-    sum_waves<kWhole<kN>>(acc, space, wave, lane, [&](int i, f32x4 sum) {
+    __syncthreads();  // all have read their A
+    sum_waves<kWhole<kM>>(acc, reinterpret_cast<f32x4*>(smem), wave, lane, [&](int i, f32x4 sum) {
         const int row = 16 * (i / kN) + r;
         const long long col = col0 + 16 * (i % kN) + 4 * q;
         if (row < m && col < n)
@@ -323,8 +355,7 @@ __global__ __launch_bounds__(256) void cut_rows(const void* __restrict__ a, long
 // multiple of 16). A step's pieces are loaded before the next step's weights,
 // because loads arrive in order; where they would take too many registers, by
 // instruction. Bound by A's pieces, which every block reads from its L2 (at most
-// 64 bytes a cycle): 32 fp16 rows by 4096x4096 in 8.6 us after 1.7 of cutting,
-// 512 KiB a block; 300x1001x1023 fp32 in 7.1 after 3.7.
+// 64 bytes a cycle): 300x1001x1023 fp32 in 7.1 us after 3.7 of cutting.
 template <int kPieceRows, int kN>
 struct Direct {
     static constexpr bool kPiecesFirst = kPieceRows <= 4;
@@ -553,8 +584,8 @@ int launch_few(const Product& p) {
 template <int kIn, int kM, int kN, int kOut>
 int launch_whole(const Product& p) {
     const long long blocks = tiles(p.n, 16 * kN);
-    if (!fits_launch(blocks, kWhole<kN> * 64)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((weights_whole<kIn, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWhole<kN> * 64), 0,
+    if (!fits_launch(blocks, kWhole<kM> * 64)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((weights_whole<kIn, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWhole<kM> * 64), 0,
                        p.stream, p.a, static_cast<int>(p.lda), p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
     return hipGetLastError();
 }
@@ -597,20 +628,17 @@ int launch(const Product& p) {
     // k = 4096, 64 per block, in 8.9 us, 32 (two rounds) in 11.4.
     const auto cost = [&](int wide) { return tiles(tiles(p.n, 16 * wide), device_cus()) * (2 * wide + 3); };
     if constexpr (kIn != kF32) {
-        if (p.m <= kWholeRows && aligned(p.a, 4) && p.lda % 2 == 0 && p.lda < (1 << 26)) {
+        if (p.m <= kWholeRows && aligned(p.a, 4) && p.lda % 2 == 0 && p.lda < (1 << 25)) {
             const bool by_16 = cost(1) <= cost(2) && cost(1) <= cost(4);
             if (p.m > 16) {
-                // 32 rows by 4096x8192 bf16 (pieces then need no cutting) in 11.7 us both ways, by 4096x14336
-                // 21.2 and 19.3 by weights_direct, by 4096x4096 7.6 and 8.0.
-                if (!by_16) {
-                    if (cost(4) < cost(2)) return launch_whole<kIn, 2, 4, kOut>(p);
-                    return launch_whole<kIn, 2, 2, kOut>(p);
-                }
-                if (kIn == kF16 || p.k <= 8192) return launch_whole<kIn, 2, 1, kOut>(p);
-            } else if (by_16 && p.k > kWhole<1> * kStep && (kIn == kF16 || p.m >= 8)) {
+                if (by_16) return launch_whole<kIn, 2, 1, kOut>(p);
+                if (cost(4) < cost(2)) return launch_whole<kIn, 2, 4, kOut>(p);
+                return launch_whole<kIn, 2, 2, kOut>(p);
+            }
+            if (by_16 && p.k > kWhole<1> * kStep && (kIn == kF16 || p.m >= 8)) {
                 // From a wave's second step on; weights_few's short code is faster below (12 rows by 1000x1000
-                // in 4.1 us, 4.6 here), for wide blocks (16 fp16 rows by 14336x4096: 11.2 and 13.9), and for bf16
-                // rows that are too few to crowd its loads (2 by 4096x4096: 4.3 and 5.1; 8: 5.4 and 5.2).
+                // in 4.1 us, 4.6 here), for wide blocks (16 fp16 rows by 14336x4096: 11.3 and 13.9), and for bf16
+                // rows that are too few to crowd its loads (2 by 4096x4096: 4.3 and 5.1; 8: 5.4 and 5.0).
                 return launch_whole<kIn, 1, 1, kOut>(p);
             }
         }

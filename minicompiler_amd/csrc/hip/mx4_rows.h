@@ -41,22 +41,19 @@ struct Rows {
 
     __device__ __forceinline__ static int offset(int q, int s) { return kQuant ? 32 * q + 8 * s : 32 * s + 8 * q; }
 
-    // first(i): tile i's first row of `all`, the same in every lane. pitch: elements between 16-bit rows,
-    // where they are not their length (16 pitch < 2^30).
+    // first(i): tile i's first row of `all`, the same in every lane.
     template <typename First>
-    __device__ __forceinline__ void open(const void* base, const unsigned char* scales, int k_, long long all, First first,
-                                         int pitch = 0) {
+    __device__ __forceinline__ void open(const void* base, const unsigned char* scales, int k_, long long all, First first) {
         const int lane = threadIdx.x % 64;
         r = lane % 16, q = lane / 16, part = lane % 4, from = (4 * r + q) * 4, k = k_;
-        const int row_bytes = kQuant ? padded(k) / 2 : 2 * (pitch != 0 ? pitch : k);
-        const int gap = kQuant || pitch == 0 ? 0 : 2 * (pitch - k);
+        const int row_bytes = kQuant ? padded(k) / 2 : 2 * k;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
             const long long row = first(i), left = all - row;
             const unsigned char* p = static_cast<const unsigned char*>(base) + row * row_bytes;
             const int odd = kOdd ? static_cast<int>(reinterpret_cast<std::uintptr_t>(p) & 2) : 0;
             // Whole dwords, to the one with the last element: what lies past it reads as zeros.
-            const int bytes = (odd + (left < 16 ? static_cast<int>(left) : 16) * row_bytes - gap + 3) & ~3;
+            const int bytes = (odd + (left < 16 ? static_cast<int>(left) : 16) * row_bytes + 3) & ~3;
             rows[i] = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p - odd), 0, bytes, 0x00020000);
             const int start = odd + lane / 4 * row_bytes;
             shift[i] = kOdd ? start & 2 : 0;
