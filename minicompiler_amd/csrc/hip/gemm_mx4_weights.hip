@@ -7,7 +7,7 @@
 // multiplied by the same weights into the same fp32 sum.
 //
 //   weights_few     up to 16 rows: A cut by every wave as it reads it;
-//   weights_whole   up to 32 rows of 16 bits, not cut: fp16 ones by the fp16
+//   weights_whole   up to 64 rows of 16 bits, not cut: fp16 ones by the fp16
 //                   instruction, scales applied to its sums;
 //   cut_rows        A's pieces into the workspace, for the two below:
 //   weights_direct  few tiles: a block's waves share out k, fragments come
@@ -23,7 +23,7 @@ namespace {
 using namespace mx4;
 
 constexpr int kFew = 16;
-constexpr int kWholeRows = 32;
+constexpr int kWholeRows = 64;
 constexpr int kFewWaves = 16;
 
 // ---------------------------------------------------------------- few rows
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __rest
 // weights_direct), by 6144x2048 6.9 (11.0), by 14336x4096 16.5 (17.9); bf16 6.6
 // (7.9), 5.6 (8.3) and 13.7 (15.0); 16 fp16 rows by 4096x4096 5.8 (7.2 by
 // weights_few), bf16 5.3 (6.5).
-// 16 waves of 16 rows, 8 of 32: two steps of A each are 128 KiB of LDS.
+// 16 waves of 16 rows, 8 of 32, 4 of 64: two steps of A each are 128 KiB of LDS.
 template <int kM>
 constexpr int kWhole = 16 / kM;
 
@@ -628,14 +628,21 @@ int launch(const Product& p) {
     // k = 4096, 64 per block, in 8.9 us, 32 (two rounds) in 11.4.
     const auto cost = [&](int wide) { return tiles(tiles(p.n, 16 * wide), device_cus()) * (2 * wide + 3); };
     if constexpr (kIn != kF32) {
-        if (p.m <= kWholeRows && aligned(p.a, 4) && p.lda % 2 == 0 && p.lda < (1 << 25)) {
+        // (32-bit offsets over all rows.)
+        if (p.m <= kWholeRows && aligned(p.a, 4) && p.lda % 2 == 0 && p.lda < (p.m <= 32 ? 1 << 25 : 1 << 23)) {
             const bool by_16 = cost(1) <= cost(2) && cost(1) <= cost(4);
-            if (p.m > 16) {
+            if (p.m > 32) {
+                // One round, four steps per wave: 64 fp16 rows by 6144x2048 in 10.7 us (11.5 in two launches), bf16
+                // 7.7 (9.8), 33 by 1024x1024 4.6 (7.1). By 4096x4096, eight steps of which a CU holds as many,
+                // 13.3 (11.4).
+                if (p.k <= 2048 && tiles(p.n, 32) <= device_cus())
+                    return by_16 ? launch_whole<kIn, 4, 1, kOut>(p) : launch_whole<kIn, 4, 2, kOut>(p);
+            } else if (p.m > 16) {
                 if (by_16) return launch_whole<kIn, 2, 1, kOut>(p);
                 if (cost(4) < cost(2)) return launch_whole<kIn, 2, 4, kOut>(p);
                 return launch_whole<kIn, 2, 2, kOut>(p);
             }
-            if (by_16 && p.k > kWhole<1> * kStep && (kIn == kF16 || p.m >= 8)) {
+            if (p.m <= 16 && by_16 && p.k > kWhole<1> * kStep && (kIn == kF16 || p.m >= 8)) {
                 // From a wave's second step on; weights_few's short code is faster below (12 rows by 1000x1000
                 // in 4.1 us, 4.6 here), for wide blocks (16 fp16 rows by 14336x4096: 11.3 and 13.9), and for bf16
                 // rows that are too few to crowd its loads (2 by 4096x4096: 4.3 and 5.1; 8: 5.4 and 5.0).

@@ -388,3 +388,10 @@ def test_scales_at_the_ends_and_of_no_number(device, mc, kind, n):
                                        (32, 70, 9000, 0)])
 def test_few_rows_of_16_bits_and_a_long_k(device, mc, kind, m, n, k, pad):
     test_rows_of_16_bits_that_start_at_dwords(device, mc, kind, m, n, k, pad)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("m,n,k,pad", [(33, 16, 128, 0), (49, 100, 2050, 2), (64, 4200, 1100, 0), (63, 9000, 333, 1),
+                                       (64, 40, 4100, 0)])
+def test_up_to_64_rows_of_16_bits(device, mc, kind, m, n, k, pad):
+    test_rows_of_16_bits_that_start_at_dwords(device, mc, kind, m, n, k, pad)
