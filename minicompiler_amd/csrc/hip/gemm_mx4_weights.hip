@@ -633,8 +633,8 @@ int launch(const Product& p) {
             const bool by_16 = cost(1) <= cost(2) && cost(1) <= cost(4);
             if (p.m > 32) {
                 // One round, four steps per wave: 64 fp16 rows by 6144x2048 in 10.7 us (11.5 in two launches), bf16
-                // 7.7 (9.8), 33 by 1024x1024 4.6 (7.1). By 4096x4096, eight steps of which a CU holds as many,
-                // 13.3 (11.4).
+                // 7.7 (9.8), 33 by 1024x1024 4.8 (7.1). By 4096x4096, eight steps for each of the four
+                // waves, 13.3 (11.4).
                 if (p.k <= 2048 && tiles(p.n, 32) <= device_cus())
                     return by_16 ? launch_whole<kIn, 4, 1, kOut>(p) : launch_whole<kIn, 4, 2, kOut>(p);
             } else if (p.m > 16) {
