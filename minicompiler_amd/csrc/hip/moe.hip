@@ -89,8 +89,9 @@ int down_shares(const Sizes& s) {
 }
 
 int pieces_of(int dtype) { return dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1; }  // at most
-// h is an fp32 sum: 24 bits of it for an fp32 result, 16 otherwise.
-int h_pieces_of(int dtype) { return dtype == kF32 ? 3 : 2; }
+// h is an fp32 number, kept whole whatever the result's type (cut to 16 bits for 16-bit results it was 2^-15 too
+// small at worst, and turned last bits of y).
+constexpr int kPiecesH = 3;
 
 std::size_t round_up(std::size_t v) { return (v + 255) / 256 * 256; }
 
@@ -110,7 +111,7 @@ std::size_t lay_out(const Sizes& s, int dtype, unsigned char* base, Workspace* w
     w->x = reinterpret_cast<unsigned short*>(
         take(2 * static_cast<std::size_t>(pieces_of(dtype)) * s.tokens * s.dp));
     w->h = reinterpret_cast<unsigned short*>(
-        take(2 * static_cast<std::size_t>(h_pieces_of(dtype)) * s.max_jobs * 16 * s.hp));
+        take(2 * static_cast<std::size_t>(kPiecesH) * s.max_jobs * 16 * s.hp));
     w->y = reinterpret_cast<float*>(
         take(sizeof(float) * static_cast<std::size_t>(down_shares(s)) * s.tokens * column_tiles(s.d) * kCols));
     return at;
@@ -349,7 +350,7 @@ __device__ __forceinline__ void cut_tokens(const void* __restrict__ x, long long
     }
 
     // h's columns past its last tile of 16, in all jobs, to zeros.
-    const int pad = s.hp / 8 - (s.h + 15) / 16 * 2, pads = (kIn == kF32 ? 3 : 2) * s.max_jobs * pad * 16;
+    const int pad = s.hp / 8 - (s.h + 15) / 16 * 2, pads = kPiecesH * s.max_jobs * pad * 16;
     for (int i = block * kThreads + threadIdx.x; i < pads; i += blocks * kThreads) {
         const long long row = i / (pad * 16) + 1LL;  // ends of jobs, of all pieces
         *reinterpret_cast<u32x4*>(w.h + row * 16 * s.hp - (i % (pad * 16) + 1) * 8) = u32x4{0, 0, 0, 0};
@@ -500,7 +501,7 @@ __device__ __forceinline__ float activate(float u, float up) {
 template <int kType>
 constexpr int kUpWaves = kType == kMx4 ? 8 : 4;  // 16-bit weights take the registers of two mx4 waves
 
-template <int kType, int kP, int kHP, int kAct, bool kOdd, bool kHalf>
+template <int kType, int kP, int kAct, bool kOdd, bool kHalf>
 __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __restrict__ w1,
                                                                const unsigned char* __restrict__ w1_scales,
                                                                const float* __restrict__ b1, Workspace w, Sizes s,
@@ -605,10 +606,10 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
                 a += b1[static_cast<long long>(of_expert) * h_rows + col];
                 if (kGated) up += b1[static_cast<long long>(of_expert) * h_rows + s.h + col];
             }
-            float piece[kHP];
-            cut<kHP>(in_h ? activate<kAct>(a, up) : 0.0f, piece);
+            float piece[kPiecesH];
+            cut<kPiecesH>(in_h ? activate<kAct>(a, up) : 0.0f, piece);
 #pragma unroll
-            for (int p = 0; p < kHP; ++p)
+            for (int p = 0; p < kPiecesH; ++p)
                 w.h[p * h_plane + static_cast<long long>(of_job) * 16 * s.hp + (col / 8 * 16 + er) * 8 + col % 8] =
                     static_cast<unsigned short>(__builtin_bit_cast(unsigned, piece[p]) >> 16);
         }
@@ -619,7 +620,7 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
 // in a row, cut evenly over the shares' waves). A wave adds each of its jobs'
 // parts, weighed, to its own LDS tile (no two lanes the same element); the tiles
 // are added in wave order, the shares in their order by the last block to arrive.
-template <int kType, int kP, int kOut, bool kOdd>
+template <int kType, int kOut, bool kOdd>
 __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2, const unsigned char* __restrict__ w2_scales,
                                                      const float* __restrict__ b2, Workspace w, Sizes s,
                                                      void* __restrict__ y) {
@@ -637,7 +638,7 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
     const int from = index * each + (index < more ? index : more), to = from + each + (index < more ? 1 : 0);
     const long long h_plane = static_cast<long long>(s.max_jobs) * 16 * s.hp;
 
-    typedef Stream<kType, kTiles, kP, kOdd, false> In;
+    typedef Stream<kType, kTiles, kPiecesH, kOdd, false> In;
     In in;
     typename In::Step now, next;
     int expert = 0, token = kNone;
@@ -724,7 +725,6 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
 
 template <int kIn, int kType, int kAct, bool kOdd>
 int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, hipStream_t stream) {
-    constexpr int kHP = kIn == kF32 ? 3 : 2;
     constexpr int kUpCols = kAct == MCHIP_MOE_SWIGLU ? 16 : 32;
     constexpr bool kHalf = kIn == kF16 && kType == kF16;
     // As many blocks as the registers let run at once, about.
@@ -734,11 +734,11 @@ int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, 
     const long long grid = std::min(blocks, units);
     const std::size_t jobs = s.tokens <= kFew ? s.max_jobs : std::min<long long>(s.max_jobs, s.max_jobs / grid + 2);
     const std::size_t lds = sizeof(Job) * jobs + (s.tokens <= kFew ? sizeof(float) * s.tokens * s.experts : 0);
-    hipLaunchKernelGGL((moe_up<kType, kHalf ? 1 : kPieces<kIn>, kHP, kAct, kOdd, kHalf>),
+    hipLaunchKernelGGL((moe_up<kType, kHalf ? 1 : kPieces<kIn>, kAct, kOdd, kHalf>),
                        dim3(static_cast<unsigned>(grid)), dim3(64 * kUpWaves<kType>), lds, stream, a.w1,
                        static_cast<const unsigned char*>(a.w1_scales), a.b1, w, s, router_parts(s.d), a.normalize != 0,
                        a.chosen, a.gates);
-    hipLaunchKernelGGL((moe_down<kType, kHP, kIn, kOdd>),
+    hipLaunchKernelGGL((moe_down<kType, kIn, kOdd>),
                        dim3(static_cast<unsigned>(column_tiles(s.d)), static_cast<unsigned>(down_shares(s))),
                        dim3(kThreads), sizeof(float) * kWaves * s.tokens * kCols, stream, a.w2,
                        static_cast<const unsigned char*>(a.w2_scales), a.b2, w, s, a.y);
