@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void moe_router(const void* __restrict__ 
                                                        const float* __restrict__ router, Workspace w, Sizes s,
                                                        bool normalize, int* __restrict__ chosen_out,
                                                        float* __restrict__ gates_out) {
-    extern __shared__ float logits[];  // [16, experts], in the last block of 16 tokens
+    extern __shared__ __attribute__((aligned(16))) float logits[];  // [16, experts], in the last block of 16 tokens
     __shared__ f32x4 space[kWaves * 64];
     __shared__ int chosen[kMaxTokens][kMaxTopK];
     __shared__ float gate[kMaxTokens][kMaxTopK];
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(64 * kUpWaves<kType>) void moe_up(const void* __res
     constexpr int kTiles = 2, kUpCols = kGated ? 16 : 32, kWaves = kUpWaves<kType>, kThreads = 64 * kWaves;
     typedef Stream<kType, kTiles, kP, kOdd, kHalf> In;
     __shared__ f32x4 space[2][kWaves][kTiles][64];
-    extern __shared__ float logits[];  // for few tokens: [tokens, experts], then their jobs
+    extern __shared__ __attribute__((aligned(16))) float logits[];  // for few tokens: [tokens, experts], then their jobs
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16;
     const int tiles = (s.h + kUpCols - 1) / kUpCols, steps = s.dp / kStep;
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(kThreads) void moe_down(const void* __restrict__ w2
                                                      const float* __restrict__ b2, Workspace w, Sizes s,
                                                      void* __restrict__ y) {
     constexpr int kTiles = kCols / 16;
-    extern __shared__ float tile[];  // [kWaves][tokens][kCols]
+    extern __shared__ __attribute__((aligned(16))) float tile[];  // [kWaves][tokens][kCols]
     __shared__ int flag;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16;
