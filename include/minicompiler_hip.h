@@ -272,7 +272,10 @@ MC_API int mc_matmul_supported(int kernel);              /* tensor_core_supporte
  * element 2 i in the low half of byte i (bit 3 the sign, bits 0-2 one of 0,
  * 0.5, 1, 1.5, 2, 3, 4, 6); scales [rows, kp / 32], one byte s per 32
  * elements, worth 2^(s - 127), 255: NaN. 16-byte aligned codes, 4-byte
- * aligned scales. Padding must be zero codes and no scale of 255. */
+ * aligned scales. Padding must be zero codes and no scale of 255. Quantising
+ * gives scales up to 252. As the weights of mc_launch_matmul_mx4_weights and
+ * mc_launch_moe, numbers past fp32's range (codes from 4 up at 253, from 2 up
+ * at 254) count as infinities or NaN; mc_launch_matmul_mx4 takes them as they are. */
 MC_API long long mc_mx4_code_bytes(int rows, int k);
 MC_API long long mc_mx4_scale_bytes(int rows, int k);
 /* x [rows, k], rows ld elements apart, to an mx4 operand: per block of 32,

@@ -242,7 +242,9 @@ __global__ __launch_bounds__(kWhole<kM> * 64) void weights_whole(const void* __r
     const auto of_column = [&](int j, int column, unsigned v) {
         return static_cast<unsigned>(__builtin_amdgcn_ds_bpermute((16 * j + column) * 4, static_cast<int>(v)));
     };
-    unsigned nans = 0;  // high bits of bytes: a scale of 255 in lane's column
+    // A scale of 255 in lane's column (high bits of bytes); tiles whose column r has a weight past fp32's largest
+    // number among the lane's, which the sums could hold but the weights of the other kernels are not.
+    unsigned nans = 0, past = 0;
     int t = wave, half = 0;
     if (t < steps) load(t, 0);
     while (t < steps) {
@@ -266,7 +268,22 @@ __global__ __launch_bounds__(kWhole<kM> * 64) void weights_whole(const void* __r
                 *of_row = x;
             }
         }
-        if constexpr (kIn == kF16) nans |= (~now.scales - 0x01010101u) & now.scales & 0x80808080u;
+        // Scales from 253 up: of no number, or past the type with some codes.
+        if constexpr (kIn == kF16) {
+            if (__ballot(((now.scales & 0x7f7f7f7fu) + 0x03030303u) & now.scales & 0x80808080u) != 0) {
+                nans |= (~now.scales - 0x01010101u) & now.scales & 0x80808080u;
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    const unsigned of_row = of_column(j, r, now.scales);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const unsigned w = static_cast<unsigned>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(now.w[j][s])));
+                        const unsigned byte = of_row >> 8 * s & 255u, four = w & 0x44444444u;  // 2, 3, 4 and 6
+                        if (byte == 254u ? four != 0 : byte == 253u && (four & w << 1) != 0) past |= 1u << j;
+                    }
+                }
+            }
+        }
         unsigned scales[kN][kIn == kF16 ? 4 : 1];
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
@@ -313,6 +330,11 @@ __global__ __launch_bounds__(kWhole<kM> * 64) void weights_whole(const void* __r
         half ^= 1;
     }
     if constexpr (kIn == kF16) {
+        if (__ballot(past != 0) != 0) {
+            past |= static_cast<unsigned>(__shfl_xor(static_cast<int>(past), 16));
+            past |= static_cast<unsigned>(__shfl_xor(static_cast<int>(past), 32));
+            nans |= past >> q & 1u;
+        }
 #pragma unroll
         for (int j = 0; j < kN; ++j)
 #pragma unroll

@@ -6,7 +6,10 @@
  * A quantised operand of `rows` rows of k numbers: k padded with zeros to
  * kp = mchip_mx4_k(k), a multiple of 128; codes [rows, kp / 2], two e2m1 codes
  * per byte, the first in the low half; scales [rows, kp / 32], one byte s per
- * 32 elements, worth 2^(s - 127), 255 for a block that holds no number.
+ * 32 elements, worth 2^(s - 127), 255 for a block that holds no number. As the
+ * weights of unquantised rows and of experts, its numbers are fp32's: codes
+ * from 4 up at byte 253 and from 2 up at 254 (quantising gives at most 252)
+ * pass its range, and no product with them is finite.
  *
  * Each launcher returns 0 or a hipError_t value; for hipErrorInvalidValue (1)
  * *why names the argument at fault. Types are MCHIP_DTYPE_* (matmul.h). */

@@ -210,7 +210,8 @@ template <int kType>
 constexpr int kPieces = kType == kBf16 ? 1 : kType == kF16 ? 2 : 3;
 
 // Eight codes (a dword) with their block's scale as the bf16 matrix
-// instruction's operand: exact, two significant bits at any scale.
+// instruction's operand: exact, two significant bits, subnormal ones too; an
+// infinity past fp32's range (codes from 4 up at byte 253, from 2 up at 254).
 __device__ __forceinline__ u32x4 decode_eight(unsigned codes, float scale) {
     u32x4 r;
     r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));

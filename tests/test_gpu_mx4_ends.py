@@ -1,0 +1,51 @@
+"""Products with 4-bit weights on the GPU where the numbers end: the largest and smallest scales, small fp32 rows,
+infinities and NaNs in the rows, for every kernel that a number of rows leads to. Expected values are exact: each
+result is one product, or a sum whose every partial sum fp32 holds."""
+
+import numpy as np
+import pytest
+
+import mx4_oracle as ref
+from test_gpu_mx4 import Out, bits_type, device_rows
+
+pytestmark = pytest.mark.gpu
+
+# Rows, columns and k: few rows at a short and at a long k, up to 32 and 64 rows at once, pieces, large tiles.
+SHAPES = [(3, 70, 300), (16, 70, 2300), (20, 70, 300), (32, 70, 300), (40, 70, 300), (64, 70, 300), (64, 70, 2300),
+          (200, 70, 300), (2050, 2060, 300)]
+
+
+def multiply(mc, dtype, bits, codes, scales, n, k):
+    """[m, n] fp32 results of rows `bits` and weights given by their codes and scales, on guarded memory."""
+    m = bits.shape[0]
+    a, bc, bs = device_rows(mc, bits, k), mc.DeviceBuffer.from_array(codes), mc.DeviceBuffer.from_array(scales)
+    c = Out(mc, m * n * 4)
+    workspace = mc.DeviceBuffer(max(1, mc.matmul_mx4_weights_workspace_bytes(dtype, m, n, k)))
+    mc.launch_matmul_mx4_weights(dtype, a.ptr, k, bc.ptr, bs.ptr, ref.F32, c.ptr, m, n, k, None, workspace.ptr)
+    mc.synchronize()
+    return c.get(np.float32, (m, n)).astype(np.float64)
+
+
+@pytest.mark.parametrize("kind", sorted(ref.TYPES))
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_the_largest_scales(device, mc, kind, m, n, k):
+    """One code per column at each scale byte from 248 to 254, met by small rows: exact up to fp32's largest number;
+    a weight past it makes no finite product, in any kernel."""
+    print(f"case largest scales {kind} {m}x{n}x{k}", flush=True)
+    kp = ref.padded(k)
+    codes, scales = np.zeros((n, kp // 2), np.uint8), np.full((n, kp // 32), 127, np.uint8)
+    column = np.arange(n)
+    code = column % 8 | (column // 16 % 2) << 3
+    byte = 248 + column // 8 % 7
+    at = np.array([0, 100, 299])[column % 3]
+    codes[column, at // 2] = code << (4 * (at % 2))
+    scales[column, at // 32] = byte
+    weight = ref.MAGNITUDES[code & 7] * np.where(code & 8, -1.0, 1.0) * 2.0 ** (byte.astype(np.float64) - 127)
+    finite = np.abs(weight) <= np.finfo(np.float32).max
+    assert (~finite).sum() >= 6
+    row = 2.0 ** -20 * (1 + np.arange(m) % 4)
+    bits = ref.to_type(np.tile(row.reshape(m, 1), (1, k)), ref.TYPES[kind])
+    got = multiply(mc, ref.TYPES[kind], bits, codes, scales, n, k)
+    want = row.reshape(m, 1) * weight
+    assert np.array_equal(got[:, finite], want[:, finite])
+    assert not np.isfinite(got[:, ~finite]).any()
