@@ -295,7 +295,8 @@ MC_API int mc_quantize_mx4_columns(int dtype, const void* b, long long ld, void*
 MC_API int mc_launch_matmul_mx4(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
                                 int c_dtype, void* c, int m, int n, int k, void* stream);
 /* C[m, n] = A B for A [m, k] of type a_dtype (rows lda elements apart), not
- * rounded, and B of n mx4 rows; fp32 sums, C in c_dtype. workspace: of
+ * rounded (fp32 numbers below 2^-110 are cut to multiples of 2^-133, towards
+ * zero), and B of n mx4 rows; fp32 sums, C in c_dtype. workspace: of
  * mc_matmul_mx4_weights_workspace_bytes bytes (0: may be NULL), 256-byte
  * aligned; calls that overlap need one each. */
 MC_API long long mc_matmul_mx4_weights_workspace_bytes(int a_dtype, int m, int n, int k);
@@ -313,8 +314,10 @@ MC_API int mc_launch_matmul_mx4_weights(int a_dtype, const void* a, long long ld
  * product's inner dimension; b1 [experts, h], b2 [experts, d] fp32 or NULL.
  * activation: 0 ReLU, 1 GELU (tanh form), 2 SwiGLU: W1 and b1 have 2 h rows,
  * h gate rows first, act = gate sigmoid(gate) up. chosen, gates: [tokens,
- * top_k], largest first, NULL if not wanted. Sums in fp32 throughout. At most
- * 512 experts and 16 per token.
+ * top_k], largest first, NULL if not wanted. Sums and act(...) in fp32; of
+ * fp32 x and of act(...), numbers below 2^-110 are cut to multiples of 2^-133.
+ * An infinite weight, or an infinite act(...) on fp16 weights, may give NaN
+ * where fp32 would give an infinity. At most 512 experts and 16 per token.
  * workspace: mc_moe_workspace_bytes bytes, 256-byte aligned, zero before the
  * first call that uses it; calls leave it ready for the next, of any sizes
  * that fit it. Calls that overlap need one each. */

@@ -3,8 +3,9 @@
 //
 // The matrix instruction on bf16 multiplies exactly, and every operand is
 // exact in bf16: a weight (two significant bits and a power of two), and A cut
-// into one, two or three bf16 pieces (8, 11 or 24 significant bits), each
-// multiplied by the same weights into the same fp32 sum.
+// into one, two or three bf16 pieces (8, 11 or 24 significant bits; of fp32 below
+// 2^-110 those from 2^-133 up), each multiplied by the same weights into the same
+// fp32 sum.
 //
 //   weights_few     up to 16 rows: A cut by every wave as it reads it;
 //   weights_whole   up to 64 rows of 16 bits, not cut: fp16 ones by the fp16

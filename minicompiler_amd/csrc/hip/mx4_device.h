@@ -180,8 +180,10 @@ __device__ __forceinline__ unsigned high_halves(float a, float b) {
 }
 
 // An fp32 value as a sum of bf16 pieces, each the leading 8 bits of what is
-// left: one piece holds a bf16 exactly, two an fp16, three an fp32 (24 bits).
-// Cutting, unlike rounding, never overflows; an infinity is its first piece.
+// left: one piece holds a bf16 exactly, two an fp16, three an fp32 (24 bits) from
+// 2^-110 up, below that its multiple of 2^-133, the smallest bf16. Cutting,
+// unlike rounding, never overflows; an infinity is its first piece, the others
+// zeros (which an infinite other operand turns into NaN).
 template <int kPieces>
 __device__ __forceinline__ void cut(float v, float (&piece)[kPieces]) {
 #pragma unroll

@@ -51,3 +51,46 @@ def test_hidden_activations_keep_the_bits_of_fp32(device, mc, kind, weights, tok
     want = np.zeros((tokens, d))
     want[:, 5] = 2.0 ** -bits
     assert np.array_equal(y, want)
+
+
+@pytest.mark.parametrize("weights", [ref.BF16, ref.F16, ref.MX4])
+@pytest.mark.parametrize("tokens", [2, 12])
+def test_an_infinite_hidden_activation(device, mc, weights, tokens):
+    """Through weights of one piece an infinity is one of the sign of its weight; through fp16 weights, cut into two,
+    the result is not finite."""
+    print(f"case moe infinite h weights {weights} tokens {tokens}", flush=True)
+    d, h = 40, 33
+    sign = np.where(np.arange(d) % 3 == 0, -1.0, 1.0)
+    net = weights_of(mc, weights, np.ones((1, h, d)), np.tile(sign.reshape(1, d, 1), (1, 1, h)))
+    b1 = np.zeros((1, h), dtype=np.float32)
+    b1[0, 30] = np.inf
+    net["keep"].append(mc.DeviceBuffer.from_array(b1))
+    net["b1"] = net["keep"][-1].ptr
+    router = np.zeros((1, d), dtype=np.float32)
+    y, _, _ = run(mc, net, np.ones((tokens, d), dtype=np.float32), ref.F32, router, weights, h, 1, "relu", True)
+    if weights == ref.F16:
+        assert not np.isfinite(y).any()
+    else:
+        assert np.array_equal(y, np.tile(np.inf * sign, (tokens, 1)))
+
+
+@pytest.mark.parametrize("weights", [ref.BF16, ref.F16, ref.MX4])
+@pytest.mark.parametrize("tokens", [2, 12])
+def test_small_fp32_activations(device, mc, weights, tokens):
+    """x and h of fp32: whole from 2^-110 up, below that the multiple of 2^-133 towards zero. W1 and W2 bring the token's
+    number to its place, and 2^14 (of a type that has no more) up to where every fp32 holds the result."""
+    print(f"case moe small x weights {weights} tokens {tokens}", flush=True)
+    d = h = 32
+    w1, w2 = np.zeros((1, h, d)), np.zeros((1, d, h))
+    w1[0, 3, 7] = 1.0
+    w2[0, 5, 3] = 2.0 ** 14
+    net = weights_of(mc, weights, w1, w2)
+    rng = np.random.default_rng(tokens)
+    value = (rng.integers(1 << 23, 1 << 24, tokens) * 2.0 ** (-136 + np.arange(tokens))).astype(np.float32)
+    x = np.zeros((tokens, d), dtype=np.float32)
+    x[:, 7] = value
+    router = np.zeros((1, d), dtype=np.float32)
+    y, _, _ = run(mc, net, x, ref.F32, router, weights, h, 1, "relu", True)
+    want = np.zeros((tokens, d))
+    want[:, 5] = np.trunc(value.astype(np.float64) * 2.0 ** 133) * 2.0 ** -133 * 2.0 ** 14
+    assert np.array_equal(y, want)

@@ -49,3 +49,21 @@ def test_the_largest_scales(device, mc, kind, m, n, k):
     want = row.reshape(m, 1) * weight
     assert np.array_equal(got[:, finite], want[:, finite])
     assert not np.isfinite(got[:, ~finite]).any()
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_small_fp32_rows(device, mc, m, n, k):
+    """fp32 rows of one number each, down to the smallest subnormal, against a weight of 2^100: whole from 2^-110 up,
+    below that the multiple of 2^-133 towards zero."""
+    print(f"case small rows {m}x{n}x{k}", flush=True)
+    kp = ref.padded(k)
+    codes, scales = np.zeros((n, kp // 2), np.uint8), np.full((n, kp // 32), 227, np.uint8)
+    at = np.arange(n) * 37 % k
+    codes[np.arange(n), at // 2] = 2 << (4 * (at % 2))  # 1
+    rng = np.random.default_rng(m + k)
+    x = (rng.integers(1 << 23, 1 << 24, m) * 2.0 ** (-149 + np.arange(m) * 5 % 45)).astype(np.float32)
+    x[::3] *= -1.0
+    x[1] = 2.0 ** -149
+    got = multiply(mc, ref.F32, np.tile(x.reshape(m, 1), (1, k)), codes, scales, n, k)
+    kept = np.where(np.abs(x) < 2.0 ** -110, np.trunc(x.astype(np.float64) * 2.0 ** 133) * 2.0 ** -133, x.astype(np.float64))
+    assert np.array_equal(got, np.tile((kept * 2.0 ** 100).reshape(m, 1), (1, n)))
