@@ -802,6 +802,7 @@ const char* refusal(const mchip_moe_args& a) {
         !aligned(a.b1, 4) || !aligned(a.b2, 4) || !aligned(a.chosen, 4) || !aligned(a.gates, 4) ||
         !aligned(a.w1, a.weights == kMx4 ? 16 : 2) || !aligned(a.w2, a.weights == kMx4 ? 16 : 2))
         return "an address that is no multiple of its element's size (mx4 codes: of 16)";
+    if (a.weights == kMx4 && (!aligned(a.w1_scales, 4) || !aligned(a.w2_scales, 4))) return "scales not 4-byte aligned";
     if (!aligned(a.workspace, 256)) return "a workspace that is not 256-byte aligned";
     return nullptr;
 }

@@ -1,0 +1,20 @@
+"""Refusals of the 4-bit and mixture-of-experts calls whose reason, or whose being refused at all, depends on more than
+one argument; before anything reaches a device."""
+
+import pytest
+
+from test_mx4_refusals import P, refused
+
+
+def moe(mc, **kw):
+    good = dict(dtype=1, x=P, ldx=64, router=P, weights=4, w1=P, w1_scales=P, b1=None, w2=P, w2_scales=P, b2=None, y=P,
+                chosen=None, gates=None, tokens=2, d=64, h=64, experts=4, top_k=2, activation="swiglu", normalize=True,
+                stream=None, workspace=P)
+    mc.launch_moe(**{**good, **kw})
+
+
+@pytest.mark.parametrize("name", ["w1_scales", "w2_scales"])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_moe_scales_off_their_dwords(mc, name, offset):
+    """Four scales at a time are read."""
+    refused(mc, "scales.*4", moe, mc, **{name: P + offset})
