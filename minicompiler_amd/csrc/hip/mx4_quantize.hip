@@ -250,7 +250,8 @@ int launch_columns(const void* w, long long ld, void* codes, void* scales, int k
     const auto go = [&](auto kernel, int per) {
         const unsigned cols = static_cast<unsigned>((static_cast<long long>(n) + 64 * per - 1) / (64 * per));
         if (cols > 65535u) {
-            *why = "more columns than one launch takes (4194240)";
+            *why = per == 2 ? "more columns than one launch takes in pairs (8388480)"
+                            : "more columns than one launch takes (4194240)";
             return static_cast<int>(hipErrorInvalidValue);
         }
         for (int step = 0; step < k_blocks / 4; step += most) {

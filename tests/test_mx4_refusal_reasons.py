@@ -18,3 +18,10 @@ def moe(mc, **kw):
 def test_moe_scales_off_their_dwords(mc, name, offset):
     """Four scales at a time are read."""
     refused(mc, "scales.*4", moe, mc, **{name: P + offset})
+
+
+@pytest.mark.parametrize("dtype,n,most", [(0, 4194241, 4194240), (0, 8388482, 4194240), (1, 4194241, 4194240),
+                                          (1, 8388482, 8388480), (2, 1 << 30, 8388480)])
+def test_columns_beyond_a_launch(mc, dtype, n, most):
+    """16-bit columns are taken in pairs where their number is even: twice as many."""
+    refused(mc, f"columns.*\\({most}\\)", mc.quantize_mx4_columns, dtype, P, n, P, P, 40, n)
