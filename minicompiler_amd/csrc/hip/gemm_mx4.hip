@@ -102,6 +102,7 @@ struct Product {
     void* c;
     int m, n, steps;
     hipStream_t stream;
+    const char** why;
 };
 
 long long tiles(int size, int tile) { return (static_cast<long long>(size) + tile - 1) / tile; }
@@ -110,11 +111,12 @@ template <int kM, int kN, int kOut>
 int launch_direct(const Product& p) {
     constexpr int kWaves = 8;
     const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
-    if (!fits_launch(blocks, kWaves * 64)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((product_direct<kM, kN, kWaves, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWaves * 64),
-                       0, p.stream, p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps,
-                       static_cast<unsigned>(tn));
-    return hipGetLastError();
+    if (!fits_launch(blocks, kWaves * 64)) {
+        *p.why = "more tiles of C than one launch takes";
+        return hipErrorInvalidValue;
+    }
+    return launch_kernel(product_direct<kM, kN, kWaves, kOut>, static_cast<unsigned>(blocks), kWaves * 64, 0, p.stream,
+                         p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps, static_cast<unsigned>(tn));
 }
 
 template <int kOut>
@@ -122,9 +124,8 @@ int launch_tiles(const Product& p) {
     const int tn = static_cast<int>(tiles(p.n, kTileCols)), all = static_cast<int>(tiles(p.m, kTileRows)) * tn;
     const int cus = device_cus(), rest = all % cus;
     const int halves = rest <= cus / 2 ? rest : 0;
-    hipLaunchKernelGGL(product_tiles<kOut>, dim3(static_cast<unsigned>(all + halves)), dim3(kTileThreads), 0, p.stream,
-                       p.a_codes, p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps, tn, all - halves, p.n % 8 == 0);
-    return hipGetLastError();
+    return launch_kernel(product_tiles<kOut>, static_cast<unsigned>(all + halves), kTileThreads, 0, p.stream, p.a_codes,
+                         p.a_scales, p.b_codes, p.b_scales, p.c, p.m, p.n, p.steps, tn, all - halves, p.n % 8 == 0);
 }
 
 // Four steps at least (a slot of scales), and 32-bit offsets from a tile's origin.
@@ -178,8 +179,6 @@ extern "C" int mchip_launch_matmul_mx4(const void* a_codes, const void* a_scales
     Product p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
               static_cast<const unsigned char*>(b_codes), static_cast<const unsigned char*>(b_scales),
               c, m, n, static_cast<int>(mchip_mx4_k(k) / kStep),
-              static_cast<hipStream_t>(stream)};
-    const int rc = c_dtype == kF32 ? launch<kF32>(p) : c_dtype == kBf16 ? launch<kBf16>(p) : launch<kF16>(p);
-    if (rc == hipErrorInvalidValue) *why = "more tiles of C than one launch takes";
-    return rc;
+              static_cast<hipStream_t>(stream), why};
+    return c_dtype == kF32 ? launch<kF32>(p) : c_dtype == kBf16 ? launch<kBf16>(p) : launch<kF16>(p);
 }

@@ -584,7 +584,13 @@ struct Product {
     int m, n, k;
     unsigned short* pieces;
     hipStream_t stream;
+    const char** why;
 };
+
+int too_many(const Product& p) {
+    *p.why = "more tiles of C than one launch takes";
+    return hipErrorInvalidValue;
+}
 
 long long tiles(long long size, int tile) { return (size + tile - 1) / tile; }
 int piece_rows(int m) { return (m + 15) / 16 * 16; }
@@ -594,11 +600,10 @@ int launch_few(const Product& p) {
     const long long size = kSize<kIn>;
     const bool loose = !aligned(p.a, 4) || p.lda * size % 4 != 0 || ((p.m - 1) * p.lda + p.k) * size > 0x7fffff00LL;
     const long long blocks = tiles(p.n, 16 * kN);
-    if (!fits_launch(blocks, kFewWaves * 64)) return hipErrorInvalidValue;
+    if (!fits_launch(blocks, kFewWaves * 64)) return too_many(p);
     const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kFewWaves * 64), 0, p.stream, p.a,
-                           p.lda, p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
-        return static_cast<int>(hipGetLastError());
+        return launch_kernel(kernel, static_cast<unsigned>(blocks), kFewWaves * 64, 0, p.stream, p.a, p.lda, p.b_codes,
+                             p.b_scales, p.c, p.m, p.n, p.k);
     };
     if (loose) return go(weights_few<kIn, kN, kOut, true>);
     return go(weights_few<kIn, kN, kOut, false>);
@@ -607,21 +612,34 @@ int launch_few(const Product& p) {
 template <int kIn, int kM, int kN, int kOut>
 int launch_whole(const Product& p) {
     const long long blocks = tiles(p.n, 16 * kN);
-    if (!fits_launch(blocks, kWhole<kM> * 64)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((weights_whole<kIn, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(kWhole<kM> * 64), 0,
-                       p.stream, p.a, static_cast<int>(p.lda), p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
-    return hipGetLastError();
+    if (!fits_launch(blocks, kWhole<kM> * 64)) return too_many(p);
+    return launch_kernel(weights_whole<kIn, kM, kN, kOut>, static_cast<unsigned>(blocks), kWhole<kM> * 64, 0, p.stream, p.a,
+                         static_cast<int>(p.lda), p.b_codes, p.b_scales, p.c, p.m, p.n, p.k);
+}
+
+// A's pieces, once the launch that multiplies them is known to fit.
+template <int kP>
+int cut_a(const Product& p) {
+    constexpr int kIn = kP == 1 ? kBf16 : kP == 2 ? kF16 : kF32;
+    const int rows = piece_rows(p.m), chunks = padded(p.k) / 8;
+    const long long blocks = tiles(static_cast<long long>(rows) * chunks, 256);
+    if (!fits_launch(blocks, 256)) {
+        *p.why = "more of A than one launch cuts into pieces";
+        return hipErrorInvalidValue;
+    }
+    return launch_kernel(cut_rows<kIn>, static_cast<unsigned>(blocks), 256, 0, p.stream, p.a, p.lda, p.pieces, p.m, rows, p.k,
+                         chunks);
 }
 
 template <int kP, int kM, int kN, int kOut>
 int launch_direct(const Product& p) {
     typedef Direct<kP * kM, kN> Shape;
     const long long tn = tiles(p.n, 16 * kN), blocks = tiles(p.m, 16 * kM) * tn;
-    if (!fits_launch(blocks, 64 * Shape::kWaves)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((weights_direct<Shape, kP, kM, kN, kOut>), dim3(static_cast<unsigned>(blocks)), dim3(64 * Shape::kWaves),
-                       0, p.stream, p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
-                       static_cast<unsigned>(tn));
-    return hipGetLastError();
+    if (!fits_launch(blocks, 64 * Shape::kWaves)) return too_many(p);
+    if (const int rc = cut_a<kP>(p); rc != hipSuccess) return rc;
+    return launch_kernel(weights_direct<Shape, kP, kM, kN, kOut>, static_cast<unsigned>(blocks), 64 * Shape::kWaves, 0,
+                         p.stream, p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
+                         static_cast<unsigned>(tn));
 }
 
 template <int kP, int kOut>
@@ -632,10 +650,10 @@ int launch_pieces(const Product& p) {
     // 42 us, by the direct kernel in 33; fp16 64 in 76 and 27, which grows with their number).
     // (32-bit offsets from a tile's origin.)
     if (4 * blocks(8, 8) >= 3 * cus && p.k <= (1 << 22) && fits_launch(blocks(8, 8), kTileThreads)) {
-        hipLaunchKernelGGL((weights_tiles<kP, kOut>), dim3(static_cast<unsigned>(blocks(8, 8))), dim3(kTileThreads), 0, p.stream,
-                           p.pieces, p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
-                           static_cast<int>(tiles(p.n, kTile)));
-        return hipGetLastError();
+        if (const int rc = cut_a<kP>(p); rc != hipSuccess) return rc;
+        return launch_kernel(weights_tiles<kP, kOut>, static_cast<unsigned>(blocks(8, 8)), kTileThreads, 0, p.stream, p.pieces,
+                             p.b_codes, p.b_scales, p.c, p.m, piece_rows(p.m), p.n, p.k,
+                             static_cast<int>(tiles(p.n, kTile)));
     }
     if constexpr (kP < 3) {  // three pieces of 64 rows do not fit the registers
         if (p.m > 32 && blocks(4, 2) >= cus) return launch_direct<kP, 4, 2, kOut>(p);
@@ -680,13 +698,6 @@ int launch(const Product& p) {
         if (cost(2) < cost(1)) return launch_few<kIn, 2, kOut>(p);
         return launch_few<kIn, 1, kOut>(p);
     }
-    const int rows = piece_rows(p.m), chunks = padded(p.k) / 8;
-    const long long blocks = tiles(static_cast<long long>(rows) * chunks, 256);
-    if (!fits_launch(blocks, 256)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(cut_rows<kIn>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, p.stream, p.a, p.lda, p.pieces, p.m,
-                       rows, p.k, chunks);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
     return launch_pieces<kPieces<kIn>, kOut>(p);
 }
 
@@ -725,12 +736,10 @@ int mchip_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, c
         *why = "no workspace, or one that is not 256-byte aligned";
     if (*why != nullptr) return hipErrorInvalidValue;
     Product p{a, lda, static_cast<const unsigned char*>(b_codes), static_cast<const unsigned char*>(b_scales),
-              c, m, n, k, static_cast<unsigned short*>(workspace), static_cast<hipStream_t>(stream)};
-    const int rc = a_dtype == kF32   ? launch_out<kF32>(c_dtype, p)
-                   : a_dtype == kBf16 ? launch_out<kBf16>(c_dtype, p)
-                                      : launch_out<kF16>(c_dtype, p);
-    if (rc == hipErrorInvalidValue) *why = "more tiles of C than one launch takes";
-    return rc;
+              c, m, n, k, static_cast<unsigned short*>(workspace), static_cast<hipStream_t>(stream), why};
+    return a_dtype == kF32    ? launch_out<kF32>(c_dtype, p)
+           : a_dtype == kBf16 ? launch_out<kBf16>(c_dtype, p)
+                              : launch_out<kF16>(c_dtype, p);
 }
 
 }  // extern "C"

@@ -735,15 +735,14 @@ int launch_experts(const mchip_moe_args& a, const Workspace& w, const Sizes& s, 
     const long long grid = std::min(blocks, units);
     const std::size_t jobs = s.tokens <= kFew ? s.max_jobs : std::min<long long>(s.max_jobs, s.max_jobs / grid + 2);
     const std::size_t lds = sizeof(Job) * jobs + (s.tokens <= kFew ? sizeof(float) * s.tokens * s.experts : 0);
-    hipLaunchKernelGGL((moe_up<kType, kHalf ? 1 : kPieces<kIn>, kAct, kOdd, kHalf>),
-                       dim3(static_cast<unsigned>(grid)), dim3(64 * kUpWaves<kType>), lds, stream, a.w1,
-                       static_cast<const unsigned char*>(a.w1_scales), a.b1, w, s, router_parts(s.d), a.normalize != 0,
-                       a.chosen, a.gates);
-    hipLaunchKernelGGL((moe_down<kType, kIn, kOdd>),
-                       dim3(static_cast<unsigned>(column_tiles(s.d)), static_cast<unsigned>(down_shares(s))),
-                       dim3(kThreads), sizeof(float) * kWaves * s.tokens * kCols, stream, a.w2,
-                       static_cast<const unsigned char*>(a.w2_scales), a.b2, w, s, a.y);
-    return hipGetLastError();
+    const int rc = launch_kernel(moe_up<kType, kHalf ? 1 : kPieces<kIn>, kAct, kOdd, kHalf>, static_cast<unsigned>(grid),
+                                 64 * kUpWaves<kType>, lds, stream, a.w1, static_cast<const unsigned char*>(a.w1_scales),
+                                 a.b1, w, s, router_parts(s.d), a.normalize != 0, a.chosen, a.gates);
+    if (rc != hipSuccess) return rc;
+    return launch_kernel(moe_down<kType, kIn, kOdd>,
+                         dim3(static_cast<unsigned>(column_tiles(s.d)), static_cast<unsigned>(down_shares(s))), kThreads,
+                         sizeof(float) * kWaves * s.tokens * kCols, stream, a.w2,
+                         static_cast<const unsigned char*>(a.w2_scales), a.b2, w, s, a.y);
 }
 
 template <int kIn, int kType, int kAct>
@@ -770,15 +769,11 @@ int launch(const mchip_moe_args& a, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>((s.experts + 15) / 16), static_cast<unsigned>((s.tokens + 15) / 16),
                     static_cast<unsigned>(2 * router_parts(s.d)));
     const auto router = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), sizeof(float) * 16 * s.experts, stream, a.x, a.ldx,
-                           a.router, w, s, a.normalize != 0, a.chosen, a.gates);
+        return launch_kernel(kernel, grid, kThreads, sizeof(float) * 16 * s.experts, stream, a.x, a.ldx, a.router, w, s,
+                             a.normalize != 0, a.chosen, a.gates);
     };
-    if (kIn == kF16 && a.weights == kF16)
-        router(moe_router<kIn, kIn == kF16>);
-    else
-        router(moe_router<kIn, false>);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    const int rc = kIn == kF16 && a.weights == kF16 ? router(moe_router<kIn, kIn == kF16>) : router(moe_router<kIn, false>);
+    if (rc != hipSuccess) return rc;
     if (a.weights == kBf16) return launch_act<kIn, kBf16>(a, w, s, stream);
     if (a.weights == kF16) return launch_act<kIn, kF16>(a, w, s, stream);
     return launch_act<kIn, kMx4>(a, w, s, stream);

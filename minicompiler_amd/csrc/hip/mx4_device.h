@@ -16,6 +16,7 @@
 #include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <tuple>
 
 #include "mx4.h"
 
@@ -280,6 +281,20 @@ inline bool is_float_type(int dtype) {
 
 // A launch takes fewer than 2^32 threads along a dimension of its grid.
 inline bool fits_launch(long long blocks, int threads) { return blocks < (1LL << 32) / threads; }
+
+// A launch's own status (hipGetLastError() would report, and take away, what an
+// earlier call of the program left behind).
+template <typename... Params, typename... Args>
+inline int launch_kernel(void (*kernel)(Params...), dim3 grid, unsigned threads, std::size_t lds, hipStream_t stream,
+                         Args... args) {
+    std::tuple<Params...> values(static_cast<Params>(args)...);
+    return std::apply(
+        [&](auto&... value) {
+            void* list[] = {const_cast<void*>(static_cast<const volatile void*>(&value))...};
+            return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), list, lds, stream);
+        },
+        values);
+}
 
 // CUs of the current device, asked once per device.
 inline int device_cus() {

@@ -232,12 +232,11 @@ int launch_rows(const void* x, long long ld, void* codes, void* scales, int rows
     for (long long from = 0; from < rows; from += most) {
         const long long count = std::min(most, rows - from);
         const unsigned blocks = static_cast<unsigned>((count * per_row + kThreads - 1) / kThreads);
-        hipLaunchKernelGGL(quantize_rows<kType>, dim3(blocks), dim3(kThreads), 0, stream, offset<kType>(x, from * ld), ld,
-                           static_cast<unsigned*>(codes) + from * per_row,
-                           static_cast<unsigned char*>(scales) + from * (per_row / 4), offset<kType>(values, from * k), count,
-                           k, per_row);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        const int rc = launch_kernel(quantize_rows<kType>, blocks, kThreads, 0, stream, offset<kType>(x, from * ld), ld,
+                                     static_cast<unsigned*>(codes) + from * per_row,
+                                     static_cast<unsigned char*>(scales) + from * (per_row / 4),
+                                     offset<kType>(values, from * k), count, k, per_row);
+        if (rc != hipSuccess) return rc;
     }
     return hipSuccess;
 }
@@ -256,12 +255,13 @@ int launch_columns(const void* w, long long ld, void* codes, void* scales, int k
         }
         for (int step = 0; step < k_blocks / 4; step += most) {
             const int steps = std::min(most, k_blocks / 4 - step), from = step * kStep;
-            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(steps), cols), dim3(kColumnThreads), 0, stream,
-                               offset<kType>(w, from * ld), ld, static_cast<unsigned*>(codes) + step * 16LL,
-                               static_cast<unsigned char*>(scales) + step * 4LL,
-                               offset<kType>(values, static_cast<long long>(from) * n), k - from, n, k_blocks);
+            const int rc = launch_kernel(kernel, dim3(static_cast<unsigned>(steps), cols), kColumnThreads, 0, stream,
+                                         offset<kType>(w, from * ld), ld, static_cast<unsigned*>(codes) + step * 16LL,
+                                         static_cast<unsigned char*>(scales) + step * 4LL,
+                                         offset<kType>(values, static_cast<long long>(from) * n), k - from, n, k_blocks);
+            if (rc != hipSuccess) return rc;
         }
-        return static_cast<int>(hipGetLastError());
+        return static_cast<int>(hipSuccess);
     };
     if constexpr (kType != kF32) {
         // Two columns to a lane load dwords (4096x14336 bf16 with values: 74 us, 80 by one).

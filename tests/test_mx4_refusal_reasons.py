@@ -25,3 +25,15 @@ def test_moe_scales_off_their_dwords(mc, name, offset):
 def test_columns_beyond_a_launch(mc, dtype, n, most):
     """16-bit columns are taken in pairs where their number is even: twice as many."""
     refused(mc, f"columns.*\\({most}\\)", mc.quantize_mx4_columns, dtype, P, n, P, P, 40, n)
+
+
+@pytest.mark.parametrize("m,n,k", [(1 << 30, 1 << 30, 32), (1 << 24, 1 << 24, 32)])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_more_tiles_than_a_launch(mc, dtype, m, n, k):
+    """Refused before A is cut into pieces, too."""
+    refused(mc, "more tiles of C", mc.launch_matmul_mx4, P, P, P, P, dtype, P, m, n, k)
+    refused(mc, "more tiles of C", mc.launch_matmul_mx4_weights, dtype, P, k, P, P, dtype, P, m, n, k, None, P)
+
+
+def test_more_rows_than_are_cut(mc):
+    refused(mc, "cuts", mc.launch_matmul_mx4_weights, 0, P, 1 << 24, P, P, 0, P, 1 << 24, 1, 1 << 24, None, P)
