@@ -768,7 +768,7 @@ def launch_moe(dtype: int, x: int, ldx: int, router: int, weights: int, w1: int,
                normalize: bool, stream=None, workspace: int | None = None) -> None:
     """A mixture-of-experts MLP of 1 to 64 tokens, router included (mc_launch_moe); the workspace
     (moe_workspace_bytes) is zero before its first use."""
-    act = MOE_ACTIVATIONS[activation] if isinstance(activation, str) else activation
+    act = MOE_ACTIVATIONS.get(activation, -1) if isinstance(activation, str) else activation
     _check_launch(library().mc_launch_moe(dtype, x, ldx, router, weights, w1, w1_scales, b1, w2, w2_scales, b2, y,
                                           chosen, gates, tokens, d, h, experts, top_k, act, int(normalize),
                                           _stream_handle(stream), workspace))

@@ -37,3 +37,9 @@ def test_more_tiles_than_a_launch(mc, dtype, m, n, k):
 
 def test_more_rows_than_are_cut(mc):
     refused(mc, "cuts", mc.launch_matmul_mx4_weights, 0, P, 1 << 24, P, P, 0, P, 1 << 24, 1, 1 << 24, None, P)
+
+
+@pytest.mark.parametrize("activation", ["silu", "", -1, 3])
+def test_moe_activations_that_are_none(mc, activation):
+    """An unknown name as an unknown number."""
+    refused(mc, "activation", moe, mc, activation=activation)
