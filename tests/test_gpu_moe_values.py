@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mx4_oracle as ref
-from test_gpu_moe import run
+from test_gpu_moe import check, run
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,14 @@ def test_small_fp32_activations(device, mc, weights, tokens):
     want = np.zeros((tokens, d))
     want[:, 5] = np.trunc(value.astype(np.float64) * 2.0 ** 133) * 2.0 ** -133 * 2.0 ** 14
     assert np.array_equal(y, want)
+
+
+@pytest.mark.parametrize("weights", [ref.BF16, ref.F16, ref.MX4])
+@pytest.mark.parametrize("tokens,d,h,experts,top_k,act", [
+    (4, 64, 48, 300, 8, "swiglu"), (8, 40, 40, 512, 16, "gelu"), (1, 48, 32, 129, 3, "relu"),  # eight logits a lane, in moe_up
+    (3, 4200, 40, 4, 2, "swiglu"), (20, 4200, 33, 5, 2, "gelu"),     # sums of nine parts of a logit
+    (2, 9000, 24, 3, 1, "relu"), (12, 9001, 16, 3, 2, "swiglu")])    # d past 16 parts; column tiles of y past the CUs
+def test_many_experts_and_long_rows(device, mc, weights, tokens, d, h, experts, top_k, act):
+    print(f"case moe weights {weights} {tokens} {d} {h} {experts} {top_k} {act}", flush=True)
+    for kind in ("f32", "f16"):
+        check(mc, 5, kind, weights, tokens, d, h, experts, top_k, act, bias=experts % 2 == 1)

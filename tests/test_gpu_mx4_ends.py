@@ -67,3 +67,63 @@ def test_small_fp32_rows(device, mc, m, n, k):
     got = multiply(mc, ref.F32, np.tile(x.reshape(m, 1), (1, k)), codes, scales, n, k)
     kept = np.where(np.abs(x) < 2.0 ** -110, np.trunc(x.astype(np.float64) * 2.0 ** 133) * 2.0 ** -133, x.astype(np.float64))
     assert np.array_equal(got, np.tile((kept * 2.0 ** 100).reshape(m, 1), (1, n)))
+
+
+@pytest.mark.parametrize("kind", sorted(ref.TYPES))
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_the_smallest_scales_and_none(device, mc, kind, m, n, k):
+    """One code per column at the scale bytes 0 to 6, and 255: exact products, those below fp32's normal numbers exact or
+    zero; a column with a scale of no number is none, whatever its code."""
+    print(f"case smallest scales {kind} {m}x{n}x{k}", flush=True)
+    kp = ref.padded(k)
+    codes, scales = np.zeros((n, kp // 2), np.uint8), np.full((n, kp // 32), 127, np.uint8)
+    column = np.arange(n)
+    code, byte = column % 8, column // 8 % 8
+    byte = np.where(byte == 7, 255, byte)
+    at = np.array([3, 130, 287])[column % 3]
+    codes[column, at // 2] = code << (4 * (at % 2))
+    scales[column, at // 32] = byte
+    none = byte == 255
+    assert none.sum() >= 6
+    weight = ref.MAGNITUDES[code] * 2.0 ** (np.where(none, 0, byte).astype(np.float64) - 127)
+    row = 2.0 ** (np.arange(m) % 4)
+    bits = ref.to_type(np.tile(row.reshape(m, 1), (1, k)), ref.TYPES[kind])
+    got = multiply(mc, ref.TYPES[kind], bits, codes, scales, n, k)
+    want = row.reshape(m, 1) * weight
+    assert np.isnan(got[:, none]).all()
+    normal = want >= 2.0 ** -126
+    equal = got == want
+    assert equal[:, ~none][normal[:, ~none]].all()
+    assert (equal | (got == 0.0))[:, ~none].all()
+
+
+@pytest.mark.parametrize("kind", sorted(ref.TYPES))
+@pytest.mark.parametrize("m,n,k", [s for s in SHAPES if s[0] >= 3])
+@pytest.mark.parametrize("pad", [1, 2])
+def test_rows_of_infinities_and_nans(device, mc, kind, m, n, k, pad):
+    """An infinity makes its row's results infinite and a NaN makes them NaN, the last element of an odd row among them;
+    the other rows, and what lies between rows (NaN), reach nothing."""
+    k, dtype = k + 1, ref.TYPES[kind]
+    print(f"case rows of no numbers {kind} {m}x{n}x{k} pad {pad}", flush=True)
+    rng = np.random.default_rng(m + k)
+    x = rng.standard_normal((m, k))
+    x[0, 7], x[1, k - 1], x[2, 190], x[m - 1, k - 1] = np.inf, np.nan, np.nan, -np.inf
+    w = np.abs(rng.standard_normal((n, k))) + 0.5  # no zero among the codes that meet an infinity
+    w[::2] *= -1.0
+    bits = ref.to_type(x, dtype)
+    wc, ws, values = ref.quantize(w)
+    a, bc, bs = device_rows(mc, bits, k + pad), mc.DeviceBuffer.from_array(wc), mc.DeviceBuffer.from_array(ws)
+    c = Out(mc, m * n * 4)
+    workspace = mc.DeviceBuffer(max(1, mc.matmul_mx4_weights_workspace_bytes(dtype, m, n, k)))
+    mc.launch_matmul_mx4_weights(dtype, a.ptr, k + pad, bc.ptr, bs.ptr, ref.F32, c.ptr, m, n, k, None, workspace.ptr)
+    mc.synchronize()
+    got = c.get(np.float32, (m, n)).astype(np.float64)
+    sign = np.where(np.arange(n) % 2 == 0, -1.0, 1.0)
+    assert np.array_equal(got[0], np.inf * sign)
+    assert np.isnan(got[1]).all()
+    if m > 3:
+        assert np.isnan(got[2]).all() and np.array_equal(got[m - 1], -np.inf * sign)
+        exact, bound = ref.product_bound(ref.from_type(bits, dtype)[3:m - 1], values, 3 * k, ref.F32)
+        assert (np.abs(got[3:m - 1] - exact) <= bound).all()
+    else:
+        assert np.isnan(got[2]).all()
