@@ -105,3 +105,11 @@ def test_many_experts_and_long_rows(device, mc, weights, tokens, d, h, experts, 
     print(f"case moe weights {weights} {tokens} {d} {h} {experts} {top_k} {act}", flush=True)
     for kind in ("f32", "f16"):
         check(mc, 5, kind, weights, tokens, d, h, experts, top_k, act, bias=experts % 2 == 1)
+
+
+@pytest.mark.parametrize("weights", [ref.BF16, ref.F16])
+@pytest.mark.parametrize("act", ["relu", "gelu", "swiglu"])
+def test_odd_rows_of_every_type(device, mc, weights, act):
+    print(f"case moe odd rows weights {weights} {act}", flush=True)
+    for kind in sorted(ref.TYPES):
+        check(mc, 6, kind, weights, 11, 133, 61, 5, 2, act)

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mx4_oracle as ref
-from test_gpu_mx4 import Out, bits_type, device_rows, operand, within
+from test_gpu_mx4 import Out, bits_type, device_rows, operand, upload_at, within
 
 pytestmark = pytest.mark.gpu
 
@@ -33,7 +33,11 @@ def test_quantised_operands(device, mc, kind, m, n, k):
 @pytest.mark.parametrize("kind", sorted(ref.TYPES))
 @pytest.mark.parametrize("m,n,k,pad", [(1, 14336, 2100, 0), (2, 14336, 300, 1), (9, 8200, 300, 1), (16, 14336, 2100, 0),
                                        (16, 14336, 2101, 2), (12, 4200, 2100, 3), (16, 8200, 2100, 0), (32, 14336, 1100, 0),
-                                       (20, 8200, 1101, 1), (64, 8192, 2048, 0), (33, 4200, 1101, 0), (64, 4096, 2200, 0)])
+                                       (20, 8200, 1101, 1), (64, 8192, 2048, 0), (33, 4200, 1101, 0), (64, 4096, 2200, 0),
+                                       (16, 4096, 2100, 0), (11, 1000, 2201, 1), (20, 8000, 1100, 2), (33, 1000, 1100, 0),
+                                       (40, 5000, 1100, 2), (5, 300, 700, 0), (5, 300, 701, 0), (9, 8200, 300, 0),
+                                       (100, 300, 129, 0), (130, 4500, 201, 0), (2050, 2060, 390, 0),
+                                       (9, 8000, 300, 0), (20, 1000, 300, 0)])
 def test_quantised_weights(device, mc, kind, m, n, k, pad):
     print(f"case mx4 weights {kind} {m}x{n}x{k} pad {pad}", flush=True)
     dtype = ref.TYPES[kind]
@@ -48,4 +52,22 @@ def test_quantised_weights(device, mc, kind, m, n, k, pad):
         mc.synchronize()
         # Up to three pieces of A per product.
         exact, bound = ref.product_bound(ref.from_type(bits, dtype), b, 3 * k, out)
+        within(ref.from_type(c.get(bits_type(out), (m, n)), out), exact, bound)
+
+
+@pytest.mark.parametrize("n", [40, 8200])
+def test_few_fp32_rows_more_than_2_gib_apart(device, mc, n):
+    m, k, lda = 2, 200, (1 << 29) + 3
+    print(f"case mx4 weights, fp32 rows far apart {n}", flush=True)
+    rng = np.random.default_rng(n)
+    bits = ref.to_type(rng.standard_normal((m, k)), ref.F32)
+    a = mc.DeviceBuffer(4 * ((m - 1) * lda + k))
+    for i in range(m):
+        upload_at(mc, a, 4 * i * lda, bits[i])
+    bc, bs, b = operand(mc, rng, n, k)
+    for out in (ref.F32, ref.BF16, ref.F16):
+        c = Out(mc, m * n * (4 if out == ref.F32 else 2))
+        mc.launch_matmul_mx4_weights(ref.F32, a.ptr, lda, bc.ptr, bs.ptr, out, c.ptr, m, n, k)
+        mc.synchronize()
+        exact, bound = ref.product_bound(ref.from_type(bits, ref.F32), b, 3 * k, out)
         within(ref.from_type(c.get(bits_type(out), (m, n)), out), exact, bound)
