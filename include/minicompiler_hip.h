@@ -297,8 +297,10 @@ MC_API int mc_launch_matmul_mx4(const void* a_codes, const void* a_scales, const
 /* C[m, n] = A B for A [m, k] of type a_dtype (rows lda elements apart), not
  * rounded (fp32 numbers below 2^-110 are cut to multiples of 2^-133, towards
  * zero), and B of n mx4 rows; fp32 sums, C in c_dtype. workspace: of
- * mc_matmul_mx4_weights_workspace_bytes bytes (0: may be NULL), 256-byte
- * aligned; calls that overlap need one each. */
+ * mc_matmul_mx4_weights_workspace_bytes bytes (0, up to 16 rows: may be NULL),
+ * 256-byte aligned; calls that overlap need one each. (The kernel for up to 64
+ * rows of 16 bits that start at dwords leaves it alone; it is asked for all the
+ * same, so that a call's needs follow from m, n, k and types.) */
 MC_API long long mc_matmul_mx4_weights_workspace_bytes(int a_dtype, int m, int n, int k);
 MC_API int mc_launch_matmul_mx4_weights(int a_dtype, const void* a, long long lda, const void* b_codes,
                                         const void* b_scales, int c_dtype, void* c, int m, int n, int k, void* stream,

@@ -13,8 +13,9 @@ using namespace mx4;
 // steps of 128 k in turn and their sums are added at the end. Fragments come
 // straight from memory, the next step's while one is multiplied. Bound by
 // latency: a launch, two trips to memory, and code read into a cold instruction
-// cache (1000x1001x1023 with 4x4 fragments: 8.5 KB of it in 7.9 us, 4.1 KB in
-// 6.3; 16x4096x4096 4.7 us).
+// cache (1000x1001x1023 with 4x4 fragments: 8.5 KB of it in 7.9 us, 4.1 KB in 6.3,
+// and 5.9 with four neighbouring lanes' loads from one row; 16x4096x4096 4.7 us and
+// so 3.6).
 template <int kM, int kN, int kWaves, int kOut>
 __global__ __launch_bounds__(kWaves * 64) void product_direct(const unsigned char* __restrict__ a_codes,
                                                               const unsigned char* __restrict__ a_scales,

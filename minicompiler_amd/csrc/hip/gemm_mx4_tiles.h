@@ -37,7 +37,9 @@
 // registers, runs at 7.4 PFLOP/s: the chip lowers its clock (1.9 GHz here). With
 // the fetch left out the loop's matrix units are busy 64% instead of 57%, with
 // the scales' work left out as well 70%, and 72% without LDS reads; the rest is
-// a tile's start and its store, which all blocks do at one time (13 of 250 us).
+// a tile's start and its store, which all blocks do at one time (13 of 250 us,
+// four tiles to a CU). In a tile's last two stages the fetches repeat its last
+// stage, where a next tile's first two could come.
 // 8 waves with quadrants of 128x64 took 261 us where 4 took 254.
 #pragma once
 

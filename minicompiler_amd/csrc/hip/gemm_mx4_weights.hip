@@ -97,9 +97,9 @@ struct Eight {
 // in turn, the next one under way while one is multiplied. Bound by the weights
 // and a launch's latency: one row by 14336x4096 in 7.6 us (31 MB at 4.1 TB/s),
 // two by 4096x4096 in 3.7. 16 bf16 rows by 14336x4096 take 10.4 us a call where
-// a launch that cuts them and one that multiplies took 12.0, 12 fp32 rows by
-// 4096x4096 10.1 and 9.7. kLoose: rows that do
-// not all start at dwords, or more than 2 GiB of them.
+// a launch that cuts them and one that multiplies took 12.0; 12 fp32 rows by
+// 4096x4096 9.8 and 9.7, three pieces of every number cut in each of 256 blocks.
+// kLoose: rows that do not all start at dwords, or more than 2 GiB of them.
 template <int kIn, int kN, int kOut, bool kLoose>
 __global__ __launch_bounds__(kFewWaves * 64) void weights_few(const void* __restrict__ a, long long lda,
                                                               const unsigned char* __restrict__ b_codes,

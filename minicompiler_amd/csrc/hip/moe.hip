@@ -21,11 +21,12 @@
 // the second. Products are exact (bf16 pieces of x, h and the weights; what of
 // fp32 numbers lies below 2^-133 is left out), sums fp32.
 //
-// Measured (router, up, down, and all of it in steady repetition): one token, 8
-// of 64 mx4 experts of 2048x1024: 3.3, 9.5, 6.8, 22 us (27 MB); 16 tokens, 8 bf16
-// experts of 512x2048, fp32: 7.7, 7.8, 8.6, 29 us (34 MB); 64 tokens, 32 fp16
-// experts of 1023x777: 12.4, 25.5, 22.4, 68 us (153 MB; with rows of 1024 and 768
-// elements 11.3, 20, 15: rows at odd places cost a quarter of the rate).
+// Measured (router, up, down, medians of a kernel trace, and all of it in steady
+// repetition): one token, 8 of 64 mx4 experts of 2048x1024: 4.0, 10.6, 8.7, 22.3
+// us (27 MB); 16 tokens, 8 bf16 experts of 512x2048, fp32: 8.0, 10.5, 10.3, 28.8 us
+// (34 MB); 64 tokens, 32 fp16 experts of 1023x777: 13.0, 31.3, 25.4, 70.7 us (153
+// MB); with rows of 1024 and 768 elements 12.3, 25.2, 21.0, 58.7: rows at odd places
+// cost a fifth of the time.
 
 #include "mx4_rows.h"
 
@@ -81,8 +82,10 @@ int router_parts(int d) { return std::min((d + 64 * kWaves - 1) / (64 * kWaves),
 
 int column_tiles(int d) { return (d + kCols - 1) / kCols; }
 
-// The shares that a column tile of y is cut into: a block for each CU (the
-// kernel's registers leave room for one), as long as a wave has a step to do.
+// The shares that a column tile of y is cut into: a block for each CU, as long as a
+// wave has a step to do. (A block is two waves to a SIMD; the kernel's registers,
+// 158 of 512 with mx4 weights and 209 to 224 with 16-bit ones, leave room for three
+// and for two.)
 int down_shares(const Sizes& s) {
     const int want = device_cus() / column_tiles(s.d);
     const int most = (s.max_jobs * (s.hp / kStep) + kWaves - 1) / kWaves;
@@ -90,8 +93,9 @@ int down_shares(const Sizes& s) {
 }
 
 int pieces_of(int dtype) { return dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1; }  // at most
-// h is an fp32 number, kept whole whatever the result's type (cut to 16 bits for 16-bit results it was 2^-15 too
-// small at worst, and turned last bits of y).
+// h is an fp32 number, kept whole whatever the result's type: cut to 16 bits for 16-bit results it was up to 2^-15 too
+// small, which turned last bits of y (2e-4 of a bf16 y, 4e-6 so), and moe_down took 8.2 us instead of 8.7 for one
+// token, 24.2 instead of 25.4 for 64.
 constexpr int kPiecesH = 3;
 
 std::size_t round_up(std::size_t v) { return (v + 255) / 256 * 256; }

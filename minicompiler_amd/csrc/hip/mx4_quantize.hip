@@ -11,7 +11,8 @@
 // Bound by memory: 2 or 4 bytes read and 17/32 written per element (and 2 or 4
 // written for `values`, past the caches: the codes are what is read next). By
 // rows 8192x2048 fp32 with values in 24.8 us (5.8 TB/s; 28.6 with plain stores),
-// 4096x14336 bf16 45 us (5.9), one row of 4096 1.5 us: a launch.
+// codes and scales alone 12.0 (6.3); 4096x14336 bf16 44 us (6.0) and 30.0 (4.9); one
+// row of 4096 1.5 us: a launch.
 
 #include <type_traits>
 
@@ -127,8 +128,9 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict
 // short, since a launch meets a cold instruction cache (32 elements per lane,
 // 5.5 KB of code: 1001x2047 fp16 in 6.9 us, so in 4.4). With values 4096x4096
 // fp32 25 us (5.8 TB/s; 37 with plain stores), 4096x14336 bf16 74 us (3.6 TB/s:
-// codes come in pieces of 4 bytes, 64 to a column and block). Loads past the
-// caches took 92: a line of x is read by several lanes' loads.
+// codes come in pieces of 4 bytes, 64 to a column and block); codes and scales
+// alone 13.6 and 46. Loads past the caches took 92: a line of x is read by several
+// lanes' loads.
 constexpr int kColumnThreads = 1024;
 
 template <int kType, int kPer>
