@@ -12,13 +12,14 @@ pytestmark = pytest.mark.gpu
 
 @pytest.fixture
 def failed(device, mc):
-    """A copy to nowhere, refused by the runtime."""
+    """A copy to nowhere, refused by the runtime; forgotten after the test."""
     a = np.zeros(4, dtype=np.float32)
 
     def fail():
         assert mc.library().mc_memcpy_htod(None, a.ctypes.data, a.nbytes) != 0
 
-    return fail
+    yield fail
+    mc.library().hipGetLastError()  # of the runtime that the library is linked with
 
 
 @pytest.mark.parametrize("columns", [False, True])
