@@ -243,8 +243,8 @@ __global__ __launch_bounds__(kWhole<kM> * 64) void weights_whole(const void* __r
     const auto of_column = [&](int j, int column, unsigned v) {
         return static_cast<unsigned>(__builtin_amdgcn_ds_bpermute((16 * j + column) * 4, static_cast<int>(v)));
     };
-    // A scale of 255 in lane's column (high bits of bytes); tiles whose column r has a weight past fp32's largest
-    // number among the lane's, which the sums could hold but the weights of the other kernels are not.
+    // A scale of 255 in lane's column (high bits of bytes); the tiles in whose column r the lane met a weight past
+    // fp32's largest number (its products might fit the sums, but are not finite in the other kernels).
     unsigned nans = 0, past = 0;
     int t = wave, half = 0;
     if (t < steps) load(t, 0);
