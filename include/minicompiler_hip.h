@@ -329,6 +329,83 @@ MC_API int mc_launch_moe(int dtype, const void* x, long long ldx, const float* r
                          const float* b2, void* y, int* chosen, float* gates, int tokens, int d, int h, int experts,
                          int top_k, int activation, int normalize, void* stream, void* workspace);
 
+/* ---- 8-bit integers, routing, experts on a plan ------------------------------
+ * No counterpart in the reference, whose lowest type is fp16. Types, errors,
+ * streams as for mx4 above: nothing waits or allocates.
+ *
+ * An i8 operand is `rows` rows of k numbers, the products' inner dimension
+ * along the row (B of C = A B as its n columns). k is padded with zeros to kp,
+ * the next multiple of 128: codes [rows, kp], signed bytes, 16-byte aligned;
+ * scales [rows], fp32. A code stands for code x scale. Padding must be zero. */
+MC_API long long mc_i8_code_bytes(int rows, int k);
+/* x [rows, k], rows ld elements apart, to an i8 operand: per row s = (largest
+ * magnitude) / 127, rounded to fp32, each code the exact quotient x / s rounded
+ * to the nearest integer, ties to the even one, -127..127. A row of zeros (or
+ * of numbers so small that s is 0) has s = 0 and zero codes; one with an
+ * infinity or a NaN s = NaN and zero codes, so that its products are NaN.
+ * values (NULL: not wanted): code x s, [rows, k] without gaps, in x's type.
+ * k at most 2^28. */
+MC_API int mc_quantize_i8(int dtype, const void* x, long long ld, void* codes, float* scales, int rows, int k,
+                          void* values, void* stream);
+/* The same of a row-major B [k, n] (rows ld elements apart), a scale for each
+ * column: an operand of n rows of k. values (NULL: not wanted): [k, n]. */
+MC_API int mc_quantize_i8_columns(int dtype, const void* b, long long ld, void* codes, float* scales, int k, int n,
+                                  void* values, void* stream);
+/* C[m, n] (row-major, of type c_dtype) = act(sum a b x a_scale x b_scale +
+ * bias) for A of m and B of n i8 rows of k: exact 32-bit sums, the rest in fp32
+ * and rounded once. bias [n], fp32, or NULL. activation: 0 ReLU, 1 GELU (tanh
+ * form), 2 SwiGLU (B and bias have 2 n rows, n gate rows first, act =
+ * gate sigmoid(gate) up), 3 none. k at most 131071 (128^2 k < 2^31). */
+MC_API int mc_launch_matmul_i8(const void* a_codes, const float* a_scales, const void* b_codes, const float* b_scales,
+                               const float* bias, int activation, int c_dtype, void* c, int m, int n, int k,
+                               void* stream);
+/* The choice of experts from logits [tokens, experts] (of type dtype, rows ld
+ * apart), any number of tokens:
+ *   score = softmax(logits) (0) or sigmoid(logits) (1), fp64;
+ *   key = score + bias ([experts], fp32, or NULL: the choice alone goes by it);
+ *   groups > 1: experts in that many equal groups, one after the other; the
+ *   top_groups groups with the largest sum of their group_best (1 or 2) largest
+ *   keys stay (1 for groups of one expert);
+ *   the top_k largest keys among them, largest first, ties to the lower index;
+ *   gates = their scores, with normalize divided by their sum (0 where that is
+ *   0), times scale.
+ * Without bias, and unless groups > 1 with group_best 2, logits are compared as they are.
+ * A logit of -infinity is never chosen before another, whatever its bias, and
+ * its score is 0 (all of a token's: gates 0); a NaN logit counts as
+ * -infinity in the choice and makes the token's gates NaN, and so does, by
+ * softmax, +infinity. A key that is NaN counts as -infinity.
+ * chosen, gates: [tokens, top_k]. order, offsets (both or neither NULL): the
+ * plan: a pair is token x top_k + place, order [tokens x top_k] all pairs, sorted
+ * by expert and for one expert by pair; expert e's "slots" are offsets[e] to
+ * offsets[e + 1] - 1 of it, offsets [experts + 1]. At most 512 experts, 16 per
+ * token, 64 groups. workspace: mc_route_workspace_bytes bytes (0: may be
+ * NULL), 256-byte aligned, needed with a plan; calls that overlap need one
+ * each. */
+MC_API long long mc_route_workspace_bytes(int tokens, int experts, int top_k);
+MC_API int mc_launch_route(int dtype, const void* logits, long long ld, const float* bias, int tokens, int experts,
+                           int top_k, int score, int groups, int top_groups, int group_best, int normalize, float scale,
+                           int* chosen, float* gates, int* order, int* offsets, void* stream, void* workspace);
+/* The experts' first product on a plan: C[slot, n] = act(x[order[slot] / top_k]
+ * W_e^T + b_e) for the expert e whose slot it is. x: an i8 operand of `tokens`
+ * rows of k; W: one of experts x n rows (SwiGLU: 2 n per expert, gates first),
+ * bias [experts, n (2 n)], fp32, or NULL; C [tokens x top_k, n], of type c_dtype.
+ * Slots outside offsets[0] .. offsets[experts] - 1 are left as they are (a part
+ * of a plan's experts, with offsets from its first on, works on that part). */
+MC_API int mc_launch_experts_up_i8(const void* x_codes, const float* x_scales, const void* w_codes,
+                                   const float* w_scales, const float* bias, int activation, int c_dtype, void* c,
+                                   const int* order, const int* offsets, int tokens, int top_k, int experts, int n,
+                                   int k, void* stream);
+/* ... and the second: y[token, n] = sum over the token's pairs, in their order,
+ * of gates[pair] (h[slot] W_e^T + b_e), in fp32. h: an i8 operand of tokens x
+ * top_k rows of k, by slot; W of experts x n rows; y [tokens, n]. The plan has
+ * every pair once. workspace: mc_experts_down_i8_workspace_bytes bytes,
+ * 256-byte aligned; calls that overlap need one each. */
+MC_API long long mc_experts_down_i8_workspace_bytes(int c_dtype, int tokens, int top_k, int n, int k);
+MC_API int mc_launch_experts_down_i8(const void* h_codes, const float* h_scales, const void* w_codes,
+                                     const float* w_scales, const float* bias, int c_dtype, void* y, const int* order,
+                                     const int* offsets, const float* gates, int tokens, int top_k, int experts, int n,
+                                     int k, void* stream, void* workspace);
+
 /* Device memory, streams and events (the thin layer, for callers with no
  * other HIP runtime in the process). */
 MC_API int mc_device_count(void);

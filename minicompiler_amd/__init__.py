@@ -121,6 +121,15 @@ _SIGNATURES = {
     "mc_moe_workspace_bytes": (_ll, [_i, _i, _i, _i, _i, _i]),
     "mc_launch_moe": (_i, [_i, _vp, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i,
                            _i, _vp, _vp]),
+    "mc_i8_code_bytes": (_ll, [_i, _i]),
+    "mc_quantize_i8": (_i, [_i, _vp, _ll, _vp, _vp, _i, _i, _vp, _vp]),
+    "mc_quantize_i8_columns": (_i, [_i, _vp, _ll, _vp, _vp, _i, _i, _vp, _vp]),
+    "mc_launch_matmul_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp]),
+    "mc_route_workspace_bytes": (_ll, [_i, _i, _i]),
+    "mc_launch_route": (_i, [_i, _vp, _ll, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_launch_experts_up_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "mc_experts_down_i8_workspace_bytes": (_ll, [_i, _i, _i, _i, _i]),
+    "mc_launch_experts_down_i8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
     "mc_sum_split_partials": (_i, [_vp, _vp, _sz, _i, _vp]),
     "mc_split_k_splits": (_i, [_i, _i, _i, _i, _i]),
     "mc_matmul_splits": (_i, [_i, _i, _i, _i, _i]),
@@ -772,6 +781,84 @@ def launch_moe(dtype: int, x: int, ldx: int, router: int, weights: int, w1: int,
     _check_launch(library().mc_launch_moe(dtype, x, ldx, router, weights, w1, w1_scales, b1, w2, w2_scales, b2, y,
                                           chosen, gates, tokens, d, h, experts, top_k, act, int(normalize),
                                           _stream_handle(stream), workspace))
+
+
+# ---------------------------------------------------------------- 8-bit integer operands, routing, experts on a plan
+
+
+def i8_code_bytes(rows: int, k: int) -> int:
+    """Bytes of the codes of an i8 operand of `rows` rows of k (one each, k padded to a multiple of 128); its scales are
+    one fp32 per row."""
+    return int(library().mc_i8_code_bytes(rows, k))
+
+
+def quantize_i8(dtype: int, x: int, ld: int, codes: int, scales: int, rows: int, k: int, values: int | None = None,
+                stream=None) -> None:
+    """x [rows, k] (rows ld elements apart; DTYPE_F32, DTYPE_BF16 or DTYPE_F16) to an i8 operand, a scale for each row;
+    values: what the codes stand for, in x's type, if wanted."""
+    _check_launch(library().mc_quantize_i8(dtype, x, ld, codes, scales, rows, k, values, _stream_handle(stream)))
+
+
+def quantize_i8_columns(dtype: int, b: int, ld: int, codes: int, scales: int, k: int, n: int,
+                        values: int | None = None, stream=None) -> None:
+    """Row-major B [k, n] to the i8 operand of its n columns, a scale for each; values: [k, n]."""
+    _check_launch(library().mc_quantize_i8_columns(dtype, b, ld, codes, scales, k, n, values, _stream_handle(stream)))
+
+
+I8_ACTIVATIONS = {**MOE_ACTIVATIONS, None: 3}
+
+
+def _i8_activation(activation: int | str | None) -> int:
+    return activation if isinstance(activation, int) else I8_ACTIVATIONS.get(activation, -1)
+
+
+def launch_matmul_i8(a_codes: int, a_scales: int, b_codes: int, b_scales: int, bias: int | None,
+                     activation: int | str | None, c_dtype: int, c: int, m: int, n: int, k: int, stream=None) -> None:
+    """C[m, n] of type c_dtype = act(A B + bias), A of m and B of n (SwiGLU: 2 n) i8 rows of k; activation: "relu",
+    "gelu", "swiglu" or None."""
+    _check_launch(library().mc_launch_matmul_i8(a_codes, a_scales, b_codes, b_scales, bias, _i8_activation(activation),
+                                                c_dtype, c, m, n, k, _stream_handle(stream)))
+
+
+ROUTE_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def route_workspace_bytes(tokens: int, experts: int, top_k: int) -> int:
+    return int(library().mc_route_workspace_bytes(tokens, experts, top_k))
+
+
+def launch_route(dtype: int, logits: int, ld: int, bias: int | None, tokens: int, experts: int, top_k: int,
+                 score: int | str, groups: int, top_groups: int, group_best: int, normalize: bool, scale: float,
+                 chosen: int, gates: int, order: int | None = None, offsets: int | None = None, stream=None,
+                 workspace: int | None = None) -> None:
+    """The top_k experts of each token by softmax or sigmoid of its logits (mc_launch_route), their gates, and with
+    order and offsets the plan that launch_experts_up_i8 and launch_experts_down_i8 run on."""
+    score = ROUTE_SCORES.get(score, -1) if isinstance(score, str) else score
+    _check_launch(library().mc_launch_route(dtype, logits, ld, bias, tokens, experts, top_k, score, groups, top_groups,
+                                            group_best, int(normalize), scale, chosen, gates, order, offsets,
+                                            _stream_handle(stream), workspace))
+
+
+def launch_experts_up_i8(x_codes: int, x_scales: int, w_codes: int, w_scales: int, bias: int | None,
+                         activation: int | str | None, c_dtype: int, c: int, order: int, offsets: int, tokens: int,
+                         top_k: int, experts: int, n: int, k: int, stream=None) -> None:
+    """The experts' first product: C[slot, n] = act(x W_e + b_e) of the slot's token and expert, as the plan has them."""
+    _check_launch(library().mc_launch_experts_up_i8(x_codes, x_scales, w_codes, w_scales, bias,
+                                                    _i8_activation(activation), c_dtype, c, order, offsets, tokens,
+                                                    top_k, experts, n, k, _stream_handle(stream)))
+
+
+def experts_down_i8_workspace_bytes(c_dtype: int, tokens: int, top_k: int, n: int, k: int) -> int:
+    return int(library().mc_experts_down_i8_workspace_bytes(c_dtype, tokens, top_k, n, k))
+
+
+def launch_experts_down_i8(h_codes: int, h_scales: int, w_codes: int, w_scales: int, bias: int | None, c_dtype: int,
+                           y: int, order: int, offsets: int, gates: int, tokens: int, top_k: int, experts: int, n: int,
+                           k: int, stream=None, workspace: int | None = None) -> None:
+    """The experts' second product and the sum by gates: y[token, n] = sum of gate (h[slot] W_e + b_e) of its pairs."""
+    _check_launch(library().mc_launch_experts_down_i8(h_codes, h_scales, w_codes, w_scales, bias, c_dtype, y, order,
+                                                      offsets, gates, tokens, top_k, experts, n, k,
+                                                      _stream_handle(stream), workspace))
 
 
 # ---------------------------------------------------------------- generator

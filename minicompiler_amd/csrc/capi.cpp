@@ -8,6 +8,7 @@
 #include "hip/hip_rt.h"
 #include "hip/kernel_compiler.hpp"
 #include "hip/matmul.h"
+#include "hip/i8.h"
 #include "hip/mx4.h"
 #include "hip/matmul_policy.hpp"
 #include "minicompiler/hip/hip_backend.hpp"
@@ -937,6 +938,73 @@ MC_API int mc_launch_moe(int dtype, const void* x, long long ldx, const float* r
                               workspace};
     const int rc = mchip_launch_moe(&args, stream, &why);
     return launched("mc_launch_moe", rc, why);
+}
+
+MC_API long long mc_i8_code_bytes(int rows, int k) {
+    return rows < 1 || k < 1 ? 0 : rows * mchip_i8_k(k);
+}
+
+MC_API int mc_quantize_i8(int dtype, const void* x, long long ld, void* codes, float* scales, int rows, int k,
+                          void* values, void* stream) {
+    const char* why = nullptr;
+    const int rc = mchip_quantize_i8(dtype, x, ld, codes, scales, rows, k, values, stream, &why);
+    return launched("mc_quantize_i8", rc, why);
+}
+
+MC_API int mc_quantize_i8_columns(int dtype, const void* b, long long ld, void* codes, float* scales, int k, int n,
+                                  void* values, void* stream) {
+    const char* why = nullptr;
+    const int rc = mchip_quantize_i8_columns(dtype, b, ld, codes, scales, k, n, values, stream, &why);
+    return launched("mc_quantize_i8_columns", rc, why);
+}
+
+MC_API int mc_launch_matmul_i8(const void* a_codes, const float* a_scales, const void* b_codes, const float* b_scales,
+                               const float* bias, int activation, int c_dtype, void* c, int m, int n, int k,
+                               void* stream) {
+    const char* why = nullptr;
+    const int rc = mchip_launch_matmul_i8(a_codes, a_scales, b_codes, b_scales, bias, activation, c_dtype, c, m, n, k,
+                                          stream, &why);
+    return launched("mc_launch_matmul_i8", rc, why);
+}
+
+MC_API long long mc_route_workspace_bytes(int tokens, int experts, int top_k) {
+    return mchip_route_workspace_bytes(tokens, experts, top_k);
+}
+
+MC_API int mc_launch_route(int dtype, const void* logits, long long ld, const float* bias, int tokens, int experts,
+                           int top_k, int score, int groups, int top_groups, int group_best, int normalize, float scale,
+                           int* chosen, float* gates, int* order, int* offsets, void* stream, void* workspace) {
+    const char* why = nullptr;
+    const mchip_route_args args{dtype,      logits,     ld,        bias,  tokens, experts, top_k, score,   groups,
+                                top_groups, group_best, normalize, scale, chosen, gates,   order, offsets, workspace};
+    const int rc = mchip_launch_route(&args, stream, &why);
+    return launched("mc_launch_route", rc, why);
+}
+
+MC_API int mc_launch_experts_up_i8(const void* x_codes, const float* x_scales, const void* w_codes,
+                                   const float* w_scales, const float* bias, int activation, int c_dtype, void* c,
+                                   const int* order, const int* offsets, int tokens, int top_k, int experts, int n,
+                                   int k, void* stream) {
+    const char* why = nullptr;
+    const mchip_experts_args args{x_codes, x_scales, w_codes, w_scales, bias,  activation, c_dtype, c, order,
+                                  offsets, nullptr,  tokens,  top_k,    experts, n,        k,       nullptr};
+    const int rc = mchip_launch_experts_up_i8(&args, stream, &why);
+    return launched("mc_launch_experts_up_i8", rc, why);
+}
+
+MC_API long long mc_experts_down_i8_workspace_bytes(int c_dtype, int tokens, int top_k, int n, int k) {
+    return mchip_experts_down_i8_workspace_bytes(c_dtype, tokens, top_k, n, k);
+}
+
+MC_API int mc_launch_experts_down_i8(const void* h_codes, const float* h_scales, const void* w_codes,
+                                     const float* w_scales, const float* bias, int c_dtype, void* y, const int* order,
+                                     const int* offsets, const float* gates, int tokens, int top_k, int experts, int n,
+                                     int k, void* stream, void* workspace) {
+    const char* why = nullptr;
+    const mchip_experts_args args{h_codes, h_scales, w_codes, w_scales, bias,    MCHIP_ACT_NONE, c_dtype, y, order,
+                                  offsets, gates,    tokens,  top_k,    experts, n,              k,       workspace};
+    const int rc = mchip_launch_experts_down_i8(&args, stream, &why);
+    return launched("mc_launch_experts_down_i8", rc, why);
 }
 
 MC_API int mc_sum_split_partials(const float* partial, float* c, size_t count, int splits, void* stream) {

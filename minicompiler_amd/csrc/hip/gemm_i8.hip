@@ -1,0 +1,315 @@
+// Products of two operands quantised to 8-bit integers (i8.h): C = A B^T in exact
+// 32-bit sums, scaled by row and column, with bias and activation; and the
+// experts' products on a plan, the same for each expert's slots.
+
+#include "i8_device.h"
+
+namespace {
+
+using namespace i8;
+
+// What the rows of C are. Dense: row i of A makes row i of C. Up: slot i takes row
+// order[i] / top_k of A and makes row i of C. Down: slot i takes row i of A and makes
+// row order[i] of the workspace, fp32 and times its gate.
+constexpr int kDense = 0, kUp = 1, kDown = 2;
+
+struct Product {
+    const unsigned char *a, *b;
+    const float *a_scales, *b_scales, *bias;
+    void* c;
+    const int *order, *offsets;
+    const float* gates;
+    int m, n;  // rows of C (slots), columns of C
+    int row_bytes, a_rows, top_k, experts, activation, c_dtype;
+    unsigned tiles_n;
+};
+
+// Where a block works: rows `first` to `end` of C, on expert `expert`.
+struct Place {
+    int expert, first, end;
+};
+
+// Job `want` of the experts' slots, up to kRows of one expert's each; end = first: none.
+// A wave looks at 64 experts at a time.
+template <int kRows>
+__device__ __forceinline__ Place find_job(const Product& p, unsigned want) {
+    const int lane = threadIdx.x % 64;
+    for (int base = 0; base < p.experts; base += 64) {
+        const int e = base + lane;
+        int from = 0, to = 0;
+        if (e < p.experts) from = p.offsets[e], to = p.offsets[e + 1];
+        from = max(from, 0), to = min(to, p.m);
+        const unsigned jobs = to > from ? static_cast<unsigned>(to - from + kRows - 1) / kRows : 0u;
+        unsigned up_to = jobs;  // of the lanes up to this one
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const unsigned o = __shfl_up(up_to, d);
+            if (lane >= d) up_to += o;
+        }
+        const unsigned long long here = __ballot(up_to > want);
+        if (here != 0) {
+            const int at = __builtin_ctzll(here);
+            const unsigned before = __builtin_amdgcn_readlane(up_to - jobs, at);
+            const int first = __builtin_amdgcn_readlane(from, at) + static_cast<int>((want - before) * kRows);
+            return {base + at, first, __builtin_amdgcn_readlane(to, at)};
+        }
+        want -= __builtin_amdgcn_readlane(up_to, 63);
+    }
+    return {0, 0, 0};
+}
+
+// A block computes 16 kM rows by 16 kN columns of C (SwiGLU: the second half of the
+// column tiles are the up rows of the first half's columns); its kWaves waves take
+// the steps of 128 k in turn and their sums are added at the end. Four neighbouring
+// lanes load 64 bytes of a row, which are then passed to the lanes that multiply them.
+template <int kMode, bool kGated, int kM, int kN, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
+    __shared__ i32x4 space[kWaves * kM * kN * 64];
+    constexpr int kCols = kGated ? kN / 2 : kN;  // column tiles of C
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int r = lane % 16, q = lane / 16, part = lane % 4, pass = (4 * r + q) * 4;
+    const unsigned chunk = blockIdx.x / p.tiles_n;
+    const int col0 = static_cast<int>(blockIdx.x % p.tiles_n) * 16 * kCols;
+    Place place{0, 0, p.m};
+    long long row0 = static_cast<long long>(chunk) * 16 * kM;
+    if constexpr (kMode != kDense) {
+        place = find_job<16 * kM>(p, chunk);
+        if (place.first >= place.end) return;
+        row0 = place.first;
+    }
+    const int end = place.end;
+    const int b_rows = kGated ? 2 * p.n : p.n;
+    const unsigned char* b0 = p.b + static_cast<long long>(place.expert) * b_rows * p.row_bytes;
+    const unsigned char *a[kM], *b[kN];
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+        long long row = row0 + 16 * i + lane / 4;
+        row = row < end ? row : end - 1;
+        if constexpr (kMode == kUp) {
+            row = p.order[row] / p.top_k;
+            row = row < 0 ? 0 : row < p.a_rows ? row : p.a_rows - 1;
+        }
+        a[i] = p.a + row * p.row_bytes + part * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        const int col = col0 + 16 * (j % kCols) + lane / 4;
+        const long long row = (col < p.n ? col : p.n - 1) + (j >= kCols ? p.n : 0LL);
+        b[j] = b0 + row * p.row_bytes + part * 16;
+    }
+    i32x4 acc[kM * kN];
+#pragma unroll
+    for (int i = 0; i < kM * kN; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    for (int at = wave * kLine; at < p.row_bytes; at += kWaves * kLine) {
+        i32x4 av[2][kM], bv[2][kN];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) av[h][i] = *reinterpret_cast<const i32x4*>(a[i] + at + 64 * h);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) bv[h][j] = *reinterpret_cast<const i32x4*>(b[j] + at + 64 * h);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int i = 0; i < kM; ++i) av[h][i][e] = __builtin_amdgcn_ds_bpermute(pass, av[h][i][e]);
+#pragma unroll
+                for (int j = 0; j < kN; ++j) bv[h][j][e] = __builtin_amdgcn_ds_bpermute(pass, bv[h][j][e]);
+            }
+#pragma unroll
+            for (int i = 0; i < kM; ++i)
+#pragma unroll
+                for (int j = 0; j < kN; ++j) acc[i * kN + j] = mfma(bv[h][j], av[h][i], acc[i * kN + j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kM * kN; ++i) space[(wave * kM * kN + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    const auto sum_of = [&](int tile) {
+        i32x4 sum = space[tile * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += space[(w * kM * kN + tile) * 64 + lane];
+        return sum;
+    };
+#pragma unroll 1
+    for (int t = wave; t < kM * kCols; t += kWaves) {
+        const int i = t / kCols, j = t % kCols;
+        const long long row = row0 + 16 * i + r;
+        const int col = col0 + 16 * j + 4 * q;
+        if (row >= end || col >= p.n) continue;
+        const int left = p.n - col;
+        long long a_row = row, c_row = row;
+        if constexpr (kMode == kUp) {
+            a_row = p.order[row] / p.top_k;
+            a_row = a_row < 0 ? 0 : a_row < p.a_rows ? a_row : p.a_rows - 1;
+        }
+        if constexpr (kMode == kDown) {
+            c_row = p.order[row];
+            if (c_row < 0 || c_row >= p.m) continue;
+        }
+        const float sa = p.a_scales[a_row];
+        const long long b_row = static_cast<long long>(place.expert) * b_rows + col;
+        // One half's four columns, scaled, with the bias.
+        const auto scaled = [&](i32x4 sum, long long at) {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = 0.0f;
+                if (e < left) {
+                    v[e] = static_cast<float>(sum[e]) * sa * p.b_scales[at + e];
+                    if (p.bias != nullptr) v[e] += p.bias[at + e];
+                }
+            }
+            return v;
+        };
+        f32x4 v = scaled(sum_of(i * kN + j), b_row);
+        if constexpr (kGated) {
+            const f32x4 up = scaled(sum_of(i * kN + kCols + j), b_row + p.n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = v[e] * sigmoid(v[e]) * up[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = activate(v[e], p.activation);
+        }
+        if constexpr (kMode == kDown) {
+            const float gate = p.gates[c_row];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= gate;
+            store_four<kF32>(p.c, c_row * p.n + col, v, left);
+        } else {
+            store_four_as(p.c_dtype, p.c, c_row * p.n + col, v, left);
+        }
+    }
+}
+
+// y[token] = the sum of its top_k rows of the workspace, in order.
+template <int kOut>
+__global__ __launch_bounds__(256) void sum_pairs(const float* __restrict__ pairs, void* __restrict__ y, int tokens,
+                                                 int top_k, int n) {
+    const unsigned per_row = (static_cast<unsigned>(n) + 3) / 4;
+    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<long long>(tokens) * per_row;
+         i += static_cast<long long>(gridDim.x) * 256) {
+        const long long t = i / per_row;
+        const int col = static_cast<int>(i % per_row) * 4;
+        f32x4 sum = load_four<kF32>(pairs, t * top_k * n + col, n - col);
+        for (int j = 1; j < top_k; ++j) sum += load_four<kF32>(pairs, (t * top_k + j) * n + col, n - col);
+        store_four<kOut>(y, t * n + col, sum, n - col);
+    }
+}
+
+long long tiles(long long size, int tile) { return (size + tile - 1) / tile; }
+
+// Jobs of up to `rows` slots that the plan may have, at most.
+long long most_jobs(long long slots, int experts, int rows) {
+    return std::min(slots, (slots + std::min<long long>(experts, slots) * (rows - 1)) / rows);
+}
+
+template <int kMode, bool kGated, int kM, int kN>
+int launch_direct(Product p, hipStream_t stream, const char** why) {
+    constexpr int kWaves = 8;
+    p.tiles_n = static_cast<unsigned>(tiles(p.n, 16 * (kGated ? kN / 2 : kN)));
+    const long long chunks = kMode == kDense ? tiles(p.m, 16 * kM) : most_jobs(p.m, p.experts, 16 * kM);
+    if (!fits_launch(chunks * p.tiles_n, kWaves * 64)) {
+        *why = "more tiles of C than one launch takes";
+        return hipErrorInvalidValue;
+    }
+    return launch_kernel(i8_direct<kMode, kGated, kM, kN, kWaves>, static_cast<unsigned>(chunks * p.tiles_n), kWaves * 64,
+                         0, stream, p);
+}
+
+template <int kMode, bool kGated>
+int launch(const Product& p, hipStream_t stream, const char** why) {
+    // Rows of one expert, on average.
+    const long long rows = kMode == kDense ? p.m : tiles(p.m, p.experts);
+    if (rows <= 16) return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
+    return launch_direct<kMode, kGated, 4, 4>(p, stream, why);
+}
+
+const char* refusal(const void* a, const float* a_scales, const void* b, const float* b_scales, const float* bias,
+                    int activation, int c_dtype, const void* c, int rows, int n, int k) {
+    if (!is_float_type(c_dtype)) return "the result's type is none of fp32 (0), bf16 (1), fp16 (2)";
+    if (activation < MCHIP_ACT_RELU || activation > MCHIP_ACT_NONE)
+        return "the activation is none of ReLU (0), GELU (1), SwiGLU (2), none (3)";
+    if (rows < 1 || n < 1 || k < 1) return "a size below 1";
+    if (k > MCHIP_I8_MAX_K) return "k above 131071, whose sums may pass 32 bits";
+    if (n > (1 << 30)) return "n above 2^30";
+    if (a == nullptr || a_scales == nullptr || b == nullptr || b_scales == nullptr || c == nullptr)
+        return "a null operand";
+    if (!aligned(a, 16) || !aligned(b, 16)) return "codes not 16-byte aligned";
+    if (!aligned(a_scales, 4) || !aligned(b_scales, 4) || !aligned(bias, 4)) return "scales or a bias not 4-byte aligned";
+    if (!aligned(c, size_of(c_dtype))) return "a result that is not aligned to its elements";
+    return nullptr;
+}
+
+const char* plan_refusal(const mchip_experts_args& x) {
+    if (x.tokens < 1 || x.top_k < 1 || x.experts < 1) return "a size below 1";
+    if (x.experts > MCHIP_ROUTE_MAX_EXPERTS) return "more than 512 experts";
+    if (x.top_k > MCHIP_ROUTE_MAX_TOP_K) return "more than 16 experts for a token";
+    if (static_cast<long long>(x.tokens) * x.top_k > (1 << 30)) return "more than 2^30 pairs of a token and an expert";
+    if (x.order == nullptr || x.offsets == nullptr) return "a null plan";
+    if (!aligned(x.order, 4) || !aligned(x.offsets, 4)) return "a plan that is not 4-byte aligned";
+    return nullptr;
+}
+
+Product product_of(const mchip_experts_args& x) {
+    return {static_cast<const unsigned char*>(x.a_codes), static_cast<const unsigned char*>(x.w_codes), x.a_scales,
+            x.w_scales, x.bias, x.c, x.order, x.offsets, x.gates, x.tokens * x.top_k, x.n, padded_k(x.k), x.tokens,
+            x.top_k, x.experts, x.activation, x.c_dtype, 0};
+}
+
+}  // namespace
+
+extern "C" {
+
+int mchip_launch_matmul_i8(const void* a_codes, const float* a_scales, const void* b_codes, const float* b_scales,
+                           const float* bias, int activation, int c_dtype, void* c, int m, int n, int k, void* stream,
+                           const char** why) {
+    *why = refusal(a_codes, a_scales, b_codes, b_scales, bias, activation, c_dtype, c, m, n, k);
+    if (*why != nullptr) return hipErrorInvalidValue;
+    const Product p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(b_codes), a_scales,
+                    b_scales, bias, c, nullptr, nullptr, nullptr, m, n, padded_k(k), m, 1, 1, activation, c_dtype, 0};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return activation == MCHIP_ACT_SWIGLU ? launch<kDense, true>(p, s, why) : launch<kDense, false>(p, s, why);
+}
+
+int mchip_launch_experts_up_i8(const mchip_experts_args* args, void* stream, const char** why) {
+    const mchip_experts_args& x = *args;
+    *why = refusal(x.a_codes, x.a_scales, x.w_codes, x.w_scales, x.bias, x.activation, x.c_dtype, x.c, x.tokens, x.n, x.k);
+    if (*why == nullptr) *why = plan_refusal(x);
+    if (*why != nullptr) return hipErrorInvalidValue;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return x.activation == MCHIP_ACT_SWIGLU ? launch<kUp, true>(product_of(x), s, why)
+                                            : launch<kUp, false>(product_of(x), s, why);
+}
+
+long long mchip_experts_down_i8_workspace_bytes(int c_dtype, int tokens, int top_k, int n, int k) {
+    if (!is_float_type(c_dtype) || tokens < 1 || top_k < 1 || n < 1 || k < 1) return 0;
+    return static_cast<long long>(tokens) * top_k * n * 4;
+}
+
+int mchip_launch_experts_down_i8(const mchip_experts_args* args, void* stream, const char** why) {
+    const mchip_experts_args& x = *args;
+    *why = refusal(x.a_codes, x.a_scales, x.w_codes, x.w_scales, x.bias, MCHIP_ACT_NONE, x.c_dtype, x.c, x.tokens, x.n, x.k);
+    if (*why == nullptr) *why = plan_refusal(x);
+    if (*why == nullptr && x.top_k > x.experts) *why = "more experts for a token than there are";
+    if (*why == nullptr && (x.gates == nullptr || x.workspace == nullptr)) *why = "null gates, or a null workspace";
+    if (*why == nullptr && (!aligned(x.gates, 4) || !aligned(x.workspace, 256)))
+        *why = "gates not 4-byte, or a workspace not 256-byte aligned";
+    if (*why != nullptr) return hipErrorInvalidValue;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Product p = product_of(x);
+    p.activation = MCHIP_ACT_NONE;
+    p.c = x.workspace;
+    const int rc = launch<kDown, false>(p, s, why);
+    if (rc != hipSuccess) return rc;
+    const auto sum = [&](auto kernel) {
+        const long long blocks = tiles(static_cast<long long>(x.tokens) * ((x.n + 3) / 4), 256);
+        return launch_kernel(kernel, static_cast<unsigned>(std::min<long long>(blocks, 1 << 20)), 256, 0, s,
+                             static_cast<const float*>(x.workspace), x.c, x.tokens, x.top_k, x.n);
+    };
+    return x.c_dtype == kF32 ? sum(sum_pairs<kF32>) : x.c_dtype == kBf16 ? sum(sum_pairs<kBf16>) : sum(sum_pairs<kF16>);
+}
+
+}  // extern "C"
