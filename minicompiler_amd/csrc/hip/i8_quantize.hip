@@ -4,7 +4,7 @@
 // each code is the exact quotient x / s rounded to the nearest integer, ties to
 // the even one: n = rint(x (1 / s)) is off by one at most, and next to a half
 // only; r = x - n s is exact in one fma (a multiple of the finer of two ulps that
-// is at most s), so comparing 2 r with s decides. Rows whose scale would be near
+// is at most s), so comparing it with s / 2 decides. Rows whose scale would be near
 // or below the smallest normal number are first taken times 2^64, exactly. A row
 // with an infinity or a NaN has the scale NaN and codes 0.
 
@@ -14,113 +14,253 @@ namespace {
 
 using namespace i8;
 
-constexpr int kThreads = 256;
-
 struct Scale {
-    float s;       // as stored
-    float up;      // a power of two that keeps what follows normal
-    float big;     // s x up
-    float inverse; // 1 / big, 0 where codes are 0
+    float s;        // as stored
+    float up;       // a power of two that keeps what follows normal
+    float big;      // s x up
+    float inverse;  // 1 / big, 0 where codes are 0
+    float past;     // the least number above big / 2
+    bool none;      // no number
 };
 
-// top: the bits of the row's largest magnitude (infinities and NaNs are above all others).
-__device__ __forceinline__ Scale scale_of(unsigned top) {
+__device__ __forceinline__ Scale of_scale(float s) {
     Scale r;
-    const float a = __builtin_bit_cast(float, top);
-    r.s = top >= 0x7f800000u ? __builtin_nanf("") : a / 127.0f;
-    r.up = r.s < 0x1p-100f ? 0x1p64f : 1.0f;
-    r.big = r.s * r.up;
-    r.inverse = r.s > 0.0f ? 1.0f / r.big : 0.0f;
+    r.s = s;
+    r.none = !(s == s);
+    r.up = s < 0x1p-100f ? 0x1p64f : 1.0f;
+    r.big = s * r.up;
+    r.inverse = s > 0.0f ? 1.0f / r.big : 0.0f;
+    r.past = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, 0.5f * r.big) + 1u);
     return r;
 }
 
+// top: the bits of the row's largest magnitude (infinities and NaNs are above all others).
+__device__ __forceinline__ float scale_of(unsigned top) {
+    return top >= 0x7f800000u ? __builtin_nanf("") : __builtin_bit_cast(float, top) / 127.0f;
+}
+
+// Of a row without a scale (0 or NaN) the caller passes zeros.
 __device__ __forceinline__ int code_of(float x, const Scale& c) {
-    // No number, or no scale: 0 (and an infinity times 0 would be no number).
-    if (c.inverse == 0.0f || !(c.s == c.s)) return 0;
     x *= c.up;
-    float n = __builtin_rintf(x * c.inverse);
-    const float r = __builtin_fmaf(-n, c.big, x), twice = __builtin_fabsf(r) * 2.0f;
-    const bool odd = (static_cast<int>(n) & 1) != 0;
-    if (twice > c.big || (twice == c.big && odd)) n += r < 0.0f ? -1.0f : 1.0f;
-    n = n > 127.0f ? 127.0f : n < -127.0f ? -127.0f : n;
-    return static_cast<int>(n);
+    const float n = __builtin_rintf(x * c.inverse);
+    const float r = __builtin_fmaf(-n, c.big, x);
+    int code = static_cast<int>(n);
+    // At a half exactly the even one is right, past it the next.
+    const float most = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, c.past) - (code & 1));
+    if (__builtin_fabsf(r) >= most) code += r < 0.0f ? -1 : 1;
+    // Past 127 only where the scale is no normal number and so rounded by much.
+    return code > 127 ? 127 : code < -127 ? -127 : code;
 }
 
 __device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
+// The low bytes of four codes.
 __device__ __forceinline__ unsigned pack(int a, int b, int c, int d) {
-    return static_cast<unsigned>(a & 255) | static_cast<unsigned>(b & 255) << 8 | static_cast<unsigned>(c & 255) << 16 |
-           static_cast<unsigned>(d) << 24;
+    const unsigned low = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), high = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return low | high << 16;
 }
 
-// What a code stands for. Both factors are exact; of a row without a scale, NaN.
-__device__ __forceinline__ float value_of(int code, const Scale& c) { return static_cast<float>(code) * c.s; }
+// Eight numbers to two dwords of codes; back: what they stand for (of a row without a scale, NaN).
+__device__ __forceinline__ u32x2 codes_of(float (&v)[8], const Scale& c) {
+    int n[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        n[e] = c.none || c.inverse == 0.0f ? 0 : code_of(v[e], c);
+        v[e] = static_cast<float>(n[e]) * c.s;
+    }
+    return u32x2{pack(n[0], n[1], n[2], n[3]), pack(n[4], n[5], n[6], n[7])};
+}
 
-// A block takes a row, twice over.
+// Values past the caches: the codes are what is read next.
 template <int kType>
-__global__ __launch_bounds__(kThreads) void quantize_rows(const void* __restrict__ x, long long ld,
-                                                          unsigned* __restrict__ codes, float* __restrict__ scales,
-                                                          void* __restrict__ values, int rows, int k, int dwords) {
-    __shared__ unsigned tops[kThreads / 64];
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        unsigned top = 0;
-        for (int i = threadIdx.x; i < dwords; i += kThreads) {
-            const f32x4 v = load_four<kType>(x, row * ld + i * 4LL, k - i * 4);
+__device__ __forceinline__ void store_eight(void* p, long long at, const float (&v)[8], int left) {
+    if (left >= 8) {
+        if constexpr (kType == kF32) {
+            f32x4_loose* d = reinterpret_cast<f32x4_loose*>(static_cast<float*>(p) + at);
+            const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+            __builtin_nontemporal_store(lo, d);
+            __builtin_nontemporal_store(hi, d + 1);
+        } else {
+            u16x8 h;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, magnitude(v[e]));
+            for (int e = 0; e < 8; ++e) h[e] = to_16<kType>(v[e]);
+            __builtin_nontemporal_store(h, reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(p) + at));
         }
-        top = wave_max(top);
-        if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < left) store_one<kType>(p, at + e, v[e]);
+}
+
+// The largest of a row over its kLanes lanes (a wave, or a block of waves).
+template <int kLanes>
+__device__ __forceinline__ unsigned row_max(unsigned top, unsigned* space) {
+    top = wave_max(top);
+    if constexpr (kLanes > 64) {
+        if (threadIdx.x % 64 == 0) space[threadIdx.x / 64] = top;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kThreads / 64; ++w) top = max(top, tops[w]);
-        const Scale c = scale_of(top);
-        if (threadIdx.x == 0) scales[row] = c.s;
-        for (int i = threadIdx.x; i < dwords; i += kThreads) {
-            const f32x4 v = load_four<kType>(x, row * ld + i * 4LL, k - i * 4);
-            int n[4];
-            f32x4 back;
+        for (int w = 0; w < kLanes / 64; ++w) top = max(top, space[w]);
+    }
+    return top;
+}
+
+// kLanes lanes take a row, each kPer chunks of eight elements, which stay in registers
+// between the row's largest magnitude and the codes; a block of 256 lanes takes four
+// rows of one wave each.
+template <int kType, int kLanes, int kPer>
+__global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void quantize_rows(const void* __restrict__ x, long long ld,
+                                                                            u32x2* __restrict__ codes,
+                                                                            float* __restrict__ scales,
+                                                                            void* __restrict__ values, int rows, int k,
+                                                                            int chunks) {
+    __shared__ unsigned space[kLanes / 64];
+    constexpr int kRows = kLanes < 256 ? 256 / kLanes : 1;
+    const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / kLanes;
+    if (kRows > 1 && row >= rows) return;
+    const int lane = threadIdx.x % kLanes;
+    float v[kPer][8];
+    unsigned top = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                n[e] = code_of(v[e], c);
-                back[e] = value_of(n[e], c);
-            }
-            codes[row * dwords + i] = pack(n[0], n[1], n[2], n[3]);
-            if (values != nullptr && i * 4 < k) store_four<kType>(values, row * k + i * 4LL, back, k - i * 4);
-        }
-        __syncthreads();
+    for (int i = 0; i < kPer; ++i) load_eight<kType>(x, row * ld + (lane + i * kLanes) * 8, k - (lane + i * kLanes) * 8, v[i]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[i][e]));
+    const Scale c = of_scale(scale_of(row_max<kLanes>(top, space)));
+    if (lane == 0) scales[row] = c.s;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = lane + i * kLanes;
+        if (at >= chunks) break;
+        codes[row * chunks + at] = codes_of(v[i], c);
+        if (values != nullptr && at * 8 < k) store_eight<kType>(values, row * k + at * 8, v[i], k - at * 8);
     }
 }
 
-// A block takes 64 columns, twice over, its waves every fourth dword of codes.
+// Longer rows: a block a row, twice over.
+constexpr int kLong = 1024;
 template <int kType>
-__global__ __launch_bounds__(kThreads) void quantize_columns(const void* __restrict__ w, long long ld,
-                                                             unsigned* __restrict__ codes, float* __restrict__ scales,
-                                                             void* __restrict__ values, int k, int n, int dwords) {
-    __shared__ unsigned tops[kThreads / 64][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const long long col = static_cast<long long>(blockIdx.x) * 64 + lane;
-    const bool has = col < n;
+__global__ __launch_bounds__(kLong) void quantize_long_rows(const void* __restrict__ x, long long ld,
+                                                            u32x2* __restrict__ codes, float* __restrict__ scales,
+                                                            void* __restrict__ values, int k, int chunks) {
+    __shared__ unsigned space[kLong / 64];
+    const long long row = blockIdx.x;
     unsigned top = 0;
-    for (int i = wave; has && i < k; i += kThreads / 64) top = max(top, magnitude(load_one<kType>(w, i * ld + col)));
-    tops[wave][lane] = top;
-    __syncthreads();
-    if (!has) return;
+    float v[8];
+    for (int at = threadIdx.x; at < chunks; at += kLong) {
+        load_eight<kType>(x, row * ld + at * 8LL, k - at * 8, v);
 #pragma unroll
-    for (int v = 0; v < kThreads / 64; ++v) top = max(top, tops[v][lane]);
-    const Scale c = scale_of(top);
-    if (wave == 0) scales[col] = c.s;
-    for (int i = wave; i < dwords; i += kThreads / 64) {
-        int code[4];
+        for (int e = 0; e < 8; ++e) top = max(top, magnitude(v[e]));
+    }
+    const Scale c = of_scale(scale_of(row_max<kLong>(top, space)));
+    if (threadIdx.x == 0) scales[row] = c.s;
+    for (int at = threadIdx.x; at < chunks; at += kLong) {
+        load_eight<kType>(x, row * ld + at * 8LL, k - at * 8, v);
+        codes[row * chunks + at] = codes_of(v, c);
+        if (values != nullptr && at * 8 < k) store_eight<kType>(values, row * k + at * 8LL, v, k - at * 8);
+    }
+}
+
+// Two neighbouring elements of a row (one where the row ends) as fp32.
+template <int kType>
+__device__ __forceinline__ f32x2 load_two(const void* p, long long at, int left) {
+    typedef f32x2 f32x2_loose __attribute__((aligned(4)));
+    if (left >= 2) {
+        if constexpr (kType == kF32) return *reinterpret_cast<const f32x2_loose*>(static_cast<const float*>(p) + at);
+        const unsigned two = *reinterpret_cast<const u32_loose*>(static_cast<const unsigned short*>(p) + at);
+        return f32x2{to_f32<kType>(two & 0xffffu), to_f32<kType>(two >> 16)};
+    }
+    return f32x2{left == 1 ? load_one<kType>(p, at) : 0.0f, 0.0f};
+}
+
+template <int kType>
+__device__ __forceinline__ void store_two(void* p, long long at, float a, float b, int left) {
+    typedef f32x2 f32x2_loose __attribute__((aligned(4)));
+    if (left >= 2) {
+        if constexpr (kType == kF32)
+            __builtin_nontemporal_store(f32x2{a, b}, reinterpret_cast<f32x2_loose*>(static_cast<float*>(p) + at));
+        else
+            __builtin_nontemporal_store(to_16<kType>(a) | static_cast<unsigned>(to_16<kType>(b)) << 16,
+                                        reinterpret_cast<u32_loose*>(static_cast<unsigned short*>(p) + at));
+    } else if (left == 1) {
+        store_one<kType>(p, at, a);
+    }
+}
+
+// A block takes 2 kAcross columns whole: kAcross lanes a row of them, two columns each,
+// and eight rows down. What one step of the block covers (8 x 1024 / kAcross rows) stays
+// in registers between the columns' largest magnitudes and the codes; of longer columns
+// the steps before the last are read a second time, from a cache.
+constexpr int kColumnThreads = 1024;
+
+template <int kType, int kAcross>
+__global__ __launch_bounds__(kColumnThreads) void quantize_columns(const void* __restrict__ w, long long ld,
+                                                                   u32x2* __restrict__ codes,
+                                                                   float* __restrict__ scales,
+                                                                   void* __restrict__ values, int k, int n,
+                                                                   int chunks) {
+    constexpr int kDown = kColumnThreads / kAcross;
+    __shared__ unsigned tops[kColumnThreads / 64][2 * kAcross];
+    __shared__ float found[2 * kAcross];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int across = threadIdx.x % kAcross, down = threadIdx.x / kAcross;
+    // Blocks go to the XCDs in turn; neighbouring columns to one, whose L2 has the lines that they share.
+    const unsigned all = gridDim.x, mine = blockIdx.x % 8 * (all / 8) + blockIdx.x / 8;
+    const unsigned block = blockIdx.x < all / 8 * 8 ? mine : blockIdx.x;
+    const long long col = static_cast<long long>(block) * 2 * kAcross + 2 * across;
+    const int left = static_cast<int>(min(static_cast<long long>(n) - col, 2LL));
+    const int steps = (chunks + kDown - 1) / kDown;
+    float v[2][8];
+    const auto load = [&](int step) {
+        const int row = (step * kDown + down) * 8;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            code[e] = 0;
-            if (i * 4 + e < k) {
-                code[e] = code_of(load_one<kType>(w, (i * 4LL + e) * ld + col), c);
-                if (values != nullptr) store_one<kType>(values, (i * 4LL + e) * n + col, value_of(code[e], c));
-            }
+        for (int e = 0; e < 8; ++e) {
+            const f32x2 two = load_two<kType>(w, (row + e) * ld + col, row + e < k ? left : 0);
+            v[0][e] = two[0], v[1][e] = two[1];
         }
-        codes[col * dwords + i] = pack(code[0], code[1], code[2], code[3]);
+    };
+    unsigned top[2] = {0, 0};
+    for (int step = 0; step < steps; ++step) {
+        load(step);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            top[0] = max(top[0], magnitude(v[0][e]));
+            top[1] = max(top[1], magnitude(v[1][e]));
+        }
+    }
+#pragma unroll
+    for (int d = kAcross; d < 64; d *= 2) {
+        top[0] = max(top[0], static_cast<unsigned>(__shfl_xor(static_cast<int>(top[0]), d)));
+        top[1] = max(top[1], static_cast<unsigned>(__shfl_xor(static_cast<int>(top[1]), d)));
+    }
+    if (lane < kAcross) tops[wave][2 * lane] = top[0], tops[wave][2 * lane + 1] = top[1];
+    __syncthreads();
+    if (threadIdx.x < 2 * kAcross) {
+        unsigned most = 0;
+#pragma unroll
+        for (int u = 0; u < kColumnThreads / 64; ++u) most = max(most, tops[u][threadIdx.x]);
+        const float s = scale_of(most);
+        found[threadIdx.x] = s;
+        if (static_cast<long long>(block) * 2 * kAcross + threadIdx.x < n)
+            scales[static_cast<long long>(block) * 2 * kAcross + threadIdx.x] = s;
+    }
+    __syncthreads();
+    const Scale c[2] = {of_scale(found[2 * across]), of_scale(found[2 * across + 1])};
+    for (int step = steps - 1; step >= 0; --step) {
+        if (step != steps - 1) load(step);
+        const int chunk = step * kDown + down;
+        if (chunk >= chunks) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const u32x2 packed = codes_of(v[j], c[j]);
+            if (j < left) codes[(col + j) * chunks + chunk] = packed;
+        }
+        if (values == nullptr) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (chunk * 8 + e < k) store_two<kType>(values, (chunk * 8LL + e) * n + col, v[0][e], v[1][e], left);
     }
 }
 
@@ -137,24 +277,68 @@ const char* refusal(int dtype, const void* x, long long ld, const void* codes, c
     return nullptr;
 }
 
+// `elements` of x's type from p on (or null).
+template <int kType>
+const void* offset(const void* p, long long elements) {
+    return p == nullptr ? nullptr : static_cast<const unsigned char*>(p) + elements * kSize<kType>;
+}
+template <int kType>
+void* offset(void* p, long long elements) {
+    return const_cast<void*>(offset<kType>(static_cast<const void*>(p), elements));
+}
+
+// As many rows at a time as a launch takes.
 template <int kType>
 int launch_rows(const void* x, long long ld, void* codes, float* scales, int rows, int k, void* values,
                 hipStream_t stream) {
-    const unsigned blocks = static_cast<unsigned>(std::min(rows, 1 << 20));
-    return launch_kernel(quantize_rows<kType>, blocks, kThreads, 0, stream, x, ld, static_cast<unsigned*>(codes), scales,
-                         values, rows, k, padded_k(k) / 4);
+    const int chunks = padded_k(k) / 8, cus = device_cus();
+    constexpr int kMost = 1 << 21;
+    for (long long from = 0; from < rows; from += kMost) {
+        const int count = static_cast<int>(std::min<long long>(kMost, rows - from));
+        const void* at = offset<kType>(x, from * ld);
+        u32x2* to = static_cast<u32x2*>(codes) + from * chunks;
+        void* back = offset<kType>(values, from * k);
+        const auto go = [&](auto kernel, int lanes) {
+            const unsigned blocks = static_cast<unsigned>(lanes < 256 ? (count + 256 / lanes - 1) / (256 / lanes) : count);
+            return launch_kernel(kernel, blocks, lanes < 256 ? 256 : lanes, 0, stream, at, ld, to, scales + from, back, count,
+                                 k, chunks);
+        };
+        // Few rows: as many lanes to a row as have something to do. Many: as few as hold it,
+        // so that no wave waits for another.
+        const bool few = count < 4 * cus;
+        int rc;
+        if (chunks <= 64) rc = go(quantize_rows<kType, 64, 1>, 64);
+        else if (!few && chunks <= 128) rc = go(quantize_rows<kType, 64, 2>, 64);
+        else if (!few && chunks <= 256) rc = go(quantize_rows<kType, 64, 4>, 64);
+        else if (chunks <= 256) rc = go(quantize_rows<kType, 256, 1>, 256);
+        else if (!few && chunks <= 512) rc = go(quantize_rows<kType, 256, 2>, 256);
+        else if (!few && chunks <= 1024) rc = go(quantize_rows<kType, 256, 4>, 256);
+        else if (chunks <= 1024) rc = go(quantize_rows<kType, 1024, 1>, 1024);
+        else if (chunks <= 2048) rc = go(quantize_rows<kType, 1024, 2>, 1024);
+        else rc = launch_kernel(quantize_long_rows<kType>, static_cast<unsigned>(count), kLong, 0, stream, at, ld, to,
+                                scales + from, back, k, chunks);
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
 }
 
 template <int kType>
 int launch_columns(const void* w, long long ld, void* codes, float* scales, int k, int n, void* values,
                    hipStream_t stream, const char** why) {
-    const long long blocks = (static_cast<long long>(n) + 63) / 64;
-    if (!fits_launch(blocks, kThreads)) {
-        *why = "more columns than one launch takes";
-        return hipErrorInvalidValue;
-    }
-    return launch_kernel(quantize_columns<kType>, static_cast<unsigned>(blocks), kThreads, 0, stream, w, ld,
-                         static_cast<unsigned*>(codes), scales, values, k, n, padded_k(k) / 4);
+    const int cus = device_cus();
+    const auto go = [&](auto kernel, int across) {
+        const long long blocks = (static_cast<long long>(n) + 2 * across - 1) / (2 * across);
+        if (!fits_launch(blocks, kColumnThreads)) {
+            *why = "more columns than one launch takes (134217696)";
+            return static_cast<int>(hipErrorInvalidValue);
+        }
+        return launch_kernel(kernel, static_cast<unsigned>(blocks), kColumnThreads, 0, stream, w, ld,
+                             static_cast<u32x2*>(codes), scales, values, k, n, padded_k(k) / 8);
+    };
+    // Wide strips read the most of a line at once, narrow ones make more blocks.
+    if (n >= 32LL * cus) return go(quantize_columns<kType, 16>, 16);
+    if (n >= 16LL * cus / 2) return go(quantize_columns<kType, 8>, 8);
+    return go(quantize_columns<kType, 4>, 4);
 }
 
 }  // namespace
