@@ -2,7 +2,7 @@
 // 32-bit sums, scaled by row and column, with bias and activation; and the
 // experts' products on a plan, the same for each expert's slots.
 
-#include "i8_device.h"
+#include "gemm_i8_tiles.h"
 
 namespace {
 
@@ -184,6 +184,155 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
     }
 }
 
+// The row of A that row `row` of C takes.
+template <int kMode>
+__device__ __forceinline__ long long a_row_of(const Product& p, long long row) {
+    if constexpr (kMode != kUp) return row;
+    const int token = p.order[row] / p.top_k;
+    return token < 0 ? 0 : token < p.a_rows ? token : p.a_rows - 1;
+}
+
+// A wave's sums (tile_sums) scaled, with bias and activation, to C: rows row0 .. up to
+// `end`, columns col0 on, by way of the wave's 32 KiB of LDS, so that a short loop (a
+// launch meets a cold instruction cache) stores whole lines. In two passes: 64 columns of
+// all rows, or (kGated) 64 rows with both halves of their 64 columns. Block c of 16
+// bytes of row r lies at c ^ (r % 16).
+template <int kMode, bool kGated, int kOut, int kRowFrags>
+__device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Product& p,
+                                           const i32x4 (&acc)[kRowFrags][kColFrags], int expert, long long row0,
+                                           long long end, int col0, int lane) {
+    constexpr int kPasses = kGated ? kRowFrags / 4 : 2, kRowBytes = kGated ? 512 : 256;
+    constexpr int kPassRows = kGated ? 64 : 16 * kRowFrags;
+    const int r = lane % 16, q = lane / 16;
+    const long long b_row = static_cast<long long>(expert) * (kGated ? 2 * p.n : p.n);
+    // What goes with rows lane and lane + 64.
+    float sa[kRowFrags / 4], gate[kRowFrags / 4];
+    int c_rows[kRowFrags / 4];  // from row0 (Down: from 0) on, -1: not stored
+#pragma unroll
+    for (int h = 0; h < kRowFrags / 4; ++h) {
+        const long long row = row0 + lane + 64 * h;
+        sa[h] = 0.0f, gate[h] = 1.0f, c_rows[h] = -1;
+        if (row < end) {
+            sa[h] = p.a_scales[a_row_of<kMode>(p, row)];
+            c_rows[h] = lane + 64 * h;
+            if constexpr (kMode == kDown) {
+                c_rows[h] = p.order[row];
+                if (c_rows[h] >= p.m) c_rows[h] = -1;
+                if (c_rows[h] >= 0) gate[h] = p.gates[c_rows[h]];
+            }
+        }
+    }
+    const auto of_row = [&](auto value, int row) {
+        return __builtin_bit_cast(decltype(value), __builtin_amdgcn_ds_bpermute(row % 64 * 4, __builtin_bit_cast(int, value)));
+    };
+#pragma unroll
+    for (int h = 0; h < kPasses; ++h) {
+        constexpr int kFirst = kGated ? 4 : kRowFrags;
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i)
+#pragma unroll
+            for (int f = 0; f < (kGated ? 8 : 4); ++f)
+                *reinterpret_cast<MX4_LDS i32x4*>(lds + (16 * i + r) * kRowBytes + ((4 * f + q) ^ r) * 16) =
+                    kGated ? acc[4 * h + i][f] : acc[i][4 * h + f];
+        const int col = col0 + (kGated ? 0 : 64 * h) + 4 * r, left = p.n - col;
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        const f32x4 scale = load_four<kF32>(p.b_scales, b_row + col, left);
+        const f32x4 bias = p.bias != nullptr ? load_four<kF32>(p.bias, b_row + col, left) : zero;
+        f32x4 up_scale = zero, up_bias = zero;
+        if constexpr (kGated) {
+            up_scale = load_four<kF32>(p.b_scales, b_row + p.n + col, left);
+            if (p.bias != nullptr) up_bias = load_four<kF32>(p.bias, b_row + p.n + col, left);
+        }
+#pragma unroll 2
+        for (int four = 0; four < kPassRows / 4; ++four) {
+            const int row = 4 * four + q;
+            const MX4_LDS unsigned char* at = lds + row * kRowBytes;
+            const i32x4 sum = *reinterpret_cast<const MX4_LDS i32x4*>(at + (r ^ row % 16) * 16);
+            const int part = kGated ? h : four / 16;
+            const float s = of_row(kRowFrags / 4 == 1 || part == 0 ? sa[0] : sa[kRowFrags / 4 - 1], row);
+            const int c_row = of_row(kRowFrags / 4 == 1 || part == 0 ? c_rows[0] : c_rows[kRowFrags / 4 - 1], row);
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(sum[e]) * s * scale[e] + bias[e];
+            if constexpr (kGated) {
+                const i32x4 other = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((16 + r) ^ row % 16) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = v[e] * sigmoid(v[e]) * (static_cast<float>(other[e]) * s * up_scale[e] + up_bias[e]);
+            } else if constexpr (kMode == kDown) {
+                const float g = of_row(kRowFrags / 4 == 1 || part == 0 ? gate[0] : gate[kRowFrags / 4 - 1], row);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= g;
+            } else if (p.activation == MCHIP_ACT_RELU) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = activate(v[e], MCHIP_ACT_RELU);
+            } else if (p.activation == MCHIP_ACT_GELU) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = gelu(v[e]);
+            }
+            if (c_row >= 0 && left > 0)
+                store_four<kOut>(p.c, ((kMode == kDown ? 0 : row0) + c_row) * p.n + col, v, left);
+        }
+    }
+}
+
+// Rows row0 .. of C up to `end` (at most kRows) by 256 (kGated: 128) columns from col0 on.
+template <int kMode, bool kGated, int kOut, int kRows>
+__device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const Product& p, int expert, long long row0,
+                                             long long end, int col0) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    constexpr int kShare = kRows / 4;  // of A's rows, a wave's to fetch
+    // A's rows, from the wave's share of the tile on, or (gathered) all.
+    const long long a0 = kMode == kUp ? 0 : row0 + wave * kShare;
+    const long long a_left = kMode == kUp ? 0 : end - a0;
+    const __amdgpu_buffer_rsrc_t a =
+        kMode == kUp ? __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a), 0, p.a_rows * p.row_bytes, 0x00020000)
+                     : rsrc_of(p.a + a0 * p.row_bytes, a_left, p.row_bytes);
+    const auto a_row = [&](int i) {
+        const int in_share = i * 8 + lane / 8;
+        if constexpr (kMode != kUp) return in_share * p.row_bytes;
+        const long long row = row0 + wave * kShare + in_share;
+        return static_cast<int>(a_row_of<kMode>(p, row < end ? row : end - 1)) * p.row_bytes;
+    };
+    // B's rows that the wave fetches: 64 of columns, of gate or of up ones.
+    const int b_col = col0 + (kGated ? wave / 2 * 64 : wave * 64), b_rows = kGated ? 2 * p.n : p.n;
+    const long long b0 = static_cast<long long>(expert) * b_rows + (kGated ? wave % 2 * static_cast<long long>(p.n) : 0) + b_col;
+    const __amdgpu_buffer_rsrc_t b = rsrc_of(p.b + b0 * p.row_bytes, p.n - b_col, p.row_bytes);
+    i32x4 acc[kRows / 32][kColFrags];
+    tile_sums<kRows>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
+    lds_barrier();  // every wave is past its reads of the ring
+    store_tile<kMode, kGated, kOut>(lds + wave * (kRingBytes / 4), p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
+                                    col0 + wave % 2 * (kGated ? 64 : 128), lane);
+}
+
+// Dense: tiles in row-major order; the grid has one block per tile of 256 rows plus
+// `halves` more, for which that many of the last tiles run as two blocks of 128 rows.
+// On a plan: an expert's slots in tiles of 256, its last of 128 where that holds it.
+template <int kMode, bool kGated, int kOut>
+__global__ __launch_bounds__(kTileThreads, 1) void i8_tiles(const Product p, unsigned full) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kRingBytes];
+    MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);  // generic -> LDS address space
+    unsigned t = blockIdx.x;
+    int half = 0;
+    if (kMode == kDense && t >= full) half = 1 + static_cast<int>((t - full) % 2), t = full + (t - full) / 2;
+    const unsigned chunk = t / p.tiles_n;
+    const int col0 = static_cast<int>(t % p.tiles_n) * (kGated ? kTileCols / 2 : kTileCols);
+    long long row0 = static_cast<long long>(chunk) * kTileRows, end = p.m;
+    int expert = 0;
+    if constexpr (kMode == kDense) {
+        if (half == 2) row0 += kTileRows / 2;
+        if (half == 1 && row0 + kTileRows / 2 < end) end = row0 + kTileRows / 2;
+    } else {
+        const Place place = find_job<kTileRows>(p, chunk);
+        expert = place.expert, row0 = place.first, end = place.end;
+    }
+    if (row0 >= end) return;
+    if (end - row0 > kTileRows / 2)
+        product_tile<kMode, kGated, kOut, 256>(lds, p, expert, row0, end, col0);
+    else
+        product_tile<kMode, kGated, kOut, 128>(lds, p, expert, row0, end, col0);
+}
+
 // y[token] = the sum of its top_k rows of the workspace, in order.
 template <int kOut>
 __global__ __launch_bounds__(256) void sum_pairs(const float* __restrict__ pairs, void* __restrict__ y, int tokens,
@@ -220,9 +369,41 @@ int launch_direct(Product p, hipStream_t stream, const char** why) {
 }
 
 template <int kMode, bool kGated>
+int launch_tiles(Product p, hipStream_t stream, const char** why) {
+    p.tiles_n = static_cast<unsigned>(tiles(p.n, kGated ? kTileCols / 2 : kTileCols));
+    const long long chunks = kMode == kDense ? tiles(p.m, kTileRows) : most_jobs(p.m, p.experts, kTileRows);
+    const long long all = chunks * p.tiles_n;
+    const int cus = device_cus(), rest = static_cast<int>(all % cus);
+    const int halves = kMode == kDense && rest <= cus / 2 ? rest : 0;
+    if (!fits_launch(all + halves, kTileThreads)) {
+        *why = "more tiles of C than one launch takes";
+        return hipErrorInvalidValue;
+    }
+    const auto go = [&](auto kernel) {
+        return launch_kernel(kernel, static_cast<unsigned>(all + halves), kTileThreads, 0, stream, p,
+                             static_cast<unsigned>(all - halves));
+    };
+    if constexpr (kMode == kDown) {
+        return go(i8_tiles<kMode, kGated, kF32>);
+    } else {
+        return p.c_dtype == kF32    ? go(i8_tiles<kMode, kGated, kF32>)
+               : p.c_dtype == kBf16 ? go(i8_tiles<kMode, kGated, kBf16>)
+                                    : go(i8_tiles<kMode, kGated, kF16>);
+    }
+}
+
+// Offsets within a tile's rows, and within A where its rows are gathered, have 32 bits.
+template <int kMode>
+bool tiles_fit(const Product& p) {
+    const long long a_rows = kMode == kUp ? p.a_rows : kTileRows;
+    return a_rows * p.row_bytes < (1LL << 31);
+}
+
+template <int kMode, bool kGated>
 int launch(const Product& p, hipStream_t stream, const char** why) {
     // Rows of one expert, on average.
     const long long rows = kMode == kDense ? p.m : tiles(p.m, p.experts);
+    if (rows > 64 && tiles_fit<kMode>(p) && tiles(p.m, 128) * tiles(p.n, 256) > 128) return launch_tiles<kMode, kGated>(p, stream, why);
     if (rows <= 16) return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
     return launch_direct<kMode, kGated, 4, 4>(p, stream, why);
 }
