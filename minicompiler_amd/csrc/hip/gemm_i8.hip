@@ -2,6 +2,8 @@
 // 32-bit sums, scaled by row and column, with bias and activation; and the
 // experts' products on a plan, the same for each expert's slots.
 
+#include <type_traits>
+
 #include "gemm_i8_tiles.h"
 
 namespace {
@@ -199,17 +201,18 @@ __device__ __forceinline__ long long a_row_of(const Product& p, long long row) {
 // bytes of row r lies at c ^ (r % 16).
 template <int kMode, bool kGated, int kOut, int kRowFrags>
 __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Product& p,
-                                           const i32x4 (&acc)[kRowFrags][kColFrags], int expert, long long row0,
+                                           const i32x16 (&acc)[kRowFrags][kColFrags], int expert, long long row0,
                                            long long end, int col0, int lane) {
-    constexpr int kPasses = kGated ? kRowFrags / 4 : 2, kRowBytes = kGated ? 512 : 256;
-    constexpr int kPassRows = kGated ? 64 : 16 * kRowFrags;
-    const int r = lane % 16, q = lane / 16;
+    constexpr int kPasses = kGated ? kRowFrags / 2 : 2, kRowBytes = kGated ? 512 : 256;
+    constexpr int kHalves = kRowFrags / 2;  // of 64 rows
+    constexpr int kPassRows = kGated ? 64 : 64 * kHalves;
     const long long b_row = static_cast<long long>(expert) * (kGated ? 2 * p.n : p.n);
+    const int line = lane % 32, half = lane / 32;
     // What goes with rows lane and lane + 64.
-    float sa[kRowFrags / 4], gate[kRowFrags / 4];
-    int c_rows[kRowFrags / 4];  // from row0 (Down: from 0) on, -1: not stored
+    float sa[kHalves], gate[kHalves];
+    int c_rows[kHalves];  // from row0 (Down: from 0) on, -1: not stored
 #pragma unroll
-    for (int h = 0; h < kRowFrags / 4; ++h) {
+    for (int h = 0; h < kHalves; ++h) {
         const long long row = row0 + lane + 64 * h;
         sa[h] = 0.0f, gate[h] = 1.0f, c_rows[h] = -1;
         if (row < end) {
@@ -225,53 +228,76 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
     const auto of_row = [&](auto value, int row) {
         return __builtin_bit_cast(decltype(value), __builtin_amdgcn_ds_bpermute(row % 64 * 4, __builtin_bit_cast(int, value)));
     };
+    const auto to_lds = [&](auto pass) {
+        constexpr int h = decltype(pass)::value;
 #pragma unroll
-    for (int h = 0; h < kPasses; ++h) {
-        constexpr int kFirst = kGated ? 4 : kRowFrags;
+        for (int i = 0; i < (kGated ? 2 : kRowFrags); ++i)
 #pragma unroll
-        for (int i = 0; i < kFirst; ++i)
+            for (int f = 0; f < (kGated ? kColFrags : 2); ++f) {
+                const i32x16& sums = kGated ? acc[2 * h % kRowFrags + i][f] : acc[i][2 * h + f];
 #pragma unroll
-            for (int f = 0; f < (kGated ? 8 : 4); ++f)
-                *reinterpret_cast<MX4_LDS i32x4*>(lds + (16 * i + r) * kRowBytes + ((4 * f + q) ^ r) * 16) =
-                    kGated ? acc[4 * h + i][f] : acc[i][4 * h + f];
-        const int col = col0 + (kGated ? 0 : 64 * h) + 4 * r, left = p.n - col;
-        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        const f32x4 scale = load_four<kF32>(p.b_scales, b_row + col, left);
-        const f32x4 bias = p.bias != nullptr ? load_four<kF32>(p.bias, b_row + col, left) : zero;
-        f32x4 up_scale = zero, up_bias = zero;
-        if constexpr (kGated) {
-            up_scale = load_four<kF32>(p.b_scales, b_row + p.n + col, left);
-            if (p.bias != nullptr) up_bias = load_four<kF32>(p.bias, b_row + p.n + col, left);
-        }
-#pragma unroll 2
-        for (int four = 0; four < kPassRows / 4; ++four) {
-            const int row = 4 * four + q;
-            const MX4_LDS unsigned char* at = lds + row * kRowBytes;
-            const i32x4 sum = *reinterpret_cast<const MX4_LDS i32x4*>(at + (r ^ row % 16) * 16);
-            const int part = kGated ? h : four / 16;
-            const float s = of_row(kRowFrags / 4 == 1 || part == 0 ? sa[0] : sa[kRowFrags / 4 - 1], row);
-            const int c_row = of_row(kRowFrags / 4 == 1 || part == 0 ? c_rows[0] : c_rows[kRowFrags / 4 - 1], row);
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(sum[e]) * s * scale[e] + bias[e];
-            if constexpr (kGated) {
-                const i32x4 other = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((16 + r) ^ row % 16) * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = v[e] * sigmoid(v[e]) * (static_cast<float>(other[e]) * s * up_scale[e] + up_bias[e]);
-            } else if constexpr (kMode == kDown) {
-                const float g = of_row(kRowFrags / 4 == 1 || part == 0 ? gate[0] : gate[kRowFrags / 4 - 1], row);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= g;
-            } else if (p.activation == MCHIP_ACT_RELU) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = activate(v[e], MCHIP_ACT_RELU);
-            } else if (p.activation == MCHIP_ACT_GELU) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = gelu(v[e]);
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<MX4_LDS i32x4*>(lds + (32 * i + line) * kRowBytes +
+                                                      ((8 * f + 2 * g + half) ^ line % 16) * 16) =
+                        i32x4{sums[4 * g], sums[4 * g + 1], sums[4 * g + 2], sums[4 * g + 3]};
             }
-            if (c_row >= 0 && left > 0)
-                store_four<kOut>(p.c, ((kMode == kDown ? 0 : row0) + c_row) * p.n + col, v, left);
+    };
+    // Columns 8 c .. + 7 of the wave's row: blocks 2 c and 2 c + 1 (the up ones 16 further on).
+    const auto sums_of = [&](int row, int block, int (&sum)[8]) {
+        const MX4_LDS unsigned char* at = lds + row * kRowBytes;
+        const i32x4 lo = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((block + lane % 8 * 2) ^ row % 16) * 16);
+        const i32x4 hi = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((block + lane % 8 * 2 + 1) ^ row % 16) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = lo[e], sum[4 + e] = hi[e];
+    };
+#pragma unroll 1
+    for (int h = 0; h < kPasses; ++h) {
+        if (h == 0) to_lds(std::integral_constant<int, 0>{});
+        else to_lds(std::integral_constant<int, 1>{});
+        // Eight columns of a row per lane, eight rows at a time, two of which are under way.
+        const int col = col0 + (kGated ? 0 : 64 * h) + lane % 8 * 8, left = p.n - col;
+        float scale[8], bias[8], up_scale[8], up_bias[8];
+        load_eight<kF32>(p.b_scales, b_row + col, left, scale);
+        load_eight<kF32>(p.bias, b_row + col, p.bias != nullptr ? left : 0, bias);
+        if constexpr (kGated) {
+            load_eight<kF32>(p.b_scales, b_row + p.n + col, left, up_scale);
+            load_eight<kF32>(p.bias, b_row + p.n + col, p.bias != nullptr ? left : 0, up_bias);
+        }
+#pragma unroll 1
+        for (int it = 0; it < kPassRows / 8; it += 2) {
+            const int part = kGated ? h : it / 8;
+            int sum[2][8], up[2][8], c_row[2];
+            float s[2], g[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int row = 8 * (it + u) + lane / 8;
+                sums_of(row, 0, sum[u]);
+                if constexpr (kGated) sums_of(row, 16, up[u]);
+                s[u] = of_row(kHalves == 1 || part == 0 ? sa[0] : sa[kHalves - 1], row);
+                c_row[u] = of_row(kHalves == 1 || part == 0 ? c_rows[0] : c_rows[kHalves - 1], row);
+                if constexpr (kMode == kDown) g[u] = of_row(kHalves == 1 || part == 0 ? gate[0] : gate[kHalves - 1], row);
+            }
+            float v[2][8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[u][e] = static_cast<float>(sum[u][e]) * s[u] * scale[e] + bias[e];
+                    if constexpr (kGated)
+                        v[u][e] *= sigmoid(v[u][e]) * (static_cast<float>(up[u][e]) * s[u] * up_scale[e] + up_bias[e]);
+                    if constexpr (kMode == kDown) v[u][e] *= g[u];
+                }
+            if (!kGated && kMode != kDown && p.activation == MCHIP_ACT_RELU) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e / 8][e % 8] = activate(v[e / 8][e % 8], MCHIP_ACT_RELU);
+            } else if (!kGated && kMode != kDown && p.activation == MCHIP_ACT_GELU) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e / 8][e % 8] = gelu(v[e / 8][e % 8]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (c_row[u] >= 0 && left > 0)
+                    store_eight<kOut>(p.c, ((kMode == kDown ? 0 : row0) + c_row[u]) * p.n + col, v[u], left);
         }
     }
 }
@@ -285,9 +311,8 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
     // A's rows, from the wave's share of the tile on, or (gathered) all.
     const long long a0 = kMode == kUp ? 0 : row0 + wave * kShare;
     const long long a_left = kMode == kUp ? 0 : end - a0;
-    const __amdgpu_buffer_rsrc_t a =
-        kMode == kUp ? __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a), 0, p.a_rows * p.row_bytes, 0x00020000)
-                     : rsrc_of(p.a + a0 * p.row_bytes, a_left, p.row_bytes);
+    const __amdgpu_buffer_rsrc_t a = kMode == kUp ? resource(p.a, p.a_rows * p.row_bytes)
+                                                  : rows_from(p.a + a0 * p.row_bytes, a_left, p.row_bytes);
     const auto a_row = [&](int i) {
         const int in_share = i * 8 + lane / 8;
         if constexpr (kMode != kUp) return in_share * p.row_bytes;
@@ -297,8 +322,8 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
     // B's rows that the wave fetches: 64 of columns, of gate or of up ones.
     const int b_col = col0 + (kGated ? wave / 2 * 64 : wave * 64), b_rows = kGated ? 2 * p.n : p.n;
     const long long b0 = static_cast<long long>(expert) * b_rows + (kGated ? wave % 2 * static_cast<long long>(p.n) : 0) + b_col;
-    const __amdgpu_buffer_rsrc_t b = rsrc_of(p.b + b0 * p.row_bytes, p.n - b_col, p.row_bytes);
-    i32x4 acc[kRows / 32][kColFrags];
+    const __amdgpu_buffer_rsrc_t b = rows_from(p.b + b0 * p.row_bytes, p.n - b_col, p.row_bytes);
+    i32x16 acc[kRows / 64][kColFrags];
     tile_sums<kRows>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
     lds_barrier();  // every wave is past its reads of the ring
     store_tile<kMode, kGated, kOut>(lds + wave * (kRingBytes / 4), p, acc, expert, row0 + wave / 2 * (kRows / 2), end,

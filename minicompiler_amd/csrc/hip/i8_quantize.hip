@@ -71,28 +71,6 @@ __device__ __forceinline__ u32x2 codes_of(float (&v)[8], const Scale& c) {
     return u32x2{pack(n[0], n[1], n[2], n[3]), pack(n[4], n[5], n[6], n[7])};
 }
 
-// Values past the caches: the codes are what is read next.
-template <int kType>
-__device__ __forceinline__ void store_eight(void* p, long long at, const float (&v)[8], int left) {
-    if (left >= 8) {
-        if constexpr (kType == kF32) {
-            f32x4_loose* d = reinterpret_cast<f32x4_loose*>(static_cast<float*>(p) + at);
-            const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
-            __builtin_nontemporal_store(lo, d);
-            __builtin_nontemporal_store(hi, d + 1);
-        } else {
-            u16x8 h;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = to_16<kType>(v[e]);
-            __builtin_nontemporal_store(h, reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(p) + at));
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < left) store_one<kType>(p, at + e, v[e]);
-}
-
 // The largest of a row over its kLanes lanes (a wave, or a block of waves).
 template <int kLanes>
 __device__ __forceinline__ unsigned row_max(unsigned top, unsigned* space) {
@@ -106,6 +84,7 @@ __device__ __forceinline__ unsigned row_max(unsigned top, unsigned* space) {
     return top;
 }
 
+// Values go past the caches: the codes are what is read next.
 // kLanes lanes take a row, each kPer chunks of eight elements, which stay in registers
 // between the row's largest magnitude and the codes; a block of 256 lanes takes four
 // rows of one wave each.
