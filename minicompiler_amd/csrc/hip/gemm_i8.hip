@@ -186,6 +186,8 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
     }
 }
 
+constexpr int kPanel = 4;
+
 // The row of A that row `row` of C takes.
 template <int kMode>
 __device__ __forceinline__ long long a_row_of(const Product& p, long long row) {
@@ -254,7 +256,7 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
     for (int h = 0; h < kPasses; ++h) {
         if (h == 0) to_lds(std::integral_constant<int, 0>{});
         else to_lds(std::integral_constant<int, 1>{});
-        // Eight columns of a row per lane, eight rows at a time, two of which are under way.
+        // Eight columns of a row per lane, eight rows at a time, four of which are under way.
         const int col = col0 + (kGated ? 0 : 64 * h) + lane % 8 * 8, left = p.n - col;
         float scale[8], bias[8], up_scale[8], up_bias[8];
         load_eight<kF32>(p.b_scales, b_row + col, left, scale);
@@ -263,41 +265,72 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
             load_eight<kF32>(p.b_scales, b_row + p.n + col, left, up_scale);
             load_eight<kF32>(p.bias, b_row + p.n + col, p.bias != nullptr ? left : 0, up_bias);
         }
+        const auto rows = [&](auto act, auto store) {
 #pragma unroll 1
-        for (int it = 0; it < kPassRows / 8; it += 2) {
-            const int part = kGated ? h : it / 8;
-            int sum[2][8], up[2][8], c_row[2];
-            float s[2], g[2];
+            for (int it = 0; it < kPassRows / 8; it += 4) {
+                const int part = kGated ? h : it / 8;
+                const float sa_here = kHalves == 1 || part == 0 ? sa[0] : sa[kHalves - 1];
+                const float gate_here = kHalves == 1 || part == 0 ? gate[0] : gate[kHalves - 1];
+                int sum[4][8], up[4][8];
+                float s[4], g[4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int row = 8 * (it + u) + lane / 8;
-                sums_of(row, 0, sum[u]);
-                if constexpr (kGated) sums_of(row, 16, up[u]);
-                s[u] = of_row(kHalves == 1 || part == 0 ? sa[0] : sa[kHalves - 1], row);
-                c_row[u] = of_row(kHalves == 1 || part == 0 ? c_rows[0] : c_rows[kHalves - 1], row);
-                if constexpr (kMode == kDown) g[u] = of_row(kHalves == 1 || part == 0 ? gate[0] : gate[kHalves - 1], row);
-            }
-            float v[2][8];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[u][e] = static_cast<float>(sum[u][e]) * s[u] * scale[e] + bias[e];
-                    if constexpr (kGated)
-                        v[u][e] *= sigmoid(v[u][e]) * (static_cast<float>(up[u][e]) * s[u] * up_scale[e] + up_bias[e]);
-                    if constexpr (kMode == kDown) v[u][e] *= g[u];
+                for (int u = 0; u < 4; ++u) {
+                    const int row = 8 * (it + u) + lane / 8;
+                    s[u] = of_row(sa_here, row);
+                    if constexpr (kMode == kDown) g[u] = of_row(gate_here, row);
+                    sums_of(row, 0, sum[u]);
+                    if constexpr (kGated) sums_of(row, 16, up[u]);
                 }
-            if (!kGated && kMode != kDown && p.activation == MCHIP_ACT_RELU) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e / 8][e % 8] = activate(v[e / 8][e % 8], MCHIP_ACT_RELU);
-            } else if (!kGated && kMode != kDown && p.activation == MCHIP_ACT_GELU) {
+                for (int u = 0; u < 4; ++u) {
+                    float v[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e / 8][e % 8] = gelu(v[e / 8][e % 8]);
+                    for (int e = 0; e < 8; ++e) {
+                        v[e] = static_cast<float>(sum[u][e]) * s[u] * scale[e] + bias[e];
+                        if constexpr (kGated)
+                            v[e] *= sigmoid(v[e]) * (static_cast<float>(up[u][e]) * s[u] * up_scale[e] + up_bias[e]);
+                        else if constexpr (kMode == kDown)
+                            v[e] *= g[u];
+                        else
+                            v[e] = act(v[e]);
+                    }
+                    store(it + u, part, v);
+                }
             }
+        };
+        const auto with_act = [&](auto store) {
+            if (kGated || kMode == kDown || p.activation == MCHIP_ACT_NONE) rows([](float u) { return u; }, store);
+            else if (p.activation == MCHIP_ACT_RELU) rows([](float u) { return activate(u, MCHIP_ACT_RELU); }, store);
+            else rows([](float u) { return gelu(u); }, store);
+        };
+        // Rows of whole eights go out through a resource of the wave's rows of C: no
+        // addresses to work out, and what lies past the last row or column is dropped.
+        constexpr int kOne = kSize<kOut>;
+        const long long row_size = static_cast<long long>(p.n) * kOne;
+        if (kMode != kDown && p.n % 8 == 0 && row_size * 16 * 16 < (1LL << 31)) {
+            const __amdgpu_buffer_rsrc_t c = rows_from(static_cast<unsigned char*>(p.c) + row0 * row_size, end - row0,
+                                                       static_cast<int>(row_size));
+            const int step = __builtin_amdgcn_readfirstlane(8 * static_cast<int>(row_size));
+            const unsigned at = left > 0 ? static_cast<unsigned>(lane / 8 * static_cast<int>(row_size) + col * kOne) : 1u << 31;
+            with_act([&](int it, int, const float(&v)[8]) {
+                const int from = static_cast<int>(at + static_cast<unsigned>((it + (kGated ? h * 8 : 0)) * step));
+                if constexpr (kOut == kF32) {
+                    const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), c, from, 0, 2);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), c, from + 16, 0, 2);
+                } else {
+                    u16x8 out;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (c_row[u] >= 0 && left > 0)
-                    store_eight<kOut>(p.c, ((kMode == kDown ? 0 : row0) + c_row[u]) * p.n + col, v[u], left);
+                    for (int e = 0; e < 8; ++e) out[e] = to_16<kOut>(v[e]);
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, out), c, from, 0, 2);
+                }
+            });
+        } else {
+            with_act([&](int it, int part, const float(&v)[8]) {
+                const int c_row = of_row(kHalves == 1 || part == 0 ? c_rows[0] : c_rows[kHalves - 1], 8 * it + lane / 8);
+                if (c_row >= 0 && left > 0)
+                    store_eight<kOut>(p.c, ((kMode == kDown ? 0 : row0) + c_row) * p.n + col, v, left);
+            });
         }
     }
 }
@@ -330,18 +363,31 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
                                     col0 + wave % 2 * (kGated ? 64 : 128), lane);
 }
 
-// Dense: tiles in row-major order; the grid has one block per tile of 256 rows plus
-// `halves` more, for which that many of the last tiles run as two blocks of 128 rows.
+// Dense: tiles in panels of kPanel rows of them, column after column; the grid has one
+// block per tile of 256 rows plus `halves` more, for which that many of the last tiles
+// run as two blocks of 128 rows. An XCD takes consecutive ones, so that the 32 which it
+// works on at a time read 4 + 8 tiles' rows through its L2.
 // On a plan: an expert's slots in tiles of 256, its last of 128 where that holds it.
 template <int kMode, bool kGated, int kOut>
 __global__ __launch_bounds__(kTileThreads, 1) void i8_tiles(const Product p, unsigned full) {
     __shared__ __attribute__((aligned(1024))) unsigned char smem[kRingBytes];
     MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);  // generic -> LDS address space
-    unsigned t = blockIdx.x;
+    unsigned t = blockIdx.x, chunk, tile;
     int half = 0;
-    if (kMode == kDense && t >= full) half = 1 + static_cast<int>((t - full) % 2), t = full + (t - full) / 2;
-    const unsigned chunk = t / p.tiles_n;
-    const int col0 = static_cast<int>(t % p.tiles_n) * (kGated ? kTileCols / 2 : kTileCols);
+    if constexpr (kMode == kDense) {
+        if (t >= full) {
+            half = 1 + static_cast<int>((t - full) % 2), t = full + (t - full) / 2;
+        } else if (t < full / 8 * 8) {
+            t = t % 8 * (full / 8) + t / 8;  // blocks go to the XCDs in turn
+        }
+        const unsigned all = static_cast<unsigned>((p.m + kTileRows - 1) / kTileRows);
+        const unsigned panel = t / (kPanel * p.tiles_n), in = t % (kPanel * p.tiles_n);
+        const unsigned high = min(static_cast<unsigned>(kPanel), all - panel * kPanel);
+        chunk = panel * kPanel + in % high, tile = in / high;
+    } else {
+        chunk = t / p.tiles_n, tile = t % p.tiles_n;
+    }
+    const int col0 = static_cast<int>(tile) * (kGated ? kTileCols / 2 : kTileCols);
     long long row0 = static_cast<long long>(chunk) * kTileRows, end = p.m;
     int expert = 0;
     if constexpr (kMode == kDense) {

@@ -57,20 +57,20 @@ struct TileLane {
     static constexpr int kFetchB = 8;
     __amdgpu_buffer_rsrc_t a, b;  // A's rows (this wave's share of the tile, or all of A), this wave's share of B's
     int a_src[kFetchA];           // the lane's offset in each fetch of A
-    int b_src[2];                 // ... in a fetch of B's rows 16 j .. + 7 and 16 j + 8 .. + 15
+    int b_src[kFetchB];           // ... of B
     int a_off[4], b_off[4];       // LDS offsets of the wave's first fragments in each step
-    int row_bytes, wave, lane;
+    int wave;
 };
 
-// Instruction i of this wave's share of stage s (A's first).
+// Instruction i of this wave's share of stage s (A's first). Rows are in the lane's
+// offset, which is held against the resource's end; the scalar one stays within a row.
 template <int kRows>
 __device__ __forceinline__ void fetch_one(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int s, int i) {
     constexpr int kA = TileLane<kRows>::kFetchA, kB = TileLane<kRows>::kFetchB;
     if (i < kA)
         buffer_to_lds(L.a, wr + (L.wave * kA + i) * 1024, L.a_src[i < kA ? i : 0], s * kLine);
     else
-        buffer_to_lds(L.b, wr + kStageB + (L.wave * kB + i - kA) * 1024, L.b_src[(i - kA) & 1],
-                      (i - kA) * 8 * L.row_bytes + s * kLine);
+        buffer_to_lds(L.b, wr + kStageB + (L.wave * kB + i - kA) * 1024, L.b_src[i < kA ? 0 : i - kA], s * kLine);
 }
 
 // One fragment of step u of the stage at `rd`. What is read is not being written;
@@ -110,12 +110,13 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
     const int r = lane % 32, h = lane / 32;
     Lane L;
     L.a = a, L.b = b;
-    L.wave = wave, L.lane = lane, L.row_bytes = row_bytes;
+    L.wave = wave;
     // The block that the lane's place in LDS takes, of row lane / 8 of a fetch.
 #pragma unroll
     for (int i = 0; i < Lane::kFetchA; ++i) L.a_src[i] = a_row(i) + (lane % 8 ^ (4 * (i & 1) + lane / 16)) * 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) L.b_src[i] = lane / 8 * row_bytes + (lane % 8 ^ (4 * i + lane / 16)) * 16;
+    for (int i = 0; i < Lane::kFetchB; ++i)
+        L.b_src[i] = (8 * i + lane / 8) * row_bytes + (lane % 8 ^ (4 * (i & 1) + lane / 16)) * 16;
     const int wave_row = wave / 2 * (kRows / 2), wave_col = wave % 2 * 128;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {

@@ -26,8 +26,9 @@ __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// x sigmoid(x), and GELU in its tanh form, u (1 + tanh(z)) / 2 = u sigmoid(2 z).
-__device__ __forceinline__ float sigmoid(float u) { return 1.0f / (1.0f + __expf(-u)); }
+// GELU in its tanh form is u (1 + tanh(z)) / 2 = u sigmoid(2 z). The reciprocal is good
+// to a unit in the last place; a division would be ten instructions.
+__device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.0f + __expf(-u)); }
 __device__ __forceinline__ float gelu(float u) {
     return u * sigmoid(1.5957691216057308f * (u + 0.044715f * u * u * u));
 }
