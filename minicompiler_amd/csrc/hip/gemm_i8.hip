@@ -31,18 +31,23 @@ struct Place {
     int expert, first, end;
 };
 
-// Job `want` of the experts' slots, up to kRows of one expert's each; end = first: none.
-// A wave looks at 64 experts at a time.
-template <int kRows>
-__device__ __forceinline__ Place find_job(const Product& p, unsigned want) {
+// Entry `want` of what count(slots of an expert) adds up to over the experts in order: the
+// expert and the entry's number there, or no expert, `want` less the sum of all. A wave
+// looks at 64 experts at a time.
+struct Entry {
+    int expert, from, to;  // the expert's slots
+    unsigned number;
+};
+template <typename Count>
+__device__ __forceinline__ bool find_entry(const Product& p, unsigned& want, Entry& found, Count count) {
     const int lane = threadIdx.x % 64;
     for (int base = 0; base < p.experts; base += 64) {
         const int e = base + lane;
         int from = 0, to = 0;
         if (e < p.experts) from = p.offsets[e], to = p.offsets[e + 1];
-        from = max(from, 0), to = min(to, p.m);
-        const unsigned jobs = to > from ? static_cast<unsigned>(to - from + kRows - 1) / kRows : 0u;
-        unsigned up_to = jobs;  // of the lanes up to this one
+        from = max(from, 0), to = max(min(to, p.m), from);
+        const unsigned mine = count(static_cast<unsigned>(to - from));
+        unsigned up_to = mine;  // of the lanes up to this one
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
             const unsigned o = __shfl_up(up_to, d);
@@ -51,12 +56,35 @@ __device__ __forceinline__ Place find_job(const Product& p, unsigned want) {
         const unsigned long long here = __ballot(up_to > want);
         if (here != 0) {
             const int at = __builtin_ctzll(here);
-            const unsigned before = __builtin_amdgcn_readlane(up_to - jobs, at);
-            const int first = __builtin_amdgcn_readlane(from, at) + static_cast<int>((want - before) * kRows);
-            return {base + at, first, __builtin_amdgcn_readlane(to, at)};
+            found = {base + at, static_cast<int>(__builtin_amdgcn_readlane(from, at)),
+                     static_cast<int>(__builtin_amdgcn_readlane(to, at)),
+                     want - __builtin_amdgcn_readlane(up_to - mine, at)};
+            return true;
         }
         want -= __builtin_amdgcn_readlane(up_to, 63);
     }
+    return false;
+}
+
+// Job `want` of the experts' slots, up to kRows of one expert's each; end = first: none.
+template <int kRows>
+__device__ __forceinline__ Place find_job(const Product& p, unsigned want) {
+    Entry e;
+    if (!find_entry(p, want, e, [](unsigned n) { return (n + kRows - 1) / kRows; })) return {0, 0, 0};
+    return {e.expert, e.from + static_cast<int>(e.number * kRows), e.to};
+}
+
+// The same in tiles of kRows, an expert's last of half as many rows where that holds it.
+// Those come after all others, so that the launch ends on short work.
+template <int kRows>
+__device__ __forceinline__ Place find_tile(const Product& p, unsigned want) {
+    Entry e;
+    if (find_entry(p, want, e, [](unsigned n) { return (n + kRows / 2 - 1) / kRows; })) {
+        const int first = e.from + static_cast<int>(e.number * kRows);
+        return {e.expert, first, min(first + kRows, e.to)};
+    }
+    if (find_entry(p, want, e, [](unsigned n) { return (n + kRows / 2 - 1) / kRows * kRows < n ? 1u : 0u; }))
+        return {e.expert, e.to - (e.to - e.from) % kRows, e.to};
     return {0, 0, 0};
 }
 
@@ -359,7 +387,7 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
     i32x16 acc[kRows / 64][kColFrags];
     tile_sums<kRows>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
     lds_barrier();  // every wave is past its reads of the ring
-    store_tile<kMode, kGated, kOut>(lds + wave * (kRingBytes / 4), p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
+    store_tile<kMode, kGated, kOut>(lds + wave * (32 * 1024), p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
                                     col0 + wave % 2 * (kGated ? 64 : 128), lane);
 }
 
@@ -394,7 +422,7 @@ __global__ __launch_bounds__(kTileThreads, 1) void i8_tiles(const Product p, uns
         if (half == 2) row0 += kTileRows / 2;
         if (half == 1 && row0 + kTileRows / 2 < end) end = row0 + kTileRows / 2;
     } else {
-        const Place place = find_job<kTileRows>(p, chunk);
+        const Place place = find_tile<kTileRows>(p, chunk);
         expert = place.expert, row0 = place.first, end = place.end;
     }
     if (row0 >= end) return;

@@ -7,15 +7,17 @@
 // loop of the instruction alone runs at 4.95 POP/s on zeros and 3.40 on random bytes,
 // where the chip lowers its clock; the 16x16x64 instruction at 2.91 and 2.71.)
 //
-// K goes in stages of 128 through two 64 KiB LDS buffers, each stage as four steps
-// of 32 and 16 products. While a step's products issue, the next step's fragments
-// are read from LDS into the other of two sets of registers. Before a stage's last
-// step a barrier: every wave has read all of stage s and its own share of stage
-// s + 1 has landed, so after it stage s + 2 is fetched over stage s, and stage s + 1
-// is read. In the last two stages the fetches repeat the last stage.
+// K goes in stages of 128 through two 32 KiB buffers of LDS for A and three for B (all
+// of LDS), each stage as four steps of 32 and 16 products. While a step's products
+// issue, the next step's fragments are read from LDS into the other of two sets of
+// registers. Before a stage's last step a barrier: every wave has read all of stage s
+// and its own share of stage s + 1 has landed, so after it A's stage s + 2 and B's
+// stage s + 3 are fetched over stage s, and stage s + 1 is read. (B, the weights, comes
+// from further away than A, whose rows all columns' tiles share.) In the last stages the
+// fetches repeat the last stage.
 //
-// LDS layout of a stage: rows of 128 bytes, A's 256 at 0 and B's at 32 KiB; block c
-// of 16 bytes of row r lies at 128 r + 16 (c ^ (r / 2 % 8)). A fetch instruction
+// LDS layout of a stage: 256 rows of 128 bytes; block c of 16 bytes of row r lies at
+// 128 r + 16 (c ^ (r / 2 % 8)). A fetch instruction
 // fills 8 rows, eight neighbouring lanes one row. A fragment read, lane (r, h) of 32
 // rows and two blocks, touches every bank once per 16 lanes that the LDS serves
 // together (lanes 0-3, 12-15 and 20-27 the first).
@@ -29,8 +31,9 @@
 namespace i8 {
 
 constexpr int kTileRows = 256, kTileCols = 256, kTileThreads = 256;
-constexpr int kStageBytes = 64 * 1024, kStageB = 32 * 1024;
-constexpr int kRingBytes = 2 * kStageBytes;
+constexpr int kStageBytes = 32 * 1024;  // of either operand
+constexpr int kRingA = 2, kRingB = 3, kFirstB = kRingA * kStageBytes;
+constexpr int kRingBytes = (kRingA + kRingB) * kStageBytes;
 constexpr int kColFrags = 4;
 
 // `bytes` bytes from p on, the same in every lane, which the compiler has to be told
@@ -62,15 +65,16 @@ struct TileLane {
     int wave;
 };
 
-// Instruction i of this wave's share of stage s (A's first). Rows are in the lane's
-// offset, which is held against the resource's end; the scalar one stays within a row.
+// Instruction i of this wave's share of a stage of A to `wr`, `at` bytes into the rows.
+// Rows are in the lane's offset, which is held against the resource's end; the scalar
+// one stays within a row.
 template <int kRows>
-__device__ __forceinline__ void fetch_one(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int s, int i) {
-    constexpr int kA = TileLane<kRows>::kFetchA, kB = TileLane<kRows>::kFetchB;
-    if (i < kA)
-        buffer_to_lds(L.a, wr + (L.wave * kA + i) * 1024, L.a_src[i < kA ? i : 0], s * kLine);
-    else
-        buffer_to_lds(L.b, wr + kStageB + (L.wave * kB + i - kA) * 1024, L.b_src[i < kA ? 0 : i - kA], s * kLine);
+__device__ __forceinline__ void fetch_a(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int at, int i) {
+    buffer_to_lds(L.a, wr + (L.wave * TileLane<kRows>::kFetchA + i) * 1024, L.a_src[i], at);
+}
+template <int kRows>
+__device__ __forceinline__ void fetch_b(MX4_LDS unsigned char* wr, const TileLane<kRows>& L, int at, int i) {
+    buffer_to_lds(L.b, wr + (L.wave * TileLane<kRows>::kFetchB + i) * 1024, L.b_src[i], at);
 }
 
 // One fragment of step u of the stage at `rd`. What is read is not being written;
@@ -83,7 +87,7 @@ __device__ __forceinline__ i32x4 read_a(const MX4_LDS unsigned char* __restrict_
 template <int kRows>
 __device__ __forceinline__ i32x4 read_b(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<kRows>& L, int u,
                                         int f) {
-    return *reinterpret_cast<const MX4_LDS i32x4*>(rd + kStageB + L.b_off[u] + f * 4096);
+    return *reinterpret_cast<const MX4_LDS i32x4*>(rd + L.b_off[u] + f * 4096);
 }
 
 // acc += a b in acc's own registers, written out because the compiler, with the
@@ -91,6 +95,13 @@ __device__ __forceinline__ i32x4 read_b(const MX4_LDS unsigned char* __restrict_
 // know that a value is there only after the instruction's passes (settle()).
 __device__ __forceinline__ void mfma_in_place(i32x16& acc, i32x4 a, i32x4 b) {
     asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+// Until all but the last kCount loads have landed, and all reads of LDS.
+template <int kCount>
+__device__ __forceinline__ void wait_for_all_but() {
+    static_assert(kCount < 64);
+    __builtin_amdgcn_s_waitcnt((kCount & 15) | (kCount >> 4) << 14 | 7 << 4);
 }
 
 // Between the last product and the first use of its value: its passes are over.
@@ -123,15 +134,27 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
         L.a_off[t] = (wave_row + r) * 128 + ((2 * t + h) ^ r / 2 % 8) * 16;
         L.b_off[t] = (wave_col + r) * 128 + ((2 * t + h) ^ r / 2 % 8) * 16;
     }
-    const auto stage = [&](int s) { return lds + (s & 1) * kStageBytes; };
-    const int stages = row_bytes / kLine;
+    const int stages = row_bytes / kLine, end = row_bytes - kLine;
+    const auto slot_a = [&](int s) { return lds + (s & 1) * kStageBytes; };
+    // B's buffers in turn: of stage s, s + 1 and s + 2.
+    MX4_LDS unsigned char *b_here = lds + kFirstB, *b_next = b_here + kStageBytes, *b_last = b_next + kStageBytes;
+    const auto offset_of = [&](int s) { return s < stages ? s * kLine : end; };
 
-    constexpr int kI = Lane::kRowFrags, kAll = Lane::kFetchA + Lane::kFetchB, kEarly = kAll / 2;
+    // What is fetched in a stage's time, A's before B's, half of it after the barrier and
+    // half in the next stage's first step.
+    constexpr int kI = Lane::kRowFrags, kA = Lane::kFetchA, kAll = kA + Lane::kFetchB, kEarly = kAll / 2;
     constexpr int kSlots = kI * kColFrags;
 #pragma unroll
-    for (int i = 0; i < kAll; ++i) fetch_one<kRows>(stage(0), L, 0, i);
+    for (int i = 0; i < kA; ++i) fetch_a<kRows>(slot_a(0), L, 0, i);
 #pragma unroll
-    for (int i = 0; i < kEarly; ++i) fetch_one<kRows>(stage(1), L, stages > 1 ? 1 : 0, i);
+    for (int i = 0; i < Lane::kFetchB; ++i) fetch_b<kRows>(b_here, L, 0, i);
+#pragma unroll
+    for (int i = 0; i < Lane::kFetchB; ++i) fetch_b<kRows>(b_next, L, offset_of(1), i);
+#pragma unroll
+    for (int i = 0; i < kEarly; ++i) {
+        if (i < kA) fetch_a<kRows>(slot_a(1), L, offset_of(1), i < kA ? i : 0);
+        else fetch_b<kRows>(b_last, L, offset_of(2), i - kA);
+    }
 #pragma unroll
     for (int i = 0; i < kI; ++i)
 #pragma unroll
@@ -140,12 +163,12 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
             for (int e = 0; e < 16; ++e) acc[i][f][e] = 0;
             asm volatile("" : "+a"(acc[i][f]));  // cleared here, while the fetch is under way
         }
-    __builtin_amdgcn_s_waitcnt(0);
+    wait_for_all_but<Lane::kFetchB + kEarly>();
     lds_barrier();
 
     i32x4 av[2][kI], bv[2][kColFrags];
 #pragma unroll
-    for (int f = 0; f < kColFrags; ++f) bv[0][f] = read_b<kRows>(lds, L, 0, f);
+    for (int f = 0; f < kColFrags; ++f) bv[0][f] = read_b<kRows>(b_here, L, 0, f);
 #pragma unroll
     for (int i = 0; i < kI; ++i) av[0][i] = read_a<kRows>(lds, L, 0, i);
 
@@ -154,12 +177,13 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
     // two steps: the address unit takes 16 cycles for an instruction, and a wave that
     // waits for it multiplies nothing.
     for (int s = 0; s < stages; ++s) {
-        const int rest = s + 1 < stages ? s + 1 : stages - 1, next = s + 2 < stages ? s + 2 : stages - 1;
+        const int a_next = offset_of(s + 1), a_after = offset_of(s + 2), b_after = offset_of(s + 3);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const MX4_LDS unsigned char* from = t < 3 ? stage(s) : stage(s + 1);
+            const MX4_LDS unsigned char *a_from = t < 3 ? slot_a(s) : slot_a(s + 1), *b_from = t < 3 ? b_here : b_next;
             if (t == 3) {
-                __builtin_amdgcn_s_waitcnt(0);
+                // All of stage s + 1; what may be missing is B's stage s + 2.
+                wait_for_all_but<Lane::kFetchB>();
                 lds_barrier();
             }
 #pragma unroll
@@ -167,19 +191,28 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
                 const int i = m / kColFrags, f = m % kColFrags;
                 mfma_in_place(acc[i][f], bv[t & 1][f], av[t & 1][i]);
                 if (m < kColFrags)
-                    bv[(t + 1) & 1][m < kColFrags ? m : 0] = read_b<kRows>(from, L, (t + 1) % 4, m);
+                    bv[(t + 1) & 1][m < kColFrags ? m : 0] = read_b<kRows>(b_from, L, (t + 1) % 4, m);
                 else if (m < kColFrags + kI)
-                    av[(t + 1) & 1][m < kColFrags + kI ? m - kColFrags : 0] = read_a<kRows>(from, L, (t + 1) % 4, m - kColFrags);
+                    av[(t + 1) & 1][m < kColFrags + kI ? m - kColFrags : 0] = read_a<kRows>(a_from, L, (t + 1) % 4, m - kColFrags);
                 // Fetch j of a step's lies behind product (j + 1) kSlots / kEarly - 1.
 #pragma unroll
                 for (int j = 0; j < kEarly; ++j)
                     if (m == (j + 1) * kSlots / kEarly - 1) {
-                        if (t == 0) fetch_one<kRows>(stage(s + 1), L, rest, kEarly + j);  // what is left of it
-                        if (t == 3) fetch_one<kRows>(stage(s), L, next, j);
+                        const int i0 = kEarly + j;
+                        if (t == 0) {
+                            if (i0 < kA) fetch_a<kRows>(slot_a(s + 1), L, a_next, i0 < kA ? i0 : 0);
+                            else fetch_b<kRows>(b_last, L, a_after, i0 - kA);
+                        }
+                        if (t == 3) {
+                            if (j < kA) fetch_a<kRows>(slot_a(s), L, a_after, j < kA ? j : 0);
+                            else fetch_b<kRows>(b_here, L, b_after, j - kA);
+                        }
                     }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        MX4_LDS unsigned char* const free = b_here;
+        b_here = b_next, b_next = b_last, b_last = free;
         // A product's operand may have been written two instructions before it at the latest.
         asm volatile("s_nop 1" ::: "memory");
     }
