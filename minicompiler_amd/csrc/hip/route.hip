@@ -1,8 +1,14 @@
 // The choice of experts: scores, groups, the top_k largest, their gates, and the
 // plan (pairs of token and place by expert) that the experts' products run on.
 //
-// Scores are in fp64: choices are compared with a bias added and in sums of two, and
-// two experts whose scores lie next to each other are then still in their order.
+// Keys are in fp64: they are compared with a bias added, or in sums of two, and two
+// experts whose scores lie next to each other are then still in their order.
+//
+// Bound by latency, and that by the code that a launch reads into a cold instruction
+// cache: sixteen lanes take a token, a lane 4 to 32 experts next to each other, keys lie
+// in LDS while loops go over them and in registers while the largest are picked, over
+// lanes by DPP. (A wave a token with LDS permutes: 8192 tokens of 256 experts in 35 us;
+// fp32 keys in unrolled code, with fp64 ones behind for what lies too near: 23.)
 
 #include "i8_device.h"
 
@@ -10,7 +16,8 @@ namespace {
 
 using namespace i8;
 
-constexpr int kWaves = 4;
+constexpr int kThreads = 512, kWaves = kThreads / 64, kTokens = kThreads / 16;  // of a block
+constexpr int kFewPairs = 128;  // of a plan that the choosing block makes itself
 constexpr double kNone = -__builtin_inf();
 
 struct Route {
@@ -21,181 +28,334 @@ struct Route {
     float scale;
     int* chosen;
     float* gates;
-    bool by_logit;  // one score by itself is as large as its logit
+    int *order, *offsets;
+    unsigned short* ids;  // of all pairs, for the plan's launch, or null
+    bool by_logit;        // one score by itself is as large as its logit
+    bool plans;           // the only block makes the plan, too
 };
 
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v = fmax(v, __shfl_xor(v, d));
-    return v;
-}
-__device__ __forceinline__ double wave_add(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
+// Place j of a token.
+__device__ __forceinline__ void put(const Route& p, unsigned short* few, long long token, int j, int expert, float gate) {
+    const long long at = token * p.top_k + j;
+    p.chosen[at] = expert;
+    p.gates[at] = gate;
+    if (p.plans) few[at] = static_cast<unsigned short>(expert);
+    if (p.ids != nullptr) p.ids[at] = static_cast<unsigned short>(expert);
 }
 
-// The largest key of the wave and the lowest place that has it.
-__device__ __forceinline__ void wave_first(double& key, int& at) {
+// Over the 16 lanes of a token: the two neighbours of a pair, of four, of eight, of all.
+template <int kCtrl>
+__device__ __forceinline__ double of_lane(double v) {
+    const u32x2 u = __builtin_bit_cast(u32x2, v);
+    u32x2 r;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double k = __shfl_xor(key, d);
-        const int a = __shfl_xor(at, d);
-        if (k > key || (k == key && a < at)) key = k, at = a;
+    for (int i = 0; i < 2; ++i)
+        r[i] = static_cast<unsigned>(
+            __builtin_amdgcn_update_dpp(static_cast<int>(u[i]), static_cast<int>(u[i]), kCtrl, 0xf, 0xf, false));
+    return __builtin_bit_cast(double, r);
+}
+template <typename Op>
+__device__ __forceinline__ double over_token(double v, Op op) {
+    v = op(v, of_lane<0xb1>(v));
+    v = op(v, of_lane<0x4e>(v));
+    v = op(v, of_lane<0x141>(v));
+    return op(v, of_lane<0x140>(v));
+}
+// Of a number and a NaN the number.
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ double both(double a, double b) { return a + b; }
+
+// The plan of few pairs by the block that chose them: pair i's slot is how many pairs come
+// before it, expert e's first how many have a lower one. `few` is padded with experts past
+// the last.
+__device__ __forceinline__ void plan_few(const Route& p, const unsigned short* few) {
+    const int pairs = p.tokens * p.top_k, i = threadIdx.x;
+    const int mine = i < pairs ? few[i] : 0;
+    int before = 0, below = 0;
+#pragma unroll 2
+    for (int j = 0; j < pairs; j += 8) {
+        const u16x8 eight = *reinterpret_cast<const u16x8*>(few + j);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int e = eight[u];
+            before += e < mine + (j + u < i);
+            below += e < i;
+        }
     }
+    if (i < pairs) p.order[before] = i;
+    if (i < p.experts) p.offsets[i] = below;
+    if (i == 0) p.offsets[p.experts] = pairs;
 }
 
-// A wave takes a token; lane l experts l, l + 64, ...
+// Sixteen lanes take a token, lane l experts l kPer .. + kPer - 1. An expert that may not
+// be chosen (it is none, is not in a group that stays, or has been chosen) has a NaN key.
 template <int kType, int kPer>
-__global__ __launch_bounds__(kWaves * 64) void route_tokens(const Route p) {
-    __shared__ double keys[kWaves][kPer * 64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const long long token = static_cast<long long>(blockIdx.x) * kWaves + wave;
-    if (token >= p.tokens) return;
-    double score[kPer], key[kPer];
-    bool bad = false;
-    double top = kNone;
+__global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
+    // Two spare words behind a lane's experts and a token's: lanes and groups meet in
+    // different banks.
+    constexpr int kLane = kPer + 2, kWords = 16 * kLane + 2;
+    __shared__ __attribute__((aligned(16))) double space[kTokens * kWords];
+    __shared__ float bias[kPer * 16];
+    __shared__ __attribute__((aligned(16))) unsigned short few[kFewPairs];
+    __shared__ int picked[kTokens][MCHIP_ROUTE_MAX_TOP_K];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l = lane % 16, row = lane / 16;
+    const long long token = (static_cast<long long>(blockIdx.x) * kWaves + wave) * 4 + row;
+    const bool has = token < p.tokens;
+    const long long from = (has ? token : 0) * p.ld;
+    const int e0 = l * kPer;
+    double* mine = space + (wave * 4 + row) * kWords;
+    const auto slot = [](int e) { return e / kPer * kLane + e % kPer; };
+    if (p.plans && threadIdx.x < kFewPairs) few[threadIdx.x] = 0xffff;
+    f32x4 four[kPer / 4];
+    if (p.experts % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int e = lane + 64 * i;
-        const float l = e < p.experts ? load_one<kType>(p.logits, token * p.ld + e) : -__builtin_inff();
-        bad |= l != l;
-        key[i] = l != l ? kNone : static_cast<double>(l);
-        top = fmax(top, key[i]);
-    }
-    bad = __any(bad);
-    top = wave_max(top);
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        if (p.score == MCHIP_ROUTE_SOFTMAX)
-            score[i] = top == kNone ? 0.0 : exp(key[i] - top);  // +inf - inf: no number
-        else
-            score[i] = 1.0 / (1.0 + exp(-key[i]));
-        sum += score[i];
-    }
-    if (p.score == MCHIP_ROUTE_SOFTMAX) {
-        sum = wave_add(sum);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) score[i] = sum > 0.0 || sum != sum ? score[i] / sum : 0.0;
-    }
-    if (!p.by_logit) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = lane + 64 * i;
-            // An expert that is masked out stays so whatever its bias.
-            if (key[i] != kNone) key[i] = score[i] + (p.bias != nullptr && e < p.experts ? static_cast<double>(p.bias[e]) : 0.0);
-            if (key[i] != key[i]) key[i] = kNone;
-        }
-    }
-    int place[kPer];  // by it ties are settled: experts of no chosen group come last
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) place[i] = lane + 64 * i;
-    if (p.groups > 1) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) keys[wave][lane + 64 * i] = key[i];
-        __builtin_amdgcn_wave_barrier();
-        double mine = kNone;
-        if (lane < p.groups) {
-            double first = kNone, second = kNone;
-            for (int i = 0; i < p.each; ++i) {
-                const double k = keys[wave][lane * p.each + i];
-                if (k > first) second = first, first = k;
-                else if (k > second) second = k;
-            }
-            mine = p.group_best == 2 && p.each > 1 ? first + second : first;
-            if (mine != mine) mine = kNone;
-        }
-        unsigned long long kept = 0;
-        int at_mine = lane < p.groups ? lane : 1 << 20;
-        for (int g = 0; g < p.top_groups; ++g) {
-            double k = mine;
-            int at = at_mine;
-            wave_first(k, at);
-            kept |= 1ull << at;
-            if (lane == at) mine = kNone, at_mine = 1 << 21;
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = lane + 64 * i;
-            if (e >= p.experts || !(kept >> (e / p.each) & 1)) key[i] = kNone, place[i] = e + (1 << 20);
+        for (int i = 0; i < kPer / 4; ++i) {
+            four[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (e0 + 4 * i < p.experts) four[i] = load_four<kType>(p.logits, from + e0 + 4 * i, 4);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (place[i] >= p.experts) place[i] += 1 << 20;
+        for (int i = 0; i < kPer / 4; ++i) four[i] = load_four<kType>(p.logits, from + e0 + 4 * i, p.experts - e0 - 4 * i);
     }
-    int expert = 0;
-    double gate = 0.0, total = 0.0;
+    if (static_cast<int>(threadIdx.x) < p.experts) bias[threadIdx.x] = p.bias != nullptr ? p.bias[threadIdx.x] : 0.0f;
+    __syncthreads();
+    bool bad = false;
+    double key[kPer], top = kNone;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const float v = four[i / 4][i % 4];
+        bad |= v != v;
+        key[i] = v != v ? kNone : static_cast<double>(v);
+        key[i] = e0 + i < p.experts ? key[i] : __builtin_nan("");
+        top = larger(top, key[i]);
+    }
+    top = over_token(top, larger);
+    bad = (__ballot(bad) >> (16 * row) & 0xffffull) != 0;
+    const bool soft = p.score == MCHIP_ROUTE_SOFTMAX;
+    double total = 0.0;
+    if (!p.by_logit || (soft && !p.normalize) || p.groups > 1) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mine[l * kLane + i] = key[i];
+        // An expert that is masked out stays so whatever its bias.
+        const auto key_of = [&](double s, int i) {
+            const double k = s + static_cast<double>(bias[e0 + i]);
+            return k != k ? kNone : k;
+        };
+        if (!p.by_logit || (soft && !p.normalize)) {
+            const int count = min(kPer, p.experts - e0);
+#pragma unroll 2
+            for (int i = 0; i < count; ++i) {
+                const double logit = mine[l * kLane + i];
+                const double e = exp(soft ? logit - top : -logit);
+                const double s = soft ? e : 1.0 / (1.0 + e);
+                // A softmax's before the division, -1 where masked out.
+                if (logit != kNone) total += s;
+                if (!p.by_logit) mine[l * kLane + i] = logit == kNone ? (soft ? -1.0 : kNone) : soft ? s : key_of(s, i);
+            }
+            total = over_token(total, both);
+            if (!p.by_logit && soft) {
+                const double share = 1.0 / total;
+#pragma unroll 2
+                for (int i = 0; i < count; ++i) {
+                    const double s = mine[l * kLane + i];
+                    mine[l * kLane + i] = s < 0.0 ? kNone : key_of(s * share, i);
+                }
+            }
+        }
+    }
+    unsigned long long kept = ~0ull;
+    if (p.groups > 1) {
+        __builtin_amdgcn_wave_barrier();
+        // Its score goes to the group's first expert's place in `sums`.
+        double* sums = mine;  // once every lane has read its groups
+        kept = 0;
+        double sum[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            sum[q] = kNone;
+            const int g = l + 16 * q;
+            if (16 * q >= p.groups) continue;
+            if (g < p.groups) {
+                double first = kNone, second = kNone;
+#pragma unroll 4
+                for (int i = 0; i < p.each; ++i) {
+                    const double k = mine[slot(g * p.each + i)];
+                    second = larger(second, __builtin_fmin(first, k));
+                    first = larger(first, k);
+                }
+                sum[q] = p.group_best == 2 && p.each > 1 ? first + second : first;
+                if (sum[q] != sum[q]) sum[q] = kNone;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) key[i] = mine[l * kLane + i];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (l + 16 * q < p.groups) sums[l + 16 * q] = sum[q];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (16 * q >= p.groups) continue;
+            const int g = l + 16 * q;
+            int before = 0;
+#pragma unroll 2
+            for (int o = 0; o < p.groups; ++o) {
+                const double s = sums[o];
+                before += s > sum[q] || (s == sum[q] && o < g);
+            }
+            kept |= (__ballot(g < p.groups && before < p.top_groups) >> (16 * row) & 0xffffull) << (16 * q);
+        }
+        int group = e0 / p.each, in_group = e0 - group * p.each;
+        bool stays = (kept >> (group & 63) & 1) != 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            key[i] = stays ? key[i] : __builtin_nan("");
+            if (++in_group == p.each) in_group = 0, ++group, stays = (kept >> (group & 63) & 1) != 0;
+        }
+    } else if (!p.by_logit) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) key[i] = mine[l * kLane + i];
+    }
+    // The chosen one after the other, lane j the j-th.
+    int* const places = picked[wave * 4 + row];
+#pragma unroll 1
     for (int j = 0; j < p.top_k; ++j) {
-        double k = key[0];
-        int at = place[0];
+        double most[kPer / 2];
 #pragma unroll
-        for (int i = 1; i < kPer; ++i)
-            if (key[i] > k || (key[i] == k && place[i] < at)) k = key[i], at = place[i];
-        wave_first(k, at);
-        double s = 0.0;
+        for (int i = 0; i < kPer / 2; ++i) most[i] = larger(key[2 * i], key[2 * i + 1]);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (at == lane + 64 * i) s = score[i], key[i] = kNone, place[i] = at + (1 << 21);
-        s = __shfl(s, at % 64);
-        total += s;
-        if (lane == j) expert = at, gate = s;
+        for (int n = kPer / 4; n > 0; n /= 2)
+#pragma unroll
+            for (int i = 0; i < n; ++i) most[i] = larger(most[2 * i], most[2 * i + 1]);
+        const double best = over_token(most[0], larger);
+        const unsigned lanes = static_cast<unsigned>(__ballot(most[0] == best) >> (16 * row)) & 0xffffu;
+        const bool winner = l == __builtin_ctz(lanes | 0x10000u);
+        int at = kPer;
+#pragma unroll
+        for (int i = kPer - 1; i >= 0; --i) at = key[i] == best ? i : at;
+        if (winner) places[j] = e0 + at;
+        at = winner ? at : kPer;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            u32x2 u = __builtin_bit_cast(u32x2, key[i]);
+            u[1] = at == i ? 0x7ff80000u : u[1];
+            key[i] = __builtin_bit_cast(double, u);
+        }
     }
-    if (lane >= p.top_k) return;
-    if (p.normalize) gate = total != 0.0 ? gate / total : 0.0;
-    float g = static_cast<float>(gate * static_cast<double>(p.scale));
-    if (bad) g = __builtin_nanf("");
-    p.chosen[token * p.top_k + lane] = expert;
-    p.gates[token * p.top_k + lane] = g;
+    __builtin_amdgcn_wave_barrier();
+    const int expert = l < p.top_k ? places[l] : 0;
+    double gate = 0.0;
+    if (l < p.top_k) {
+        const double logit = load_one<kType>(p.logits, from + expert);
+        const double e = exp(soft ? logit - top : -logit);
+        gate = logit == kNone ? 0.0 : soft ? e : 1.0 / (1.0 + e);
+    }
+    const double over = p.normalize ? over_token(gate, both) : soft ? total : 1.0;
+    gate = over != 0.0 ? gate / over : 0.0;
+    if (bad) gate = __builtin_nan("");
+    if (has && l < p.top_k) put(p, few, token, l, expert, static_cast<float>(gate * static_cast<double>(p.scale)));
+    if (!p.plans) return;
+    __syncthreads();
+    plan_few(p, few);
 }
 
 // A block takes an expert: how many pairs have a lower one is where its slots begin,
-// and its own pairs follow in order, each wave a range of them.
-__global__ __launch_bounds__(1024) void make_plan(const int* __restrict__ chosen, int pairs, int experts,
-                                                  int* __restrict__ order, int* __restrict__ offsets) {
-    __shared__ int lower[16], own[16];
+// and its own pairs follow in order. A wave takes 4096 pairs at a time, a lane eight of
+// 512 next to each other (whole lines to a load; 64 to a lane took three times as long).
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kSteps = 8;
+
+// The sum over the lanes up to this one.
+__device__ __forceinline__ unsigned sum_to(unsigned v) {
+#define ROUTE_STEP(ctrl, rows) \
+    v += static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl, rows, 0xf, false));
+    ROUTE_STEP(0x111, 0xf) ROUTE_STEP(0x112, 0xf) ROUTE_STEP(0x114, 0xf) ROUTE_STEP(0x118, 0xf)
+    ROUTE_STEP(0x142, 0xa) ROUTE_STEP(0x143, 0xc)
+#undef ROUTE_STEP
+    return v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void make_plan(const unsigned short* __restrict__ ids, int pairs, int experts,
+                                                          int* __restrict__ order, int* __restrict__ offsets) {
+    constexpr int kPart = kPlanThreads * 8 * kSteps;
+    __shared__ int own[kPlanWaves], lower[kPlanWaves];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, e = static_cast<int>(blockIdx.x);
-    const int share = (pairs + 16 * 64 - 1) / (16 * 64) * 64;
-    const int from = min(wave * static_cast<long long>(share), static_cast<long long>(pairs));
-    const int to = min(from + static_cast<long long>(share), static_cast<long long>(pairs));
-    int below = 0, mine = 0;
-    for (int i = from + lane; i < to; i += 64) {
-        const int c = chosen[i];
-        below += c < e;
-        mine += c == e;
-    }
+    const int parts = (pairs + kPart - 1) / kPart;
+    unsigned below = 0, mine[kSteps];  // mine: bit j: the lane's pair j of the step, of the part that was read last
+    int at = 0;
+    const auto read = [&](int part) {
+        at = part * kPart + (wave * kSteps * 64 + lane) * 8;
+        u16x8 eight[kSteps];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) below += __shfl_xor(below, d), mine += __shfl_xor(mine, d);
-    if (lane == 0) lower[wave] = below, own[wave] = mine;
+        for (int i = 0; i < kSteps; ++i) {
+            const int from = at + i * 512;
+            eight[i] = *reinterpret_cast<const u16x8*>(ids + (from < pairs ? from : 0));
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            mine[i] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int id = at + i * 512 + j < pairs ? eight[i][j] : 0xffff;
+                below += static_cast<unsigned>(id - e) >> 31;
+                mine[i] |= id == e ? 1u << j : 0u;
+            }
+        }
+    };
+    for (int part = 0; part < parts; ++part) read(part);
+    below = sum_to(below);
+    if (lane == 63) lower[wave] = static_cast<int>(below);
     __syncthreads();
-    int at = 0, all = 0;
-    for (int w = 0; w < 16; ++w) {
-        at += lower[w];
-        if (w < wave) at += own[w];
-        all += lower[w] + own[w];
+    int first = 0;
+    for (int w = 0; w < kPlanWaves; ++w) first += lower[w];
+    const int start = first;
+    for (int part = 0; part < parts; ++part) {
+        if (parts > 1) read(part);
+        // Three steps' counts to a word: at most 512 each.
+        unsigned packed[3] = {0, 0, 0}, up_to[3];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) packed[i / 3] += static_cast<unsigned>(__popc(mine[i])) << i % 3 * 10;
+        unsigned before[kSteps], all = 0;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) up_to[w] = sum_to(packed[w]);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            before[i] = all + ((up_to[i / 3] - packed[i / 3]) >> i % 3 * 10 & 1023u);
+            all += __builtin_amdgcn_readlane(static_cast<int>(up_to[i / 3]), 63) >> i % 3 * 10 & 1023u;
+        }
+        if (lane == 0) own[wave] = static_cast<int>(all);
+        __syncthreads();
+        int to = first;
+        for (int w = 0; w < kPlanWaves; ++w) {
+            if (w < wave) to += own[w];
+            first += own[w];
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            int slot = to + static_cast<int>(before[i]);
+            for (unsigned bits = mine[i]; bits != 0; bits &= bits - 1) order[slot++] = at + i * 512 + __builtin_ctz(bits);
+        }
+        __syncthreads();
     }
     if (threadIdx.x == 0) {
-        offsets[e] = at;
-        if (e == experts - 1) offsets[experts] = all;
-    }
-    for (int i = from; i < to; i += 64) {
-        const bool is = i + lane < to && chosen[i + lane] == e;
-        const unsigned long long here = __ballot(is);
-        if (is) order[at + __popcll(here & ((1ull << lane) - 1))] = i + lane;
-        at += __popcll(here);
+        offsets[e] = start;
+        if (e == experts - 1) offsets[experts] = first;
     }
 }
 
 template <int kType>
 int launch_tokens(const Route& p, hipStream_t stream) {
-    const unsigned blocks = static_cast<unsigned>((static_cast<long long>(p.tokens) + kWaves - 1) / kWaves);
-    const auto go = [&](auto kernel) { return launch_kernel(kernel, blocks, kWaves * 64, 0, stream, p); };
-    if (p.experts <= 64) return go(route_tokens<kType, 1>);
-    if (p.experts <= 128) return go(route_tokens<kType, 2>);
-    if (p.experts <= 256) return go(route_tokens<kType, 4>);
-    return go(route_tokens<kType, 8>);
+    const unsigned blocks = static_cast<unsigned>((static_cast<long long>(p.tokens) + kTokens - 1) / kTokens);
+    const auto go = [&](auto kernel) { return launch_kernel(kernel, blocks, kThreads, 0, stream, p); };
+    if (p.experts <= 64) return go(route_tokens<kType, 4>);
+    if (p.experts <= 128) return go(route_tokens<kType, 8>);
+    if (p.experts <= 256) return go(route_tokens<kType, 16>);
+    return go(route_tokens<kType, 32>);
 }
+
+// Whether the block that chooses makes the plan, too.
+bool plans_itself(int tokens, int top_k) { return tokens <= kTokens && tokens * top_k <= kFewPairs; }
 
 const char* refusal(const mchip_route_args& x) {
     if (!is_float_type(x.dtype)) return "the type is none of fp32 (0), bf16 (1), fp16 (2)";
@@ -213,6 +373,8 @@ const char* refusal(const mchip_route_args& x) {
     if (x.ld < x.experts) return "rows closer together than they are long";
     if (x.logits == nullptr || x.chosen == nullptr || x.gates == nullptr) return "null logits, chosen or gates";
     if ((x.order == nullptr) != (x.offsets == nullptr)) return "one half of a plan";
+    if (x.order != nullptr && !plans_itself(x.tokens, x.top_k) && (x.workspace == nullptr || !aligned(x.workspace, 256)))
+        return "a null workspace, or one that is not 256-byte aligned";
     if (!aligned(x.logits, size_of(x.dtype))) return "an address that is no multiple of its element's size";
     if (!aligned(x.bias, 4) || !aligned(x.chosen, 4) || !aligned(x.gates, 4) || !aligned(x.order, 4) || !aligned(x.offsets, 4))
         return "a bias or an output that is not 4-byte aligned";
@@ -223,22 +385,27 @@ const char* refusal(const mchip_route_args& x) {
 
 extern "C" {
 
-long long mchip_route_workspace_bytes(int tokens, int experts, int top_k) { return 0; }
+long long mchip_route_workspace_bytes(int tokens, int experts, int top_k) {
+    if (tokens < 1 || experts < 1 || top_k < 1 || top_k > MCHIP_ROUTE_MAX_TOP_K || plans_itself(tokens, top_k)) return 0;
+    return (static_cast<long long>(tokens) * top_k * 2 + 255) / 256 * 256;
+}
 
 int mchip_launch_route(const mchip_route_args* args, void* stream, const char** why) {
     const mchip_route_args& x = *args;
     *why = refusal(x);
     if (*why != nullptr) return hipErrorInvalidValue;
+    const bool plans = x.order != nullptr && plans_itself(x.tokens, x.top_k);
+    unsigned short* ids = x.order != nullptr && !plans ? static_cast<unsigned short*>(x.workspace) : nullptr;
     const Route p{x.logits, x.ld, x.bias, x.tokens, x.experts, x.top_k, x.score, x.groups, x.experts / x.groups,
-                  x.top_groups, x.group_best, x.normalize, x.scale, x.chosen, x.gates,
-                  x.bias == nullptr && (x.groups == 1 || x.group_best == 1)};
+                  x.top_groups, x.group_best, x.normalize, x.scale, x.chosen, x.gates, x.order, x.offsets, ids,
+                  x.bias == nullptr && (x.groups == 1 || x.group_best == 1), plans};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int rc = x.dtype == kF32    ? launch_tokens<kF32>(p, s)
                    : x.dtype == kBf16 ? launch_tokens<kBf16>(p, s)
                                       : launch_tokens<kF16>(p, s);
-    if (rc != hipSuccess || x.order == nullptr) return rc;
-    return launch_kernel(make_plan, static_cast<unsigned>(x.experts), 1024, 0, s, x.chosen, x.tokens * x.top_k, x.experts,
-                         x.order, x.offsets);
+    if (rc != hipSuccess || ids == nullptr) return rc;
+    return launch_kernel(make_plan, static_cast<unsigned>(x.experts), kPlanThreads, 0, s, ids, x.tokens * x.top_k,
+                         x.experts, x.order, x.offsets);
 }
 
 }  // extern "C"

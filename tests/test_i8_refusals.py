@@ -63,8 +63,11 @@ def test_route(mc):
                       ("than the chosen groups", {"groups": 16, "top_groups": 1}), ("closer", {"ld": 63}),
                       ("pairs", {"tokens": 1 << 28}), ("null", {"logits": None}), ("null", {"gates": None}),
                       ("one half", {"order": None}), ("one half", {"offsets": None}), ("element", {"logits": P + 2}),
-                      ("aligned", {"bias": P + 2}), ("aligned", {"order": P + 1})]:
+                      ("aligned", {"bias": P + 2}), ("aligned", {"order": P + 1}),
+                      ("workspace", {"tokens": 64, "workspace": None}), ("workspace", {"tokens": 64, "workspace": P + 64})]:
         refused(mc, match, call, **kw)
+    assert mc.route_workspace_bytes(1, 64, 8) == 0 and mc.route_workspace_bytes(64, 64, 8) > 0
+    assert mc.route_workspace_bytes(0, 64, 8) == 0 and mc.route_workspace_bytes(64, 64, 17) == 0
 
 
 @pytest.mark.parametrize("down", [False, True])
