@@ -2,6 +2,7 @@
 // 32-bit sums, scaled by row and column, with bias and activation; and the
 // experts' products on a plan, the same for each expert's slots.
 
+#include <cmath>
 #include <type_traits>
 
 #include "gemm_i8_tiles.h"
@@ -66,6 +67,22 @@ __device__ __forceinline__ bool find_entry(const Product& p, unsigned& want, Ent
     return false;
 }
 
+// What all experts' slots add up to.
+template <typename Count>
+__device__ __forceinline__ unsigned sum_of_entries(const Product& p, Count count) {
+    unsigned all = 0;
+    for (int base = 0; base < p.experts; base += 64) {
+        const int e = base + static_cast<int>(threadIdx.x % 64);
+        int from = 0, to = 0;
+        if (e < p.experts) from = p.offsets[e], to = p.offsets[e + 1];
+        from = max(from, 0), to = max(min(to, p.m), from);
+        all += count(static_cast<unsigned>(to - from));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+    return __builtin_amdgcn_readfirstlane(all);
+}
+
 // Job `want` of the experts' slots, up to kRows of one expert's each; end = first: none.
 template <int kRows>
 __device__ __forceinline__ Place find_job(const Product& p, unsigned want) {
@@ -98,8 +115,14 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
     constexpr int kCols = kGated ? kN / 2 : kN;  // column tiles of C
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int r = lane % 16, q = lane / 16, part = lane % 4, pass = (4 * r + q) * 4;
-    const unsigned chunk = blockIdx.x / p.tiles_n;
-    const int col0 = static_cast<int>(blockIdx.x % p.tiles_n) * 16 * kCols;
+    unsigned chunk = blockIdx.x / p.tiles_n, tile = blockIdx.x % p.tiles_n;
+    if constexpr (kMode == kDense) {
+        // A column tile's rows one after the other on one XCD, whose L2 has its weights.
+        const unsigned all = gridDim.x, t = blockIdx.x < all / 8 * 8 ? blockIdx.x % 8 * (all / 8) + blockIdx.x / 8 : blockIdx.x;
+        const unsigned chunks = all / p.tiles_n;
+        chunk = t % chunks, tile = t / chunks;
+    }
+    const int col0 = static_cast<int>(tile) * 16 * kCols;
     Place place{0, 0, p.m};
     long long row0 = static_cast<long long>(chunk) * 16 * kM;
     if constexpr (kMode != kDense) {
@@ -214,8 +237,6 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
     }
 }
 
-constexpr int kPanel = 4;
-
 // The row of A that row `row` of C takes.
 template <int kMode>
 __device__ __forceinline__ long long a_row_of(const Product& p, long long row) {
@@ -225,17 +246,19 @@ __device__ __forceinline__ long long a_row_of(const Product& p, long long row) {
 }
 
 // A wave's sums (tile_sums) scaled, with bias and activation, to C: rows row0 .. up to
-// `end`, columns col0 on, by way of the wave's 32 KiB of LDS, so that a short loop (a
-// launch meets a cold instruction cache) stores whole lines. In two passes: 64 columns of
-// all rows, or (kGated) 64 rows with both halves of their 64 columns. Block c of 16
-// bytes of row r lies at c ^ (r % 16).
-template <int kMode, bool kGated, int kOut, int kRowFrags>
-__device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Product& p,
-                                           const i32x16 (&acc)[kRowFrags][kColFrags], int expert, long long row0,
-                                           long long end, int col0, int lane) {
-    constexpr int kPasses = kGated ? kRowFrags / 2 : 2, kRowBytes = kGated ? 512 : 256;
+// `end`, columns col0 on, by way of the wave's share of LDS (`lds`), so that a short loop
+// (a launch meets a cold instruction cache) stores whole lines. In passes: 64 columns of
+// all rows, or (kGated) 64 rows with both halves of their columns. Block c of 16 bytes of
+// row r lies at c ^ (r % 16).
+template <int kMode, bool kGated, int kOut, typename T>
+__device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Product& p, const typename T::Sums& acc,
+                                           int expert, long long row0, long long end, int col0, int lane) {
+    constexpr int kRowFrags = T::kRowFrags, kColFrags = T::kColFrags;
     constexpr int kHalves = kRowFrags / 2;  // of 64 rows
-    constexpr int kPassRows = kGated ? 64 : 64 * kHalves;
+    constexpr int kPasses = kGated ? kHalves : kColFrags / 2, kPassFrags = kGated ? kColFrags : 2;
+    constexpr int kRowBytes = kPassFrags * 128, kPassRows = kGated ? 64 : 64 * kHalves;
+    constexpr int kAcross = (kGated ? kColFrags / 2 : 2) * 4, kBatch = 64 / kAcross;  // lanes along a row, rows at a time
+    static_assert(kPasses <= 2 && kPassRows / kBatch % 4 == 0);
     const long long b_row = static_cast<long long>(expert) * (kGated ? 2 * p.n : p.n);
     const int line = lane % 32, half = lane / 32;
     // What goes with rows lane and lane + 64.
@@ -263,8 +286,8 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
 #pragma unroll
         for (int i = 0; i < (kGated ? 2 : kRowFrags); ++i)
 #pragma unroll
-            for (int f = 0; f < (kGated ? kColFrags : 2); ++f) {
-                const i32x16& sums = kGated ? acc[2 * h % kRowFrags + i][f] : acc[i][2 * h + f];
+            for (int f = 0; f < kPassFrags; ++f) {
+                const i32x16& sums = kGated ? acc[2 * h % kRowFrags + i][f] : acc[i][2 * h % kColFrags + f];
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *reinterpret_cast<MX4_LDS i32x4*>(lds + (32 * i + line) * kRowBytes +
@@ -272,11 +295,11 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
                         i32x4{sums[4 * g], sums[4 * g + 1], sums[4 * g + 2], sums[4 * g + 3]};
             }
     };
-    // Columns 8 c .. + 7 of the wave's row: blocks 2 c and 2 c + 1 (the up ones 16 further on).
+    // Columns 8 c .. + 7 of the wave's row: blocks 2 c and 2 c + 1 (the up ones behind all gate ones).
     const auto sums_of = [&](int row, int block, int (&sum)[8]) {
         const MX4_LDS unsigned char* at = lds + row * kRowBytes;
-        const i32x4 lo = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((block + lane % 8 * 2) ^ row % 16) * 16);
-        const i32x4 hi = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((block + lane % 8 * 2 + 1) ^ row % 16) * 16);
+        const i32x4 lo = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((block + lane % kAcross * 2) ^ row % 16) * 16);
+        const i32x4 hi = *reinterpret_cast<const MX4_LDS i32x4*>(at + ((block + lane % kAcross * 2 + 1) ^ row % 16) * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = lo[e], sum[4 + e] = hi[e];
     };
@@ -284,8 +307,8 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
     for (int h = 0; h < kPasses; ++h) {
         if (h == 0) to_lds(std::integral_constant<int, 0>{});
         else to_lds(std::integral_constant<int, 1>{});
-        // Eight columns of a row per lane, eight rows at a time, four of which are under way.
-        const int col = col0 + (kGated ? 0 : 64 * h) + lane % 8 * 8, left = p.n - col;
+        // Eight columns of a row per lane, kBatch rows at a time, four times that under way.
+        const int col = col0 + (kGated ? 0 : 64 * h) + lane % kAcross * 8, left = p.n - col;
         float scale[8], bias[8], up_scale[8], up_bias[8];
         load_eight<kF32>(p.b_scales, b_row + col, left, scale);
         load_eight<kF32>(p.bias, b_row + col, p.bias != nullptr ? left : 0, bias);
@@ -295,19 +318,19 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
         }
         const auto rows = [&](auto act, auto store) {
 #pragma unroll 1
-            for (int it = 0; it < kPassRows / 8; it += 4) {
-                const int part = kGated ? h : it / 8;
+            for (int it = 0; it < kPassRows / kBatch; it += 4) {
+                const int part = kGated ? h : it * kBatch / 64;
                 const float sa_here = kHalves == 1 || part == 0 ? sa[0] : sa[kHalves - 1];
                 const float gate_here = kHalves == 1 || part == 0 ? gate[0] : gate[kHalves - 1];
                 int sum[4][8], up[4][8];
                 float s[4], g[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const int row = 8 * (it + u) + lane / 8;
+                    const int row = kBatch * (it + u) + lane / kAcross;
                     s[u] = of_row(sa_here, row);
                     if constexpr (kMode == kDown) g[u] = of_row(gate_here, row);
                     sums_of(row, 0, sum[u]);
-                    if constexpr (kGated) sums_of(row, 16, up[u]);
+                    if constexpr (kGated) sums_of(row, 2 * kAcross, up[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -338,10 +361,10 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
         if (kMode != kDown && p.n % 8 == 0 && row_size * 16 * 16 < (1LL << 31)) {
             const __amdgpu_buffer_rsrc_t c = rows_from(static_cast<unsigned char*>(p.c) + row0 * row_size, end - row0,
                                                        static_cast<int>(row_size));
-            const int step = __builtin_amdgcn_readfirstlane(8 * static_cast<int>(row_size));
-            const unsigned at = left > 0 ? static_cast<unsigned>(lane / 8 * static_cast<int>(row_size) + col * kOne) : 1u << 31;
+            const int step = __builtin_amdgcn_readfirstlane(kBatch * static_cast<int>(row_size));
+            const unsigned at = left > 0 ? static_cast<unsigned>(lane / kAcross * static_cast<int>(row_size) + col * kOne) : 1u << 31;
             with_act([&](int it, int, const float(&v)[8]) {
-                const int from = static_cast<int>(at + static_cast<unsigned>((it + (kGated ? h * 8 : 0)) * step));
+                const int from = static_cast<int>(at + static_cast<unsigned>((it + (kGated ? h * (64 / kBatch) : 0)) * step));
                 if constexpr (kOut == kF32) {
                     const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), c, from, 0, 2);
@@ -355,51 +378,54 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
             });
         } else {
             with_act([&](int it, int part, const float(&v)[8]) {
-                const int c_row = of_row(kHalves == 1 || part == 0 ? c_rows[0] : c_rows[kHalves - 1], 8 * it + lane / 8);
+                const int c_row = of_row(kHalves == 1 || part == 0 ? c_rows[0] : c_rows[kHalves - 1], kBatch * it + lane / kAcross);
                 if (c_row >= 0 && left > 0)
-                    store_eight<kOut>(p.c, ((kMode == kDown ? 0 : row0) + c_row) * p.n + col, v, left);
+                    store_eight<kOut, kMode != kDown>(p.c, ((kMode == kDown ? 0 : row0) + c_row) * p.n + col, v, left);
             });
         }
     }
 }
 
-// Rows row0 .. of C up to `end` (at most kRows) by 256 (kGated: 128) columns from col0 on.
-template <int kMode, bool kGated, int kOut, int kRows>
+// Rows row0 .. of C up to `end` (at most kRows) by kCols (kGated: half of it) columns from
+// col0 on.
+template <int kMode, bool kGated, int kOut, int kRows, int kCols, int kSlotRows>
 __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const Product& p, int expert, long long row0,
                                              long long end, int col0) {
+    typedef Tile<kRows, kCols, kSlotRows> T;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-    constexpr int kShare = kRows / 4;  // of A's rows, a wave's to fetch
+    constexpr int kShareA = kRows / 4, kShareB = kCols / 4;  // rows, a wave's to fetch
     // A's rows, from the wave's share of the tile on, or (gathered) all.
-    const long long a0 = kMode == kUp ? 0 : row0 + wave * kShare;
-    const long long a_left = kMode == kUp ? 0 : end - a0;
+    const long long a0 = kMode == kUp ? 0 : row0 + wave * kShareA;
     const __amdgpu_buffer_rsrc_t a = kMode == kUp ? resource(p.a, p.a_rows * p.row_bytes)
-                                                  : rows_from(p.a + a0 * p.row_bytes, a_left, p.row_bytes);
+                                                  : rows_from(p.a + a0 * p.row_bytes, end - a0, p.row_bytes);
     const auto a_row = [&](int i) {
         const int in_share = i * 8 + lane / 8;
         if constexpr (kMode != kUp) return in_share * p.row_bytes;
-        const long long row = row0 + wave * kShare + in_share;
+        const long long row = row0 + wave * kShareA + in_share;
         return static_cast<int>(a_row_of<kMode>(p, row < end ? row : end - 1)) * p.row_bytes;
     };
-    // B's rows that the wave fetches: 64 of columns, of gate or of up ones.
-    const int b_col = col0 + (kGated ? wave / 2 * 64 : wave * 64), b_rows = kGated ? 2 * p.n : p.n;
+    // B's rows that the wave fetches: of columns, of gate or of up ones.
+    const int b_col = col0 + (kGated ? wave / 2 : wave) * kShareB, b_rows = kGated ? 2 * p.n : p.n;
     const long long b0 = static_cast<long long>(expert) * b_rows + (kGated ? wave % 2 * static_cast<long long>(p.n) : 0) + b_col;
     const __amdgpu_buffer_rsrc_t b = rows_from(p.b + b0 * p.row_bytes, p.n - b_col, p.row_bytes);
-    i32x16 acc[kRows / 64][kColFrags];
-    tile_sums<kRows>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
+    typename T::Sums acc;
+    tile_sums<T>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
     lds_barrier();  // every wave is past its reads of the ring
-    store_tile<kMode, kGated, kOut>(lds + wave * (32 * 1024), p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
-                                    col0 + wave % 2 * (kGated ? 64 : 128), lane);
+    store_tile<kMode, kGated, kOut, T>(lds + wave * T::kSlotBytes, p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
+                                       col0 + wave % 2 * (kGated ? kCols / 4 : kCols / 2), lane);
 }
 
-// Dense: tiles in panels of kPanel rows of them, column after column; the grid has one
-// block per tile of 256 rows plus `halves` more, for which that many of the last tiles
-// run as two blocks of 128 rows. An XCD takes consecutive ones, so that the 32 which it
-// works on at a time read 4 + 8 tiles' rows through its L2.
-// On a plan: an expert's slots in tiles of 256, its last of 128 where that holds it.
-template <int kMode, bool kGated, int kOut>
-__global__ __launch_bounds__(kTileThreads, 1) void i8_tiles(const Product p, unsigned full) {
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[kRingBytes];
+// kTile 256: dense tiles are 256 rows high; the grid has one block per tile plus `halves`
+// more, for which that many of the last tiles run as two blocks of 128 rows; on a plan an
+// expert's last tile is of 128 rows where that holds it. kTile 128: tiles of 128x128.
+// Dense tiles go in panels of kPanel rows of them, column after column. An XCD takes
+// consecutive ones, so that those which it works on at a time read few rows through its
+// L2 (4 + 8 tiles' rows of 256).
+template <int kMode, bool kGated, int kOut, int kTile>
+__global__ __launch_bounds__(kTileThreads, kTile == 256 ? 1 : 2) void i8_tiles(const Product p, unsigned full) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile<kTile, kTile, kTile>::kRingBytes];
     MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);  // generic -> LDS address space
+    constexpr int kPanel = kTile == 256 ? 4 : 8;
     unsigned t = blockIdx.x, chunk, tile;
     int half = 0;
     if constexpr (kMode == kDense) {
@@ -408,28 +434,39 @@ __global__ __launch_bounds__(kTileThreads, 1) void i8_tiles(const Product p, uns
         } else if (t < full / 8 * 8) {
             t = t % 8 * (full / 8) + t / 8;  // blocks go to the XCDs in turn
         }
-        const unsigned all = static_cast<unsigned>((p.m + kTileRows - 1) / kTileRows);
+        const unsigned all = static_cast<unsigned>((p.m + kTile - 1) / kTile);
         const unsigned panel = t / (kPanel * p.tiles_n), in = t % (kPanel * p.tiles_n);
         const unsigned high = min(static_cast<unsigned>(kPanel), all - panel * kPanel);
         chunk = panel * kPanel + in % high, tile = in / high;
     } else {
+        // An XCD takes an eighth of the tiles that the plan has, consecutive ones, so that
+        // an expert's weights and a chunk's rows come through one L2.
+        const unsigned long long have =
+            static_cast<unsigned long long>(sum_of_entries(p, [](unsigned n) { return (n + kTile - 1) / kTile; })) * p.tiles_n;
+        const unsigned first = static_cast<unsigned>(have * (t % 8) / 8), last = static_cast<unsigned>(have * (t % 8 + 1) / 8);
+        t = first + t / 8;
+        if (t >= last) return;
         chunk = t / p.tiles_n, tile = t % p.tiles_n;
     }
-    const int col0 = static_cast<int>(tile) * (kGated ? kTileCols / 2 : kTileCols);
-    long long row0 = static_cast<long long>(chunk) * kTileRows, end = p.m;
+    const int col0 = static_cast<int>(tile) * (kGated ? kTile / 2 : kTile);
+    long long row0 = static_cast<long long>(chunk) * kTile, end = p.m;
     int expert = 0;
     if constexpr (kMode == kDense) {
-        if (half == 2) row0 += kTileRows / 2;
-        if (half == 1 && row0 + kTileRows / 2 < end) end = row0 + kTileRows / 2;
+        if (half == 2) row0 += kTile / 2;
+        if (half == 1 && row0 + kTile / 2 < end) end = row0 + kTile / 2;
     } else {
-        const Place place = find_tile<kTileRows>(p, chunk);
+        const Place place = kTile == 256 ? find_tile<256>(p, chunk) : find_job<kTile>(p, chunk);
         expert = place.expert, row0 = place.first, end = place.end;
     }
     if (row0 >= end) return;
-    if (end - row0 > kTileRows / 2)
-        product_tile<kMode, kGated, kOut, 256>(lds, p, expert, row0, end, col0);
-    else
-        product_tile<kMode, kGated, kOut, 128>(lds, p, expert, row0, end, col0);
+    if constexpr (kTile == 256) {
+        if (end - row0 > 128)
+            product_tile<kMode, kGated, kOut, 256, 256, 256>(lds, p, expert, row0, end, col0);
+        else
+            product_tile<kMode, kGated, kOut, 128, 256, 256>(lds, p, expert, row0, end, col0);
+    } else {
+        product_tile<kMode, kGated, kOut, 128, 128, 128>(lds, p, expert, row0, end, col0);
+    }
 }
 
 // y[token] = the sum of its top_k rows of the workspace, in order.
@@ -467,13 +504,14 @@ int launch_direct(Product p, hipStream_t stream, const char** why) {
                          0, stream, p);
 }
 
-template <int kMode, bool kGated>
+template <int kMode, bool kGated, int kTile>
 int launch_tiles(Product p, hipStream_t stream, const char** why) {
-    p.tiles_n = static_cast<unsigned>(tiles(p.n, kGated ? kTileCols / 2 : kTileCols));
-    const long long chunks = kMode == kDense ? tiles(p.m, kTileRows) : most_jobs(p.m, p.experts, kTileRows);
-    const long long all = chunks * p.tiles_n;
+    p.tiles_n = static_cast<unsigned>(tiles(p.n, kGated ? kTile / 2 : kTile));
+    const long long chunks = kMode == kDense ? tiles(p.m, kTile) : most_jobs(p.m, p.experts, kTile);
+    // On a plan eight XCDs with the same number of blocks each.
+    const long long all = kMode == kDense ? chunks * p.tiles_n : (chunks * p.tiles_n + 7) / 8 * 8;
     const int cus = device_cus(), rest = static_cast<int>(all % cus);
-    const int halves = kMode == kDense && rest <= cus / 2 ? rest : 0;
+    const int halves = kMode == kDense && kTile == 256 && rest <= cus / 2 ? rest : 0;
     if (!fits_launch(all + halves, kTileThreads)) {
         *why = "more tiles of C than one launch takes";
         return hipErrorInvalidValue;
@@ -483,28 +521,72 @@ int launch_tiles(Product p, hipStream_t stream, const char** why) {
                              static_cast<unsigned>(all - halves));
     };
     if constexpr (kMode == kDown) {
-        return go(i8_tiles<kMode, kGated, kF32>);
+        return go(i8_tiles<kMode, kGated, kF32, kTile>);
     } else {
-        return p.c_dtype == kF32    ? go(i8_tiles<kMode, kGated, kF32>)
-               : p.c_dtype == kBf16 ? go(i8_tiles<kMode, kGated, kBf16>)
-                                    : go(i8_tiles<kMode, kGated, kF16>);
+        return p.c_dtype == kF32    ? go(i8_tiles<kMode, kGated, kF32, kTile>)
+               : p.c_dtype == kBf16 ? go(i8_tiles<kMode, kGated, kBf16, kTile>)
+                                    : go(i8_tiles<kMode, kGated, kF16, kTile>);
     }
 }
 
 // Offsets within a tile's rows, and within A where its rows are gathered, have 32 bits.
 template <int kMode>
 bool tiles_fit(const Product& p) {
-    const long long a_rows = kMode == kUp ? p.a_rows : kTileRows;
+    const long long a_rows = kMode == kUp ? p.a_rows : 256;
     return a_rows * p.row_bytes < (1LL << 31);
 }
 
+// What a variant takes, in microseconds: a launch and `k` (in units of 4096) times its rounds.
+// Measured, 4096 wide and deep unless said: 16x32 blocks 5.5 (16 rows, 128 of them), 5.8 (32,
+// 256), 8.3 (64, 512), 12.0 (128), 20.6 (256); 32x32 6.5 (32 rows), 7.0 (64), 10.1 (128),
+// 15.9 (256); 32x64 9.1, 8.9, 8.6, 13.6 and 23.2 (512); 128x128 tiles 17.3 (64 rows), 18.5
+// (512), 22.1 (1024), 35.0 (2048), 215 (4096 by 14336); 256x256 39 (512), 51 (2048), 57
+// (4096), 212 (4096 by 14336). 64x64 blocks were nowhere a fifth faster than the next.
+// On a plan tiles take longer (rows gathered, weights from memory: 2048 tokens x 8 of 64
+// experts, 2048 deep, 1024 gated columns: 128x128 117, 256x256 105; 1024 tokens 78 and 98;
+// 128 tokens 55.8, 60.4 and 60.1 by 16x32 blocks; 64 tokens 55.5, 60.6 and 48.3).
+struct Cost {
+    double k, cus;
+    double few(double blocks, double one, double each, bool plan) const {
+        return 2.5 + k * (plan ? 1.8 : 1.0) * (blocks <= cus ? one : each * std::max(1.0, blocks / (2.0 * cus)));
+    }
+    double small_tiles(double tiles, bool plan) const {
+        if (plan) return 5.0 + 50.0 * k * std::ceil(tiles / (2.0 * cus));
+        return 5.0 + k * (2.0 * tiles <= cus ? 13.0 : tiles <= cus ? 17.0 : 30.0 * std::ceil(tiles / (2.0 * cus)));
+    }
+    double large_tiles(double rounds, bool plan) const { return 4.0 + rounds * (8.0 + (plan ? 66.0 : 48.0) * k); }
+};
+
 template <int kMode, bool kGated>
 int launch(const Product& p, hipStream_t stream, const char** why) {
-    // Rows of one expert, on average.
-    const long long rows = kMode == kDense ? p.m : tiles(p.m, p.experts);
-    if (rows > 64 && tiles_fit<kMode>(p) && tiles(p.m, 128) * tiles(p.n, 256) > 128) return launch_tiles<kMode, kGated>(p, stream, why);
-    if (rows <= 16) return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
-    return launch_direct<kMode, kGated, 4, 4>(p, stream, why);
+    constexpr bool kPlan = kMode != kDense;
+    const double cus = device_cus(), experts = static_cast<double>(std::min(p.experts, p.m));
+    const Cost cost{p.row_bytes / 4096.0, cus};
+    const double columns = kGated ? 2.0 * p.n : p.n;
+    // Blocks, of rows by columns of B; on a plan every second expert's last is half full.
+    const auto blocks = [&](int rows, int cols) {
+        const double down = kPlan ? std::max(experts, p.m / static_cast<double>(rows) + experts / 2)
+                                  : static_cast<double>(tiles(p.m, rows));
+        return down * std::ceil(columns / cols);
+    };
+    const double b16 = cost.few(blocks(16, 32), 3.2, 5.0, kPlan), b32 = cost.few(blocks(32, 32), 4.4, 7.3, kPlan),
+                 b64 = cost.few(blocks(32, 64), 6.2, 10.8, kPlan);
+    double t128 = 1e30, t256 = 1e30;
+    if (tiles_fit<kMode>(p)) {
+        t128 = cost.small_tiles(blocks(128, 128), kPlan);
+        // In rounds and halves of them; dense tiles that leave half a round or more empty run
+        // as halves, on a plan a third of the experts' last ones.
+        const double all = kPlan ? std::max(experts / 2, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus
+                                 : blocks(256, 256) / cus;
+        const double rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
+        t256 = cost.large_tiles(rounds, kPlan);
+    }
+    const double best = std::min({b16, b32, b64, t128, t256});
+    if (best == t256) return launch_tiles<kMode, kGated, 256>(p, stream, why);
+    if (best == t128) return launch_tiles<kMode, kGated, 128>(p, stream, why);
+    if (best == b64) return launch_direct<kMode, kGated, 2, 4>(p, stream, why);
+    if (best == b32) return launch_direct<kMode, kGated, 2, 2>(p, stream, why);
+    return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
 }
 
 const char* refusal(const void* a, const float* a_scales, const void* b, const float* b_scales, const float* bias,
