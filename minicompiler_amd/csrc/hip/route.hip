@@ -34,13 +34,19 @@ struct Route {
     bool plans;           // the only block makes the plan, too
 };
 
-// Place j of a token.
+// Place j of a token. Behind the last pair the ids go on to a multiple of eight with an
+// expert past all others.
 __device__ __forceinline__ void put(const Route& p, unsigned short* few, long long token, int j, int expert, float gate) {
     const long long at = token * p.top_k + j;
     p.chosen[at] = expert;
     p.gates[at] = gate;
     if (p.plans) few[at] = static_cast<unsigned short>(expert);
-    if (p.ids != nullptr) p.ids[at] = static_cast<unsigned short>(expert);
+    if (p.ids != nullptr) {
+        p.ids[at] = static_cast<unsigned short>(expert);
+        const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
+        if (at == pairs - 1)
+            for (long long i = pairs; i % 8 != 0; ++i) p.ids[i] = 0xffff;
+    }
 }
 
 // Over the 16 lanes of a token: the two neighbours of a pair, of four, of eight, of all.
@@ -95,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
     // different banks.
     constexpr int kLane = kPer + 2, kWords = 16 * kLane + 2;
     __shared__ __attribute__((aligned(16))) double space[kTokens * kWords];
-    __shared__ float bias[kPer * 16];
+    __shared__ float bias[kPer * 16];  // zeros without one
     __shared__ __attribute__((aligned(16))) unsigned short few[kFewPairs];
     __shared__ int picked[kTokens][MCHIP_ROUTE_MAX_TOP_K];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l = lane % 16, row = lane / 16;
@@ -117,7 +123,8 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
 #pragma unroll
         for (int i = 0; i < kPer / 4; ++i) four[i] = load_four<kType>(p.logits, from + e0 + 4 * i, p.experts - e0 - 4 * i);
     }
-    if (static_cast<int>(threadIdx.x) < p.experts) bias[threadIdx.x] = p.bias != nullptr ? p.bias[threadIdx.x] : 0.0f;
+    if (threadIdx.x < kPer * 16)
+        bias[threadIdx.x] = p.bias != nullptr && static_cast<int>(threadIdx.x) < p.experts ? p.bias[threadIdx.x] : 0.0f;
     __syncthreads();
     bool bad = false;
     double key[kPer], top = kNone;
@@ -136,30 +143,43 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
     if (!p.by_logit || (soft && !p.normalize) || p.groups > 1) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) mine[l * kLane + i] = key[i];
-        // An expert that is masked out stays so whatever its bias.
-        const auto key_of = [&](double s, int i) {
-            const double k = s + static_cast<double>(bias[e0 + i]);
-            return k != k ? kNone : k;
-        };
-        if (!p.by_logit || (soft && !p.normalize)) {
-            const int count = min(kPer, p.experts - e0);
-#pragma unroll 2
-            for (int i = 0; i < count; ++i) {
-                const double logit = mine[l * kLane + i];
-                const double e = exp(soft ? logit - top : -logit);
-                const double s = soft ? e : 1.0 / (1.0 + e);
-                // A softmax's before the division, -1 where masked out.
-                if (logit != kNone) total += s;
-                if (!p.by_logit) mine[l * kLane + i] = logit == kNone ? (soft ? -1.0 : kNone) : soft ? s : key_of(s, i);
+        // Four experts at a time, straight through, so that their chains of dependent steps
+        // run beside each other. An expert that is masked out stays so whatever its bias.
+        const auto fours = [&](auto step) {
+#pragma unroll 1
+            for (int i = 0; i < kPer; i += 4) {
+                double* at = mine + l * kLane + i;
+                double v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = at[e];
+                step(v, i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) at[e] = v[e];
             }
-            total = over_token(total, both);
-            if (!p.by_logit && soft) {
-                const double share = 1.0 / total;
-#pragma unroll 2
-                for (int i = 0; i < count; ++i) {
-                    const double s = mine[l * kLane + i];
-                    mine[l * kLane + i] = s < 0.0 ? kNone : key_of(s * share, i);
-                }
+        };
+        const auto key_of = [&](double s, double logit, int e) {
+            const double k = s + static_cast<double>(bias[e0 + e]);
+            return logit != logit ? logit : logit == kNone || k != k ? kNone : k;
+        };
+        if (!p.by_logit && !soft) {
+            fours([&](double (&v)[4], int i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = key_of(1.0 / (1.0 + exp(-v[e])), v[e], i + e);
+            });
+        } else if (soft && (!p.by_logit || !p.normalize)) {
+            double share = 0.0;
+#pragma unroll 1
+            for (int pass = 0; pass < (p.by_logit ? 1 : 2); ++pass) {
+                // The sum of the exponentials, and the keys behind it.
+                fours([&](double (&v)[4], int i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const double logit = v[e], x = exp(logit - top);
+                        if (pass == 0) total += logit > kNone ? x : 0.0;  // none that is masked out, or no expert
+                        else v[e] = key_of(x * share, logit, i + e);
+                    }
+                });
+                if (pass == 0) total = over_token(total, both), share = 1.0 / total;
             }
         }
     }
@@ -290,14 +310,15 @@ __global__ __launch_bounds__(kPlanThreads) void make_plan(const unsigned short* 
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const int from = at + i * 512;
-            eight[i] = *reinterpret_cast<const u16x8*>(ids + (from < pairs ? from : 0));
+            eight[i] = u16x8{0xffff, 0xffff, 0xffff, 0xffff, 0xffff, 0xffff, 0xffff, 0xffff};
+            if (from < pairs) eight[i] = *reinterpret_cast<const u16x8*>(ids + from);
         }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             mine[i] = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int id = at + i * 512 + j < pairs ? eight[i][j] : 0xffff;
+                const int id = eight[i][j];
                 below += static_cast<unsigned>(id - e) >> 31;
                 mine[i] |= id == e ? 1u << j : 0u;
             }
@@ -387,7 +408,7 @@ extern "C" {
 
 long long mchip_route_workspace_bytes(int tokens, int experts, int top_k) {
     if (tokens < 1 || experts < 1 || top_k < 1 || top_k > MCHIP_ROUTE_MAX_TOP_K || plans_itself(tokens, top_k)) return 0;
-    return (static_cast<long long>(tokens) * top_k * 2 + 255) / 256 * 256;
+    return (static_cast<long long>(tokens) * top_k * 2 + 255) / 256 * 256;  // whole eights of ids
 }
 
 int mchip_launch_route(const mchip_route_args* args, void* stream, const char** why) {
