@@ -42,20 +42,23 @@ __device__ __forceinline__ float activate(float u, int act) {
 // (a large result: 4096x4096 bf16 sums of one step in 14.6 us, 16.8 with plain stores).
 template <int kType, bool kPast = true>
 __device__ __forceinline__ void store_eight(void* c, long long at, const float (&v)[8], int left) {
-    const auto put = [](auto value, auto* to) {
-        if constexpr (kPast) __builtin_nontemporal_store(value, to);
-        else *to = value;
-    };
     if (left >= 8) {
         if constexpr (kType == kF32) {
             f32x4_loose* d = reinterpret_cast<f32x4_loose*>(static_cast<float*>(c) + at);
-            put(f32x4{v[0], v[1], v[2], v[3]}, d);
-            put(f32x4{v[4], v[5], v[6], v[7]}, d + 1);
+            const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+            if constexpr (kPast) {
+                __builtin_nontemporal_store(lo, d);
+                __builtin_nontemporal_store(hi, d + 1);
+            } else {
+                d[0] = lo, d[1] = hi;
+            }
         } else {
             u16x8 h;
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] = to_16<kType>(v[e]);
-            put(h, reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(c) + at));
+            u16x8_loose* d = reinterpret_cast<u16x8_loose*>(static_cast<unsigned short*>(c) + at);
+            if constexpr (kPast) __builtin_nontemporal_store(h, d);
+            else *d = h;
         }
         return;
     }

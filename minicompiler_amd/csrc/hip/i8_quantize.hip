@@ -169,9 +169,8 @@ __device__ __forceinline__ void store_two(void* p, long long at, float a, float 
 }
 
 // A block takes 2 kAcross columns whole: kAcross lanes a row of them, two columns each,
-// and eight rows down. What one step of the block covers (8 x 1024 / kAcross rows) stays
-// in registers between the columns' largest magnitudes and the codes; of longer columns
-// the steps before the last are read a second time, from a cache.
+// and eight rows down, which stay in registers between the columns' largest magnitudes
+// and the codes. For up to 8 x 1024 / kAcross rows.
 constexpr int kColumnThreads = 1024;
 
 template <int kType, int kAcross>
@@ -180,34 +179,26 @@ __global__ __launch_bounds__(kColumnThreads) void quantize_columns(const void* _
                                                                    float* __restrict__ scales,
                                                                    void* __restrict__ values, int k, int n,
                                                                    int chunks) {
-    constexpr int kDown = kColumnThreads / kAcross;
     __shared__ unsigned tops[kColumnThreads / 64][2 * kAcross];
     __shared__ float found[2 * kAcross];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int across = threadIdx.x % kAcross, down = threadIdx.x / kAcross;
+    const int across = threadIdx.x % kAcross, chunk = threadIdx.x / kAcross;
     // Blocks go to the XCDs in turn; neighbouring columns to one, whose L2 has the lines that they share.
     const unsigned all = gridDim.x, mine = blockIdx.x % 8 * (all / 8) + blockIdx.x / 8;
     const unsigned block = blockIdx.x < all / 8 * 8 ? mine : blockIdx.x;
     const long long col = static_cast<long long>(block) * 2 * kAcross + 2 * across;
     const int left = static_cast<int>(min(static_cast<long long>(n) - col, 2LL));
-    const int steps = (chunks + kDown - 1) / kDown;
     float v[2][8];
-    const auto load = [&](int step) {
-        const int row = (step * kDown + down) * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const f32x2 two = load_two<kType>(w, (row + e) * ld + col, row + e < k ? left : 0);
-            v[0][e] = two[0], v[1][e] = two[1];
-        }
-    };
     unsigned top[2] = {0, 0};
-    for (int step = 0; step < steps; ++step) {
-        load(step);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            top[0] = max(top[0], magnitude(v[0][e]));
-            top[1] = max(top[1], magnitude(v[1][e]));
-        }
+    for (int e = 0; e < 8; ++e) {
+        const f32x2 two = load_two<kType>(w, (chunk * 8 + e) * ld + col, chunk * 8 + e < k ? left : 0);
+        v[0][e] = two[0], v[1][e] = two[1];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        top[0] = max(top[0], magnitude(v[0][e]));
+        top[1] = max(top[1], magnitude(v[1][e]));
     }
 #pragma unroll
     for (int d = kAcross; d < 64; d *= 2) {
@@ -226,21 +217,87 @@ __global__ __launch_bounds__(kColumnThreads) void quantize_columns(const void* _
             scales[static_cast<long long>(block) * 2 * kAcross + threadIdx.x] = s;
     }
     __syncthreads();
-    const Scale c[2] = {of_scale(found[2 * across]), of_scale(found[2 * across + 1])};
-    for (int step = steps - 1; step >= 0; --step) {
-        if (step != steps - 1) load(step);
-        const int chunk = step * kDown + down;
-        if (chunk >= chunks) continue;
+    if (chunk >= chunks) return;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const u32x2 packed = codes_of(v[j], c[j]);
-            if (j < left) codes[(col + j) * chunks + chunk] = packed;
-        }
-        if (values == nullptr) continue;
+    for (int j = 0; j < 2; ++j) {
+        const u32x2 packed = codes_of(v[j], of_scale(found[2 * across + j]));
+        if (j < left) codes[(col + j) * chunks + chunk] = packed;
+    }
+    if (values == nullptr) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (chunk * 8 + e < k) store_two<kType>(values, (chunk * 8LL + e) * n + col, v[0][e], v[1][e], left);
+}
+
+// More rows, in three launches: scales cleared, found (the largest of the scales of parts
+// of a column is the column's: rounding keeps the order), and the codes. A block of the
+// last two takes 128 columns, a wave whole lines of a row, two columns a lane.
+constexpr int kAcrossAll = 128, kPartRows = 512;
+
+__global__ __launch_bounds__(256) void clear_scales(float* __restrict__ scales, int n) {
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
+    if (i < static_cast<unsigned>(n)) scales[i] = 0.0f;
+}
+
+template <int kType>
+__global__ __launch_bounds__(kColumnThreads) void column_scales(const void* __restrict__ w, long long ld,
+                                                                unsigned* __restrict__ scales, int k, int n) {
+    constexpr int kWaves = kColumnThreads / 64;
+    __shared__ unsigned tops[kWaves][kAcrossAll];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const long long col = static_cast<long long>(blockIdx.x) * kAcrossAll + 2 * lane;
+    const int left = static_cast<int>(min(static_cast<long long>(n) - col, 2LL));
+    unsigned top[2] = {0, 0};
+#pragma unroll 8
+    for (int i = 0; i < kPartRows / kWaves; ++i) {
+        const long long row = static_cast<long long>(blockIdx.y) * kPartRows + i * kWaves + wave;
+        const f32x2 two = load_two<kType>(w, row * ld + col, row < k ? left : 0);
+        top[0] = max(top[0], magnitude(two[0]));
+        top[1] = max(top[1], magnitude(two[1]));
+    }
+    tops[wave][2 * lane] = top[0], tops[wave][2 * lane + 1] = top[1];
+    __syncthreads();
+    if (threadIdx.x >= kAcrossAll) return;
+    unsigned most = 0;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) most = max(most, tops[u][threadIdx.x]);
+    const long long at = static_cast<long long>(blockIdx.x) * kAcrossAll + threadIdx.x;
+    if (at < n && most != 0) atomicMax(scales + at, __builtin_bit_cast(unsigned, scale_of(most)));
+}
+
+// A wave eight rows, the block 128: a line of codes for each column, by way of LDS.
+template <int kType>
+__global__ __launch_bounds__(kColumnThreads) void column_codes(const void* __restrict__ w, long long ld,
+                                                               unsigned char* __restrict__ codes,
+                                                               const float* __restrict__ scales,
+                                                               void* __restrict__ values, int k, int n, int row_bytes) {
+    constexpr int kStride = kLine + 16;
+    __shared__ __attribute__((aligned(16))) unsigned char lines[kAcrossAll * kStride];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const long long col0 = static_cast<long long>(blockIdx.x) * kAcrossAll, col = col0 + 2 * lane;
+    const long long row = static_cast<long long>(blockIdx.y) * kLine + wave * 8;
+    const int left = static_cast<int>(min(static_cast<long long>(n) - col, 2LL));
+    float v[2][8], s[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j] = j < left ? scales[col + j] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const f32x2 two = load_two<kType>(w, (row + e) * ld + col, row + e < k ? left : 0);
+        v[0][e] = two[0], v[1][e] = two[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<u32x2*>(lines + (2 * lane + j) * kStride + wave * 8) = codes_of(v[j], of_scale(s[j]));
+    if (values != nullptr) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (chunk * 8 + e < k) store_two<kType>(values, (chunk * 8LL + e) * n + col, v[0][e], v[1][e], left);
+            if (row + e < k) store_two<kType>(values, (row + e) * n + col, v[0][e], v[1][e], left);
     }
+    __syncthreads();
+    const int c = threadIdx.x / 8, part = threadIdx.x % 8 * 16;
+    if (col0 + c < n)
+        *reinterpret_cast<u32x4*>(codes + (col0 + c) * row_bytes + static_cast<long long>(blockIdx.y) * kLine + part) =
+            *reinterpret_cast<const u32x4*>(lines + c * kStride + part);
 }
 
 const char* refusal(int dtype, const void* x, long long ld, const void* codes, const float* scales, int outer, int inner,
@@ -304,20 +361,37 @@ int launch_rows(const void* x, long long ld, void* codes, float* scales, int row
 template <int kType>
 int launch_columns(const void* w, long long ld, void* codes, float* scales, int k, int n, void* values,
                    hipStream_t stream, const char** why) {
-    const int cus = device_cus();
-    const auto go = [&](auto kernel, int across) {
+    const auto whole = [&](auto kernel, int across) {
         const long long blocks = (static_cast<long long>(n) + 2 * across - 1) / (2 * across);
-        if (!fits_launch(blocks, kColumnThreads)) {
-            *why = "more columns than one launch takes (134217696)";
-            return static_cast<int>(hipErrorInvalidValue);
-        }
         return launch_kernel(kernel, static_cast<unsigned>(blocks), kColumnThreads, 0, stream, w, ld,
                              static_cast<u32x2*>(codes), scales, values, k, n, padded_k(k) / 8);
     };
-    // Wide strips read the most of a line at once, narrow ones make more blocks.
-    if (n >= 32LL * cus) return go(quantize_columns<kType, 16>, 16);
-    if (n >= 16LL * cus / 2) return go(quantize_columns<kType, 8>, 8);
-    return go(quantize_columns<kType, 4>, 4);
+    // Few enough rows for one launch, and not so many columns that their narrow strips take
+    // longer than the two launches more (2048 rows by 8192 columns of fp32 103 us).
+    if (k <= 1024 && n <= (1 << 22)) return whole(quantize_columns<kType, 8>, 8);
+    if (k <= 2048 && static_cast<long long>(k) * n <= (1 << 22)) return whole(quantize_columns<kType, 4>, 4);
+    const unsigned across = static_cast<unsigned>((static_cast<long long>(n) + kAcrossAll - 1) / kAcrossAll);
+    if (!fits_launch(across, kColumnThreads)) {
+        *why = "more columns than one launch takes (536870784)";
+        return hipErrorInvalidValue;
+    }
+    int rc = launch_kernel(clear_scales, static_cast<unsigned>((static_cast<long long>(n) + 255) / 256), 256, 0, stream, scales, n);
+    // As much of k at a time as a launch takes.
+    constexpr int kParts = 65535;
+    for (long long from = 0; rc == hipSuccess && from < k; from += static_cast<long long>(kParts) * kPartRows) {
+        const int rows = static_cast<int>(std::min<long long>(k - from, static_cast<long long>(kParts) * kPartRows));
+        rc = launch_kernel(column_scales<kType>, dim3(across, static_cast<unsigned>((rows + kPartRows - 1) / kPartRows)),
+                           kColumnThreads, 0, stream, offset<kType>(w, from * ld), ld, reinterpret_cast<unsigned*>(scales),
+                           rows, n);
+    }
+    for (long long from = 0; rc == hipSuccess && from < k; from += static_cast<long long>(kParts) * kLine) {
+        const int rows = static_cast<int>(std::min<long long>(k - from, static_cast<long long>(kParts) * kLine));
+        rc = launch_kernel(column_codes<kType>, dim3(across, static_cast<unsigned>((rows + kLine - 1) / kLine)),
+                           kColumnThreads, 0, stream, offset<kType>(w, from * ld), ld,
+                           static_cast<unsigned char*>(codes) + from, scales, offset<kType>(values, from * n), rows, n,
+                           padded_k(k));
+    }
+    return rc;
 }
 
 }  // namespace
