@@ -153,15 +153,32 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
     i32x4 acc[kM * kN];
 #pragma unroll
     for (int i = 0; i < kM * kN; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    // Of small dense blocks the next line is on its way while one is multiplied (one row by
+    // 14336x4096 10.5 us, 10.9 without); larger ones lose a block per CU to it (1000x1001x1023
+    // 8.0 and 6.3), and on a plan it gains nothing.
+    constexpr bool kAhead = kMode == kDense && kM * kN <= 4;
+    i32x4 a_next[2][kM], b_next[2][kN];
+    const auto load = [&](int at) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < kM; ++i) a_next[h][i] = *reinterpret_cast<const i32x4*>(a[i] + at + 64 * h);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) b_next[h][j] = *reinterpret_cast<const i32x4*>(b[j] + at + 64 * h);
+        }
+    };
+    if (kAhead && wave * kLine < p.row_bytes) load(wave * kLine);
     for (int at = wave * kLine; at < p.row_bytes; at += kWaves * kLine) {
+        if (!kAhead) load(at);
         i32x4 av[2][kM], bv[2][kN];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int i = 0; i < kM; ++i) av[h][i] = *reinterpret_cast<const i32x4*>(a[i] + at + 64 * h);
+            for (int i = 0; i < kM; ++i) av[h][i] = a_next[h][i];
 #pragma unroll
-            for (int j = 0; j < kN; ++j) bv[h][j] = *reinterpret_cast<const i32x4*>(b[j] + at + 64 * h);
+            for (int j = 0; j < kN; ++j) bv[h][j] = b_next[h][j];
         }
+        if (kAhead && at + kWaves * kLine < p.row_bytes) load(at + kWaves * kLine);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -536,32 +553,35 @@ bool tiles_fit(const Product& p) {
     return a_rows * p.row_bytes < (1LL << 31);
 }
 
-// What a variant takes, in microseconds: a launch and `k` (in units of 4096) times its rounds.
-// Measured, 4096 wide and deep unless said: 16x32 blocks 5.5 (16 rows, 128 of them), 5.8 (32,
-// 256), 8.3 (64, 512), 12.0 (128), 20.6 (256); 32x32 6.5 (32 rows), 7.0 (64), 10.1 (128),
-// 15.9 (256); 32x64 9.1, 8.9, 8.6, 13.6 and 23.2 (512); 128x128 tiles 17.3 (64 rows), 18.5
-// (512), 22.1 (1024), 35.0 (2048), 215 (4096 by 14336); 256x256 39 (512), 51 (2048), 57
-// (4096), 212 (4096 by 14336). 64x64 blocks were nowhere a fifth faster than the next.
-// On a plan tiles take longer (rows gathered, weights from memory: 2048 tokens x 8 of 64
+// What a variant takes, in microseconds, by its rounds of blocks and k (in units of 4096).
+// Measured, 4096 wide and deep unless said: 16x32 blocks 5.5 (16 rows, 128 of them), 5.8 (32
+// rows, 256), 8.3 (64, 512), 12.0 (128), 20.6 (256); 32x32 6.5 (32 rows), 7.0 (64), 10.1
+// (128), 15.9 (256); 32x64 9.1, 8.9, 8.6, 13.6 and 23.2 (512); 128x128 tiles 17.3 (64 rows),
+// 18.5 (512), 22.1 (1024), 35.0 (2048), 215 (4096 by 14336); 256x256 39 (512), 51 (2048),
+// 57 (4096), 212 (4096 by 14336). 4096x4096 of k = 128 and 1024: 57 and 113, 61 and 109, 40
+// and 74, 12.7 and 22.4, 12.5 and 21.6. 64x64 blocks were nowhere a fifth faster than the next.
+// On a plan all take longer (rows gathered, weights from memory: 2048 tokens x 8 of 64
 // experts, 2048 deep, 1024 gated columns: 128x128 117, 256x256 105; 1024 tokens 78 and 98;
 // 128 tokens 55.8, 60.4 and 60.1 by 16x32 blocks; 64 tokens 55.5, 60.6 and 48.3).
 struct Cost {
     double k, cus;
-    double few(double blocks, double one, double each, bool plan) const {
-        return 2.5 + k * (plan ? 1.8 : 1.0) * (blocks <= cus ? one : each * std::max(1.0, blocks / (2.0 * cus)));
+    bool plan;
+    double few(double blocks, double one, double fixed, double each) const {
+        return 2.5 + (plan ? 1.8 : 1.0) * (blocks <= cus ? 0.5 + one * k : (fixed + each * k) * std::max(1.0, blocks / (2.0 * cus)));
     }
-    double small_tiles(double tiles, bool plan) const {
+    double small_tiles(double tiles) const {
         if (plan) return 5.0 + 50.0 * k * std::ceil(tiles / (2.0 * cus));
-        return 5.0 + k * (2.0 * tiles <= cus ? 13.0 : tiles <= cus ? 17.0 : 30.0 * std::ceil(tiles / (2.0 * cus)));
+        if (tiles <= cus) return 5.0 + k * (2.0 * tiles <= cus ? 13.0 : 17.0);
+        return 5.0 + (3.5 + 24.0 * k) * std::max(1.0, std::ceil(tiles / cus) / 2.0);
     }
-    double large_tiles(double rounds, bool plan) const { return 4.0 + rounds * (8.0 + (plan ? 66.0 : 48.0) * k); }
+    double large_tiles(double rounds) const { return 4.0 + rounds * (8.0 + (plan ? 66.0 : 48.0) * k); }
 };
 
 template <int kMode, bool kGated>
 int launch(const Product& p, hipStream_t stream, const char** why) {
     constexpr bool kPlan = kMode != kDense;
     const double cus = device_cus(), experts = static_cast<double>(std::min(p.experts, p.m));
-    const Cost cost{p.row_bytes / 4096.0, cus};
+    const Cost cost{p.row_bytes / 4096.0, cus, kPlan};
     const double columns = kGated ? 2.0 * p.n : p.n;
     // Blocks, of rows by columns of B; on a plan every second expert's last is half full.
     const auto blocks = [&](int rows, int cols) {
@@ -569,17 +589,17 @@ int launch(const Product& p, hipStream_t stream, const char** why) {
                                   : static_cast<double>(tiles(p.m, rows));
         return down * std::ceil(columns / cols);
     };
-    const double b16 = cost.few(blocks(16, 32), 3.2, 5.0, kPlan), b32 = cost.few(blocks(32, 32), 4.4, 7.3, kPlan),
-                 b64 = cost.few(blocks(32, 64), 6.2, 10.8, kPlan);
+    const double b16 = cost.few(blocks(16, 32), 3.0, 0.8, 4.1), b32 = cost.few(blocks(32, 32), 4.2, 1.6, 7.0),
+                 b64 = cost.few(blocks(32, 64), 6.0, 2.1, 9.5);
     double t128 = 1e30, t256 = 1e30;
     if (tiles_fit<kMode>(p)) {
-        t128 = cost.small_tiles(blocks(128, 128), kPlan);
+        t128 = cost.small_tiles(blocks(128, 128));
         // In rounds and halves of them; dense tiles that leave half a round or more empty run
         // as halves, on a plan a third of the experts' last ones.
         const double all = kPlan ? std::max(experts / 2, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus
                                  : blocks(256, 256) / cus;
         const double rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
-        t256 = cost.large_tiles(rounds, kPlan);
+        t256 = cost.large_tiles(rounds);
     }
     const double best = std::min({b16, b32, b64, t128, t256});
     if (best == t256) return launch_tiles<kMode, kGated, 256>(p, stream, why);

@@ -103,6 +103,22 @@ def test_many_tokens(device, mc, kind, tokens, experts, top_k, n, k, skew):
     check_down(mc, 3, tokens, experts, top_k, n, k, kind, bias=True, skew=skew)
 
 
+# Each kernel by sizes that its rule gives it: blocks of 16x32, 32x32 and 32x64, tiles of 128x128, and of 256x256 with
+# whole, half and short last tiles; even plans and one expert with nearly all.
+VARIANTS = [(40, 16, 4, 520, 256, 1.0), (100, 4, 2, 960, 512, 0.3), (90, 4, 2, 520, 256, 0.5), (200, 4, 2, 1032, 256, 0.5), (700, 8, 4, 1030, 256, 1.0),
+            (1500, 4, 2, 2056, 128, 0.3), (1300, 3, 2, 4100, 256, 4.0), (4000, 2, 1, 4104, 128, 0.3),
+            (4200, 8, 4, 2056, 384, 1.0), (2100, 4, 2, 4096, 1600, 0.4), (2100, 3, 2, 4100, 1500, 3.0)]
+
+
+@pytest.mark.parametrize("kind", sorted(ref.TYPES))
+@pytest.mark.parametrize("tokens,experts,top_k,n,k,skew", VARIANTS)
+def test_by_every_kernel(device, mc, kind, tokens, experts, top_k, n, k, skew):
+    for act in (ref.ACTS[(tokens // 10 + sorted(ref.TYPES).index(kind)) % 3], "swiglu"):
+        print(f"case kernel {kind} {tokens} of {experts} top {top_k} {n}x{k} {act}", flush=True)
+        check_up(mc, n, tokens, experts, top_k, n // 2 if act == "swiglu" else n, k, kind, act, bias=k == 256, skew=skew)
+    check_down(mc, n + 1, tokens, experts, top_k, n, k, kind, bias=k == 128, skew=skew)
+
+
 @pytest.mark.parametrize("tokens", [3, 60, 900])
 @pytest.mark.parametrize("part", [(0, 3), (2, 7), (7, 8), (4, 4 + 1)])
 def test_a_part_of_a_plan_leaves_the_others_alone(device, mc, tokens, part):

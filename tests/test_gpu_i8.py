@@ -153,6 +153,43 @@ def test_product_of_many_tiles(device, mc, kind, m, n, k, act):
     check_product(mc, m + n, m, n, k, kind, act, bias=act is not None)
 
 
+# Each kernel by sizes that its rule gives it: blocks of 16x32, 32x32 and 32x64, tiles of 128x128 and of 256x256 (whole
+# rounds, halves, short last rows), every activation and type, columns that are and are not eights, short k.
+VARIANTS = [(16, 1056, 512), (32, 4104, 200), (60, 4099, 300), (128, 4096, 130), (250, 4090, 260), (600, 4104, 384),
+            (640, 4100, 129), (1025, 2056, 256), (1100, 2049, 1100), (4000, 4090, 128), (3850, 4096, 600), (6100, 4096, 1000)]
+
+
+@pytest.mark.parametrize("kind", sorted(ref.TYPES))
+@pytest.mark.parametrize("m,n,k", VARIANTS)
+def test_product_by_every_kernel(device, mc, kind, m, n, k):
+    for act in (ref.ACTS[(m + sorted(ref.TYPES).index(kind)) % 3], "swiglu"):
+        print(f"case kernel {kind} {m}x{n}x{k} {act}", flush=True)
+        check_product(mc, m + n + k, m, n // 2 if act == "swiglu" else n, k, kind, act, bias=n % 2 == 0)
+
+
+def test_columns_of_b_past_32_bits(device, mc):
+    """B of 2.2 GB: the last columns' offsets pass 2^31."""
+    m, n, k = 20, 17500, 131000
+    kp = ref.padded(k)
+    rng = np.random.default_rng(2)
+    b = mc.DeviceBuffer(n * kp)
+    b.fill_bytes(0)
+    mc.synchronize()
+    last = rng.integers(-127, 128, (64, kp)).astype(np.int8)
+    last[:, k:] = 0
+    assert mc.library().mc_memcpy_htod(b.ptr + (n - 64) * kp, last.ctypes.data, last.nbytes) == 0
+    sb = np.ones(n, dtype=np.float32)
+    a, sa = random_operand(rng, m, k, 20)
+    da, ds = operand(mc, a, sa), mc.DeviceBuffer.from_array(sb)
+    c = Out(mc, m * n * 4)
+    mc.launch_matmul_i8(da[0].ptr, da[1].ptr, b.ptr, ds.ptr, None, None, 0, c.ptr, m, n, k)
+    mc.synchronize()
+    got = c.get(np.float32, (m, n))
+    want, err = ref.scaled(a, sa, last, sb[-64:], None)
+    assert np.all(got[:, :-64] == 0)
+    assert np.all(np.abs(got[:, -64:] - want) <= ref.rounded(want, err, ref.F32))
+
+
 @pytest.mark.parametrize("m", [1, 20, 300])
 def test_sums_at_the_end_of_32_bits(device, mc, m):
     """k = 131071 codes of -128 (never quantised, but codes) and 127: sums up to 2147467264."""
