@@ -157,29 +157,39 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
                 for (int e = 0; e < 4; ++e) at[e] = v[e];
             }
         };
-        const auto key_of = [&](double s, double logit, int e) {
+        // Of a softmax's score, below 0 where masked out; no expert's is no number and stays so.
+        const auto key_of = [&](double s, int e) {
             const double k = s + static_cast<double>(bias[e0 + e]);
-            return logit != logit ? logit : logit == kNone || k != k ? kNone : k;
+            return s != s ? s : s < 0.0 || k != k ? kNone : k;
         };
         if (!p.by_logit && !soft) {
             fours([&](double (&v)[4], int i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = key_of(1.0 / (1.0 + exp(-v[e])), v[e], i + e);
+                for (int e = 0; e < 4; ++e) {
+                    const double logit = v[e], k = 1.0 / (1.0 + exp(-logit)) + static_cast<double>(bias[e0 + i + e]);
+                    v[e] = logit != logit ? logit : logit == kNone || k != k ? kNone : k;
+                }
             });
         } else if (soft && (!p.by_logit || !p.normalize)) {
-            double share = 0.0;
-#pragma unroll 1
-            for (int pass = 0; pass < (p.by_logit ? 1 : 2); ++pass) {
-                // The sum of the exponentials, and the keys behind it.
+            fours([&](double (&v)[4], int i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double logit = v[e], x = exp(logit - top);
+                    total += logit > kNone ? x : 0.0;  // none that is masked out, or no expert
+                    // (+infinity less itself is no number, either: a key of none.)
+                    if (!p.by_logit) v[e] = logit != logit ? logit : logit == kNone || x != x ? -1.0 : x;
+                }
+            });
+            total = over_token(total, both);
+            if (!p.by_logit) {
+                const double share = 1.0 / total;
                 fours([&](double (&v)[4], int i) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const double logit = v[e], x = exp(logit - top);
-                        if (pass == 0) total += logit > kNone ? x : 0.0;  // none that is masked out, or no expert
-                        else v[e] = key_of(x * share, logit, i + e);
+                        const double s = v[e] * share;
+                        v[e] = key_of(s != s && v[e] == v[e] ? -1.0 : s, i + e);
                     }
                 });
-                if (pass == 0) total = over_token(total, both), share = 1.0 / total;
             }
         }
     }

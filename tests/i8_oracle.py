@@ -86,6 +86,7 @@ def route(logits, bias, top_k, score, groups, top_groups, group_best, normalize,
         if score == "softmax":
             top = l.max(-1, keepdims=True)
             e = np.where(top == -np.inf, 0.0, np.exp(l - np.where(top == -np.inf, 0.0, top)))
+            e = np.where(l == -np.inf, 0.0, e)
             total = e.sum(-1, keepdims=True)
             s = np.where(total == 0, 0.0, e / np.where(total == 0, 1.0, total))
         else:

@@ -105,7 +105,8 @@ def test_many_tokens(device, mc, kind, tokens, experts, top_k, n, k, skew):
 
 # Each kernel by sizes that its rule gives it: blocks of 16x32, 32x32 and 32x64, tiles of 128x128, and of 256x256 with
 # whole, half and short last tiles; even plans and one expert with nearly all.
-VARIANTS = [(40, 16, 4, 520, 256, 1.0), (100, 4, 2, 960, 512, 0.3), (90, 4, 2, 520, 256, 0.5), (200, 4, 2, 1032, 256, 0.5), (700, 8, 4, 1030, 256, 1.0),
+VARIANTS = [(40, 16, 4, 520, 256, 1.0), (100, 4, 2, 960, 512, 0.3), (90, 4, 2, 520, 256, 0.5),
+            (200, 4, 2, 1032, 256, 0.5), (700, 8, 4, 1030, 256, 1.0),
             (1500, 4, 2, 2056, 128, 0.3), (1300, 3, 2, 4100, 256, 4.0), (4000, 2, 1, 4104, 128, 0.3),
             (4200, 8, 4, 2056, 384, 1.0), (2100, 4, 2, 4096, 1600, 0.4), (2100, 3, 2, 4100, 1500, 3.0)]
 
