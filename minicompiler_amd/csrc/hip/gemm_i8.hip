@@ -131,8 +131,8 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
         row0 = place.first;
     }
     const int end = place.end;
-    const int b_rows = kGated ? 2 * p.n : p.n;
-    const unsigned char* b0 = p.b + static_cast<long long>(place.expert) * b_rows * p.row_bytes;
+    const long long b_rows = kGated ? 2LL * p.n : p.n;
+    const unsigned char* b0 = p.b + place.expert * b_rows * p.row_bytes;
     const unsigned char *a[kM], *b[kN];
 #pragma unroll
     for (int i = 0; i < kM; ++i) {
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
             if (c_row < 0 || c_row >= p.m) continue;
         }
         const float sa = p.a_scales[a_row];
-        const long long b_row = static_cast<long long>(place.expert) * b_rows + col;
+        const long long b_row = place.expert * b_rows + col;
         // One half's four columns, scaled, with the bias.
         const auto scaled = [&](i32x4 sum, long long at) {
             f32x4 v;
@@ -276,7 +276,7 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
     constexpr int kRowBytes = kPassFrags * 128, kPassRows = kGated ? 64 : 64 * kHalves;
     constexpr int kAcross = (kGated ? kColFrags / 2 : 2) * 4, kBatch = 64 / kAcross;  // lanes along a row, rows at a time
     static_assert(kPasses <= 2 && kPassRows / kBatch % 4 == 0);
-    const long long b_row = static_cast<long long>(expert) * (kGated ? 2 * p.n : p.n);
+    const long long b_row = expert * (kGated ? 2LL * p.n : p.n);
     const int line = lane % 32, half = lane / 32;
     // What goes with rows lane and lane + 64.
     float sa[kHalves], gate[kHalves];
@@ -422,8 +422,8 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
         return static_cast<int>(a_row_of<kMode>(p, row < end ? row : end - 1)) * p.row_bytes;
     };
     // B's rows that the wave fetches: of columns, of gate or of up ones.
-    const int b_col = col0 + (kGated ? wave / 2 : wave) * kShareB, b_rows = kGated ? 2 * p.n : p.n;
-    const long long b0 = static_cast<long long>(expert) * b_rows + (kGated ? wave % 2 * static_cast<long long>(p.n) : 0) + b_col;
+    const int b_col = col0 + (kGated ? wave / 2 : wave) * kShareB;
+    const long long b0 = expert * (kGated ? 2LL * p.n : p.n) + (kGated ? wave % 2 * static_cast<long long>(p.n) : 0) + b_col;
     const __amdgpu_buffer_rsrc_t b = rows_from(p.b + b0 * p.row_bytes, p.n - b_col, p.row_bytes);
     typename T::Sums acc;
     tile_sums<T>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(kTileThreads, kTile == 256 ? 1 : 2) void i8_tiles(c
         } else if (t < full / 8 * 8) {
             t = t % 8 * (full / 8) + t / 8;  // blocks go to the XCDs in turn
         }
-        const unsigned all = static_cast<unsigned>((p.m + kTile - 1) / kTile);
+        const unsigned all = (static_cast<unsigned>(p.m) + kTile - 1) / kTile;
         const unsigned panel = t / (kPanel * p.tiles_n), in = t % (kPanel * p.tiles_n);
         const unsigned high = min(static_cast<unsigned>(kPanel), all - panel * kPanel);
         chunk = panel * kPanel + in % high, tile = in / high;
