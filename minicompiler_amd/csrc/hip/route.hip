@@ -7,8 +7,10 @@
 // Bound by latency, and that by the code that a launch reads into a cold instruction
 // cache: sixteen lanes take a token, a lane 4 to 32 experts next to each other, keys lie
 // in LDS while loops go over them and in registers while the largest are picked, over
-// lanes by DPP. (A wave a token with LDS permutes: 8192 tokens of 256 experts in 35 us;
-// fp32 keys in unrolled code, with fp64 ones behind for what lies too near: 23.)
+// lanes by DPP. 8192 tokens, 8 of 256 experts in groups: 20.3 us, 14.9 of them here and 6.5 in
+// the plan's launch; one token on 64 experts 4.3, plan included. (A wave a token with LDS
+// permutes: 35 us for the choice alone; fp32 keys in unrolled code, with fp64 ones behind for
+// what lies too near: 23.)
 
 #include "i8_device.h"
 
@@ -294,6 +296,8 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
 // A block takes an expert: how many pairs have a lower one is where its slots begin,
 // and its own pairs follow in order. A wave takes 4096 pairs at a time, a lane eight of
 // 512 next to each other (whole lines to a load; 64 to a lane took three times as long).
+// 65536 pairs of 256 experts in 6.5 us; every block reads all ids, twice where they are
+// more than 65536 (16384 tokens, 8 of 384: 64 us with the choice).
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kSteps = 8;
 
 // The sum over the lanes up to this one.
