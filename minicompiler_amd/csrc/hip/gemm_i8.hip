@@ -459,10 +459,13 @@ __global__ __launch_bounds__(kTileThreads, kTile == 256 ? 1 : 2) void i8_tiles(c
     unsigned t = blockIdx.x, chunk, tile;
     int half = 0;
     if constexpr (kMode == kDense) {
+        // Blocks go to the XCDs in turn.
+        const auto in_turn = [](unsigned i, unsigned all) { return i < all / 8 * 8 ? i % 8 * (all / 8) + i / 8 : i; };
         if (t >= full) {
-            half = 1 + static_cast<int>((t - full) % 2), t = full + (t - full) / 2;
-        } else if (t < full / 8 * 8) {
-            t = t % 8 * (full / 8) + t / 8;  // blocks go to the XCDs in turn
+            const unsigned part = in_turn(t - full, gridDim.x - full);
+            half = 1 + static_cast<int>(part % 2), t = full + part / 2;
+        } else {
+            t = in_turn(t, full);
         }
         const unsigned all = (static_cast<unsigned>(p.m) + kTile - 1) / kTile;
         const unsigned panel = t / (kPanel * p.tiles_n), in = t % (kPanel * p.tiles_n);
@@ -571,9 +574,11 @@ bool tiles_fit(const Product& p) {
 // Measured, 4096 wide and deep unless said: 16x32 blocks 5.5 (16 rows, 128 of them), 5.8 (32
 // rows, 256), 8.3 (64, 512), 12.0 (128), 20.6 (256); 32x32 6.5 (32 rows), 7.0 (64), 10.1
 // (128), 15.9 (256); 32x64 9.1, 8.9, 8.6, 13.6 and 23.2 (512); 128x128 tiles 17.3 (64 rows),
-// 18.5 (512), 22.1 (1024), 35.0 (2048), 215 (4096 by 14336); 256x256 39 (512), 51 (2048),
-// 57 (4096), 212 (4096 by 14336). 4096x4096 of k = 128 and 1024: 57 and 113, 61 and 109, 40
-// and 74, 12.7 and 22.4, 12.5 and 21.6. 64x64 blocks were nowhere a fifth faster than the next.
+// 18.4 (512), 20.8 (1024), 35.3 (2048), 68.8 (4096), 103 (6144), 237 (4096 by 14336), 251 (4096, k
+// 16384), 516 (8192^3); 256x256 39.5 (1024), 50.7 (2048), 58.9, 108, 222, 204, 432. 4096x4096 of k =
+// 128 and 1024: 57 and 113, 61 and 109, 40 and 74, 12.0 and 24.6, 12.2 and 22.9; 4096x14336 of
+// 1024: 78.0 and 78.5 by tiles. 64x64 blocks were nowhere a fifth faster than the next. (Half of
+// a large tile takes 0.87 of it: fetches bound it.)
 // On a plan all take longer (rows gathered, weights from memory: 2048 tokens x 8 of 64
 // experts, 2048 deep, 1024 gated columns: 128x128 117, 256x256 105; 1024 tokens 78 and 98;
 // 128 tokens 55.8, 60.4 and 60.1 by 16x32 blocks; 64 tokens 55.5, 60.6 and 48.3).
@@ -586,9 +591,9 @@ struct Cost {
     double small_tiles(double tiles) const {
         if (plan) return 5.0 + 50.0 * k * std::ceil(tiles / (2.0 * cus));
         if (tiles <= cus) return 5.0 + k * (2.0 * tiles <= cus ? 13.0 : 17.0);
-        return 5.0 + (3.5 + 24.0 * k) * std::max(1.0, std::ceil(tiles / cus) / 2.0);
+        return 3.0 + (3.0 + 30.5 * k) * std::ceil(tiles / cus) / 2.0;
     }
-    double large_tiles(double rounds) const { return 4.0 + rounds * (8.0 + (plan ? 66.0 : 48.0) * k); }
+    double large_tiles(double rounds) const { return plan ? 4.0 + rounds * (8.0 + 66.0 * k) : 3.5 + rounds * (6.5 + 49.5 * k); }
 };
 
 template <int kMode, bool kGated>
@@ -608,11 +613,16 @@ int launch(const Product& p, hipStream_t stream, const char** why) {
     double t128 = 1e30, t256 = 1e30;
     if (tiles_fit<kMode>(p)) {
         t128 = cost.small_tiles(blocks(128, 128));
-        // In rounds and halves of them; dense tiles that leave half a round or more empty run
-        // as halves, on a plan a third of the experts' last ones.
-        const double all = kPlan ? std::max(experts / 2, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus
-                                 : blocks(256, 256) / cus;
-        const double rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
+        double rounds;
+        if (kPlan) {
+            // In rounds and halves of them; a third of the experts' last tiles are halves.
+            const double all = std::max(experts / 2, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus;
+            rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
+        } else {
+            // Tiles that leave half a round or more empty run as halves.
+            const double all = blocks(256, 256), rest = std::fmod(all, cus);
+            rounds = std::floor(all / cus) + (rest == 0.0 ? 0.0 : rest <= cus / 2 ? 0.87 : 1.0);
+        }
         t256 = cost.large_tiles(rounds);
     }
     const double best = std::min({b16, b32, b64, t128, t256});
