@@ -579,9 +579,10 @@ bool tiles_fit(const Product& p) {
 // 128 and 1024: 57 and 113, 61 and 109, 40 and 74, 12.0 and 24.6, 12.2 and 22.9; 4096x14336 of
 // 1024: 78.0 and 78.5 by tiles. 64x64 blocks were nowhere a fifth faster than the next. (Half of
 // a large tile takes 0.87 of it: fetches bound it.)
-// On a plan all take longer (rows gathered, weights from memory: 2048 tokens x 8 of 64
-// experts, 2048 deep, 1024 gated columns: 128x128 117, 256x256 105; 1024 tokens 78 and 98;
-// 128 tokens 55.8, 60.4 and 60.1 by 16x32 blocks; 64 tokens 55.5, 60.6 and 48.3).
+// On a plan all take longer (rows gathered, weights from memory). Tokens x 8 of 64 experts, 2048
+// deep, 1024 gated columns, by 128x128 and 256x256: 128 tokens 56.1 and 61.3, 512 58 and 62,
+// 1024 84 and 79, 2048 121 and 123, 4096 200 and 186; by 16x32 blocks, 128 tokens 60.1, 64 tokens
+// 48.3 (55.5, 60.6). Down, 1024 deep, 2048 columns: 512 tokens 45 and 49, 2048 110 and 121.
 struct Cost {
     double k, cus;
     bool plan;
@@ -615,8 +616,9 @@ int launch(const Product& p, hipStream_t stream, const char** why) {
         t128 = cost.small_tiles(blocks(128, 128));
         double rounds;
         if (kPlan) {
-            // In rounds and halves of them; a third of the experts' last tiles are halves.
-            const double all = std::max(experts / 2, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus;
+            // In rounds and halves of them; a third of the experts' last tiles are halves, which
+            // take 0.7 of a tile.
+            const double all = std::max(experts * 0.7, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus;
             rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
         } else {
             // Tiles that leave half a round or more empty run as halves.
