@@ -355,7 +355,7 @@ MC_API int mc_quantize_i8_columns(int dtype, const void* b, long long ld, void* 
  * bias) for A of m and B of n i8 rows of k: exact 32-bit sums, the rest in fp32
  * and rounded once. bias [n], fp32, or NULL. activation: 0 ReLU, 1 GELU (tanh
  * form), 2 SwiGLU (B and bias have 2 n rows, n gate rows first, act =
- * gate sigmoid(gate) up), 3 none. k at most 131071 (128^2 k < 2^31). */
+ * gate sigmoid(gate) up), 3 none. k at most 131071 (128^2 k < 2^31), n 2^30. */
 MC_API int mc_launch_matmul_i8(const void* a_codes, const float* a_scales, const void* b_codes, const float* b_scales,
                                const float* bias, int activation, int c_dtype, void* c, int m, int n, int k,
                                void* stream);

@@ -9,7 +9,7 @@
 // experts, 2048 by 2 x 1024, 8.9). Blocks of 16x32 to 32x64 take all of k, without LDS
 // before the end: a wave's loads are in flight at once (1000x1001x1023 7.0 us, 4096 of k and
 // columns by 32 rows 5.5). Many rows: tiles of 128x128 or 256x256 (gemm_i8_tiles.h; on the
-// plan of 2048 tokens, 8 of 64 experts, up 105-116 us, down 111).
+// plan of 2048 tokens, 8 of 64 experts, up 105-124 us by the chip, down 111).
 //
 // Down keeps each pair's product in fp32 until the token's pairs are summed in their order:
 // 16-bit ones would save half of 268 MB there (2048 tokens, 21 of 111 us in the sum) and

@@ -9,8 +9,8 @@
 // with an infinity or a NaN has the scale NaN and codes 0.
 //
 // Bound by HBM, and for little by the launch. Numbers are read once and stay in registers
-// between the largest magnitude and the codes: 8192x2048 fp32 with its values 27.7 us (151
-// MB at 5.5 TB/s; 32.7 where a second pass reads again), 4096x14336 bf16 52 (5.65 TB/s),
+// between the largest magnitude and the codes: 8192x2048 fp32 with its values 28-29 us (151
+// MB at 5.3 TB/s; 32.7 where a second pass reads again), 4096x14336 bf16 52 (5.65 TB/s),
 // one row of 4096 4.3 (2.1 in the kernel). By columns too where a block holds them
 // (1001x2047 fp16 7.6 us); taller ones are read twice, mostly from the last-level cache
 // (k = 14336 by 1000 fp16 35 us; k = 4096 by 14336 bf16 101).
