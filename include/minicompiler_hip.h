@@ -365,15 +365,18 @@ MC_API int mc_launch_matmul_i8(const void* a_codes, const float* a_scales, const
  *   key = score + bias ([experts], fp32, or NULL: the choice alone goes by it);
  *   groups > 1: experts in that many equal groups, one after the other; the
  *   top_groups groups with the largest sum of their group_best (1 or 2) largest
- *   keys stay (1 for groups of one expert);
+ *   keys stay, ties to the lower group; a key of -infinity is left out of the
+ *   sum (of one key where a group has no second), and a group of none but such
+ *   comes after all others;
  *   the top_k largest keys among them, largest first, ties to the lower index;
  *   gates = their scores, with normalize divided by their sum (0 where that is
  *   0), times scale.
  * Without bias, and unless groups > 1 with group_best 2, logits are compared as they are.
- * A logit of -infinity is never chosen before another, whatever its bias, and
- * its score is 0 (all of a token's: gates 0); a NaN logit counts as
- * -infinity in the choice and makes the token's gates NaN, and so does, by
- * softmax, +infinity. A key that is NaN counts as -infinity.
+ * A logit of -infinity is never chosen before another of the groups that stay,
+ * whatever its bias (its key is -infinity), and its score is 0 (all of a
+ * token's: gates 0); a NaN logit counts as -infinity in the choice and makes the
+ * token's gates NaN, and so does, by softmax, +infinity. A key that is NaN
+ * counts as -infinity.
  * chosen, gates: [tokens, top_k]. order, offsets (both or neither NULL): the
  * plan: a pair is token x top_k + place, order [tokens x top_k] all pairs, sorted
  * by expert and for one expert by pair; expert e's "slots" are offsets[e] to

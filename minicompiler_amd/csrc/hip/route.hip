@@ -215,8 +215,9 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
                     second = larger(second, __builtin_fmin(first, k));
                     first = larger(first, k);
                 }
-                sum[q] = p.group_best == 2 && p.each > 1 ? first + second : first;
-                if (sum[q] != sum[q]) sum[q] = kNone;
+                // An expert that is masked out takes nothing from the group's others: only a group
+                // of none but such is worth none.
+                sum[q] = p.group_best == 2 && second > kNone ? first + second : first;
             }
         }
         __builtin_amdgcn_wave_barrier();
