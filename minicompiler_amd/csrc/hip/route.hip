@@ -139,8 +139,9 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
         top = larger(top, key[i]);
     }
     top = over_token(top, larger);
-    bad = (__ballot(bad) >> (16 * row) & 0xffffull) != 0;
     const bool soft = p.score == MCHIP_ROUTE_SOFTMAX;
+    // Over +infinity a softmax is no number, though the experts that are chosen may be others.
+    bad = (__ballot(bad) >> (16 * row) & 0xffffull) != 0 || (soft && top == -kNone);
     double total = 0.0;
     if (!p.by_logit || (soft && !p.normalize) || p.groups > 1) {
 #pragma unroll
