@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
             c_row = p.order[row];
             if (c_row < 0 || c_row >= p.m) continue;
         }
-        const float sa = p.a_scales[a_row];
+        const RowScale sa = row_scale(p.a_scales[a_row]);
         const long long b_row = place.expert * b_rows + col;
         // One half's four columns, scaled, with the bias.
         const auto scaled = [&](i32x4 sum, long long at) {
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
             for (int e = 0; e < 4; ++e) {
                 v[e] = 0.0f;
                 if (e < left) {
-                    v[e] = static_cast<float>(sum[e]) * sa * p.b_scales[at + e];
+                    v[e] = static_cast<float>(sum[e]) * sa.s * p.b_scales[at + e] * sa.back;
                     if (p.bias != nullptr) v[e] += p.bias[at + e];
                 }
             }
@@ -279,10 +279,12 @@ __device__ __forceinline__ long long a_row_of(const Product& p, long long row) {
 // `end`, columns col0 on, by way of the wave's share of LDS (`lds`), so that a short loop
 // (a launch meets a cold instruction cache) stores whole lines. In passes: 64 columns of
 // all rows, or (kGated) 64 rows with both halves of their columns. Block c of 16 bytes of
-// row r lies at c ^ (r % 16).
+// row r lies at c ^ (r % 16). What goes with a row lies in `side`, 16 bytes each: in
+// registers it would be held through everything, and the large tiles have none to spare.
 template <int kMode, bool kGated, int kOut, typename T>
-__device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Product& p, const typename T::Sums& acc,
-                                           int expert, long long row0, long long end, int col0, int lane) {
+__device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, MX4_LDS unsigned char* side, const Product& p,
+                                           const typename T::Sums& acc, int expert, long long row0, long long end, int col0,
+                                           int lane) {
     constexpr int kRowFrags = T::kRowFrags, kColFrags = T::kColFrags;
     constexpr int kHalves = kRowFrags / 2;  // of 64 rows
     constexpr int kPasses = kGated ? kHalves : kColFrags / 2, kPassFrags = kGated ? kColFrags : 2;
@@ -291,25 +293,32 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
     static_assert(kPasses <= 2 && kPassRows / kBatch % 4 == 0);
     const long long b_row = expert * (kGated ? 2LL * p.n : p.n);
     const int line = lane % 32, half = lane / 32;
-    // What goes with rows lane and lane + 64.
+    // Rows lane and lane + 64: on their way while sums go to LDS.
     float sa[kHalves], gate[kHalves];
-    int c_rows[kHalves];  // from row0 (Down: from 0) on, -1: not stored
+    int c_row[kHalves];  // Down: of the workspace, -1: not stored
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
         const long long row = row0 + lane + 64 * h;
-        sa[h] = 0.0f, gate[h] = 1.0f, c_rows[h] = -1;
+        sa[h] = 0.0f, gate[h] = 0.0f, c_row[h] = -1;
         if (row < end) {
             sa[h] = p.a_scales[a_row_of<kMode>(p, row)];
-            c_rows[h] = lane + 64 * h;
             if constexpr (kMode == kDown) {
-                c_rows[h] = p.order[row];
-                if (c_rows[h] >= p.m) c_rows[h] = -1;
-                if (c_rows[h] >= 0) gate[h] = p.gates[c_rows[h]];
+                c_row[h] = p.order[row];
+                if (c_row[h] >= p.m) c_row[h] = -1;
+                if (c_row[h] >= 0) gate[h] = p.gates[c_row[h]];
             }
         }
     }
-    const auto of_row = [&](auto value, int row) {
-        return __builtin_bit_cast(decltype(value), __builtin_amdgcn_ds_bpermute(row % 64 * 4, __builtin_bit_cast(int, value)));
+    const auto rows_to_lds = [&] {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            const RowScale r = row_scale(sa[h]);
+            MX4_LDS unsigned char* at = side + (lane + 64 * h) * 16;
+            if constexpr (kMode == kDown)
+                *reinterpret_cast<MX4_LDS f32x4*>(at) = f32x4{r.s, r.back, gate[h], __builtin_bit_cast(float, c_row[h])};
+            else
+                *reinterpret_cast<MX4_LDS f32x2*>(at) = f32x2{r.s, r.back};
+        }
     };
     const auto to_lds = [&](auto pass) {
         constexpr int h = decltype(pass)::value;
@@ -335,8 +344,12 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
     };
 #pragma unroll 1
     for (int h = 0; h < kPasses; ++h) {
-        if (h == 0) to_lds(std::integral_constant<int, 0>{});
-        else to_lds(std::integral_constant<int, 1>{});
+        if (h == 0) {
+            to_lds(std::integral_constant<int, 0>{});
+            rows_to_lds();
+        } else {
+            to_lds(std::integral_constant<int, 1>{});
+        }
         // Eight columns of a row per lane, kBatch rows at a time, four times that under way.
         const int col = col0 + (kGated ? 0 : 64 * h) + lane % kAcross * 8, left = p.n - col;
         float scale[8], bias[8], up_scale[8], up_bias[8];
@@ -349,33 +362,33 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
         const auto rows = [&](auto act, auto store) {
 #pragma unroll 1
             for (int it = 0; it < kPassRows / kBatch; it += 4) {
-                const int part = kGated ? h : it * kBatch / 64;
-                const float sa_here = kHalves == 1 || part == 0 ? sa[0] : sa[kHalves - 1];
-                const float gate_here = kHalves == 1 || part == 0 ? gate[0] : gate[kHalves - 1];
                 int sum[4][8], up[4][8];
-                float s[4], g[4];
+                f32x2 scale_of[4];
+                float g[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const int row = kBatch * (it + u) + lane / kAcross;
-                    s[u] = of_row(sa_here, row);
-                    if constexpr (kMode == kDown) g[u] = of_row(gate_here, row);
+                    const MX4_LDS unsigned char* with = side + (row + (kGated ? 64 * h : 0)) * 16;
+                    scale_of[u] = *reinterpret_cast<const MX4_LDS f32x2*>(with);
+                    if constexpr (kMode == kDown) g[u] = *reinterpret_cast<const MX4_LDS float*>(with + 8);
                     sums_of(row, 0, sum[u]);
                     if constexpr (kGated) sums_of(row, 2 * kAcross, up[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
+                    const float s = scale_of[u][0], back = scale_of[u][1];
                     float v[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        v[e] = static_cast<float>(sum[u][e]) * s[u] * scale[e] + bias[e];
+                        v[e] = static_cast<float>(sum[u][e]) * s * scale[e] * back + bias[e];
                         if constexpr (kGated)
-                            v[e] *= sigmoid(v[e]) * (static_cast<float>(up[u][e]) * s[u] * up_scale[e] + up_bias[e]);
+                            v[e] *= sigmoid(v[e]) * (static_cast<float>(up[u][e]) * s * up_scale[e] * back + up_bias[e]);
                         else if constexpr (kMode == kDown)
                             v[e] *= g[u];
                         else
                             v[e] = act(v[e]);
                     }
-                    store(it + u, part, v);
+                    store(it + u, v);
                 }
             }
         };
@@ -393,7 +406,7 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
                                                        static_cast<int>(row_size));
             const int step = __builtin_amdgcn_readfirstlane(kBatch * static_cast<int>(row_size));
             const unsigned at = left > 0 ? static_cast<unsigned>(lane / kAcross * static_cast<int>(row_size) + col * kOne) : 1u << 31;
-            with_act([&](int it, int, const float(&v)[8]) {
+            with_act([&](int it, const float(&v)[8]) {
                 const int from = static_cast<int>(at + static_cast<unsigned>((it + (kGated ? h * (64 / kBatch) : 0)) * step));
                 if constexpr (kOut == kF32) {
                     const f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
@@ -407,10 +420,15 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, const Pro
                 }
             });
         } else {
-            with_act([&](int it, int part, const float(&v)[8]) {
-                const int c_row = of_row(kHalves == 1 || part == 0 ? c_rows[0] : c_rows[kHalves - 1], kBatch * it + lane / kAcross);
-                if (c_row >= 0 && left > 0)
-                    store_eight<kOut, kMode != kDown>(p.c, ((kMode == kDown ? 0 : row0) + c_row) * p.n + col, v, left);
+            with_act([&](int it, const float(&v)[8]) {
+                const int row = kBatch * it + lane / kAcross;
+                if constexpr (kMode == kDown) {
+                    const int c_row = *reinterpret_cast<const MX4_LDS int*>(side + row * 16 + 12);
+                    if (c_row >= 0 && left > 0) store_eight<kOut, false>(p.c, static_cast<long long>(c_row) * p.n + col, v, left);
+                } else {
+                    const long long c_row = row0 + (kGated ? 64 * h : 0) + row;
+                    if (c_row < end && left > 0) store_eight<kOut>(p.c, c_row * p.n + col, v, left);
+                }
             });
         }
     }
@@ -441,7 +459,8 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
     typename T::Sums acc;
     tile_sums<T>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
     lds_barrier();  // every wave is past its reads of the ring
-    store_tile<kMode, kGated, kOut, T>(lds + wave * T::kSlotBytes, p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
+    static_assert(kRingA + kRingB > 4);  // behind the waves' shares
+    store_tile<kMode, kGated, kOut, T>(lds + wave * T::kSlotBytes, lds + 4 * T::kSlotBytes + wave * 2048, p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
                                        col0 + wave % 2 * (kGated ? kCols / 4 : kCols / 2), lane);
 }
 

@@ -26,6 +26,17 @@ __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
+// A row's scale for sum x s x (a column's scale) x back, of which no part leaves fp32's range unless the
+// whole does: rows of numbers past 2^97 have scales with which a sum of up to 2^31 alone would. What
+// is taken times 2^-64 stays above 2^26, so that no column's scale (2^-149 at least) makes it subnormal.
+struct RowScale {
+    float s, back;
+};
+__device__ __forceinline__ RowScale row_scale(float s) {
+    const bool far = __builtin_fabsf(s) >= 0x1p90f;
+    return {far ? s * 0x1p-64f : s, far ? 0x1p64f : 1.0f};
+}
+
 // GELU in its tanh form is u (1 + tanh(z)) / 2 = u sigmoid(2 z). The reciprocal is good
 // to a unit in the last place; a division would be ten instructions.
 __device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.0f + __expf(-u)); }
