@@ -557,14 +557,20 @@ int launch_direct(Product p, hipStream_t stream, const char** why) {
                          0, stream, p);
 }
 
+// How many of `all` dense tiles of 256x256 run as two of 128 rows: those that would leave half
+// of a last round or more empty.
+int halves_of(long long all, int cus) {
+    const int rest = static_cast<int>(all % cus);
+    return rest <= cus / 2 ? rest : 0;
+}
+
 template <int kMode, bool kGated, int kTile>
 int launch_tiles(Product p, hipStream_t stream, const char** why) {
     p.tiles_n = static_cast<unsigned>(tiles(p.n, kGated ? kTile / 2 : kTile));
     const long long chunks = kMode == kDense ? tiles(p.m, kTile) : most_jobs(p.m, p.experts, kTile);
     // On a plan eight XCDs with the same number of blocks each.
     const long long all = kMode == kDense ? chunks * p.tiles_n : (chunks * p.tiles_n + 7) / 8 * 8;
-    const int cus = device_cus(), rest = static_cast<int>(all % cus);
-    const int halves = kMode == kDense && kTile == 256 && rest <= cus / 2 ? rest : 0;
+    const int halves = kMode == kDense && kTile == 256 ? halves_of(all, device_cus()) : 0;
     if (!fits_launch(all + halves, kTileThreads)) {
         *why = "more tiles of C than one launch takes";
         return hipErrorInvalidValue;
@@ -616,10 +622,11 @@ struct Cost {
     double large_tiles(double rounds) const { return plan ? 4.0 + rounds * (8.0 + 66.0 * k) : 3.5 + rounds * (6.5 + 49.5 * k); }
 };
 
+// The kernel of least cost (MCHIP_I8_*).
 template <int kMode, bool kGated>
-int launch(const Product& p, hipStream_t stream, const char** why) {
+int choose(const Product& p, int cu_count) {
     constexpr bool kPlan = kMode != kDense;
-    const double cus = device_cus(), experts = static_cast<double>(std::min(p.experts, p.m));
+    const double cus = cu_count, experts = static_cast<double>(std::min(p.experts, p.m));
     const Cost cost{p.row_bytes / 4096.0, cus, kPlan};
     const double columns = kGated ? 2.0 * p.n : p.n;
     // Blocks, of rows by columns of B; on a plan every second expert's last is half full.
@@ -647,11 +654,19 @@ int launch(const Product& p, hipStream_t stream, const char** why) {
         t256 = cost.large_tiles(rounds);
     }
     const double best = std::min({b16, b32, b64, t128, t256});
-    if (best == t256) return launch_tiles<kMode, kGated, 256>(p, stream, why);
-    if (best == t128) return launch_tiles<kMode, kGated, 128>(p, stream, why);
-    if (best == b64) return launch_direct<kMode, kGated, 2, 4>(p, stream, why);
-    if (best == b32) return launch_direct<kMode, kGated, 2, 2>(p, stream, why);
-    return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
+    return best == t256 ? MCHIP_I8_TILES_256 : best == t128 ? MCHIP_I8_TILES_128 : best == b64 ? MCHIP_I8_BLOCKS_32X64
+           : best == b32 ? MCHIP_I8_BLOCKS_32X32 : MCHIP_I8_BLOCKS_16X32;
+}
+
+template <int kMode, bool kGated>
+int launch(const Product& p, hipStream_t stream, const char** why) {
+    switch (choose<kMode, kGated>(p, device_cus())) {
+        case MCHIP_I8_TILES_256: return launch_tiles<kMode, kGated, 256>(p, stream, why);
+        case MCHIP_I8_TILES_128: return launch_tiles<kMode, kGated, 128>(p, stream, why);
+        case MCHIP_I8_BLOCKS_32X64: return launch_direct<kMode, kGated, 2, 4>(p, stream, why);
+        case MCHIP_I8_BLOCKS_32X32: return launch_direct<kMode, kGated, 2, 2>(p, stream, why);
+        default: return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
+    }
 }
 
 const char* refusal(const void* a, const float* a_scales, const void* b, const float* b_scales, const float* bias,
@@ -699,6 +714,22 @@ int mchip_launch_matmul_i8(const void* a_codes, const float* a_scales, const voi
                     b_scales, bias, c, nullptr, nullptr, nullptr, m, n, padded_k(k), m, 1, 1, activation, c_dtype, 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
     return activation == MCHIP_ACT_SWIGLU ? launch<kDense, true>(p, s, why) : launch<kDense, false>(p, s, why);
+}
+
+int mchip_matmul_i8_plan(int activation, int m, int n, int k, int cu_count, int* halves) {
+    Product p{};
+    p.m = p.a_rows = m, p.n = n, p.row_bytes = padded_k(k), p.experts = 1;
+    const bool gated = activation == MCHIP_ACT_SWIGLU;
+    const int kernel = gated ? choose<kDense, true>(p, cu_count) : choose<kDense, false>(p, cu_count);
+    *halves = kernel == MCHIP_I8_TILES_256 ? halves_of(tiles(m, 256) * tiles(n, gated ? 128 : 256), cu_count) : 0;
+    return kernel;
+}
+
+int mchip_experts_i8_plan(int down, int activation, int tokens, int top_k, int experts, int n, int k, int cu_count) {
+    Product p{};
+    p.m = tokens * top_k, p.a_rows = tokens, p.n = n, p.row_bytes = padded_k(k), p.top_k = top_k, p.experts = experts;
+    if (down != 0) return choose<kDown, false>(p, cu_count);
+    return activation == MCHIP_ACT_SWIGLU ? choose<kUp, true>(p, cu_count) : choose<kUp, false>(p, cu_count);
 }
 
 int mchip_launch_experts_up_i8(const mchip_experts_args* args, void* stream, const char** why) {
