@@ -118,6 +118,8 @@ __device__ __forceinline__ Place find_tile(const Product& p, unsigned want) {
     return {0, 0, 0};
 }
 
+constexpr int kDirectWaves = 8;
+
 // A block computes 16 kM rows by 16 kN columns of C (SwiGLU: the second half of the
 // column tiles are the up rows of the first half's columns); its kWaves waves take
 // the steps of 128 k in turn and their sums are added at the end. Four neighbouring
@@ -435,8 +437,8 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, MX4_LDS u
 }
 
 // Rows row0 .. of C up to `end` (at most kRows) by kCols (kGated: half of it) columns from
-// col0 on.
-template <int kMode, bool kGated, int kOut, int kRows, int kCols, int kSlotRows>
+// col0 on. kFar: gathered rows of an A past what a resource reaches.
+template <int kMode, bool kGated, int kOut, int kRows, int kCols, int kSlotRows, bool kFar = false>
 __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const Product& p, int expert, long long row0,
                                              long long end, int col0) {
     typedef Tile<kRows, kCols, kSlotRows> T;
@@ -444,24 +446,38 @@ __device__ __forceinline__ void product_tile(MX4_LDS unsigned char* lds, const P
     constexpr int kShareA = kRows / 4, kShareB = kCols / 4;  // rows, a wave's to fetch
     // A's rows, from the wave's share of the tile on, or (gathered) all.
     const long long a0 = kMode == kUp ? 0 : row0 + wave * kShareA;
-    const __amdgpu_buffer_rsrc_t a = kMode == kUp ? resource(p.a, p.a_rows * p.row_bytes)
-                                                  : rows_from(p.a + a0 * p.row_bytes, end - a0, p.row_bytes);
+    const __amdgpu_buffer_rsrc_t a = kFar            ? resource(p.a, 0)
+                                     : kMode == kUp ? resource(p.a, p.a_rows * p.row_bytes)
+                                                    : rows_from(p.a + a0 * p.row_bytes, end - a0, p.row_bytes);
     const auto a_row = [&](int i) {
         const int in_share = i * 8 + lane / 8;
         if constexpr (kMode != kUp) return in_share * p.row_bytes;
         const long long row = row0 + wave * kShareA + in_share;
-        return static_cast<int>(a_row_of<kMode>(p, row < end ? row : end - 1)) * p.row_bytes;
+        const long long token = a_row_of<kMode>(p, row < end ? row : end - 1);
+        if constexpr (kFar) return p.a + token * p.row_bytes;
+        else return static_cast<int>(token) * p.row_bytes;
     };
     // B's rows that the wave fetches: of columns, of gate or of up ones.
     const int b_col = col0 + (kGated ? wave / 2 : wave) * kShareB;
     const long long b0 = expert * (kGated ? 2LL * p.n : p.n) + (kGated ? wave % 2 * static_cast<long long>(p.n) : 0) + b_col;
     const __amdgpu_buffer_rsrc_t b = rows_from(p.b + b0 * p.row_bytes, p.n - b_col, p.row_bytes);
     typename T::Sums acc;
-    tile_sums<T>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
+    tile_sums<T, kFar>(lds, a, a_row, b, p.row_bytes, wave, lane, acc);
     lds_barrier();  // every wave is past its reads of the ring
     static_assert(kRingA + kRingB > 4);  // behind the waves' shares
     store_tile<kMode, kGated, kOut, T>(lds + wave * T::kSlotBytes, lds + 4 * T::kSlotBytes + wave * 2048, p, acc, expert, row0 + wave / 2 * (kRows / 2), end,
                                        col0 + wave % 2 * (kGated ? kCols / 4 : kCols / 2), lane);
+}
+
+// Block t's tile on a plan: an XCD takes an eighth of the tiles that the plan has, consecutive
+// ones, so that an expert's weights and a chunk's rows come through one L2.
+template <int kTile>
+__device__ __forceinline__ bool tile_on_plan(const Product& p, unsigned& t) {
+    const unsigned long long have =
+        static_cast<unsigned long long>(sum_of_entries(p, [](unsigned n) { return (n + kTile - 1) / kTile; })) * p.tiles_n;
+    const unsigned first = static_cast<unsigned>(have * (t % 8) / 8), last = static_cast<unsigned>(have * (t % 8 + 1) / 8);
+    t = first + t / 8;
+    return t < last;
 }
 
 // kTile 256: dense tiles are 256 rows high; the grid has one block per tile plus `halves`
@@ -491,13 +507,7 @@ __global__ __launch_bounds__(kTileThreads, kTile == 256 ? 1 : 2) void i8_tiles(c
         const unsigned high = min(static_cast<unsigned>(kPanel), all - panel * kPanel);
         chunk = panel * kPanel + in % high, tile = in / high;
     } else {
-        // An XCD takes an eighth of the tiles that the plan has, consecutive ones, so that
-        // an expert's weights and a chunk's rows come through one L2.
-        const unsigned long long have =
-            static_cast<unsigned long long>(sum_of_entries(p, [](unsigned n) { return (n + kTile - 1) / kTile; })) * p.tiles_n;
-        const unsigned first = static_cast<unsigned>(have * (t % 8) / 8), last = static_cast<unsigned>(have * (t % 8 + 1) / 8);
-        t = first + t / 8;
-        if (t >= last) return;
+        if (!tile_on_plan<kTile>(p, t)) return;
         chunk = t / p.tiles_n, tile = t % p.tiles_n;
     }
     const int col0 = static_cast<int>(tile) * (kGated ? kTile / 2 : kTile);
@@ -519,6 +529,23 @@ __global__ __launch_bounds__(kTileThreads, kTile == 256 ? 1 : 2) void i8_tiles(c
     } else {
         product_tile<kMode, kGated, kOut, 128, 128, 128>(lds, p, expert, row0, end, col0);
     }
+}
+
+// Up by 256x256 tiles where A has 2 GiB or more: 524288 tokens of 4096 on 8 experts, 2 x 1024
+// columns, 4.1 ms, as long as 64 tokens less take through a resource (by 32x64 blocks 12.4).
+template <bool kGated, int kOut>
+__global__ __launch_bounds__(kTileThreads, 1) void i8_far_rows(const Product p, unsigned) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[Tile<256, 256, 256>::kRingBytes];
+    MX4_LDS unsigned char* lds = (MX4_LDS unsigned char*)(smem);  // generic -> LDS address space
+    unsigned t = blockIdx.x;
+    if (!tile_on_plan<256>(p, t)) return;
+    const Place place = find_tile<256>(p, t / p.tiles_n);
+    const int col0 = static_cast<int>(t % p.tiles_n) * (kGated ? 128 : 256);
+    if (place.first >= place.end) return;
+    if (place.end - place.first > 128)
+        product_tile<kUp, kGated, kOut, 256, 256, 256, true>(lds, p, place.expert, place.first, place.end, col0);
+    else
+        product_tile<kUp, kGated, kOut, 128, 256, 256, true>(lds, p, place.expert, place.first, place.end, col0);
 }
 
 // y[token] = the sum of its top_k rows of the workspace, in order: 134 MB in 21.7 us, 6.5
@@ -544,17 +571,21 @@ long long most_jobs(long long slots, int experts, int rows) {
     return std::min(slots, (slots + std::min<long long>(experts, slots) * (rows - 1)) / rows);
 }
 
+// Blocks of a launch in blocks or tiles of rows by columns of B. On a plan of tiles eight XCDs
+// have the same number each.
+template <int kMode, bool kGated>
+long long grid_of(const Product& p, int rows, int cols) {
+    const long long chunks = kMode == kDense ? tiles(p.m, rows) : most_jobs(p.m, p.experts, rows);
+    const long long all = chunks * tiles(p.n, kGated ? cols / 2 : cols);
+    return kMode != kDense && rows >= 128 ? (all + 7) / 8 * 8 : all;
+}
+
 template <int kMode, bool kGated, int kM, int kN>
-int launch_direct(Product p, hipStream_t stream, const char** why) {
-    constexpr int kWaves = 8;
-    p.tiles_n = static_cast<unsigned>(tiles(p.n, 16 * (kGated ? kN / 2 : kN)));
-    const long long chunks = kMode == kDense ? tiles(p.m, 16 * kM) : most_jobs(p.m, p.experts, 16 * kM);
-    if (!fits_launch(chunks * p.tiles_n, kWaves * 64)) {
-        *why = "more tiles of C than one launch takes";
-        return hipErrorInvalidValue;
-    }
-    return launch_kernel(i8_direct<kMode, kGated, kM, kN, kWaves>, static_cast<unsigned>(chunks * p.tiles_n), kWaves * 64,
-                         0, stream, p);
+int launch_direct(Product p, hipStream_t stream) {
+    constexpr int kCols = kGated ? kN / 2 : kN;
+    p.tiles_n = static_cast<unsigned>(tiles(p.n, 16 * kCols));
+    return launch_kernel(i8_direct<kMode, kGated, kM, kN, kDirectWaves>,
+                         static_cast<unsigned>(grid_of<kMode, kGated>(p, 16 * kM, 16 * kN)), kDirectWaves * 64, 0, stream, p);
 }
 
 // How many of `all` dense tiles of 256x256 run as two of 128 rows: those that would leave half
@@ -564,23 +595,22 @@ int halves_of(long long all, int cus) {
     return rest <= cus / 2 ? rest : 0;
 }
 
-template <int kMode, bool kGated, int kTile>
-int launch_tiles(Product p, hipStream_t stream, const char** why) {
+template <int kMode, bool kGated, int kTile, bool kFar = false>
+int launch_tiles(Product p, hipStream_t stream) {
     p.tiles_n = static_cast<unsigned>(tiles(p.n, kGated ? kTile / 2 : kTile));
-    const long long chunks = kMode == kDense ? tiles(p.m, kTile) : most_jobs(p.m, p.experts, kTile);
-    // On a plan eight XCDs with the same number of blocks each.
-    const long long all = kMode == kDense ? chunks * p.tiles_n : (chunks * p.tiles_n + 7) / 8 * 8;
+    const long long all = grid_of<kMode, kGated>(p, kTile, kTile);
     const int halves = kMode == kDense && kTile == 256 ? halves_of(all, device_cus()) : 0;
-    if (!fits_launch(all + halves, kTileThreads)) {
-        *why = "more tiles of C than one launch takes";
-        return hipErrorInvalidValue;
-    }
     const auto go = [&](auto kernel) {
         return launch_kernel(kernel, static_cast<unsigned>(all + halves), kTileThreads, 0, stream, p,
                              static_cast<unsigned>(all - halves));
     };
     if constexpr (kMode == kDown) {
         return go(i8_tiles<kMode, kGated, kF32, kTile>);
+    } else if constexpr (kFar) {
+        static_assert(kMode == kUp && kTile == 256);
+        return p.c_dtype == kF32    ? go(i8_far_rows<kGated, kF32>)
+               : p.c_dtype == kBf16 ? go(i8_far_rows<kGated, kBf16>)
+                                    : go(i8_far_rows<kGated, kF16>);
     } else {
         return p.c_dtype == kF32    ? go(i8_tiles<kMode, kGated, kF32, kTile>)
                : p.c_dtype == kBf16 ? go(i8_tiles<kMode, kGated, kBf16, kTile>)
@@ -588,11 +618,10 @@ int launch_tiles(Product p, hipStream_t stream, const char** why) {
     }
 }
 
-// Offsets within a tile's rows, and within A where its rows are gathered, have 32 bits.
+// Offsets within A have 32 bits where its rows are gathered through a resource.
 template <int kMode>
-bool tiles_fit(const Product& p) {
-    const long long a_rows = kMode == kUp ? p.a_rows : 256;
-    return a_rows * p.row_bytes < (1LL << 31);
+bool one_resource(const Product& p) {
+    return kMode != kUp || static_cast<long long>(p.a_rows) * p.row_bytes < (1LL << 31);
 }
 
 // What a variant takes, in microseconds, by its rounds of blocks and k (in units of 4096).
@@ -622,7 +651,7 @@ struct Cost {
     double large_tiles(double rounds) const { return plan ? 4.0 + rounds * (8.0 + 66.0 * k) : 3.5 + rounds * (6.5 + 49.5 * k); }
 };
 
-// The kernel of least cost (MCHIP_I8_*).
+// The kernel of least cost (MCHIP_I8_*) of those that one launch takes, -1: none.
 template <int kMode, bool kGated>
 int choose(const Product& p, int cu_count) {
     constexpr bool kPlan = kMode != kDense;
@@ -635,38 +664,50 @@ int choose(const Product& p, int cu_count) {
                                   : static_cast<double>(tiles(p.m, rows));
         return down * std::ceil(columns / cols);
     };
-    const double b16 = cost.few(blocks(16, 32), 3.0, 0.8, 4.1), b32 = cost.few(blocks(32, 32), 4.2, 1.6, 7.0),
-                 b64 = cost.few(blocks(32, 64), 6.0, 2.1, 9.5);
-    double t128 = 1e30, t256 = 1e30;
-    if (tiles_fit<kMode>(p)) {
-        t128 = cost.small_tiles(blocks(128, 128));
-        double rounds;
-        if (kPlan) {
-            // In rounds and halves of them; a third of the experts' last tiles are halves, which
-            // take 0.7 of a tile.
-            const double all = std::max(experts * 0.7, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus;
-            rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
-        } else {
-            // Tiles that leave half a round or more empty run as halves.
-            const double all = blocks(256, 256), rest = std::fmod(all, cus);
-            rounds = std::floor(all / cus) + (rest == 0.0 ? 0.0 : rest <= cus / 2 ? 0.87 : 1.0);
-        }
-        t256 = cost.large_tiles(rounds);
+    // None where a launch has no room for it.
+    const auto or_none = [&](double microseconds, int rows, int cols, int threads) {
+        return fits_launch(grid_of<kMode, kGated>(p, rows, cols), threads) ? microseconds : 1e30;
+    };
+    constexpr int kDirectThreads = kDirectWaves * 64;
+    const double b16 = or_none(cost.few(blocks(16, 32), 3.0, 0.8, 4.1), 16, 32, kDirectThreads),
+                 b32 = or_none(cost.few(blocks(32, 32), 4.2, 1.6, 7.0), 32, 32, kDirectThreads),
+                 b64 = or_none(cost.few(blocks(32, 64), 6.0, 2.1, 9.5), 32, 64, kDirectThreads);
+    double rounds;
+    if (kPlan) {
+        // In rounds and halves of them; a third of the experts' last tiles are halves, which
+        // take 0.7 of a tile.
+        const double all = std::max(experts * 0.7, p.m / 256.0 + experts * 0.35) * std::ceil(columns / 256.0) / cus;
+        rounds = std::max(1.0, std::ceil(2.0 * all) / 2.0);
+    } else {
+        // Tiles that leave half a round or more empty run as halves.
+        const double all = blocks(256, 256), rest = std::fmod(all, cus);
+        rounds = std::floor(all / cus) + (rest == 0.0 ? 0.0 : rest <= cus / 2 ? 0.87 : 1.0);
     }
+    const bool near = one_resource<kMode>(p);
+    const double t128 = near ? or_none(cost.small_tiles(blocks(128, 128)), 128, 128, kTileThreads) : 1e30;
+    const double t256 = or_none(cost.large_tiles(rounds), 256, 256, kTileThreads);
     const double best = std::min({b16, b32, b64, t128, t256});
-    return best == t256 ? MCHIP_I8_TILES_256 : best == t128 ? MCHIP_I8_TILES_128 : best == b64 ? MCHIP_I8_BLOCKS_32X64
-           : best == b32 ? MCHIP_I8_BLOCKS_32X32 : MCHIP_I8_BLOCKS_16X32;
+    return best == 1e30 ? -1
+           : best == t256 ? (near ? MCHIP_I8_TILES_256 : MCHIP_I8_TILES_FAR)
+           : best == t128 ? MCHIP_I8_TILES_128
+           : best == b64  ? MCHIP_I8_BLOCKS_32X64
+           : best == b32  ? MCHIP_I8_BLOCKS_32X32
+                          : MCHIP_I8_BLOCKS_16X32;
 }
 
 template <int kMode, bool kGated>
 int launch(const Product& p, hipStream_t stream, const char** why) {
     switch (choose<kMode, kGated>(p, device_cus())) {
-        case MCHIP_I8_TILES_256: return launch_tiles<kMode, kGated, 256>(p, stream, why);
-        case MCHIP_I8_TILES_128: return launch_tiles<kMode, kGated, 128>(p, stream, why);
-        case MCHIP_I8_BLOCKS_32X64: return launch_direct<kMode, kGated, 2, 4>(p, stream, why);
-        case MCHIP_I8_BLOCKS_32X32: return launch_direct<kMode, kGated, 2, 2>(p, stream, why);
-        default: return launch_direct<kMode, kGated, 1, 2>(p, stream, why);
+        case MCHIP_I8_TILES_256: return launch_tiles<kMode, kGated, 256>(p, stream);
+        case MCHIP_I8_TILES_128: return launch_tiles<kMode, kGated, 128>(p, stream);
+        case MCHIP_I8_BLOCKS_32X64: return launch_direct<kMode, kGated, 2, 4>(p, stream);
+        case MCHIP_I8_BLOCKS_32X32: return launch_direct<kMode, kGated, 2, 2>(p, stream);
+        case MCHIP_I8_BLOCKS_16X32: return launch_direct<kMode, kGated, 1, 2>(p, stream);
+        case MCHIP_I8_TILES_FAR:
+            if constexpr (kMode == kUp) return launch_tiles<kMode, kGated, 256, true>(p, stream);
     }
+    *why = "more tiles of C than one launch takes";
+    return hipErrorInvalidValue;
 }
 
 const char* refusal(const void* a, const float* a_scales, const void* b, const float* b_scales, const float* bias,

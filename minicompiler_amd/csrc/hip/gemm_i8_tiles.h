@@ -67,10 +67,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const unsigned char*
     return resource(p, most * row_bytes);
 }
 
-template <typename T>
+typedef const __attribute__((address_space(1))) unsigned char* global_bytes;
+
+// kFar: A's rows have addresses of their own, for gathered rows further apart than a resource reaches.
+template <typename T, bool kFar>
 struct TileLane {
     __amdgpu_buffer_rsrc_t a, b;             // A's rows (this wave's share of the tile, or all of A), this wave's of B's
     int a_src[T::kFetchA], b_src[T::kFetchB];  // the lane's offset in each fetch
+    global_bytes a_far[kFar ? T::kFetchA : 1];   // kFar: where it begins
     int a_off[4], b_off[4];                  // LDS offsets of the wave's first fragments in each step
     int wave;
 };
@@ -78,23 +82,28 @@ struct TileLane {
 // Instruction i of this wave's share of a stage of A to `wr`, `at` bytes into the rows.
 // Rows are in the lane's offset, which is held against the resource's end; the scalar
 // one stays within a row.
-template <typename T>
-__device__ __forceinline__ void fetch_a(MX4_LDS unsigned char* wr, const TileLane<T>& L, int at, int i) {
-    buffer_to_lds(L.a, wr + (L.wave * T::kFetchA + i) * 1024, L.a_src[i], at);
+template <typename T, bool kFar>
+__device__ __forceinline__ void fetch_a(MX4_LDS unsigned char* wr, const TileLane<T, kFar>& L, int at, int i) {
+    MX4_LDS unsigned char* const to = wr + (L.wave * T::kFetchA + i) * 1024;
+    if constexpr (kFar)
+        __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) void*>(L.a_far[i] + at),
+                                         reinterpret_cast<MX4_LDS void*>(to), 16, 0, 0);
+    else
+        buffer_to_lds(L.a, to, L.a_src[i], at);
 }
-template <typename T>
-__device__ __forceinline__ void fetch_b(MX4_LDS unsigned char* wr, const TileLane<T>& L, int at, int i) {
+template <typename T, bool kFar>
+__device__ __forceinline__ void fetch_b(MX4_LDS unsigned char* wr, const TileLane<T, kFar>& L, int at, int i) {
     buffer_to_lds(L.b, wr + (L.wave * T::kFetchB + i) * 1024, L.b_src[i], at);
 }
 
 // One fragment of step u of the stage at `rd`. What is read is not being written;
 // __restrict__ says so, or the compiler would wait for the fetches in flight.
-template <typename T>
-__device__ __forceinline__ i32x4 read_a(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<T>& L, int u, int f) {
+template <typename T, bool kFar>
+__device__ __forceinline__ i32x4 read_a(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<T, kFar>& L, int u, int f) {
     return *reinterpret_cast<const MX4_LDS i32x4*>(rd + L.a_off[u] + f * 4096);
 }
-template <typename T>
-__device__ __forceinline__ i32x4 read_b(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<T>& L, int u, int f) {
+template <typename T, bool kFar>
+__device__ __forceinline__ i32x4 read_b(const MX4_LDS unsigned char* __restrict__ rd, const TileLane<T, kFar>& L, int u, int f) {
     return *reinterpret_cast<const MX4_LDS i32x4*>(rd + L.b_off[u] + f * 4096);
 }
 
@@ -120,19 +129,23 @@ __device__ __forceinline__ void settle() {
 
 // acc[i][f][v] = the sum of row wave_row + 32 i + lane % 32 and of the wave's column
 // 32 f + 8 (v / 4) + 4 (lane / 32) + v % 4. a_row(i): where the lane's row of the wave's
-// fetch i of A begins, in bytes from A's resource on.
-template <typename T, typename RowOf>
+// fetch i of A begins, in bytes from A's resource on (kFar: its address).
+template <typename T, bool kFar, typename RowOf>
 __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_buffer_rsrc_t a, RowOf a_row,
                                           __amdgpu_buffer_rsrc_t b, int row_bytes, int wave, int lane,
                                           typename T::Sums& acc) {
     constexpr int kColFrags = T::kColFrags;
     const int r = lane % 32, h = lane / 32;
-    TileLane<T> L;
+    TileLane<T, kFar> L;
     L.a = a, L.b = b;
     L.wave = wave;
     // The block that the lane's place in LDS takes, of row lane / 8 of a fetch.
 #pragma unroll
-    for (int i = 0; i < T::kFetchA; ++i) L.a_src[i] = a_row(i) + (lane % 8 ^ (4 * (i & 1) + lane / 16)) * 16;
+    for (int i = 0; i < T::kFetchA; ++i) {
+        const int block = (lane % 8 ^ (4 * (i & 1) + lane / 16)) * 16;
+        if constexpr (kFar) L.a_far[i] = (global_bytes)(a_row(i)) + block;  // generic -> global address space
+        else L.a_src[i] = a_row(i) + block;
+    }
 #pragma unroll
     for (int i = 0; i < T::kFetchB; ++i)
         L.b_src[i] = (8 * i + lane / 8) * row_bytes + (lane % 8 ^ (4 * (i & 1) + lane / 16)) * 16;
@@ -153,15 +166,15 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
     constexpr int kI = T::kRowFrags, kA = T::kFetchA, kAll = kA + T::kFetchB, kEarly = kAll / 2;
     constexpr int kSlots = kI * kColFrags;
 #pragma unroll
-    for (int i = 0; i < kA; ++i) fetch_a<T>(slot_a(0), L, 0, i);
+    for (int i = 0; i < kA; ++i) fetch_a<T, kFar>(slot_a(0), L, 0, i);
 #pragma unroll
-    for (int i = 0; i < T::kFetchB; ++i) fetch_b<T>(b_here, L, 0, i);
+    for (int i = 0; i < T::kFetchB; ++i) fetch_b<T, kFar>(b_here, L, 0, i);
 #pragma unroll
-    for (int i = 0; i < T::kFetchB; ++i) fetch_b<T>(b_next, L, offset_of(1), i);
+    for (int i = 0; i < T::kFetchB; ++i) fetch_b<T, kFar>(b_next, L, offset_of(1), i);
 #pragma unroll
     for (int i = 0; i < kEarly; ++i) {
-        if (i < kA) fetch_a<T>(slot_a(1), L, offset_of(1), i < kA ? i : 0);
-        else fetch_b<T>(b_last, L, offset_of(2), i - kA);
+        if (i < kA) fetch_a<T, kFar>(slot_a(1), L, offset_of(1), i < kA ? i : 0);
+        else fetch_b<T, kFar>(b_last, L, offset_of(2), i - kA);
     }
 #pragma unroll
     for (int i = 0; i < kI; ++i)
@@ -176,9 +189,9 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
 
     i32x4 av[2][kI], bv[2][kColFrags];
 #pragma unroll
-    for (int f = 0; f < kColFrags; ++f) bv[0][f] = read_b<T>(b_here, L, 0, f);
+    for (int f = 0; f < kColFrags; ++f) bv[0][f] = read_b<T, kFar>(b_here, L, 0, f);
 #pragma unroll
-    for (int i = 0; i < kI; ++i) av[0][i] = read_a<T>(lds, L, 0, i);
+    for (int i = 0; i < kI; ++i) av[0][i] = read_a<T, kFar>(lds, L, 0, i);
 
     // Every product is held in its place, with at most a fragment's read and a fetch
     // behind it: the matrix unit is busy meanwhile. The fetch of a stage is spread over
@@ -199,21 +212,21 @@ __device__ __forceinline__ void tile_sums(MX4_LDS unsigned char* lds, __amdgpu_b
                 const int i = m / kColFrags, f = m % kColFrags;
                 mfma_in_place(acc[i][f], bv[t & 1][f], av[t & 1][i]);
                 if (m < kColFrags)
-                    bv[(t + 1) & 1][m < kColFrags ? m : 0] = read_b<T>(b_from, L, (t + 1) % 4, m);
+                    bv[(t + 1) & 1][m < kColFrags ? m : 0] = read_b<T, kFar>(b_from, L, (t + 1) % 4, m);
                 else if (m < kColFrags + kI)
-                    av[(t + 1) & 1][m < kColFrags + kI ? m - kColFrags : 0] = read_a<T>(a_from, L, (t + 1) % 4, m - kColFrags);
+                    av[(t + 1) & 1][m < kColFrags + kI ? m - kColFrags : 0] = read_a<T, kFar>(a_from, L, (t + 1) % 4, m - kColFrags);
                 // Fetch j of a step's lies behind product (j + 1) kSlots / kEarly - 1.
 #pragma unroll
                 for (int j = 0; j < kEarly; ++j)
                     if (m == (j + 1) * kSlots / kEarly - 1) {
                         const int i0 = kEarly + j;
                         if (t == 0) {
-                            if (i0 < kA) fetch_a<T>(slot_a(s + 1), L, a_next, i0 < kA ? i0 : 0);
-                            else fetch_b<T>(b_last, L, a_after, i0 - kA);
+                            if (i0 < kA) fetch_a<T, kFar>(slot_a(s + 1), L, a_next, i0 < kA ? i0 : 0);
+                            else fetch_b<T, kFar>(b_last, L, a_after, i0 - kA);
                         }
                         if (t == 3) {
-                            if (j < kA) fetch_a<T>(slot_a(s), L, a_after, j < kA ? j : 0);
-                            else fetch_b<T>(b_here, L, b_after, j - kA);
+                            if (j < kA) fetch_a<T, kFar>(slot_a(s), L, a_after, j < kA ? j : 0);
+                            else fetch_b<T, kFar>(b_here, L, b_after, j - kA);
                         }
                     }
                 __builtin_amdgcn_sched_barrier(0);

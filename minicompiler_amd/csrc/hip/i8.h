@@ -82,14 +82,15 @@ typedef struct mchip_experts_args {
 int mchip_launch_experts_up_i8(const mchip_experts_args* args, void* stream, const char** why);
 
 /* The kernel that a product of these sizes runs on a chip of cu_count CUs, for the
- * tests: blocks or tiles of rows x columns. *halves: how many of the last 256x256
+ * tests: blocks or tiles of rows x columns; -1: none, one launch is too small. *halves: how many of the last 256x256
  * tiles run as two of 128 rows. */
 enum {
     MCHIP_I8_BLOCKS_16X32 = 0,
     MCHIP_I8_BLOCKS_32X32 = 1,
     MCHIP_I8_BLOCKS_32X64 = 2,
     MCHIP_I8_TILES_128 = 3,
-    MCHIP_I8_TILES_256 = 4
+    MCHIP_I8_TILES_256 = 4,
+    MCHIP_I8_TILES_FAR = 5 /* as 256x256, gathered from 2 GiB of A or more */
 };
 int mchip_matmul_i8_plan(int activation, int m, int n, int k, int cu_count, int* halves);
 int mchip_experts_i8_plan(int down, int activation, int tokens, int top_k, int experts, int n, int k, int cu_count);

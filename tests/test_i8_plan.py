@@ -9,7 +9,7 @@ import test_gpu_experts_i8 as experts
 import test_gpu_i8 as operators
 import test_gpu_i8_halves as halves
 
-BLOCKS_16X32, BLOCKS_32X32, BLOCKS_32X64, TILES_128, TILES_256 = range(5)
+BLOCKS_16X32, BLOCKS_32X32, BLOCKS_32X64, TILES_128, TILES_256, TILES_FAR = range(6)
 
 
 def dense(mc, m, n, k, gated):
@@ -55,3 +55,16 @@ def test_plans_of_every_kernel(mc, at):
     (4096, 14336, 4096, TILES_256, 128), (1, 1, 1, BLOCKS_16X32, 0)])
 def test_the_rule(mc, m, n, k, kernel, split):
     assert dense(mc, m, n, k, False) == (kernel, split)
+
+
+# Gathered rows whose bytes reach 2 GiB: as large tiles as below it, from one row to the next, and never more blocks than
+# a launch takes.
+@pytest.mark.parametrize("tokens,count,top_k,n,k,gated,kernel", [
+    (524287, 64, 8, 2048, 4096, True, TILES_256), (524288, 64, 8, 2048, 4096, True, TILES_FAR),
+    (524288, 8, 2, 14336, 4096, True, TILES_FAR), (1 << 27, 8, 8, 128, 128, False, TILES_FAR),
+    (16383, 4, 2, 1000, 131071, False, TILES_256), (16384, 4, 2, 1000, 131071, False, TILES_FAR),
+    (2000000, 512, 16, 4096, 4096, True, TILES_FAR)])
+def test_gathered_rows_past_2_gib(mc, tokens, count, top_k, n, k, gated, kernel):
+    assert on_plan(mc, False, gated, tokens, count, top_k, n, k) == kernel
+    # The second product reads its rows in their order, wherever they lie.
+    assert on_plan(mc, True, False, tokens, count, top_k, n, k) in (TILES_128, TILES_256)
