@@ -34,6 +34,7 @@ struct Route {
     unsigned short* ids;  // of all pairs, for the plan's launch, or null
     bool by_logit;        // one score by itself is as large as its logit
     bool plans;           // the only block makes the plan, too
+    long long first;      // the launch's first token
 };
 
 // Place j of a token. Behind the last pair the ids go on to a multiple of eight with an
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
     __shared__ __attribute__((aligned(16))) unsigned short few[kFewPairs];
     __shared__ int picked[kTokens][MCHIP_ROUTE_MAX_TOP_K];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, l = lane % 16, row = lane / 16;
-    const long long token = (static_cast<long long>(blockIdx.x) * kWaves + wave) * 4 + row;
+    const long long token = p.first + (static_cast<long long>(blockIdx.x) * kWaves + wave) * 4 + row;
     const bool has = token < p.tokens;
     const long long from = (has ? token : 0) * p.ld;
     const int e0 = l * kPer;
@@ -381,10 +382,19 @@ __global__ __launch_bounds__(kPlanThreads) void make_plan(const unsigned short* 
     }
 }
 
+// As many tokens at a time as a launch takes.
 template <int kType>
-int launch_tokens(const Route& p, hipStream_t stream) {
-    const unsigned blocks = static_cast<unsigned>((static_cast<long long>(p.tokens) + kTokens - 1) / kTokens);
-    const auto go = [&](auto kernel) { return launch_kernel(kernel, blocks, kThreads, 0, stream, p); };
+int launch_tokens(Route p, hipStream_t stream) {
+    constexpr long long kMost = 1LL << 27;
+    static_assert(kMost / kTokens * kThreads < 1LL << 32);
+    const auto go = [&](auto kernel) {
+        int rc = hipSuccess;
+        for (p.first = 0; rc == hipSuccess && p.first < p.tokens; p.first += kMost) {
+            const long long count = std::min(kMost, p.tokens - p.first);
+            rc = launch_kernel(kernel, static_cast<unsigned>((count + kTokens - 1) / kTokens), kThreads, 0, stream, p);
+        }
+        return rc;
+    };
     if (p.experts <= 64) return go(route_tokens<kType, 4>);
     if (p.experts <= 128) return go(route_tokens<kType, 8>);
     if (p.experts <= 256) return go(route_tokens<kType, 16>);
@@ -435,7 +445,7 @@ int mchip_launch_route(const mchip_route_args* args, void* stream, const char** 
     unsigned short* ids = x.order != nullptr && !plans ? static_cast<unsigned short*>(x.workspace) : nullptr;
     const Route p{x.logits, x.ld, x.bias, x.tokens, x.experts, x.top_k, x.score, x.groups, x.experts / x.groups,
                   x.top_groups, x.group_best, x.normalize, x.scale, x.chosen, x.gates, x.order, x.offsets, ids,
-                  x.bias == nullptr && (x.groups == 1 || x.group_best == 1), plans};
+                  x.bias == nullptr && (x.groups == 1 || x.group_best == 1), plans, 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int rc = x.dtype == kF32    ? launch_tokens<kF32>(p, s)
                    : x.dtype == kBf16 ? launch_tokens<kBf16>(p, s)
