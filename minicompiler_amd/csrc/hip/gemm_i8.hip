@@ -350,8 +350,10 @@ __device__ __forceinline__ void store_tile(MX4_LDS unsigned char* lds, MX4_LDS u
             to_lds(std::integral_constant<int, 0>{});
             rows_to_lds();
         } else {
+            wave_lds_order();  // behind the first pass's reads
             to_lds(std::integral_constant<int, 1>{});
         }
+        wave_lds_order();
         // Eight columns of a row per lane, kBatch rows at a time, four times that under way.
         const int col = col0 + (kGated ? 0 : 64 * h) + lane % kAcross * 8, left = p.n - col;
         float scale[8], bias[8], up_scale[8], up_bias[8];

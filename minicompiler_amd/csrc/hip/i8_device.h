@@ -37,6 +37,13 @@ __device__ __forceinline__ RowScale row_scale(float s) {
     return {far ? s * 0x1p-64f : s, far ? 0x1p64f : 1.0f};
 }
 
+// Between one lane's writes to LDS and another's reads of the same wave, or back. The hardware
+// keeps a wave's LDS accesses in order; the compiler, which sees one lane, is held to it here.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // GELU in its tanh form is u (1 + tanh(z)) / 2 = u sigmoid(2 z). The reciprocal is good
 // to a unit in the last place; a division would be ten instructions.
 __device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.0f + __expf(-u)); }

@@ -199,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
     }
     unsigned long long kept = ~0ull;
     if (p.groups > 1) {
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
         // Its score goes to the group's first expert's place in `sums`.
         double* sums = mine;  // once every lane has read its groups
         kept = 0;
@@ -222,14 +222,14 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
                 sum[q] = p.group_best == 2 && second > kNone ? first + second : first;
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int i = 0; i < kPer; ++i) key[i] = mine[l * kLane + i];
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if (l + 16 * q < p.groups) sums[l + 16 * q] = sum[q];
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (16 * q >= p.groups) continue;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
             key[i] = __builtin_bit_cast(double, u);
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_lds_order();
     const int expert = l < p.top_k ? places[l] : 0;
     double gate = 0.0;
     if (l < p.top_k) {
