@@ -111,4 +111,4 @@ def test_results_past_the_range(device, mc, m):
     c = Out(mc, m * n * 4)
     mc.launch_matmul_i8(da.ptr, ca.ptr, db.ptr, cb.ptr, None, None, 0, c.ptr, m, n, k)
     mc.synchronize()
-    assert np.array_equal(c.get(np.float32, (m, n)), np.where(sums == 0, 0.0, np.sign(sums) * np.inf))
+    assert np.array_equal(c.get(np.float32, (m, n)), np.where(sums == 0, 0.0, np.copysign(np.inf, sums)))
