@@ -348,7 +348,8 @@ MC_API long long mc_i8_code_bytes(int rows, int k);
 MC_API int mc_quantize_i8(int dtype, const void* x, long long ld, void* codes, float* scales, int rows, int k,
                           void* values, void* stream);
 /* The same of a row-major B [k, n] (rows ld elements apart), a scale for each
- * column: an operand of n rows of k. values (NULL: not wanted): [k, n]. */
+ * column: an operand of n rows of k. values (NULL: not wanted): [k, n]. n at most
+ * 536870784. */
 MC_API int mc_quantize_i8_columns(int dtype, const void* b, long long ld, void* codes, float* scales, int k, int n,
                                   void* values, void* stream);
 /* C[m, n] (row-major, of type c_dtype) = act(sum a b x a_scale x b_scale +
@@ -401,7 +402,7 @@ MC_API int mc_launch_experts_up_i8(const void* x_codes, const float* x_scales, c
 /* ... and the second: y[token, n] = sum over the token's pairs, in their order,
  * of gates[pair] (h[slot] W_e^T + b_e), in fp32. h: an i8 operand of tokens x
  * top_k rows of k, by slot; W of experts x n rows; y [tokens, n]. The plan has
- * every pair once. workspace: mc_experts_down_i8_workspace_bytes bytes,
+ * every pair once: unlike the first product, not a part of the experts. workspace: mc_experts_down_i8_workspace_bytes bytes,
  * 256-byte aligned; calls that overlap need one each. */
 MC_API long long mc_experts_down_i8_workspace_bytes(int c_dtype, int tokens, int top_k, int n, int k);
 MC_API int mc_launch_experts_down_i8(const void* h_codes, const float* h_scales, const void* w_codes,

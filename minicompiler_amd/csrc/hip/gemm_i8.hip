@@ -9,11 +9,12 @@
 // experts, 2048 by 2 x 1024, 8.9). Blocks of 16x32 to 32x64 take all of k, without LDS
 // before the end: a wave's loads are in flight at once (1000x1001x1023 7.0 us, 4096 of k and
 // columns by 32 rows 5.5). Many rows: tiles of 128x128 or 256x256 (gemm_i8_tiles.h; on the
-// plan of 2048 tokens, 8 of 64 experts, up 105-124 us by the chip, down 111).
+// plan of 2048 tokens, 8 of 64 experts, up 105-126 us by the chip, down 111-115).
 //
 // Down keeps each pair's product in fp32 until the token's pairs are summed in their order:
 // 16-bit ones would save half of 268 MB there (2048 tokens, 21 of 111 us in the sum) and
-// round each term, atomic sums would depend on the order.
+// round each term, atomic sums would depend on the order. So its plan has every pair; a part of a
+// plan's experts is Up's alone.
 
 #include <cmath>
 #include <type_traits>
@@ -639,6 +640,8 @@ bool one_resource(const Product& p) {
 // deep, 1024 gated columns, by 128x128 and 256x256: 128 tokens 56.1 and 61.3, 512 58 and 62,
 // 1024 84 and 79, 2048 121 and 123, 4096 200 and 186; by 16x32 blocks, 128 tokens 60.1, 64 tokens
 // 48.3 (55.5, 60.6). Down, 1024 deep, 2048 columns: 512 tokens 45 and 49, 2048 110 and 121.
+// (Fitted to that one plan. Where two kernels are near each other it may take the slower: 1024
+// tokens' up product runs by 128x128.)
 struct Cost {
     double k, cus;
     bool plan;

@@ -8,7 +8,7 @@
 // loop of the instruction alone runs at 4.95 POP/s on zeros and 3.40 on random bytes,
 // where the chip lowers its clock; the 16x16x64 instruction at 2.91 and 2.71.)
 //
-// 8192^3 413-432 us (by the chip; 2.65 POP/s), 4096x14336x4096 213-222 (the library's 32-bit
+// 8192^3 413-432 us (by the chip; 2.65 POP/s), 4096x14336x4096 204-222 (the library's 32-bit
 // sums alone 231). Matrix units are busy 76% of the time, at 1.65 GHz, in
 // 4096x4096x16384 (204 us); without any fetch 79%, at 1.83: power bounds the loop. A tile's
 // results take 16 thousand cycles, the loop over k = 4096 72 thousand; two blocks of 128x128

@@ -200,8 +200,8 @@ __global__ __launch_bounds__(kThreads) void route_tokens(const Route p) {
     unsigned long long kept = ~0ull;
     if (p.groups > 1) {
         wave_lds_order();
-        // Its score goes to the group's first expert's place in `sums`.
-        double* sums = mine;  // once every lane has read its groups
+        // sums[g]: group g's score, over the token's keys once all lanes have theirs in registers.
+        double* sums = mine;
         kept = 0;
         double sum[4];
 #pragma unroll
