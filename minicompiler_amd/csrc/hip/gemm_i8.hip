@@ -239,14 +239,15 @@ __global__ __launch_bounds__(kWaves * 64) void i8_direct(const Product p) {
         const long long b_row = place.expert * b_rows + col;
         // One half's four columns, scaled, with the bias.
         const auto scaled = [&](i32x4 sum, long long at) {
-            f32x4 v;
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = 0.0f;
-                if (e < left) {
-                    v[e] = static_cast<float>(sum[e]) * sa.s * p.b_scales[at + e] * sa.back;
-                    if (p.bias != nullptr) v[e] += p.bias[at + e];
-                }
+            for (int e = 0; e < 4; ++e)
+                if (e < left) v[e] = static_cast<float>(sum[e]) * sa.s * p.b_scales[at + e];
+            if (sa.back != 1.0f) v *= sa.back;
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < left) v[e] += p.bias[at + e];
             }
             return v;
         };
